@@ -243,7 +243,7 @@ def _run_own(state):
         if case["bits"] == 16:
             out["k"], out["v"] = pool.k, pool.v
         else:
-            out["k"], out["v"] = fv_sdpa.paged_read(pool, batch)
+            out["k"], out["v"] = fv_sdpa.paged_read(pool, batch, state["k"].shape[0])
     if case["kind"] in ("attend", "step"):
         out["out"] = fv_sdpa.paged_attention(q, pool, batch, fv_sdpa.BlockCausal(case["block"], case["window"], case["sink"]))
     return out
