@@ -1,0 +1,559 @@
+// Attention over a paged KV cache (declarations: include/fv_sdpa_hip.h): for every row (token t of a sequence, query head h)
+// at position p, o = sum_j softmax_j(scale q . k_j) v_j over the keys j that it sees: block(j) <= block(p), and within the
+// window of blocks or among the sink blocks.
+//
+// Rows of one key head lie together (token by token, the heads of its group in turn), so a step over 32 keys serves all of
+// them with one load of K and V.
+#include <limits.h>
+#include <math.h>
+
+#include "../../include/fv_sdpa_hip.h"
+#include "fv_common.h"
+#include "fv_internal.h"
+#include "paged.h"
+
+namespace fv {
+namespace {
+
+constexpr int kStep = 32;       // keys a wave takes at a time
+constexpr int kWaves = 4;
+
+struct PagedAttnParams {
+    PagedPool pool;
+    PagedBatch b;
+    const uint16_t* q;
+    long q_stride;              // elements between tokens
+    void* out;                  // [tokens, heads, d]
+    int out_is_bf16;
+    int heads, group;           // query heads, of which `group` share a key head
+    float sl2;                  // scale * log2(e)
+    int block_tokens, window, sink;   // blocks; window 0: all
+    int tiles;                  // row tiles of a (sequence, key head)
+    int chunk, chunks;          // steps a workgroup takes of its walk, workgroups a walk
+    float* part_o;              // [chunks][tokens * heads][d], each normalised, and the base-2 logarithm of its sum
+    float* part_lse;            // [chunks][tokens * heads]
+};
+
+// The keys that a row at position p of a sequence of `len` tokens sees: [0, a) and [lo, hi), a <= hi.
+struct PagedSight {
+    int a, lo, hi;
+    // bit j: key k + j, j < 8. (Bits and selects: the comparisons key by key under divergent branches were compiled into
+    // code that lost the stores of -inf.)
+    FV_DEV unsigned eight(int k) const {
+        return below(a - k) | (below(hi - k) & ~below(lo - k));
+    }
+    static FV_DEV unsigned below(int n) { return (1u << min(max(n, 0), 8)) - 1u; }
+};
+template <class Params>
+FV_DEV PagedSight paged_sight(const Params& p, int pos, int len) {
+    if (pos < 0) return {0, 0, 0};
+    const int bt = p.block_tokens, block = bt == 1 ? pos : pos / bt;
+    const long hi = (long)(block + 1) * bt, sink = (long)p.sink * bt;
+    PagedSight s;
+    s.hi = (int)min(hi, (long)len);
+    s.lo = p.window > 0 ? max(0, block - p.window + 1) * bt : 0;
+    s.a = (int)min(sink, (long)s.hi);
+    return s;
+}
+
+// The walk of a tile of rows (tokens t0 .. t1 of the sequence): steps [0, ns) hold the sink, then [b0, b0 + n - ns).
+struct PagedWalk {
+    int ns, b0, n;
+    PagedSight any, all;        // the keys that some row sees (as a range: every key of the walk that none sees is outside), that all rows see
+    FV_DEV int key(int e) const { return (e < ns ? e : b0 + e - ns) * kStep; }
+    FV_DEV bool whole(int k) const {   // of the step at key k
+        const int e = k + kStep;
+        return e <= all.a || (k >= all.lo && e <= all.hi) || (all.a >= all.lo && e <= all.hi);
+    }
+};
+template <class Params>
+FV_DEV PagedWalk paged_walk(const Params& p, const PagedSeq& s, int t0, int t1) {
+    const int p0 = s.first_pos() + t0, p1 = s.first_pos() + t1;
+    PagedWalk w;
+    const PagedSight f = paged_sight(p, p0, s.len), l = paged_sight(p, p1, s.len);
+    w.all = {f.a, l.lo, f.hi};
+    w.any = {l.a, paged_sight(p, max(p0, 0), s.len).lo, l.hi};
+    w.ns = (w.any.a + kStep - 1) / kStep;
+    w.b0 = max(w.any.lo / kStep, w.ns);
+    w.n = w.ns + max(0, (w.any.hi + kStep - 1) / kStep - w.b0);
+    return w;
+}
+
+// What a lane holds of one step: lane l takes part in the products as row l % 16 and K group l / 16.
+//   K: its rows of two blocks of 16 keys. Row r of block b is key 8 (r / 4) + 4 b + r % 4, so that the scores S = K Q^T, whose
+//      lane has rows 4 (l / 16) .. + 3 of both blocks, are those of keys 8 (l / 16) .. + 7 in order: the probabilities are
+//      the operand of the second product as they stand.
+//   V: 8 keys, 8 (l / 16) .. + 7, of D / 16 channels, (D / 16) (l % 16) .. : turned over within the lane (v_perm_b32) they are the
+//      operands V^T of D / 16 products, channel (D / 16) r + c in row r of the c-th. Nothing passes through LDS.
+template <int D, bool FOUR>
+struct PagedStage;
+template <int D>
+struct PagedStage<D, false> {
+    static constexpr int kWords = D / 32;                  // words of D / 16 channels
+    typedef __attribute__((ext_vector_type(kWords))) unsigned vwords;
+    u32x4 k[2][D / 32];
+    vwords v[8];
+};
+template <int D>
+struct PagedStage<D, true> {
+    static constexpr int kWords = D / 32;
+    typedef __attribute__((ext_vector_type(D / 32))) unsigned kwords;   // D / 4 codes of a key
+    kwords k[2];
+    unsigned kscale[2];
+    unsigned v[8];                                          // D / 16 codes of a key (D = 64: in the low half)
+    u32x4 vscale[D / 64];                                   // the scales of the lane's 8 keys
+};
+
+template <int D, bool FOUR>
+struct PagedLane {
+    const uint8_t *k, *v, *ks, *vs;    // the lane's place in a half step of 16 keys at the pool's first row
+};
+
+template <int D, bool FOUR>
+FV_DEV void paged_load(PagedStage<D, FOUR>& s, const PagedLane<D, FOUR>& at, size_t row0, size_t row1, int lane) {
+    constexpr int kRow = PagedGeo<D, FOUR>::kRow;
+    const size_t rk = (lane & 8) ? row1 : row0, rv = (lane & 32) ? row1 : row0;
+    const uint8_t* k = at.k + rk * kRow;
+    const uint8_t* v = at.v + rv * kRow;
+    if constexpr (FOUR) {
+        constexpr int kS = PagedGeo<D, true>::kScales;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            s.k[b] = *reinterpret_cast<const typename PagedStage<D, true>::kwords*>(k + 4 * b * kRow);
+            s.kscale[b] = at.ks[rk * kS + 4 * b * kS];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (D == 128) s.v[j] = *reinterpret_cast<const unsigned*>(v + j * kRow);
+            else s.v[j] = *reinterpret_cast<const uint16_t*>(v + j * kRow);
+        }
+#pragma unroll
+        for (int j = 0; j < D / 64; j++) s.vscale[j] = *reinterpret_cast<const u32x4*>(at.vs + rv * kS + 16 * j);
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int dk = 0; dk < D / 32; dk++) s.k[b][dk] = *reinterpret_cast<const u32x4*>(k + 4 * b * kRow + 64 * dk);
+#pragma unroll
+        for (int j = 0; j < 8; j++) s.v[j] = *reinterpret_cast<const typename PagedStage<D, false>::vwords*>(v + j * kRow);
+    }
+}
+
+template <int D, bool FOUR>
+FV_DEV void paged_lane(PagedLane<D, FOUR>& at, const PagedPool& pool, int lane) {
+    constexpr int kRow = PagedGeo<D, FOUR>::kRow, kS = PagedGeo<D, FOUR>::kScales;
+    const int r = lane & 15, g = lane >> 4;
+    const int krow = 8 * ((r >> 2) & 1) + (r & 3), vrow = 8 * (g & 1);
+    at.k = (const uint8_t*)pool.k + krow * kRow + (FOUR ? g * (D / 8) : 16 * g);
+    at.v = (const uint8_t*)pool.v + vrow * kRow + r * (kRow / 16);
+    if constexpr (FOUR) {
+        at.ks = pool.ks + krow * kS + g * kS / 4;
+        at.vs = pool.vs + vrow * kS;
+    } else {
+        at.ks = at.vs = nullptr;
+    }
+}
+
+// The K operand of block b, piece dk: channels 32 dk + 8 g .. + 7 of a bf16 key, (D / 4) g + 8 dk .. + 7 of a 4-bit one.
+template <int D, bool FOUR>
+FV_DEV bf16x8 k_frag(const PagedStage<D, FOUR>& s, int b, int dk) {
+    if constexpr (FOUR) return __builtin_bit_cast(bf16x8, fp4_eight(s.k[b][dk], e8m0_scale(s.kscale[b])));
+    else return __builtin_bit_cast(bf16x8, s.k[b][dk]);
+}
+// The lane's V as bf16 words: D / 16 channels of key j.
+template <int D, bool FOUR>
+FV_DEV void v_words(const PagedStage<D, FOUR>& s, int lane, unsigned (&w)[8][D / 32]) {
+    if constexpr (FOUR) {
+        constexpr int kS = D / 32;                            // scale bytes a key
+        const int blk = (lane & 15) * (D / 16) / 32;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const unsigned bytes = s.vscale[j * kS / 16][(j * kS / 4) & 3];
+            const float scale = e8m0_scale((bytes >> (8 * ((j * kS & 3) + blk))) & 255u);
+            w[j][0] = fp4_pair<0>(s.v[j], scale);
+            w[j][1] = fp4_pair<1>(s.v[j], scale);
+            if constexpr (D == 128) {
+                w[j][2] = fp4_pair<2>(s.v[j], scale);
+                w[j][3] = fp4_pair<3>(s.v[j], scale);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int x = 0; x < D / 32; x++) w[j][x] = s.v[j][x];
+    }
+}
+
+// One workgroup: a share of the walk of a tile of 16 NT rows of one (sequence, key head); its four waves take the share's
+// steps in turn, each with a running maximum of its own, and join through LDS. The loads of a step go out while the one
+// before is computed.
+template <int D, bool FOUR, int NT>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParams p) {
+    constexpr int kNO = D / 16, kPad = D + 4;
+    __shared__ float lds_o[kWaves][16][kPad];
+    __shared__ float lds_ml[kWaves][16][2], lds_row[16][2];   // a wave's (offset, sum) of its rows; (1 / sum, log2 of the sum) of all
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    int item = blockIdx.x;
+    const int tile = item % p.tiles;
+    item /= p.tiles;
+    const int kvh = item % p.pool.kv_heads;
+    item /= p.pool.kv_heads;
+    const int chunk = item % p.chunks, seq = item / p.chunks;
+    const PagedSeq sq = paged_seq(p.b, seq);
+    const int rows = sq.count * p.group, row0 = tile * 16 * NT;
+    if (row0 >= rows) return;
+    const int t0 = row0 / p.group, t1 = (min(row0 + 16 * NT, rows) - 1) / p.group;
+    const PagedWalk w = paged_walk(p, sq, t0, t1);
+    const int e0 = chunk * p.chunk, e1 = min(w.n, e0 + p.chunk);
+    if (chunk > 0 && e0 >= e1) return;
+
+    PagedSight see[NT];
+    bf16x8 qf[NT][D / 32];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = row0 + 16 * n + col, t = r / p.group, h = kvh * p.group + r - t * p.group;
+        const bool ok = r < rows;
+        see[n] = paged_sight(p, ok ? sq.first_pos() + t : -1, sq.len);
+        const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + h * D + (FOUR ? (D / 4) * g : 8 * g);
+#pragma unroll
+        for (int dk = 0; dk < D / 32; dk++) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (ok) x = *reinterpret_cast<const u32x4*>(q + (FOUR ? 8 : 32) * dk);
+            qf[n][dk] = __builtin_bit_cast(bf16x8, x);
+        }
+    }
+    f32x4 o[NT][kNO];
+    float off[NT], l[NT];       // the offset of the lane's row in raw scores, the lane's share of its sum
+    bool some[NT];              // whether the row has seen a score (its offset is set)
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int c = 0; c < kNO; c++) o[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        off[n] = l[n] = 0.f;
+        some[n] = false;
+    }
+    PagedLane<D, FOUR> at;
+    paged_lane<D, FOUR>(at, p.pool, lane);
+    const int* table = p.b.table + (size_t)seq * p.b.table_stride;
+    const int lg = p.pool.lg, slots = (1 << lg) - 1, columns = (p.b.max_len + slots) >> lg;
+
+    auto compute = [&](const PagedStage<D, FOUR>& s, int k0, bool good0, bool good1) {
+        const bool whole = w.whole(k0) && good0 && good1;
+        bf16x8 pr[NT];
+        f32x4 x[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float m = -off[n];
+            x[n][0] = x[n][1] = f32x4{m, m, m, m};
+        }
+#pragma unroll
+        for (int dk = 0; dk < D / 32; dk++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const bf16x8 kf = k_frag<D, FOUR>(s, b, dk);
+#pragma unroll
+                for (int n = 0; n < NT; n++) x[n][b] = mfma16(kf, qf[n][dk], x[n][b]);
+            }
+        unsigned vw[8][D / 32];
+        v_words<D, FOUR>(s, lane, vw);
+        const int kl = k0 + 8 * g;
+        if (!whole) {   // keys that a row does not see, keys of pages that are none, values that no row sees (whatever they are)
+            const unsigned good = (g < 2 ? good0 : good1) ? 0xffu : 0u;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const unsigned seen = see[n].eight(kl) & good;
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[n][j >> 2][j & 3] = (seen >> j) & 1 ? x[n][j >> 2][j & 3] : neg_inf();
+            }
+            const unsigned used = w.any.eight(kl) & good;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) vw[j][i] = (used >> j) & 1 ? vw[j][i] : 0u;
+        }
+        bool need = false;
+        float mx[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float m = x[n][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) m = __builtin_fmaxf(m, x[n][j >> 2][j & 3]);
+            mx[n] = quad_max(m);
+            need |= mx[n] * p.sl2 > 6.0f || (!some[n] && mx[n] > neg_inf());
+        }
+        if (__builtin_amdgcn_ballot_w64(need) != 0) {   // rare: a row's maximum has outgrown its offset by 2^6, or is its first
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const bool move = mx[n] > neg_inf() && (!some[n] || mx[n] > 0.f);
+                const float delta = move ? mx[n] : 0.f;
+                const float alpha = some[n] ? fast_exp2(-delta * p.sl2) : 0.f;
+                l[n] *= alpha;
+                off[n] += delta;
+                some[n] |= mx[n] > neg_inf();
+#pragma unroll
+                for (int c = 0; c < kNO; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[n][c][i] *= alpha;
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[n][b][i] -= delta;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            f32x8 e;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                e[j] = fast_exp2(x[n][j >> 2][j & 3] * p.sl2);
+                l[n] += e[j];
+            }
+            pr[n] = __builtin_convertvector(e, bf16x8);
+        }
+#pragma unroll
+        for (int c = 0; c < kNO; c++) {
+            constexpr unsigned kLow = 0x05040100u, kHigh = 0x07060302u;
+            u32x4 t;
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[i] = __builtin_amdgcn_perm(vw[2 * i + 1][c >> 1], vw[2 * i][c >> 1], (c & 1) ? kHigh : kLow);
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, t);
+#pragma unroll
+            for (int n = 0; n < NT; n++) o[n][c] = mfma16(vf, pr[n], o[n][c]);
+        }
+    };
+
+    // groups of 64 steps of the wave: their page numbers are fetched at once, one a lane
+    for (int first = e0 + wave; first < e1; first += 64 * kWaves) {
+        const int mine = first + lane * kWaves;
+        const int my_key = w.key(min(mine, e1 - 1));
+        const int my_page = my_key >> lg;
+        const int id0 = table[my_page];
+        const int id1 = lg == 4 ? table[min(my_page + 1, columns - 1)] : id0;
+        const int count = min(64, (e1 - first + kWaves - 1) / kWaves);
+        auto fetch = [&](PagedStage<D, FOUR>& s, int i, int& k0, bool& good0, bool& good1) {
+            i = min(i, count - 1);
+            const int a = __builtin_amdgcn_readlane(id0, i), b = __builtin_amdgcn_readlane(id1, i);
+            k0 = w.key(first + i * kWaves);
+            good0 = (unsigned)a < (unsigned)p.pool.pages;
+            good1 = (unsigned)b < (unsigned)p.pool.pages;
+            const size_t r0 = (((size_t)(good0 ? a : 0) * p.pool.kv_heads + kvh) << lg) + (k0 & slots);
+            const size_t r1 = lg == 4 ? ((size_t)(good1 ? b : 0) * p.pool.kv_heads + kvh) << lg : r0 + 16;
+            paged_load<D, FOUR>(s, at, r0, r1, lane);
+        };
+        PagedStage<D, FOUR> sa, sb;
+        int ka, kb;
+        bool a0, a1, b0, b1;
+        fetch(sa, 0, ka, a0, a1);
+        for (int i = 0; i < count; i += 2) {   // (a fetch past the group's end takes its last step again)
+            fetch(sb, i + 1, kb, b0, b1);
+            compute(sa, ka, a0, a1);
+            if (i + 1 >= count) break;
+            fetch(sa, i + 2, ka, a0, a1);
+            compute(sb, kb, b0, b1);
+        }
+    }
+
+    // join the waves: each brings its rows' offsets and sums, and its O scaled to the common offset
+    const bool split = w.n > p.chunk;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float sum = quad_sum(l[n]);
+        const float m2 = some[n] ? off[n] * p.sl2 : neg_inf();
+        if (g == 0) lds_ml[wave][col][0] = m2, lds_ml[wave][col][1] = sum;
+        __syncthreads();
+        float top = neg_inf(), total = 0.f;
+#pragma unroll
+        for (int x = 0; x < kWaves; x++) top = __builtin_fmaxf(top, lds_ml[x][col][0]);
+#pragma unroll
+        for (int x = 0; x < kWaves; x++) {
+            const float mx = lds_ml[x][col][0];
+            total += mx == neg_inf() ? lds_ml[x][col][1] : lds_ml[x][col][1] * fast_exp2(mx - top);
+        }
+        const float scale = m2 == neg_inf() ? 1.f : fast_exp2(m2 - top);
+        // lane: channels (D / 4) g + kNO i + c of its row
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int c = 0; c < kNO; c += 4)
+                *reinterpret_cast<f32x4*>(&lds_o[wave][col][(D / 4) * g + kNO * i + c]) =
+                    f32x4{o[n][c][i] * scale, o[n][c + 1][i] * scale, o[n][c + 2][i] * scale, o[n][c + 3][i] * scale};
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        if (wave == 0 && g == 0) lds_row[col][0] = inv, lds_row[col][1] = top == neg_inf() ? (total == 0.f ? neg_inf() : total) : top + __log2f(total);
+        __syncthreads();
+        {
+            constexpr int kPer = D / 16;   // channels a thread stores
+            const int rr = threadIdx.x >> 4, cc = (threadIdx.x & 15) * kPer;
+            const int r = row0 + 16 * n + rr;
+            if (r < rows) {
+                const int t = r / p.group;
+                const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
+                const float k = lds_row[rr][0];
+                float val[kPer];
+#pragma unroll
+                for (int c = 0; c < kPer; c++) {
+                    float a = 0.f;
+#pragma unroll
+                    for (int x = 0; x < kWaves; x++) a += lds_o[x][rr][cc + c];
+                    val[c] = a * k;
+                }
+                if (split) {
+                    const size_t all = (size_t)p.b.tokens * p.heads;
+                    float* po = p.part_o + ((size_t)chunk * all + dst) * D + cc;
+#pragma unroll
+                    for (int c = 0; c < kPer; c += 4) *reinterpret_cast<f32x4*>(po + c) = f32x4{val[c], val[c + 1], val[c + 2], val[c + 3]};
+                    if (cc == 0) p.part_lse[(size_t)chunk * all + dst] = lds_row[rr][1];
+                } else if (p.out_is_bf16) {
+                    __attribute__((ext_vector_type(kPer))) float f;
+#pragma unroll
+                    for (int c = 0; c < kPer; c++) f[c] = val[c];
+                    typedef __attribute__((ext_vector_type(kPer))) __bf16 bfv;
+                    *reinterpret_cast<bfv*>((uint16_t*)p.out + dst * D + cc) = __builtin_convertvector(f, bfv);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kPer; c += 4)
+                        *reinterpret_cast<f32x4*>((float*)p.out + dst * D + cc + c) = f32x4{val[c], val[c + 1], val[c + 2], val[c + 3]};
+                }
+            }
+        }
+        if (NT > 1) __syncthreads();
+    }
+}
+
+// The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). A workgroup takes 256 / (D / 4)
+// rows of one sequence; rows whose walk one workgroup made have their result already.
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
+    constexpr int kPer = D / 4, kRows = 256 / kPer;
+    const int seq = blockIdx.x / p.pool.kv_heads, kvh = blockIdx.x % p.pool.kv_heads;
+    const PagedSeq sq = paged_seq(p.b, seq);
+    const int rows = sq.count * p.group, r = blockIdx.y * kRows + threadIdx.x / kPer, c = (threadIdx.x % kPer) * 4;
+    if (r >= rows || r >= p.tiles * ROWS) return;
+    const int row0 = r / ROWS * ROWS;
+    const PagedWalk w = paged_walk(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group);
+    if (w.n <= p.chunk) return;
+    const int chunks = (w.n + p.chunk - 1) / p.chunk, t = r / p.group;
+    const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group), all = (size_t)p.b.tokens * p.heads;
+    float top = neg_inf();
+    bool nan = false;   // (a share whose sum is not a number: max drops it)
+    for (int s = 0; s < chunks; s++) {
+        const float x = p.part_lse[s * all + dst];
+        top = __builtin_fmaxf(top, x);
+        nan |= x != x;
+    }
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+    if (top != neg_inf() || nan) {
+        for (int s = 0; s < chunks; s++) {
+            const float k = fast_exp2(p.part_lse[s * all + dst] - top);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + (s * all + dst) * D + c);
+            total += k;
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] += k * x[i];
+        }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] *= inv;
+    if (p.out_is_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.out + dst * D + c) = __builtin_convertvector(acc, bf16x4);
+    else *reinterpret_cast<f32x4*>((float*)p.out + dst * D + c) = acc;
+}
+
+// How a call is cut. (Host arithmetic on the call's bounds: the lengths themselves are the device's.)
+struct PagedCut {
+    size_t nt, tiles, steps, chunk, chunks;
+};
+PagedCut paged_cut(size_t heads, size_t kv_heads, size_t seqs, size_t max_q, size_t max_len, size_t block_tokens, size_t window, size_t sink) {
+    PagedCut c;
+    const size_t group = heads / kv_heads, rows = max_q * group;
+    c.nt = rows <= 16 ? 1 : 2;
+    c.tiles = (rows + 16 * c.nt - 1) / (16 * c.nt);
+    c.steps = (max_len + kStep - 1) / kStep;
+    if (window > 0) {   // the window, the tile's tokens (which lie in as many blocks, or in two), a step at either end; the sink
+        const size_t tokens = (16 * c.nt + group - 1) / group + 1, blocks = window + tokens;
+        const size_t far = (size_t)1 << 31;
+        const size_t band = blocks < far / block_tokens ? blocks * block_tokens : far, keep = sink < far / block_tokens ? sink * block_tokens : far;
+        const size_t most = (band + kStep - 1) / kStep + 1 + (keep + kStep - 1) / kStep;
+        if (most < c.steps) c.steps = most;
+    }
+    if (c.steps == 0) c.steps = 1;
+    const size_t base = seqs * kv_heads * c.tiles, slots = 4 * (size_t)fv_compute_units();
+    size_t chunk = (base * c.steps + slots - 1) / slots;
+    chunk = (chunk + kWaves - 1) / kWaves * kWaves;
+    if (chunk < kWaves) chunk = kWaves;
+    c.chunks = (c.steps + chunk - 1) / chunk;
+    if (c.chunks > 64) c.chunks = 64;
+    c.chunk = ((c.steps + c.chunks - 1) / c.chunks + kWaves - 1) / kWaves * kWaves;
+    c.chunks = (c.steps + c.chunk - 1) / c.chunk;
+    return c;
+}
+size_t part_bytes(size_t chunks, size_t tokens, size_t heads, size_t d) {
+    if (chunks <= 1) return 0;
+    const size_t rows = chunks * tokens * heads, lse = (rows * 4 + 255) / 256 * 256;
+    return rows * d * 4 + lse;
+}
+
+}  // namespace
+}  // namespace fv
+
+extern "C" {
+
+size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q, size_t max_len,
+                                          size_t block_tokens, size_t window, size_t sink) {
+    if (kv_heads == 0 || heads < kv_heads || heads % kv_heads != 0 || block_tokens == 0 || seqs == 0 || tokens == 0 || max_q == 0) return 0;
+    const fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, max_q, max_len, block_tokens, window, sink);
+    return fv::part_bytes(c.chunks, tokens, heads, d);
+}
+
+int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is_bf16, size_t heads, const void* k_pages,
+                       const void* v_pages, const void* k_scales, const void* v_scales, size_t pages, size_t page_tokens, size_t kv_heads,
+                       size_t d, const int32_t* q_start, const int32_t* lens, const int32_t* table, size_t table_stride, size_t table_pages,
+                       size_t seqs, size_t tokens, size_t max_q, size_t max_len, float scale, size_t block_tokens, size_t window,
+                       size_t sink, void* workspace, size_t workspace_bytes, void* stream) {
+    fv::PagedAttnParams p;
+    const int rc = fv_paged_args("paged attention", k_pages, v_pages, k_scales, v_scales, pages, page_tokens, kv_heads, d, q_start, lens,
+                                 table, table_stride, table_pages, seqs, tokens, &max_len, &p.pool, &p.b);
+    if (rc != FV_OK) return rc;
+    if (!q || !out) return fv_invalid("paged attention: null operand");
+    if (heads == 0 || heads % kv_heads != 0) return fv_invalid("paged attention: query heads must be a multiple of the key heads");
+    if (heads > 65535) return fv_decline("paged attention: too many heads");
+    if (q_stride < heads * d) return fv_invalid("paged attention: tokens overlap (a stride below heads * d)");
+    if (q_stride % 8 != 0 || q_stride > (size_t)INT_MAX / 4) return fv_decline("paged attention: the stride must be a multiple of 8 elements");
+    if (((uintptr_t)q & 15) != 0 || ((uintptr_t)out & 15) != 0) return fv_invalid("paged attention: operands must be 16-byte aligned");
+    if (!(scale > 0.f) || !(scale <= 2e38f)) return fv_decline("paged attention: scale must be positive and finite");
+    if (block_tokens == 0) return fv_invalid("paged attention: block_tokens must be positive");
+    if (block_tokens > (size_t)INT_MAX / 2 || window > (size_t)INT_MAX / 2 || sink > (size_t)INT_MAX / 2)
+        return fv_decline("paged attention: mask too large");
+    if (max_q > tokens) max_q = tokens;
+    if (seqs == 0 || tokens == 0 || max_q == 0) return FV_OK;
+    fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, max_q, max_len, block_tokens, window, sink);
+    const size_t need = fv::part_bytes(c.chunks, tokens, heads, d);
+    if (need > 0 && (!workspace || workspace_bytes < need)) c.chunks = 1, c.chunk = (c.steps + fv::kWaves - 1) / fv::kWaves * fv::kWaves;
+    if (c.chunks > 1 && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
+    const size_t blocks = seqs * kv_heads * c.tiles * c.chunks;
+    const dim3 join((unsigned)(seqs * kv_heads), (unsigned)((max_q * (heads / kv_heads) * (d / 4) + 255) / 256));
+    if (blocks >= (size_t)1 << 24 || seqs * kv_heads * join.y >= (size_t)1 << 24) return fv_decline("paged attention: too large for one launch");
+    p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
+    p.heads = (int)heads, p.group = (int)(heads / kv_heads);
+    p.sl2 = (float)((double)scale * 1.4426950408889634);
+    p.block_tokens = (int)block_tokens, p.window = (int)window, p.sink = (int)sink;
+    p.tiles = (int)c.tiles, p.chunk = (int)c.chunk, p.chunks = (int)c.chunks;
+    p.part_o = (float*)workspace;
+    p.part_lse = p.part_o ? p.part_o + c.chunks * tokens * heads * d : nullptr;
+    const bool four = k_scales != nullptr;
+    hipStream_t st = (hipStream_t)stream;
+    fv::paged_pick(d == 128, [&](auto d128) {
+        fv::paged_pick(four, [&](auto f) {
+            fv::paged_pick(c.nt == 1, [&](auto one) {
+                constexpr int D = d128() ? 128 : 64, NT = one() ? 1 : 2;
+                hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), NT>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+                if (c.chunks > 1) hipLaunchKernelGGL((fv::paged_join_kernel<D, 16 * NT>), join, dim3(256), 0, st, p);
+            });
+        });
+    });
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? FV_OK : fv_fail_hip(e, "paged_attention");
+}
+
+}  // extern "C"

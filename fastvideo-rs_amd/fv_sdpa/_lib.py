@@ -53,6 +53,13 @@ SIGNATURES = {
     "fv_kv_cache_pointers": (C.c_int, [_vp, _sz, _vp]),
     "fv_kv_cache_bytes": (_sz, [_vp]),
     "fv_kv_cache_update": (C.c_int, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp]),
+    "fv_paged_append": (C.c_int, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, C.c_int, _sz, _vp, _vp, _sz, _vp, C.c_int, _vp, _vp, _vp,
+                                  _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
+    "fv_paged_read": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _sz,
+                                _vp]),
+    "fv_paged_attention_workspace_bytes": (_sz, [_sz] * 10),
+    "fv_paged_attention": (C.c_int, [_vp, _sz, _vp, C.c_int, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz,
+                                     _sz, _sz, _sz, _sz, _sz, C.c_float, _sz, _sz, _sz, _vp, _sz, _vp]),
     "fv_sdpa_block_causal_bf16": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, _sz, _sz, _sz, _sz, C.c_float,
                                             _sz, _sz, _sz, _vp]),
     "fv_cast_f32_bf16": (C.c_int, [_vp, _vp, _sz, _vp]),

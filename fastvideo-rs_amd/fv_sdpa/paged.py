@@ -1,0 +1,172 @@
+"""A paged KV cache and the attention over it (include/fv_sdpa_hip.h, `fv_paged_*`; no counterpart in the reference): many
+sequences of different lengths in one pool of pages of bf16 or of 4 bits, new tokens appended with the rotation of their
+positions applied on the way, attention under the block mask with a window and sinks, single tokens to long prompts.
+"""
+import math
+
+import torch
+
+from . import _lib
+
+__all__ = ["PagedKv", "PagedBatch", "paged_append", "paged_read", "paged_attention"]
+
+_BF16, _F32, _U8, _I32 = torch.bfloat16, torch.float32, torch.uint8, torch.int32
+
+
+class PagedKv:
+    """One layer's pool: k, v [pages, kv_heads, page_tokens, d] bf16, or 4-bit codes [.., d / 2] with k_scales, v_scales
+    [.., d / 32] (uint8 all four). The tensors are the caller's, used in place."""
+
+    __slots__ = ("k", "v", "k_scales", "v_scales", "d", "_args")
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
+        four = k_scales is not None
+        shape = k.shape
+        if (v_scales is None) == four or len(shape) != 4 or v.shape != shape:
+            raise ValueError("PagedKv: want k and v [pages, kv_heads, page_tokens, d] of one shape, with scales for both or neither")
+        dtype, dev = (_U8 if four else _BF16), k.get_device()
+        if k.dtype is not dtype or v.dtype is not dtype or not k.is_contiguous() or not v.is_contiguous() or dev < 0 or v.get_device() != dev:
+            raise ValueError(f"PagedKv: want contiguous CUDA tensors of {dtype} on one device")
+        d = shape[3] * 2 if four else shape[3]
+        if four:
+            want = (*shape[:3], d // 32)
+            for t in (k_scales, v_scales):
+                if t.dtype is not _U8 or tuple(t.shape) != want or not t.is_contiguous() or t.get_device() != dev:
+                    raise ValueError(f"PagedKv: want contiguous uint8 scales {want} on the pages' device")
+        self.k, self.v, self.k_scales, self.v_scales, self.d = k, v, k_scales, v_scales, d
+        self._args = (k.data_ptr(), v.data_ptr(), k_scales.data_ptr() if four else None, v_scales.data_ptr() if four else None,
+                      shape[0], shape[2], shape[1], d)
+
+    @staticmethod
+    def new(pages, page_tokens, kv_heads, d, four_bits=False, device="cuda"):
+        """A pool of zeros."""
+        shape = (pages, kv_heads, page_tokens)
+        if not four_bits:
+            return PagedKv(*(torch.zeros((*shape, d), dtype=_BF16, device=device) for _ in range(2)))
+        return PagedKv(*(torch.zeros((*shape, n), dtype=_U8, device=device) for n in (d // 2, d // 2, d // 32, d // 32)))
+
+    @property
+    def four_bits(self):
+        return self.k_scales is not None
+
+    @property
+    def page_tokens(self):
+        return self.k.shape[2]
+
+    @property
+    def kv_heads(self):
+        return self.k.shape[1]
+
+
+class PagedBatch:
+    """The sequences of a call: int32 CUDA tensors q_start [n + 1] (rows of sequence s: q_start[s] .. q_start[s + 1]), lens [n]
+    (tokens in the cache, the new ones among them) and table [n, columns] (page numbers); max_q and max_len bound the rows of
+    a sequence and its length (host numbers: the launches are sized by them; max_len None: what the table's columns hold)."""
+
+    __slots__ = ("q_start", "lens", "table", "max_q", "max_len", "_args", "_device")
+
+    def __init__(self, q_start, lens, table, max_q, max_len=None):
+        n, dev = lens.shape[0], lens.get_device()
+        if lens.dim() != 1 or q_start.shape != (n + 1,) or table.dim() != 2 or table.shape[0] != n:
+            raise ValueError("PagedBatch: want q_start [n + 1], lens [n] and table [n, columns]")
+        for t in (q_start, lens, table):
+            if t.dtype is not _I32 or t.get_device() != dev or dev < 0:
+                raise ValueError("PagedBatch: want int32 CUDA tensors on one device")
+        if not q_start.is_contiguous() or not lens.is_contiguous() or (table.shape[1] > 1 and table.stride(1) != 1) or (n > 1 and table.stride(0) < table.shape[1]):
+            raise ValueError("PagedBatch: want contiguous arrays (of the table: rows)")
+        if max_q < 0 or (max_len is not None and max_len < 0):
+            raise ValueError("PagedBatch: bounds must not be negative")
+        self.q_start, self.lens, self.table, self.max_q, self.max_len, self._device = q_start, lens, table, max_q, max_len, dev
+        self._args = (q_start.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0) if n > 1 else table.shape[1], table.shape[1], n)
+
+
+def _rows(t, name, heads, d, dtypes, device):
+    """Elements between the tokens of t [tokens, heads, d], whose heads are contiguous."""
+    if t.dim() != 3 or t.dtype not in dtypes or t.get_device() != device:
+        raise ValueError(f"{name}: want a [tokens, heads, d] tensor of {' or '.join(str(x) for x in dtypes)} on the pool's device")
+    n, h, dd = t.shape
+    if (heads and h != heads) or dd != d:
+        raise ValueError(f"{name}: want [tokens, {heads or 'heads'}, {d}], got {tuple(t.shape)}")
+    a, b, c = t.stride()
+    if c != 1 or (h > 1 and b != d):
+        raise ValueError(f"{name}: the heads of a token must be contiguous")
+    return a if n > 1 else h * d
+
+
+def _on(device, name):
+    if torch._C._cuda_getDevice() != device:
+        raise ValueError(f"{name}: the tensors are on cuda:{device}, which is not the current device")
+
+
+def paged_append(pool, batch, k, v, rope=None, halves=False, rope_at=None, q=None):
+    """The new tokens' k, v [tokens, kv_heads, d] (f32 or bf16) into the pool, the keys turned by their positions (rows of
+    rope = (cos, sin), f32 [rows, d]; rope_at: int32 [tokens], rows in place of the positions). q [tokens, heads, d]: turned
+    likewise and returned, bf16. halves: pairs (i, i + d / 2) instead of (2i, 2i + 1)."""
+    dev, kvh, d = pool.k.get_device(), pool.kv_heads, pool.d
+    _on(dev, "paged_append")
+    tokens = k.shape[0]
+    dtypes = (k.dtype,) if k.dtype in (_F32, _BF16) else (_F32, _BF16)
+    ks, vs = _rows(k, "k", kvh, d, dtypes, dev), _rows(v, "v", kvh, d, dtypes, dev)
+    if v.shape[0] != tokens or batch._device != dev:
+        raise ValueError("paged_append: k and v differ in tokens, or the batch is on another device")
+    qs, heads, q_out = 0, 0, None
+    if q is not None:
+        qs, heads = _rows(q, "q", 0, d, dtypes, dev), q.shape[1]
+        if q.shape[0] != tokens:
+            raise ValueError("paged_append: q and k differ in tokens")
+        q_out = torch.empty((tokens, heads, d), device=q.device, dtype=_BF16)
+    cos = sin = None
+    rows = 0
+    if rope is not None:
+        cos, sin = rope
+        rows = cos.shape[0]
+        for t in rope:
+            if t.dtype is not _F32 or t.shape != (rows, d) or not t.is_contiguous() or t.get_device() != dev:
+                raise ValueError(f"paged_append: rope tables must be contiguous f32 [rows, {d}] on the pool's device")
+        if rope_at is not None and (rope_at.dtype is not _I32 or rope_at.shape != (tokens,) or not rope_at.is_contiguous() or rope_at.get_device() != dev):
+            raise ValueError("paged_append: rope_at must be contiguous int32 [tokens] on the pool's device")
+    elif rope_at is not None:
+        raise ValueError("paged_append: rope_at without tables")
+    _lib.check(_lib.lib().fv_paged_append(
+        k.data_ptr(), ks, v.data_ptr(), vs, q.data_ptr() if q is not None else None, qs, q_out.data_ptr() if q is not None else None,
+        1 if k.dtype is _BF16 else 0, heads, cos.data_ptr() if rows else None, sin.data_ptr() if rows else None, rows,
+        rope_at.data_ptr() if rope_at is not None else None, 1 if halves else 0, *pool._args, *batch._args, tokens, _lib.stream()))
+    return q_out
+
+
+def paged_read(pool, batch, tokens, out_bf16=True):
+    """(k, v) [tokens, kv_heads, d] of the batch's tokens; rows behind the last sequence are not written."""
+    dev = pool.k.get_device()
+    _on(dev, "paged_read")
+    if batch._device != dev:
+        raise ValueError("paged_read: the batch is on another device")
+    k, v = (torch.empty((tokens, pool.kv_heads, pool.d), device=pool.k.device, dtype=_BF16 if out_bf16 else _F32) for _ in range(2))
+    _lib.check(_lib.lib().fv_paged_read(k.data_ptr(), v.data_ptr(), 1 if out_bf16 else 0, *pool._args, *batch._args, tokens, _lib.stream()))
+    return k, v
+
+
+def paged_attention(q, pool, batch, mask=None, scale=None, out_bf16=True, out=None):
+    """softmax(scale q k^T) v of the rows q [tokens, heads, d] (bf16) over the cached keys of their sequences, [tokens, heads, d].
+    mask: a BlockCausal; None: causal by token. A sink block is not seen before its time (BlockCausal.allows has it always
+    seen). Rows behind the last sequence are not written."""
+    dev, kvh, d = pool.k.get_device(), pool.kv_heads, pool.d
+    _on(dev, "paged_attention")
+    qs = _rows(q, "q", 0, d, (_BF16,), dev)
+    if batch._device != dev:
+        raise ValueError("paged_attention: the batch is on another device")
+    tokens, heads, _ = q.shape
+    dtype = _BF16 if out_bf16 else _F32
+    if out is None:
+        out = torch.empty((tokens, heads, d), device=q.device, dtype=dtype)
+    elif out.dtype is not dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(q.shape)} on {q.device}")
+    max_len = batch.max_len if batch.max_len is not None else batch.table.shape[1] * pool.page_tokens
+    bt, window, sink = (mask.block_tokens, mask.window, mask.sink) if mask is not None else (1, 0, 0)
+    n = batch._args[5]
+    lib = _lib.lib()
+    nbytes = lib.fv_paged_attention_workspace_bytes(heads, kvh, d, n, tokens, batch.max_q, max_len, bt, window, sink)
+    work = torch.empty(nbytes, device=q.device, dtype=_U8) if nbytes else None
+    _lib.check(lib.fv_paged_attention(
+        q.data_ptr(), qs, out.data_ptr(), 1 if out_bf16 else 0, heads, *pool._args, *batch._args, tokens, batch.max_q, max_len,
+        1.0 / math.sqrt(d) if scale is None else scale, bt, window, sink, work.data_ptr() if nbytes else None, nbytes, _lib.stream()))
+    return out

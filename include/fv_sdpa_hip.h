@@ -350,6 +350,60 @@ size_t fv_kv_cache_bytes(const fv_kv_cache* c);
 int fv_kv_cache_update(fv_kv_cache* c, size_t layer, const fv_tensor* k, const fv_tensor* v, size_t current_start,
                        fv_tensor* k_window, fv_tensor* v_window, void* stream);
 
+/* ---- the paged KV cache (no counterpart in the reference) ---------------------------------------
+ * Many sequences of different lengths in one pool of pages. The pool: k_pages / v_pages [pages, kv_heads, page_tokens, d],
+ * page_tokens a power of two of 16 to 65536, d 64 or 128, 16-byte aligned;
+ *   k_scales == v_scales == NULL: bf16 bits;
+ *   else 4 bits: codes [pages, kv_heads, page_tokens, d / 2] (e2m1: 0 .5 1 1.5 2 3 4 6 and their negatives, channel 2i in the low
+ *   half of byte i) and scales [pages, kv_heads, page_tokens, d / 32] (e8m0: 2^(byte - 127) for 32 channels, 255: not a number).
+ * The batch, int32 device arrays: sequence s has lens[s] tokens in the cache, this call's new ones among them, which are rows
+ * q_start[s] .. q_start[s + 1] (ascending, q_start[0] is the first row's number) of the ragged tensors [tokens, heads, d]: the last
+ * tokens of the sequence, in order. Token j lies in slot j % page_tokens of page table[s * table_stride + j / page_tokens],
+ * of table_pages columns. Entries of pages that a call does not reach are not read; sequences may share pages that none of
+ * them appends to (two tokens of one call in one slot: either is kept). A page number outside the pool is no fault: nothing is
+ * written there, it reads as zeros, and its keys are seen by no query. Rows at q_start[seqs] and behind are left as they were, so
+ * a padded batch may be captured into a graph and replayed with other lengths, tables and counts. The arrays are read when the
+ * call's work runs.
+ *
+ * fv_paged_append: the new tokens' keys k and values v [tokens, kv_heads, d] into the cache, the keys (and the queries q
+ * [tokens, heads, d], into q_out, contiguous bf16 bits; both NULL: none) turned by row rope_at[token] (NULL: by the token's
+ * position) of the f32 tables cos_t / sin_t [rope_rows, d] (both NULL: not turned). halves == 0: pairs (2i, 2i + 1), the angle in
+ * slot 2i, as fv_rope_bhsd; else pairs (i, i + d / 2), the angle in slot i. Inputs are f32 or bf16 bits (in_is_bf16, all three),
+ * tokens k_stride / v_stride / q_stride elements apart (multiples of 8; a slice of a fused projection). f32 arithmetic, products
+ * unfused, one rounding: to bf16, or to 4 bits with the smallest power of two for each 32 channels that takes none of them past
+ * the largest code (ties to the even code; a value that is not finite makes its 32 channels not a number). A token whose
+ * table row lies outside the tables, or that lies before the first token of its sequence (more rows than tokens), is not
+ * stored and its query is zeros. */
+int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q, size_t q_stride,
+                    uint16_t* q_out, int in_is_bf16, size_t heads, const float* cos_t, const float* sin_t, size_t rope_rows,
+                    const int32_t* rope_at, int halves, void* k_pages, void* v_pages, void* k_scales, void* v_scales,
+                    size_t pages, size_t page_tokens, size_t kv_heads, size_t d, const int32_t* q_start, const int32_t* lens,
+                    const int32_t* table, size_t table_stride, size_t table_pages, size_t seqs, size_t tokens, void* stream);
+/* The batch's tokens out of the cache: k_out, v_out [tokens, kv_heads, d], contiguous, f32 or bf16 bits (both exact; a
+ * 4-bit value of 2^128 or more is infinite). With
+ * q_start the running sums of lens, whole sequences (a contiguous copy for the dense entries, for keeping elsewhere). */
+int fv_paged_read(void* k_out, void* v_out, int out_is_bf16, const void* k_pages, const void* v_pages, const void* k_scales,
+                  const void* v_scales, size_t pages, size_t page_tokens, size_t kv_heads, size_t d, const int32_t* q_start,
+                  const int32_t* lens, const int32_t* table, size_t table_stride, size_t table_pages, size_t seqs,
+                  size_t tokens, void* stream);
+/* out [tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale * q k^T) v of the batch's rows over the cached keys of
+ * their sequences; q bf16 bits, tokens q_stride elements apart; heads / kv_heads neighbouring heads share a key head. Under the
+ * block mask of fv_sdpa_block_causal_bf16 with one difference: the query at position i sees key j iff, t = position / block_tokens,
+ * tj <= ti && (window == 0 || ti - tj < window || tj < sink): a sink block is not seen before its time. block_tokens == 1: causal by
+ * token, a window of tokens, sink tokens. A row that sees no key is zeros. max_q / max_len: bounds of the rows of a sequence and of
+ * lens, host numbers that the launch is sized by (longer lengths are cut to max_len, rows past max_q may not be written).
+ * workspace: fv_paged_attention_workspace_bytes of the same numbers (0: none), 256-byte aligned, this call's alone until its work
+ * is done; where it is too small or NULL long walks are not split, which costs time only (and bits: shares are
+ * normalised before they are joined). The results of a call with the same bounds and workspace are the same bits. */
+size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q,
+                                          size_t max_len, size_t block_tokens, size_t window, size_t sink);
+int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is_bf16, size_t heads, const void* k_pages,
+                       const void* v_pages, const void* k_scales, const void* v_scales, size_t pages, size_t page_tokens,
+                       size_t kv_heads, size_t d, const int32_t* q_start, const int32_t* lens, const int32_t* table,
+                       size_t table_stride, size_t table_pages, size_t seqs, size_t tokens, size_t max_q, size_t max_len,
+                       float scale, size_t block_tokens, size_t window, size_t sink, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 /* ---- Video Sparse Attention (rt/vsa.rs, rt/ops.rs:811-1619) --------------------------
  * Geometry: 64-token cubes (4x4x4 in t,h,w), TilePlan arrays as rt/vsa.rs:42-109:
  * slot_src [num_tiles*64] (token of each padded slot, -1 = padding), block_sizes
