@@ -5,9 +5,11 @@
 // Rows of one key head lie together (token by token, the heads of its group in turn), so a step over 32 keys serves all of
 // them with one load of K and V.
 #include <limits.h>
-#include <math.h>
+
+#include <algorithm>
 
 #include "../../include/fv_sdpa_hip.h"
+#include "attn_core.h"
 #include "fv_common.h"
 #include "fv_internal.h"
 #include "paged.h"
@@ -28,8 +30,14 @@ struct PagedAttnParams {
     int heads, group;           // query heads, of which `group` share a key head
     float sl2;                  // scale * log2(e)
     int block_tokens, window, sink;   // blocks; window 0: all
-    int tiles;                  // row tiles of a (sequence, key head)
-    int chunk, chunks;          // steps a workgroup takes of its walk, workgroups a walk
+    // Two kernels share a call: sequences of up to `few` rows a key head go to paged_rows_kernel, the others to
+    // paged_tiles_kernel. How each cuts its part:
+    int few;
+    struct Cut {
+        int tiles;              // row tiles of a (sequence, key head)
+        int chunk, chunks;      // steps of the walk that a workgroup takes, workgroups a walk
+    } rows, big;
+    int big_total, big_per_xcd; // workgroups of paged_tiles_kernel, an eighth of them
     float* part_o;              // [chunks][tokens * heads][d], each normalised, and the base-2 logarithm of its sum
     float* part_lse;            // [chunks][tokens * heads]
 };
@@ -56,26 +64,31 @@ FV_DEV PagedSight paged_sight(const Params& p, int pos, int len) {
     return s;
 }
 
-// The walk of a tile of rows (tokens t0 .. t1 of the sequence): steps [0, ns) hold the sink, then [b0, b0 + n - ns).
+// The walk of a tile of rows (tokens t0 .. t1 of the sequence) in steps of STEP keys: [0, ns) hold the sink, then
+// [b0, b0 + n - ns).
+template <int STEP>
 struct PagedWalk {
     int ns, b0, n;
-    PagedSight any, all;        // the keys that some row sees (as a range: every key of the walk that none sees is outside), that all rows see
-    FV_DEV int key(int e) const { return (e < ns ? e : b0 + e - ns) * kStep; }
-    FV_DEV bool whole(int k) const {   // of the step at key k
-        const int e = k + kStep;
-        return e <= all.a || (k >= all.lo && e <= all.hi) || (all.a >= all.lo && e <= all.hi);
-    }
+    PagedSight any;             // the keys that some row sees
+    FV_DEV int key(int e) const { return (e < ns ? e : b0 + e - ns) * STEP; }
 };
+// Whether rows all of which see `all` see every key of [k, e).
+FV_DEV bool paged_whole(const PagedSight& all, int k, int e) {
+    return e <= all.a || (k >= all.lo && e <= all.hi) || (all.a >= all.lo && e <= all.hi);
+}
 template <class Params>
-FV_DEV PagedWalk paged_walk(const Params& p, const PagedSeq& s, int t0, int t1) {
-    const int p0 = s.first_pos() + t0, p1 = s.first_pos() + t1;
-    PagedWalk w;
-    const PagedSight f = paged_sight(p, p0, s.len), l = paged_sight(p, p1, s.len);
-    w.all = {f.a, l.lo, f.hi};
-    w.any = {l.a, paged_sight(p, max(p0, 0), s.len).lo, l.hi};
-    w.ns = (w.any.a + kStep - 1) / kStep;
-    w.b0 = max(w.any.lo / kStep, w.ns);
-    w.n = w.ns + max(0, (w.any.hi + kStep - 1) / kStep - w.b0);
+FV_DEV PagedSight paged_all(const Params& p, const PagedSeq& s, int t0, int t1) {   // what the tokens t0 .. t1 all see
+    const PagedSight f = paged_sight(p, s.first_pos() + t0, s.len), l = paged_sight(p, s.first_pos() + t1, s.len);
+    return {f.a, l.lo, f.hi};
+}
+template <int STEP, class Params>
+FV_DEV PagedWalk<STEP> paged_walk(const Params& p, const PagedSeq& s, int t0, int t1) {
+    PagedWalk<STEP> w;
+    const PagedSight l = paged_sight(p, s.first_pos() + t1, s.len);
+    w.any = {l.a, paged_sight(p, max(s.first_pos() + t0, 0), s.len).lo, l.hi};
+    w.ns = (w.any.a + STEP - 1) / STEP;
+    w.b0 = max(w.any.lo / STEP, w.ns);
+    w.n = w.ns + max(0, (w.any.hi + STEP - 1) / STEP - w.b0);
     return w;
 }
 
@@ -196,17 +209,18 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     int item = blockIdx.x;
-    const int tile = item % p.tiles;
-    item /= p.tiles;
+    const int tile = item % p.rows.tiles;
+    item /= p.rows.tiles;
     const int kvh = item % p.pool.kv_heads;
     item /= p.pool.kv_heads;
-    const int chunk = item % p.chunks, seq = item / p.chunks;
+    const int chunk = item % p.rows.chunks, seq = item / p.rows.chunks;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group, row0 = tile * 16 * NT;
-    if (row0 >= rows) return;
+    if (row0 >= rows || rows > p.few) return;
     const int t0 = row0 / p.group, t1 = (min(row0 + 16 * NT, rows) - 1) / p.group;
-    const PagedWalk w = paged_walk(p, sq, t0, t1);
-    const int e0 = chunk * p.chunk, e1 = min(w.n, e0 + p.chunk);
+    const PagedWalk<kStep> w = paged_walk<kStep>(p, sq, t0, t1);
+    const PagedSight all_see = paged_all(p, sq, t0, t1);
+    const int e0 = chunk * p.rows.chunk, e1 = min(w.n, e0 + p.rows.chunk);
     if (chunk > 0 && e0 >= e1) return;
 
     PagedSight see[NT];
@@ -240,7 +254,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     const int lg = p.pool.lg, slots = (1 << lg) - 1, columns = (p.b.max_len + slots) >> lg;
 
     auto compute = [&](const PagedStage<D, FOUR>& s, int k0, bool good0, bool good1) {
-        const bool whole = w.whole(k0) && good0 && good1;
+        const bool whole = paged_whole(all_see, k0, k0 + kStep) && good0 && good1;
         bf16x8 pr[NT];
         f32x4 x[NT][2];
 #pragma unroll
@@ -356,7 +370,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     }
 
     // join the waves: each brings its rows' offsets and sums, and its O scaled to the common offset
-    const bool split = w.n > p.chunk;
+    const bool split = w.n > p.rows.chunk;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const float sum = quad_sum(l[n]);
@@ -421,19 +435,296 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     }
 }
 
+// Sequences of many rows: a workgroup takes 128 rows of one (sequence, key head), 32 a wave, over tiles of 64 keys that pass
+// through LDS as in the dense kernels (attn_core.h): two buffers for K, two for V. A phase is one key tile: the matrix part
+// (O += P V of the tile before, S = K Q^T) with the next K and this V on their way in, the softmax, one barrier. A wave brings
+// 16 keys of each tile, which lie in one page whatever its size, so a page costs a tile one lookup:
+//   bf16 pages: loads straight to LDS through a buffer descriptor of the wave's 16 rows, whose length cuts off what lies
+//     behind the sequence's last key (zeros in LDS, whatever the page holds);
+//   4-bit pages: a lane has a quarter of a row in registers a phase ahead and writes it to LDS as bf16 between the matrix
+//     instructions, 4 conversions and a write at a time.
+constexpr int kBigRows = 128, kTileKeys = 64;
+template <int D, bool FOUR>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const PagedAttnParams p) {
+    using G = TileGeo<D>;
+    constexpr int kNO = D / 16, kTile = G::kTile;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+    lds_u8* smem = (lds_u8*)smem_raw;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q4 = lane >> 4, i16 = lane & 15;
+    // XCD x takes a contiguous eighth of the items, key head by key head, so that an L2 holds few heads' keys; the last rows,
+    // whose walks are the longest, first
+    int item = (blockIdx.x & 7) * p.big_per_xcd + (blockIdx.x >> 3);
+    if (item >= p.big_total) return;
+    const int tile = p.big.tiles - 1 - item % p.big.tiles;
+    item /= p.big.tiles;
+    const int chunk = item % p.big.chunks;
+    item /= p.big.chunks;
+    const int seq = item % p.b.seqs, kvh = item / p.b.seqs;
+    const PagedSeq sq = paged_seq(p.b, seq);
+    const int rows = sq.count * p.group, row0 = tile * kBigRows;
+    if (row0 >= rows || rows <= p.few) return;
+    const PagedWalk<kTileKeys> w = paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
+    const int e0 = chunk * p.big.chunk, e1 = min(w.n, e0 + p.big.chunk);
+    if (chunk > 0 && e0 >= e1) return;
+    const bool split = w.n > p.big.chunk;
+    const float sl2 = p.sl2;
+
+    // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
+    const int wrow = row0 + 32 * wave;
+    PagedSight all_see = {0x7fffffff, 0, 0x7fffffff}, mine = {0, 0, 0};
+    if (wrow < rows) {
+        all_see = paged_all(p, sq, wrow / p.group, (min(wrow + 32, rows) - 1) / p.group);
+        const int r = wrow + (lane & 31);
+        mine = paged_sight(p, sq.first_pos() + min(r, rows - 1) / p.group, sq.len);
+    }
+    bf16x8 qf[D / 32][2];
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const int r = wrow + 16 * g + i16, t = r / p.group;
+        const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + (kvh * p.group + r - t * p.group) * D + 8 * q4;
+#pragma unroll
+        for (int dk = 0; dk < D / 32; dk++) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (r < rows) x = *reinterpret_cast<const u32x4*>(q + 32 * dk);
+            qf[dk][g] = __builtin_bit_cast(bf16x8, x);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0) here: the compiler's own wait for them would stand among the tile loads
+
+    const int* table = p.b.table + (size_t)seq * p.b.table_stride;
+    const int lg = p.pool.lg, slots = (1 << lg) - 1, columns = (p.b.max_len + slots) >> lg;
+    // page numbers of 64 tiles of the walk, a tile a lane: that of the wave's 16 keys, and which of the tile's four 16 are in the pool
+    int ids = 0, good = 0, ids_at = e0;
+    auto look_up = [&](int e) {
+        ids_at = e;
+        const int k = w.key(min(e + lane, max(e1 - 1, 0)));
+        good = 0;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const int id = table[min((k + 16 * x) >> lg, columns - 1)];
+            const bool ok = (unsigned)id < (unsigned)p.pool.pages;
+            good |= ok ? 1 << x : 0;
+            if (x == wave) ids = ok ? id : -1;
+        }
+    };
+    const TileReadBases rb = tile_read_bases<D>(lane);
+    auto kbuf = [&](int m) -> lds_u8* { return smem + (m & 1) * kTile; };
+    auto vbuf = [&](int m) -> lds_u8* { return smem + (2 + (m & 1)) * kTile; };
+    // Where the wave's 16 keys of walk position e lie: their first key, its row in the pool, and how many of them, from the
+    // front, are keys of the sequence in a page of the pool.
+    struct Part {
+        int key;
+        unsigned row;
+        int count;
+    };
+    auto part_of = [&](int e) {
+        Part x;
+        x.key = w.key(min(e, e1 - 1)) + 16 * wave;
+        const int id = __builtin_amdgcn_readlane(ids, min(e, e1 - 1) - ids_at);
+        x.row = (((unsigned)max(id, 0) * (unsigned)p.pool.kv_heads + (unsigned)kvh) << lg) + (unsigned)(x.key & slots);
+        x.count = id < 0 ? 0 : min(max(w.any.hi - x.key, 0), 16);
+        return x;
+    };
+    // Whether no row sees row r of a part: a key between the sink and the window. (What lies there may be anything.)
+    auto some_hidden = [&](const Part& x) { return x.key < w.any.lo && x.key + 16 > w.any.a && w.any.a < w.any.lo; };
+    auto hidden = [&](const Part& x, int r) { return x.key + r >= w.any.a && x.key + r < w.any.lo; };
+
+    // bf16 pages
+    constexpr int kIter = FOUR ? 2 : TileDma<4, D>::ITER, kUnits = kIter / 2;
+    unsigned koff[kIter], voff[kIter];
+    // 4-bit pages: the lane's quarter of row lane / 4
+    constexpr int kQuarter = D / 32;   // words of codes; 16-byte pieces of bf16
+    typedef __attribute__((ext_vector_type(kQuarter))) unsigned quarter;
+    quarter kq = {}, vq = {};
+    unsigned kqs = 127, vqs = 127;
+    const int qrow = lane >> 2, qpart = lane & 3;
+    if constexpr (!FOUR) {
+#pragma unroll
+        for (int it = 0; it < kIter; it++) {
+            const int r = it * G::kRowsPerDma + lane / G::kChunks, c = lane % G::kChunks;
+            koff[it] = r * G::kRow + ((c ^ G::kswz(r)) << 4) - (it & 1) * 1024;
+            voff[it] = r * G::kRow + ((c ^ G::vswz(r)) << 4) - (it & 1) * 1024;
+        }
+    }
+    // bf16: unit u (two loads) of the wave's part of a tile
+    auto issue = [&](const void* pages, const Part& x, lds_u8* buf, const unsigned (&off)[kIter], int u) {
+        const u32x4 desc = plane_descriptor((const uint8_t*)pages + (size_t)x.row * G::kRow, (unsigned)x.count * G::kRow);
+        const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(buf + wave * 16 * G::kRow + u * 2048));
+        unsigned o0 = off[2 * u], o1 = off[2 * u + 1];
+        if (some_hidden(x)) {   // past the descriptor's end
+            const int r = 2 * u * G::kRowsPerDma + lane / G::kChunks;
+            o0 = hidden(x, r) ? 0x40000000u : o0;
+            o1 = hidden(x, r + G::kRowsPerDma) ? 0x40000000u : o1;
+        }
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                     "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds"
+                     :: "s"(m0), "v"(o0), "v"(o1), "s"(desc) : "memory");
+    };
+    // 4 bits: the lane's quarter of K or V of a part, into registers ...
+    auto fetch = [&](const void* pages, const uint8_t* scales, const Part& x, quarter& c, unsigned& sc) {
+        const size_t row = (size_t)x.row + qrow;
+        c = *reinterpret_cast<const quarter*>((const uint8_t*)pages + row * (D / 2) + qpart * (D / 8));
+        sc = scales[row * (D / 32) + qpart * (D / 32) / 4];
+    };
+    auto keep = [&](const Part& x, quarter& c, unsigned& sc) {   // what nobody sees is zeros
+        const bool none = qrow >= x.count || hidden(x, qrow);
+#pragma unroll
+        for (int j = 0; j < kQuarter; j++) c[j] = none ? 0u : c[j];
+        sc = none ? 127u : sc;
+    };
+    // ... and piece j (8 channels) of it as bf16 to its place in the tile
+    auto put = [&](lds_u8* buf, int swz, const quarter& c, unsigned sc, int j) {
+        lds_write_b128(buf + (16 * wave + qrow) * G::kRow + (((kQuarter * qpart + j) ^ swz) << 4), fp4_eight(c[j], e8m0_scale(sc)));
+    };
+
+    f32x4 o[kNO][2], s_init[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    SoftmaxOffState st;
+    st.init();
+    ProbTile pb;
+
+    auto mask_tile = [&](ScoreTile& s, int e) {
+        const int k = w.key(e), ok = __builtin_amdgcn_readlane(good, e - ids_at);
+        if (paged_whole(all_see, k, k + kTileKeys) && ok == 15) return;
+        const unsigned m[3] = {(unsigned)mine.a, (unsigned)mine.lo, (unsigned)mine.hi};
+        int both[3][2];   // the even rows of 16 lanes hold block 0's, the odd ones block 1's
+#pragma unroll
+        for (int x = 0; x < 3; x++) {
+            const auto r = __builtin_amdgcn_permlane16_swap(m[x], m[x], false, false);
+            both[x][0] = (int)r[0];
+            both[x][1] = (int)r[1];
+        }
+        const int at = k + 4 * q4;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const unsigned long long seen = first_bits(both[0][g] - at) | (first_bits(both[2][g] - at) & ~first_bits(both[1][g] - at));
+            const unsigned half[2] = {(unsigned)seen, (unsigned)(seen >> 32)};
+#pragma unroll
+            for (int kb = 0; kb < 4; kb++) {
+                const unsigned bits = (ok >> kb) & 1 ? half[kb >> 1] >> (16 * (kb & 1)) : 0u;
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[kb][g][i] = (bits >> i) & 1 ? s[kb][g][i] : neg_inf();
+            }
+        }
+    };
+
+    if (e0 < e1) {
+        look_up(e0);
+        Part cur = part_of(e0), next = part_of(e0 + 1);   // of the tile whose V is loaded next, whose K is
+        if constexpr (FOUR) {
+            fetch(p.pool.k, p.pool.ks, cur, kq, kqs);
+            keep(cur, kq, kqs);
+#pragma unroll
+            for (int j = 0; j < kQuarter; j++) put(kbuf(0), G::kswz(qrow), kq, kqs, j);
+            fetch(p.pool.v, p.pool.vs, cur, vq, vqs);
+            fetch(p.pool.k, p.pool.ks, next, kq, kqs);
+            __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+        } else {
+#pragma unroll
+            for (int u = 0; u < kUnits; u++) issue(p.pool.k, cur, kbuf(0), koff, u);
+            wait_vmcnt<0>();
+        }
+        block_barrier();
+        constexpr int kAhead = 3;
+        auto phase = [&](int m, auto first) {
+            const int e = e0 + m;
+            Part after = next;
+            ScoreTile s;
+            auto hook = [&](int i) {
+                if constexpr (FOUR) {
+                    // V of this tile and K of the next, fetched a phase ago; then the fetches for the next phase
+                    if (i == 0) keep(cur, vq, vqs), keep(next, kq, kqs);
+                    if (i < kQuarter) put(vbuf(m), G::vswz(qrow), vq, vqs, i);
+                    else if (i < 2 * kQuarter) put(kbuf(m + 1), G::kswz(qrow), kq, kqs, i - kQuarter);
+                    else if (i == 2 * kQuarter) after = part_of(e + 2), fetch(p.pool.v, p.pool.vs, next, vq, vqs);
+                    else if (i == 2 * kQuarter + 1) fetch(p.pool.k, p.pool.ks, after, kq, kqs);
+                } else {
+                    if (i < kUnits) issue(p.pool.v, cur, vbuf(m), voff, i);
+                    else if (i < 2 * kUnits) issue(p.pool.k, next, kbuf(m + 1), koff, i - kUnits);
+                    else if (i == 2 * kUnits) after = part_of(e + 2);
+                }
+            };
+            __builtin_amdgcn_s_setprio(1);
+            if constexpr (first()) {
+                mfma_phase<false, kAhead, D>(vbuf(0), kbuf(0), rb, pb, o, qf, s, s_init, hook);
+                if constexpr (FOUR) {   // (a phase without its P V part has half the gaps)
+#pragma unroll
+                    for (int i = G::kKGroups; i < 2 * kQuarter + 2; i++) hook(i);
+                }
+#pragma unroll
+                for (int db = 0; db < kNO; db++) o[db][0] = o[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            } else {
+                mfma_phase<true, kAhead, D>(vbuf(m - 1), kbuf(m), rb, pb, o, qf, s, s_init, hook);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            mask_tile(s, e);
+            if constexpr (first()) softmax_first_off<true>(s, st, s_init, sl2, pb);
+            else softmax_tile_off<true>(s, st, o, s_init, sl2, pb);
+            asm volatile("" ::"v"(pb[0][0]), "v"(pb[0][1]), "v"(pb[1][0]), "v"(pb[1][1]), "v"(st.l_acc[0]), "v"(st.l_acc[1]));
+            cur = next;
+            next = after;
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (FOUR) __builtin_amdgcn_s_waitcnt(0xC07F);
+            else wait_vmcnt<0>();
+            block_barrier();   // K(m + 1), V(m) resident; this phase's tiles read by every wave
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        phase(0, std::true_type{});
+#pragma unroll 1
+        for (int m = 1; m < e1 - e0; m++) {
+            if (e0 + m + 2 - ids_at >= 64 && e0 + m + 2 < e1) look_up(e0 + m);
+            phase(m, std::false_type{});
+        }
+        pv_tile<D>(vbuf(e1 - e0 - 1), rb.v, pb, o);
+    } else {
+#pragma unroll
+        for (int db = 0; db < kNO; db++) o[db][0] = o[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const size_t all = (size_t)p.b.tokens * p.heads;
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const float l = quad_sum(st.l_acc[g]);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int r = wrow + 16 * g + i16, t = r / p.group;
+        if (r >= rows) continue;
+        const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
+        if (split && q4 == 0) p.part_lse[(size_t)chunk * all + dst] = l == 0.f ? neg_inf() : st.log2_offset<true>(g, sl2) + __log2f(l);
+#pragma unroll
+        for (int db = 0; db < kNO; db++) {
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = o[db][g][i] * inv;
+            const size_t at = dst * D + 16 * db + 4 * q4;
+            if (split) *reinterpret_cast<f32x4*>(p.part_o + (size_t)chunk * all * D + at) = x;
+            else if (p.out_is_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.out + at) = __builtin_convertvector(x, bf16x4);
+            else *reinterpret_cast<f32x4*>((float*)p.out + at) = x;
+        }
+    }
+}
+
 // The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). A workgroup takes 256 / (D / 4)
-// rows of one sequence; rows whose walk one workgroup made have their result already.
+// rows of one sequence; rows whose walk one workgroup made have their result already. ROWS: of a tile of paged_rows_kernel.
 template <int D, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
     constexpr int kPer = D / 4, kRows = 256 / kPer;
     const int seq = blockIdx.x / p.pool.kv_heads, kvh = blockIdx.x % p.pool.kv_heads;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group, r = blockIdx.y * kRows + threadIdx.x / kPer, c = (threadIdx.x % kPer) * 4;
-    if (r >= rows || r >= p.tiles * ROWS) return;
-    const int row0 = r / ROWS * ROWS;
-    const PagedWalk w = paged_walk(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group);
-    if (w.n <= p.chunk) return;
-    const int chunks = (w.n + p.chunk - 1) / p.chunk, t = r / p.group;
+    if (r >= rows) return;
+    int chunks;
+    if (rows <= p.few) {
+        const int row0 = r / ROWS * ROWS;
+        chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
+        if (r >= p.rows.tiles * ROWS) return;
+    } else {
+        const int row0 = r / kBigRows * kBigRows;
+        chunks = (paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + p.big.chunk - 1) / p.big.chunk;
+        if (r >= p.big.tiles * kBigRows) return;
+    }
+    if (chunks <= 1) return;
+    const int t = r / p.group;
     const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group), all = (size_t)p.b.tokens * p.heads;
     float top = neg_inf();
     bool nan = false;   // (a share whose sum is not a number: max drops it)
@@ -460,32 +751,56 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     else *reinterpret_cast<f32x4*>((float*)p.out + dst * D + c) = acc;
 }
 
-// How a call is cut. (Host arithmetic on the call's bounds: the lengths themselves are the device's.)
-struct PagedCut {
-    size_t nt, tiles, steps, chunk, chunks;
-};
-PagedCut paged_cut(size_t heads, size_t kv_heads, size_t seqs, size_t max_q, size_t max_len, size_t block_tokens, size_t window, size_t sink) {
-    PagedCut c;
-    const size_t group = heads / kv_heads, rows = max_q * group;
-    c.nt = rows <= 16 ? 1 : 2;
-    c.tiles = (rows + 16 * c.nt - 1) / (16 * c.nt);
-    c.steps = (max_len + kStep - 1) / kStep;
-    if (window > 0) {   // the window, the tile's tokens (which lie in as many blocks, or in two), a step at either end; the sink
-        const size_t tokens = (16 * c.nt + group - 1) / group + 1, blocks = window + tokens;
-        const size_t far = (size_t)1 << 31;
+// Steps of `step` keys that the walk of a tile of `rows` rows may have. (Host arithmetic on the call's bounds: the lengths
+// themselves are the device's.)
+size_t walk_bound(size_t step, size_t rows, size_t group, size_t max_len, size_t block_tokens, size_t window, size_t sink) {
+    size_t steps = (max_len + step - 1) / step;
+    if (window > 0) {   // the window, the tile's tokens (which lie in as many blocks, or fewer), a step at either end; the sink
+        const size_t blocks = window + (rows + group - 1) / group + 1, far = (size_t)1 << 31;
         const size_t band = blocks < far / block_tokens ? blocks * block_tokens : far, keep = sink < far / block_tokens ? sink * block_tokens : far;
-        const size_t most = (band + kStep - 1) / kStep + 1 + (keep + kStep - 1) / kStep;
-        if (most < c.steps) c.steps = most;
+        steps = std::min(steps, (band + step - 1) / step + 1 + (keep + step - 1) / step);
     }
-    if (c.steps == 0) c.steps = 1;
-    const size_t base = seqs * kv_heads * c.tiles, slots = 4 * (size_t)fv_compute_units();
-    size_t chunk = (base * c.steps + slots - 1) / slots;
-    chunk = (chunk + kWaves - 1) / kWaves * kWaves;
-    if (chunk < kWaves) chunk = kWaves;
-    c.chunks = (c.steps + chunk - 1) / chunk;
-    if (c.chunks > 64) c.chunks = 64;
-    c.chunk = ((c.steps + c.chunks - 1) / c.chunks + kWaves - 1) / kWaves * kWaves;
-    c.chunks = (c.steps + c.chunk - 1) / c.chunk;
+    return std::max<size_t>(steps, 1);
+}
+
+// How a call is cut.
+struct PagedCut {
+    size_t few = 0;                         // rows a key head up to which a sequence is paged_rows_kernel's
+    size_t nt = 0;                          // its tiles of 16 rows; 0: not launched
+    size_t rows_tiles = 1, rows_chunk = 1, rows_chunks = 1;
+    size_t big_tiles = 0, big_chunk = 1, big_chunks = 1;   // of paged_tiles_kernel; no tiles: not launched
+    size_t chunks() const { return std::max(nt ? rows_chunks : 1, big_tiles ? big_chunks : 1); }
+};
+constexpr size_t kFewRows = 64;
+PagedCut paged_cut(size_t heads, size_t kv_heads, size_t seqs, size_t tokens, size_t max_q, size_t max_len, size_t block_tokens,
+                   size_t window, size_t sink) {
+    PagedCut c;
+    const size_t group = heads / kv_heads, rows = max_q * group, units = (size_t)fv_compute_units();
+    if (rows > kFewRows) {
+        c.big_tiles = (rows + kBigRows - 1) / kBigRows;
+        const size_t steps = walk_bound(kTileKeys, kBigRows, group, max_len, block_tokens, window, sink);
+        // tiles that hold rows: those of the longest sequence alone where one has them all
+        const size_t base = kv_heads * std::min(seqs * c.big_tiles, tokens * group / kBigRows + seqs);
+        // shares of the walk: rounds of two workgroups a unit, a fixed part of 4 steps each, against what joining moves
+        double best = 0;
+        for (size_t k = 1; k <= 32 && k <= steps; k++) {
+            const size_t chunk = (steps + k - 1) / k, rounds = (base * k + 2 * units - 1) / (2 * units);
+            const double cost = (double)rounds * (double)(chunk + 4) * 2.0 + (k > 1 ? 5.0 + (double)(k * tokens * heads) * 1024.0 / 4e6 : 0.0);
+            if (k == 1 || cost < 0.97 * best) best = cost, c.big_chunk = chunk, c.big_chunks = (steps + chunk - 1) / chunk;
+        }
+    }
+    if (rows <= kFewRows || seqs > 1) {   // (the one sequence of a long call is the tiles' whatever its rows)
+        const size_t most = std::min(rows, kFewRows);
+        c.few = rows <= kFewRows ? rows : kFewRows;
+        c.nt = most <= 16 ? 1 : 2;
+        c.rows_tiles = (most + 16 * c.nt - 1) / (16 * c.nt);
+        const size_t steps = walk_bound(kStep, 16 * c.nt, group, max_len, block_tokens, window, sink);
+        const size_t base = seqs * kv_heads * c.rows_tiles, slots = 4 * units;
+        size_t chunk = std::max<size_t>(((base * steps + slots - 1) / slots + kWaves - 1) / kWaves, 1) * kWaves;
+        chunk = std::max(chunk, ((steps + 63) / 64 + kWaves - 1) / kWaves * kWaves);
+        c.rows_chunk = chunk;
+        c.rows_chunks = (steps + chunk - 1) / chunk;
+    }
     return c;
 }
 size_t part_bytes(size_t chunks, size_t tokens, size_t heads, size_t d) {
@@ -502,8 +817,8 @@ extern "C" {
 size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q, size_t max_len,
                                           size_t block_tokens, size_t window, size_t sink) {
     if (kv_heads == 0 || heads < kv_heads || heads % kv_heads != 0 || block_tokens == 0 || seqs == 0 || tokens == 0 || max_q == 0) return 0;
-    const fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, max_q, max_len, block_tokens, window, sink);
-    return fv::part_bytes(c.chunks, tokens, heads, d);
+    const fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
+    return fv::part_bytes(c.chunks(), tokens, heads, d);
 }
 
 int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is_bf16, size_t heads, const void* k_pages,
@@ -527,29 +842,40 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
         return fv_decline("paged attention: mask too large");
     if (max_q > tokens) max_q = tokens;
     if (seqs == 0 || tokens == 0 || max_q == 0) return FV_OK;
-    fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, max_q, max_len, block_tokens, window, sink);
-    const size_t need = fv::part_bytes(c.chunks, tokens, heads, d);
-    if (need > 0 && (!workspace || workspace_bytes < need)) c.chunks = 1, c.chunk = (c.steps + fv::kWaves - 1) / fv::kWaves * fv::kWaves;
-    if (c.chunks > 1 && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
-    const size_t blocks = seqs * kv_heads * c.tiles * c.chunks;
+    fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, tokens, max_q, max_len, block_tokens, window, sink);
+    const size_t need = fv::part_bytes(c.chunks(), tokens, heads, d);
+    if (need > 0 && (!workspace || workspace_bytes < need)) {   // a share is the whole walk
+        c.rows_chunk *= c.rows_chunks, c.big_chunk *= c.big_chunks;
+        c.rows_chunks = c.big_chunks = 1;
+    }
+    const bool split = c.chunks() > 1;
+    if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
     const dim3 join((unsigned)(seqs * kv_heads), (unsigned)((max_q * (heads / kv_heads) * (d / 4) + 255) / 256));
-    if (blocks >= (size_t)1 << 24 || seqs * kv_heads * join.y >= (size_t)1 << 24) return fv_decline("paged attention: too large for one launch");
+    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_blocks = seqs * kv_heads * c.big_tiles * c.big_chunks;
+    constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
+    if (row_blocks >= kMost || big_blocks + 8 >= kMost || seqs * kv_heads * join.y >= kMost)
+        return fv_decline("paged attention: too large for one launch");
     p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
     p.heads = (int)heads, p.group = (int)(heads / kv_heads);
     p.sl2 = (float)((double)scale * 1.4426950408889634);
     p.block_tokens = (int)block_tokens, p.window = (int)window, p.sink = (int)sink;
-    p.tiles = (int)c.tiles, p.chunk = (int)c.chunk, p.chunks = (int)c.chunks;
+    p.few = (int)c.few;
+    p.rows = {(int)c.rows_tiles, (int)c.rows_chunk, (int)c.rows_chunks};
+    p.big = {(int)c.big_tiles, (int)c.big_chunk, (int)c.big_chunks};
+    p.big_total = (int)big_blocks, p.big_per_xcd = (int)((big_blocks + 7) / 8);
     p.part_o = (float*)workspace;
-    p.part_lse = p.part_o ? p.part_o + c.chunks * tokens * heads * d : nullptr;
+    p.part_lse = split ? p.part_o + c.chunks() * tokens * heads * d : nullptr;
     const bool four = k_scales != nullptr;
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(d == 128, [&](auto d128) {
         fv::paged_pick(four, [&](auto f) {
-            fv::paged_pick(c.nt == 1, [&](auto one) {
-                constexpr int D = d128() ? 128 : 64, NT = one() ? 1 : 2;
-                hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), NT>), dim3((unsigned)blocks), dim3(256), 0, st, p);
-                if (c.chunks > 1) hipLaunchKernelGGL((fv::paged_join_kernel<D, 16 * NT>), join, dim3(256), 0, st, p);
-            });
+            constexpr int D = d128() ? 128 : 64;
+            if (c.big_tiles)
+                hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3(8 * p.big_per_xcd), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
+            if (c.nt == 1) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 1>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
+            if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
+            if (split && c.nt == 1) hipLaunchKernelGGL((fv::paged_join_kernel<D, 16>), join, dim3(256), 0, st, p);
+            if (split && c.nt != 1) hipLaunchKernelGGL((fv::paged_join_kernel<D, 32>), join, dim3(256), 0, st, p);
         });
     });
     const hipError_t e = hipGetLastError();

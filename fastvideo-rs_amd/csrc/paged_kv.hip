@@ -244,6 +244,8 @@ int fv_paged_args(const char* who, const void* k_pages, const void* v_pages, con
         return say("page_tokens must be a power of two of 16 to 65536", true);
     if (kv_heads == 0 || pages == 0) return say("an empty pool", false);
     if (kv_heads > 65535 || pages > (size_t)INT_MAX) return say("pool too large", true);
+    // (row numbers are 32 bits: as many rows of K and V are more than the card holds)
+    if (pages > 0xffffffffull / kv_heads / page_tokens) return say("pool too large", true);
     if (!fv::aligned16(k_pages) || !fv::aligned16(v_pages) || !fv::aligned16(k_scales) || !fv::aligned16(v_scales))
         return say("pages and scales must be 16-byte aligned", false);
     if (table_pages > table_stride) return say("table rows shorter than their pages", false);

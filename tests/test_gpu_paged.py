@@ -309,3 +309,22 @@ def test_long_walks_are_split_and_joined(fv):
                                     None, 0, torch.cuda.current_stream().cuda_stream)
         assert rc == 0
         w.check(q, out, f"unsplit four={four} d={d}")
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("d,page", [(128, 16), (128, 64), (64, 32)])
+def test_many_rows_over_long_walks(fv, four, d, page):
+    """More tiles than page numbers are looked up at once, walks split and whole, rows of one sequence and of several, a page
+    that the pool does not have in the middle."""
+    announce(f"paged: many rows, long walks four={four} d={d} page={page}")
+    for lens, counts, mask in (([9000], [150], (1, 0, 0)), ([6000, 90, 5003], [40, 90, 3], (1, 0, 0)), ([7000, 5000], [64, 100], (1, 4500, 70)),
+                               ([4680], [1560], (1560, 0, 0))):
+        kvh, heads = (1, 2) if counts[0] > 1000 else (2, 4)
+        w = World(fv, 61 + d + len(lens), lens, counts, kvh, d, page, four, fill="nan")
+        w.table[0, 40 * 16 // page] = -3
+        w.table[-1, 1] = w.pages + 5
+        w.batch = fv.PagedBatch(w.dev(w.starts), w.dev(np.array(lens, dtype=np.int32)), w.dev(w.table), max(counts), max(lens))
+        q = w.queries(heads, 1.5)
+        for out16 in (True, False):
+            got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=out16)
+            w.check(q, got, f"long {lens} {mask} four={four} d={d} out16={out16}", *mask)
