@@ -33,7 +33,8 @@ struct PagedSeq {
     int start, count, len;   // first row, rows, tokens in the cache
     FV_DEV int first_pos() const { return len - count; }   // of row `start`; negative where there are more rows than tokens
 };
-FV_DEV PagedSeq paged_seq(const PagedBatch& b, int s) {
+template <class Batch>   // (PagedBatch, or the same struct read through another address space)
+FV_DEV PagedSeq paged_seq(const Batch& b, int s) {
     PagedSeq q;
     q.start = min(max(b.q_start[s], 0), b.tokens);
     q.count = min(max(b.q_start[s + 1], q.start), b.tokens) - q.start;

@@ -123,30 +123,39 @@ struct PagedLane {
 };
 
 template <int D, bool FOUR>
-FV_DEV void paged_load(PagedStage<D, FOUR>& s, const PagedLane<D, FOUR>& at, size_t row0, size_t row1, int lane) {
+FV_DEV void paged_load_k(PagedStage<D, FOUR>& s, const PagedLane<D, FOUR>& at, unsigned row0, unsigned row1, int lane) {
     constexpr int kRow = PagedGeo<D, FOUR>::kRow;
-    const size_t rk = (lane & 8) ? row1 : row0, rv = (lane & 32) ? row1 : row0;
-    const uint8_t* k = at.k + rk * kRow;
-    const uint8_t* v = at.v + rv * kRow;
+    const size_t row = (lane & 8) ? row1 : row0;
+    const uint8_t* k = at.k + row * kRow;
     if constexpr (FOUR) {
         constexpr int kS = PagedGeo<D, true>::kScales;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             s.k[b] = *reinterpret_cast<const typename PagedStage<D, true>::kwords*>(k + 4 * b * kRow);
-            s.kscale[b] = at.ks[rk * kS + 4 * b * kS];
+            s.kscale[b] = at.ks[row * kS + 4 * b * kS];
         }
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int dk = 0; dk < D / 32; dk++) s.k[b][dk] = *reinterpret_cast<const u32x4*>(k + 4 * b * kRow + 64 * dk);
+    }
+}
+template <int D, bool FOUR>
+FV_DEV void paged_load_v(PagedStage<D, FOUR>& s, const PagedLane<D, FOUR>& at, unsigned row0, unsigned row1, int lane) {
+    constexpr int kRow = PagedGeo<D, FOUR>::kRow;
+    const size_t row = (lane & 32) ? row1 : row0;
+    const uint8_t* v = at.v + row * kRow;
+    if constexpr (FOUR) {
+        constexpr int kS = PagedGeo<D, true>::kScales;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             if constexpr (D == 128) s.v[j] = *reinterpret_cast<const unsigned*>(v + j * kRow);
             else s.v[j] = *reinterpret_cast<const uint16_t*>(v + j * kRow);
         }
 #pragma unroll
-        for (int j = 0; j < D / 64; j++) s.vscale[j] = *reinterpret_cast<const u32x4*>(at.vs + rv * kS + 16 * j);
+        for (int j = 0; j < D / 64; j++) s.vscale[j] = *reinterpret_cast<const u32x4*>(at.vs + row * kS + 16 * j);
     } else {
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int dk = 0; dk < D / 32; dk++) s.k[b][dk] = *reinterpret_cast<const u32x4*>(k + 4 * b * kRow + 64 * dk);
 #pragma unroll
         for (int j = 0; j < 8; j++) s.v[j] = *reinterpret_cast<const typename PagedStage<D, false>::vwords*>(v + j * kRow);
     }
@@ -173,37 +182,35 @@ FV_DEV bf16x8 k_frag(const PagedStage<D, FOUR>& s, int b, int dk) {
     if constexpr (FOUR) return __builtin_bit_cast(bf16x8, fp4_eight(s.k[b][dk], e8m0_scale(s.kscale[b])));
     else return __builtin_bit_cast(bf16x8, s.k[b][dk]);
 }
-// The lane's V as bf16 words: D / 16 channels of key j.
+// Word X of the lane's V as bf16, channels 2 X and 2 X + 1 of its D / 16, of each of its 8 keys.
 template <int D, bool FOUR>
-FV_DEV void v_words(const PagedStage<D, FOUR>& s, int lane, unsigned (&w)[8][D / 32]) {
-    if constexpr (FOUR) {
-        constexpr int kS = D / 32;                            // scale bytes a key
-        const int blk = (lane & 15) * (D / 16) / 32;
+struct VScales {
+    float of[FOUR ? 8 : 1];
+    FV_DEV VScales(const PagedStage<D, FOUR>& s, int lane) {
+        if constexpr (FOUR) {
+            constexpr int kS = D / 32;                        // scale bytes a key
+            const int shift = 8 * ((lane & 15) * (D / 16) / 32);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const unsigned bytes = s.vscale[j * kS / 16][(j * kS / 4) & 3];
-            const float scale = e8m0_scale((bytes >> (8 * ((j * kS & 3) + blk))) & 255u);
-            w[j][0] = fp4_pair<0>(s.v[j], scale);
-            w[j][1] = fp4_pair<1>(s.v[j], scale);
-            if constexpr (D == 128) {
-                w[j][2] = fp4_pair<2>(s.v[j], scale);
-                w[j][3] = fp4_pair<3>(s.v[j], scale);
-            }
+            for (int j = 0; j < 8; j++) of[j] = e8m0_scale((s.vscale[j * kS / 16][(j * kS / 4) & 3] >> (shift + 8 * (j * kS & 3))) & 255u);
         }
-    } else {
+    }
+};
+template <int X, int D, bool FOUR>
+FV_DEV void v_words(const PagedStage<D, FOUR>& s, const VScales<D, FOUR>& scales, unsigned (&w)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-#pragma unroll
-            for (int x = 0; x < D / 32; x++) w[j][x] = s.v[j][x];
+    for (int j = 0; j < 8; j++) {
+        if constexpr (FOUR) w[j] = fp4_pair<X>(s.v[j], scales.of[j]);
+        else w[j] = s.v[j][X];
     }
 }
 
 // One workgroup: a share of the walk of a tile of 16 NT rows of one (sequence, key head); its four waves take the share's
-// steps in turn, each with a running maximum of its own, and join through LDS. The loads of a step go out while the one
-// before is computed.
+// steps in turn, each with a running maximum of its own, and join through LDS. One tile of rows: a whole step is loaded ahead.
+// Two: the keys of the next step go into the registers of this one's as soon as their scores are there, its values likewise
+// (a whole step ahead spilled 270 bytes a lane: 48 drafts of 5 tokens, 32 heads, a window of 2048, 136 us instead of 83).
 template <int D, bool FOUR, int NT>
 __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParams p) {
-    constexpr int kNO = D / 16, kPad = D + 4;
+    constexpr int kNO = D / 16, kPad = D + 4, kDepth = NT == 1 ? 2 : 1;
     __shared__ float lds_o[kWaves][16][kPad];
     __shared__ float lds_ml[kWaves][16][2], lds_row[16][2];   // a wave's (offset, sum) of its rows; (1 / sum, log2 of the sum) of all
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -253,10 +260,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     const int* table = p.b.table + (size_t)seq * p.b.table_stride;
     const int lg = p.pool.lg, slots = (1 << lg) - 1, columns = (p.b.max_len + slots) >> lg;
 
-    auto compute = [&](const PagedStage<D, FOUR>& s, int k0, bool good0, bool good1) {
-        const bool whole = paged_whole(all_see, k0, k0 + kStep) && good0 && good1;
-        bf16x8 pr[NT];
-        f32x4 x[NT][2];
+    // S = K Q^T of a step, relative to the rows' offsets
+    auto scores = [&](const PagedStage<D, FOUR>& s, f32x4 (&x)[NT][2]) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const float m = -off[n];
@@ -270,22 +275,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
 #pragma unroll
                 for (int n = 0; n < NT; n++) x[n][b] = mfma16(kf, qf[n][dk], x[n][b]);
             }
-        unsigned vw[8][D / 32];
-        v_words<D, FOUR>(s, lane, vw);
+    };
+    auto softmax = [&](f32x4 (&x)[NT][2], bf16x8 (&pr)[NT], int k0, unsigned good) {
         const int kl = k0 + 8 * g;
-        if (!whole) {   // keys that a row does not see, keys of pages that are none, values that no row sees (whatever they are)
-            const unsigned good = (g < 2 ? good0 : good1) ? 0xffu : 0u;
+        if (!paged_whole(all_see, k0, k0 + kStep) || good != 3) {   // keys that a row does not see, keys of pages that are none
+            const unsigned mask = (good >> (g >> 1)) & 1 ? 0xffu : 0u;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const unsigned seen = see[n].eight(kl) & good;
+                const unsigned seen = see[n].eight(kl) & mask;
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[n][j >> 2][j & 3] = (seen >> j) & 1 ? x[n][j >> 2][j & 3] : neg_inf();
             }
-            const unsigned used = w.any.eight(kl) & good;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) vw[j][i] = (used >> j) & 1 ? vw[j][i] : 0u;
         }
         bool need = false;
         float mx[NT];
@@ -326,15 +326,34 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
             }
             pr[n] = __builtin_convertvector(e, bf16x8);
         }
+    };
+    auto add_values = [&](const PagedStage<D, FOUR>& s, const bf16x8 (&pr)[NT], int k0, unsigned good) {
+        const VScales<D, FOUR> scales(s, lane);
+        const bool whole = paged_whole(all_see, k0, k0 + kStep) && good == 3;
+        // values that no row sees are zeros, whatever they are
+        const unsigned used = whole ? 0xffu : w.any.eight(k0 + 8 * g) & ((good >> (g >> 1)) & 1 ? 0xffu : 0u);
+        auto word = [&](auto x) {
+            unsigned vw[8];
+            v_words<x()>(s, scales, vw);
+            if (!whole) {
 #pragma unroll
-        for (int c = 0; c < kNO; c++) {
-            constexpr unsigned kLow = 0x05040100u, kHigh = 0x07060302u;
-            u32x4 t;
+                for (int j = 0; j < 8; j++) vw[j] = (used >> j) & 1 ? vw[j] : 0u;
+            }
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[i] = __builtin_amdgcn_perm(vw[2 * i + 1][c >> 1], vw[2 * i][c >> 1], (c & 1) ? kHigh : kLow);
-            const bf16x8 vf = __builtin_bit_cast(bf16x8, t);
+            for (int c = 0; c < 2; c++) {
+                u32x4 t;
 #pragma unroll
-            for (int n = 0; n < NT; n++) o[n][c] = mfma16(vf, pr[n], o[n][c]);
+                for (int i = 0; i < 4; i++) t[i] = __builtin_amdgcn_perm(vw[2 * i + 1], vw[2 * i], c ? 0x07060302u : 0x05040100u);
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, t);
+#pragma unroll
+                for (int n = 0; n < NT; n++) o[n][2 * x() + c] = mfma16(vf, pr[n], o[n][2 * x() + c]);
+            }
+        };
+        word(std::integral_constant<int, 0>{});
+        word(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            word(std::integral_constant<int, 2>{});
+            word(std::integral_constant<int, 3>{});
         }
     };
 
@@ -346,26 +365,53 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
         const int id0 = table[my_page];
         const int id1 = lg == 4 ? table[min(my_page + 1, columns - 1)] : id0;
         const int count = min(64, (e1 - first + kWaves - 1) / kWaves);
-        auto fetch = [&](PagedStage<D, FOUR>& s, int i, int& k0, bool& good0, bool& good1) {
+        struct Step {
+            int key;
+            unsigned row[2], good;   // of its halves of 16 keys: first row in the pool, whether the page is one of the pool's
+        };
+        auto step = [&](int i) {     // (past the group's end: its last step again)
             i = min(i, count - 1);
             const int a = __builtin_amdgcn_readlane(id0, i), b = __builtin_amdgcn_readlane(id1, i);
-            k0 = w.key(first + i * kWaves);
-            good0 = (unsigned)a < (unsigned)p.pool.pages;
-            good1 = (unsigned)b < (unsigned)p.pool.pages;
-            const size_t r0 = (((size_t)(good0 ? a : 0) * p.pool.kv_heads + kvh) << lg) + (k0 & slots);
-            const size_t r1 = lg == 4 ? ((size_t)(good1 ? b : 0) * p.pool.kv_heads + kvh) << lg : r0 + 16;
-            paged_load<D, FOUR>(s, at, r0, r1, lane);
+            Step x;
+            x.key = w.key(first + i * kWaves);
+            const bool ga = (unsigned)a < (unsigned)p.pool.pages, gb = (unsigned)b < (unsigned)p.pool.pages;
+            x.good = (ga ? 1u : 0u) | (gb ? 2u : 0u);
+            x.row[0] = (((unsigned)(ga ? a : 0) * (unsigned)p.pool.kv_heads + (unsigned)kvh) << lg) + (unsigned)(x.key & slots);
+            x.row[1] = lg == 4 ? ((unsigned)(gb ? b : 0) * (unsigned)p.pool.kv_heads + (unsigned)kvh) << lg : x.row[0] + 16;
+            return x;
         };
-        PagedStage<D, FOUR> sa, sb;
-        int ka, kb;
-        bool a0, a1, b0, b1;
-        fetch(sa, 0, ka, a0, a1);
-        for (int i = 0; i < count; i += 2) {   // (a fetch past the group's end takes its last step again)
-            fetch(sb, i + 1, kb, b0, b1);
-            compute(sa, ka, a0, a1);
-            if (i + 1 >= count) break;
-            fetch(sa, i + 2, ka, a0, a1);
-            compute(sb, kb, b0, b1);
+        PagedStage<D, FOUR> stage[kDepth];
+        Step now = step(0);
+        paged_load_k<D, FOUR>(stage[0], at, now.row[0], now.row[1], lane);
+        paged_load_v<D, FOUR>(stage[0], at, now.row[0], now.row[1], lane);
+        for (int i = 0; i < count; i += kDepth) {
+#pragma unroll
+            for (int x = 0; x < kDepth; x++) {
+                if (i + x >= count) break;
+                PagedStage<D, FOUR>&s = stage[x], &ahead = stage[kDepth - 1 - x];
+                const Step next = step(i + x + 1);
+                f32x4 sc[NT][2];
+                bf16x8 pr[NT];
+                if constexpr (kDepth > 1) {
+                    paged_load_k<D, FOUR>(ahead, at, next.row[0], next.row[1], lane);
+                    paged_load_v<D, FOUR>(ahead, at, next.row[0], next.row[1], lane);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                scores(s, sc);
+                if constexpr (kDepth == 1) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    paged_load_k<D, FOUR>(s, at, next.row[0], next.row[1], lane);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                softmax(sc, pr, now.key, now.good);
+                add_values(s, pr, now.key, now.good);
+                if constexpr (kDepth == 1) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    paged_load_v<D, FOUR>(s, at, next.row[0], next.row[1], lane);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                now = next;
+            }
         }
     }
 
@@ -444,18 +490,21 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
 //   4-bit pages: a lane has a quarter of a row in registers a phase ahead and writes it to LDS as bf16 between the matrix
 //     instructions, 4 conversions and a write at a time.
 constexpr int kBigRows = 128, kTileKeys = 64;
-template <int D, bool FOUR>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const PagedAttnParams p) {
+// FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop:
+// 8 % of one frame against 21, 9 % of three over 4 bits, 7 % of prompts under a window). Exact as long as nothing overflows or
+// vanishes, which is checked before anything is stored: the sum of every row that sees a key of the walk within 2^-60 .. 2^100 and
+// its values finite, or the workgroup makes the pass again with the running maximum (returns false).
+template <int D, bool FOUR, bool FIXED, class Params>
+FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, const int block) {
     using G = TileGeo<D>;
     constexpr int kNO = D / 16, kTile = G::kTile;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q4 = lane >> 4, i16 = lane & 15;
     // XCD x takes a contiguous eighth of the items, key head by key head, so that an L2 holds few heads' keys; the last rows,
     // whose walks are the longest, first
-    int item = (blockIdx.x & 7) * p.big_per_xcd + (blockIdx.x >> 3);
-    if (item >= p.big_total) return;
+    int item = (block & 7) * p.big_per_xcd + (block >> 3);
+    if (item >= p.big_total) return true;
     const int tile = p.big.tiles - 1 - item % p.big.tiles;
     item /= p.big.tiles;
     const int chunk = item % p.big.chunks;
@@ -463,10 +512,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
     const int seq = item % p.b.seqs, kvh = item / p.b.seqs;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group, row0 = tile * kBigRows;
-    if (row0 >= rows || rows <= p.few) return;
+    if (row0 >= rows || rows <= p.few) return true;
     const PagedWalk<kTileKeys> w = paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
     const int e0 = chunk * p.big.chunk, e1 = min(w.n, e0 + p.big.chunk);
-    if (chunk > 0 && e0 >= e1) return;
+    if (chunk > 0 && e0 >= e1) return true;
     const bool split = w.n > p.big.chunk;
     const float sl2 = p.sl2;
 
@@ -478,6 +527,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
         const int r = wrow + (lane & 31);
         mine = paged_sight(p, sq.first_pos() + min(r, rows - 1) / p.group, sq.len);
     }
+    // the walk's positions whose tiles the wave's rows see whole: [0, whole0) and [whole1, whole2)
+    auto before = [&](int t) { return min(t, w.ns) + min(max(t - w.b0, 0), w.n - w.ns); };   // positions of tiles before tile t
+    const int whole0 = before(all_see.a / kTileKeys), whole1 = all_see.a >= all_see.lo ? 0 : before((all_see.lo + kTileKeys - 1) / kTileKeys),
+              whole2 = before(all_see.hi / kTileKeys);
     bf16x8 qf[D / 32][2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
@@ -496,6 +549,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
     const int lg = p.pool.lg, slots = (1 << lg) - 1, columns = (p.b.max_len + slots) >> lg;
     // page numbers of 64 tiles of the walk, a tile a lane: that of the wave's 16 keys, and which of the tile's four 16 are in the pool
     int ids = 0, good = 0, ids_at = e0;
+    bool clean = true;   // whether all of them are
     auto look_up = [&](int e) {
         ids_at = e;
         const int k = w.key(min(e + lane, max(e1 - 1, 0)));
@@ -507,6 +561,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
             good |= ok ? 1 << x : 0;
             if (x == wave) ids = ok ? id : -1;
         }
+        clean = __builtin_amdgcn_ballot_w64(good != 15) == 0;
     };
     const TileReadBases rb = tile_read_bases<D>(lane);
     auto kbuf = [&](int m) -> lds_u8* { return smem + (m & 1) * kTile; };
@@ -526,7 +581,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
         x.count = id < 0 ? 0 : min(max(w.any.hi - x.key, 0), 16);
         return x;
     };
-    // Whether no row sees row r of a part: a key between the sink and the window. (What lies there may be anything.)
+    // Whether no row sees row r of a part: a key between the sink and the window. What lies there may be anything: scores that
+    // are not seen are replaced, but values times a probability of 0 have to be numbers.
     auto some_hidden = [&](const Part& x) { return x.key < w.any.lo && x.key + 16 > w.any.a && w.any.a < w.any.lo; };
     auto hidden = [&](const Part& x, int r) { return x.key + r >= w.any.a && x.key + r < w.any.lo; };
 
@@ -551,15 +607,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
     auto issue = [&](const void* pages, const Part& x, lds_u8* buf, const unsigned (&off)[kIter], int u) {
         const u32x4 desc = plane_descriptor((const uint8_t*)pages + (size_t)x.row * G::kRow, (unsigned)x.count * G::kRow);
         const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(buf + wave * 16 * G::kRow + u * 2048));
-        unsigned o0 = off[2 * u], o1 = off[2 * u + 1];
-        if (some_hidden(x)) {   // past the descriptor's end
-            const int r = 2 * u * G::kRowsPerDma + lane / G::kChunks;
-            o0 = hidden(x, r) ? 0x40000000u : o0;
-            o1 = hidden(x, r + G::kRowsPerDma) ? 0x40000000u : o1;
-        }
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
                      "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds"
-                     :: "s"(m0), "v"(o0), "v"(o1), "s"(desc) : "memory");
+                     :: "s"(m0), "v"(off[2 * u]), "v"(off[2 * u + 1]), "s"(desc) : "memory");
     };
     // 4 bits: the lane's quarter of K or V of a part, into registers ...
     auto fetch = [&](const void* pages, const uint8_t* scales, const Part& x, quarter& c, unsigned& sc) {
@@ -567,7 +617,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
         c = *reinterpret_cast<const quarter*>((const uint8_t*)pages + row * (D / 2) + qpart * (D / 8));
         sc = scales[row * (D / 32) + qpart * (D / 32) / 4];
     };
-    auto keep = [&](const Part& x, quarter& c, unsigned& sc) {   // what nobody sees is zeros
+    auto clear = [&](lds_u8* buf, const Part& x) {   // bf16: hidden rows of the wave's part of a V tile
+#pragma unroll
+        for (int i = 0; i < 16 * G::kRow / 1024; i++) {
+            const int r = i * G::kRowsPerDma + lane / G::kChunks;
+            if (hidden(x, r)) lds_write_b128(buf + (16 * wave + r) * G::kRow + (lane % G::kChunks << 4), u32x4{0u, 0u, 0u, 0u});
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+    };
+    auto keep = [&](const Part& x, quarter& c, unsigned& sc) {   // 4 bits: values that nobody sees
         const bool none = qrow >= x.count || hidden(x, qrow);
 #pragma unroll
         for (int j = 0; j < kQuarter; j++) c[j] = none ? 0u : c[j];
@@ -584,8 +642,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
     ProbTile pb;
 
     auto mask_tile = [&](ScoreTile& s, int e) {
+        if ((e < whole0 || (e >= whole1 && e < whole2)) && clean) return;
         const int k = w.key(e), ok = __builtin_amdgcn_readlane(good, e - ids_at);
-        if (paged_whole(all_see, k, k + kTileKeys) && ok == 15) return;
         const unsigned m[3] = {(unsigned)mine.a, (unsigned)mine.lo, (unsigned)mine.hi};
         int both[3][2];   // the even rows of 16 lanes hold block 0's, the odd ones block 1's
 #pragma unroll
@@ -613,7 +671,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
         Part cur = part_of(e0), next = part_of(e0 + 1);   // of the tile whose V is loaded next, whose K is
         if constexpr (FOUR) {
             fetch(p.pool.k, p.pool.ks, cur, kq, kqs);
-            keep(cur, kq, kqs);
 #pragma unroll
             for (int j = 0; j < kQuarter; j++) put(kbuf(0), G::kswz(qrow), kq, kqs, j);
             fetch(p.pool.v, p.pool.vs, cur, vq, vqs);
@@ -633,7 +690,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
             auto hook = [&](int i) {
                 if constexpr (FOUR) {
                     // V of this tile and K of the next, fetched a phase ago; then the fetches for the next phase
-                    if (i == 0) keep(cur, vq, vqs), keep(next, kq, kqs);
+                    if (i == 0) keep(cur, vq, vqs);
                     if (i < kQuarter) put(vbuf(m), G::vswz(qrow), vq, vqs, i);
                     else if (i < 2 * kQuarter) put(kbuf(m + 1), G::kswz(qrow), kq, kqs, i - kQuarter);
                     else if (i == 2 * kQuarter) after = part_of(e + 2), fetch(p.pool.v, p.pool.vs, next, vq, vqs);
@@ -660,13 +717,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
             __builtin_amdgcn_sched_barrier(0);
             mask_tile(s, e);
             if constexpr (first()) softmax_first_off<true>(s, st, s_init, sl2, pb);
+            else if constexpr (FIXED) softmax_off_tile<true>(s, st, sl2, pb);
             else softmax_tile_off<true>(s, st, o, s_init, sl2, pb);
             asm volatile("" ::"v"(pb[0][0]), "v"(pb[0][1]), "v"(pb[1][0]), "v"(pb[1][1]), "v"(st.l_acc[0]), "v"(st.l_acc[1]));
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (FOUR) {
+                __builtin_amdgcn_s_waitcnt(0xC07F);
+            } else {
+                wait_vmcnt<0>();
+                if (some_hidden(cur)) clear(vbuf(m), cur);
+            }
             cur = next;
             next = after;
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (FOUR) __builtin_amdgcn_s_waitcnt(0xC07F);
-            else wait_vmcnt<0>();
             block_barrier();   // K(m + 1), V(m) resident; this phase's tiles read by every wave
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -682,6 +744,32 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
         for (int db = 0; db < kNO; db++) o[db][0] = o[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    if constexpr (FIXED) {
+        // the lane's part of its rows' check; a row without a key in the walk has a sum of zero by right
+        const int from = w.key(max(e0, w.ns)), to = e1 > e0 ? w.key(e1 - 1) + kTileKeys : 0;   // of the walk past the sink
+        const bool any = e1 > e0 && wrow + (lane & 31) < rows &&
+                         ((e0 < w.ns && e0 * kTileKeys < mine.a) || (e1 > w.ns && max(mine.lo, from) < min(mine.hi, to)) || (e1 > w.ns && from < mine.a));
+        const auto sees = __builtin_amdgcn_permlane16_swap((unsigned)any, (unsigned)any, false, false);   // (exchanged as in mask_tile)
+        float chk = 0.f;
+        bool fine = true;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const float l = quad_sum(st.l_acc[g]);
+            fine = fine && (wrow + 16 * g + i16 >= rows || (l < 0x1p+100f && (l > 0x1p-60f || (l == 0.f && !sees[g]))));
+#pragma unroll
+            for (int db = 0; db < kNO; db++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) chk = __builtin_fmaf(o[db][g][i], 0.f, chk);
+        }
+        // (of rows past the last nothing is stored; their values are those of queries of zeros)
+        const bool wave_ok = wrow >= rows || __builtin_amdgcn_ballot_w64(!(fine && chk == 0.f)) == 0;
+        auto* votes = (__attribute__((address_space(3))) unsigned*)(smem + kTile);   // (K buffer 1: the last P V reads none, and a second pass writes it behind its first barrier)
+        if (lane == 0) votes[wave] = wave_ok ? 0u : 1u;
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        block_barrier();
+        const u32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(votes);
+        if (__builtin_amdgcn_readfirstlane(v[0] | v[1] | v[2] | v[3]) != 0) return false;
+    }
     const size_t all = (size_t)p.b.tokens * p.heads;
 #pragma unroll
     for (int g = 0; g < 2; g++) {
@@ -702,53 +790,103 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
             else *reinterpret_cast<f32x4*>((float*)p.out + at) = x;
         }
     }
+    return true;
+}
+// The kernel's arguments read again from their segment, of which PagedAttnParams is the whole, and the lane counted anew: the second
+// pass, which runs once in a blue moon, keeps nothing of the first in registers.
+template <int D, bool FOUR>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const PagedAttnParams p) {
+    int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = blockIdx.x;
+    if (paged_tiles_item<D, FOUR, true>(p, wave, threadIdx.x & 63, block)) return;
+    using ConstParams = const __attribute__((address_space(4))) PagedAttnParams;
+    ConstParams* again = (ConstParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(again));
+    int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(lane), "+s"(wave), "+s"(block));
+    paged_tiles_item<D, FOUR, false>(*again, wave, lane, block);
 }
 
-// The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). A workgroup takes 256 / (D / 4)
-// rows of one sequence; rows whose walk one workgroup made have their result already. ROWS: of a tile of paged_rows_kernel.
-template <int D, int ROWS>
+// The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). G groups of D / 4 threads share a
+// row's shares out, four at a time each, with a running maximum, and meet in LDS; rows whose walk one workgroup made have
+// their result already. ROWS: of a tile of paged_rows_kernel.
+template <int D, int ROWS, int G>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
-    constexpr int kPer = D / 4, kRows = 256 / kPer;
+    constexpr int kPer = D / 4, kRows = 256 / (kPer * G);
+    __shared__ float lds_top[kRows][G], lds_sum[kRows][G];
+    __shared__ f32x4 lds_acc[kRows][G][kPer];
     const int seq = blockIdx.x / p.pool.kv_heads, kvh = blockIdx.x % p.pool.kv_heads;
     const PagedSeq sq = paged_seq(p.b, seq);
-    const int rows = sq.count * p.group, r = blockIdx.y * kRows + threadIdx.x / kPer, c = (threadIdx.x % kPer) * 4;
-    if (r >= rows) return;
-    int chunks;
-    if (rows <= p.few) {
-        const int row0 = r / ROWS * ROWS;
-        chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
-        if (r >= p.rows.tiles * ROWS) return;
-    } else {
-        const int row0 = r / kBigRows * kBigRows;
-        chunks = (paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + p.big.chunk - 1) / p.big.chunk;
-        if (r >= p.big.tiles * kBigRows) return;
+    const int slot = threadIdx.x / (kPer * G), gi = threadIdx.x / kPer % G, c = threadIdx.x % kPer;
+    const int rows = sq.count * p.group, r = blockIdx.y * kRows + slot;
+    int chunks = 0;
+    if (r < rows) {
+        if (rows <= p.few) {
+            const int row0 = r / ROWS * ROWS;
+            if (r < p.rows.tiles * ROWS)
+                chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
+        } else {
+            const int row0 = r / kBigRows * kBigRows;
+            if (r < p.big.tiles * kBigRows)
+                chunks = (paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + p.big.chunk - 1) / p.big.chunk;
+        }
     }
-    if (chunks <= 1) return;
+    if (G == 1 && chunks <= 1) return;
     const int t = r / p.group;
     const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group), all = (size_t)p.b.tokens * p.heads;
-    float top = neg_inf();
-    bool nan = false;   // (a share whose sum is not a number: max drops it)
-    for (int s = 0; s < chunks; s++) {
-        const float x = p.part_lse[s * all + dst];
-        top = __builtin_fmaxf(top, x);
-        nan |= x != x;
-    }
+    float top = neg_inf(), total = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
-    if (top != neg_inf() || nan) {
-        for (int s = 0; s < chunks; s++) {
-            const float k = fast_exp2(p.part_lse[s * all + dst] - top);
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + (s * all + dst) * D + c);
-            total += k;
+    if (chunks > 1) {
+        for (int s = gi; s < chunks; s += 4 * G) {
+            float lse[4];
+            f32x4 x[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] += k * x[i];
+            for (int u = 0; u < 4; u++) {
+                const size_t at = (size_t)min(s + u * G, chunks - 1) * all + dst;
+                lse[u] = p.part_lse[at];
+                x[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * c);
+            }
+            float m = top;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (s + u * G >= chunks) lse[u] = neg_inf();
+                m = __builtin_fmaxf(m, lse[u]);
+            }
+            const float k = top == neg_inf() ? 0.f : fast_exp2(top - m);
+            total *= k;
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] *= k;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {   // (a share without a key has -inf; one whose sum is not a number makes the row that)
+                const float k = lse[u] == neg_inf() ? 0.f : fast_exp2(lse[u] - m);
+                total += k;
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[i] += lse[u] == neg_inf() ? 0.f : k * x[u][i];
+            }
+            top = m;
+        }
+    }
+    if constexpr (G > 1) {
+        if (c == 0) lds_top[slot][gi] = top, lds_sum[slot][gi] = total;
+        lds_acc[slot][gi][c] = acc;
+        __syncthreads();
+        if (chunks <= 1 || gi != 0) return;
+        float m = neg_inf();
+#pragma unroll
+        for (int x = 0; x < G; x++) m = __builtin_fmaxf(m, lds_top[slot][x]);
+        total = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < G; x++) {
+            const float k = lds_top[slot][x] == neg_inf() ? 1.f : fast_exp2(lds_top[slot][x] - m);   // (-inf: zeros, or not a number)
+            total += k * lds_sum[slot][x];
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] += k * lds_acc[slot][x][c][i];
         }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[i] *= inv;
-    if (p.out_is_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.out + dst * D + c) = __builtin_convertvector(acc, bf16x4);
-    else *reinterpret_cast<f32x4*>((float*)p.out + dst * D + c) = acc;
+    if (p.out_is_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.out + dst * D + 4 * c) = __builtin_convertvector(acc, bf16x4);
+    else *reinterpret_cast<f32x4*>((float*)p.out + dst * D + 4 * c) = acc;
 }
 
 // Steps of `step` keys that the walk of a tile of `rows` rows may have. (Host arithmetic on the call's bounds: the lengths
@@ -772,7 +910,7 @@ struct PagedCut {
     size_t chunks() const { return std::max(nt ? rows_chunks : 1, big_tiles ? big_chunks : 1); }
 };
 constexpr size_t kFewRows = 64;
-PagedCut paged_cut(size_t heads, size_t kv_heads, size_t seqs, size_t tokens, size_t max_q, size_t max_len, size_t block_tokens,
+PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t seqs, size_t tokens, size_t max_q, size_t max_len, size_t block_tokens,
                    size_t window, size_t sink) {
     PagedCut c;
     const size_t group = heads / kv_heads, rows = max_q * group, units = (size_t)fv_compute_units();
@@ -785,7 +923,7 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t seqs, size_t tokens, si
         double best = 0;
         for (size_t k = 1; k <= 32 && k <= steps; k++) {
             const size_t chunk = (steps + k - 1) / k, rounds = (base * k + 2 * units - 1) / (2 * units);
-            const double cost = (double)rounds * (double)(chunk + 4) * 2.0 + (k > 1 ? 5.0 + (double)(k * tokens * heads) * 1024.0 / 4e6 : 0.0);
+            const double cost = (double)rounds * (double)(chunk + 4) * 2.0 + (k > 1 ? 5.0 + (double)(k * tokens * heads) * 8.0 * (double)d / 4e6 : 0.0);
             if (k == 1 || cost < 0.97 * best) best = cost, c.big_chunk = chunk, c.big_chunks = (steps + chunk - 1) / chunk;
         }
     }
@@ -795,9 +933,15 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t seqs, size_t tokens, si
         c.nt = most <= 16 ? 1 : 2;
         c.rows_tiles = (most + 16 * c.nt - 1) / (16 * c.nt);
         const size_t steps = walk_bound(kStep, 16 * c.nt, group, max_len, block_tokens, window, sink);
-        const size_t base = seqs * kv_heads * c.rows_tiles, slots = 4 * units;
-        size_t chunk = std::max<size_t>(((base * steps + slots - 1) / slots + kWaves - 1) / kWaves, 1) * kWaves;
-        chunk = std::max(chunk, ((steps + 63) / 64 + kWaves - 1) / kWaves * kWaves);
+        // Shares of up to 128 steps, so that long sequences among short ones are cut (40 sessions of 15 to 100 % of 32760 tokens, 8
+        // key heads, 4 bits: whole 270 us, 256 steps 211, 128 180, 64 184), a walk of up to 192 whole (128 sessions under a
+        // window of 4096: 100 us, in two 115). Where the workgroups then hold too little to fill the memory's pipe, about 2.2 MB of
+        // steps, as many shares as do: one session of 131000 tokens over 4 bits in 32 shares 38.7 us, in 64 36.9, in 128 41.2, in
+        // 16 66; 40 heads of 13270 tokens in bf16 in 4 shares 61, in 13 68. Short walks are not worth a second launch.
+        const size_t base = seqs * kv_heads * c.rows_tiles, step_bytes = kStep * (four ? d + d / 16 : 4 * d);
+        size_t shares = steps <= 192 ? 1 : (steps + 127) / 128;
+        if (steps >= 48) shares = std::max(shares, std::min(std::min(2 * units, (size_t)2200000 / step_bytes) / base, steps / 8));
+        size_t chunk = ((steps + shares - 1) / shares + kWaves - 1) / kWaves * kWaves;
         c.rows_chunk = chunk;
         c.rows_chunks = (steps + chunk - 1) / chunk;
     }
@@ -817,8 +961,12 @@ extern "C" {
 size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q, size_t max_len,
                                           size_t block_tokens, size_t window, size_t sink) {
     if (kv_heads == 0 || heads < kv_heads || heads % kv_heads != 0 || block_tokens == 0 || seqs == 0 || tokens == 0 || max_q == 0) return 0;
-    const fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
-    return fv::part_bytes(c.chunks(), tokens, heads, d);
+    size_t most = 0;   // of both kinds of pages
+    for (const bool four : {false, true}) {
+        const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
+        most = std::max(most, fv::part_bytes(c.chunks(), tokens, heads, d));
+    }
+    return most;
 }
 
 int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is_bf16, size_t heads, const void* k_pages,
@@ -842,7 +990,8 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
         return fv_decline("paged attention: mask too large");
     if (max_q > tokens) max_q = tokens;
     if (seqs == 0 || tokens == 0 || max_q == 0) return FV_OK;
-    fv::PagedCut c = fv::paged_cut(heads, kv_heads, seqs, tokens, max_q, max_len, block_tokens, window, sink);
+    const bool four = k_scales != nullptr;
+    fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, max_q, max_len, block_tokens, window, sink);
     const size_t need = fv::part_bytes(c.chunks(), tokens, heads, d);
     if (need > 0 && (!workspace || workspace_bytes < need)) {   // a share is the whole walk
         c.rows_chunk *= c.rows_chunks, c.big_chunk *= c.big_chunks;
@@ -850,7 +999,8 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     }
     const bool split = c.chunks() > 1;
     if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
-    const dim3 join((unsigned)(seqs * kv_heads), (unsigned)((max_q * (heads / kv_heads) * (d / 4) + 255) / 256));
+    const bool many = (c.big_tiles ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
+    const dim3 join((unsigned)(seqs * kv_heads), (unsigned)((max_q * (heads / kv_heads) * (d / 4) * (many ? 8 : 1) + 255) / 256));
     const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_blocks = seqs * kv_heads * c.big_tiles * c.big_chunks;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     if (row_blocks >= kMost || big_blocks + 8 >= kMost || seqs * kv_heads * join.y >= kMost)
@@ -865,7 +1015,6 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     p.big_total = (int)big_blocks, p.big_per_xcd = (int)((big_blocks + 7) / 8);
     p.part_o = (float*)workspace;
     p.part_lse = split ? p.part_o + c.chunks() * tokens * heads * d : nullptr;
-    const bool four = k_scales != nullptr;
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(d == 128, [&](auto d128) {
         fv::paged_pick(four, [&](auto f) {
@@ -874,8 +1023,12 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
                 hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3(8 * p.big_per_xcd), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
             if (c.nt == 1) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 1>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
-            if (split && c.nt == 1) hipLaunchKernelGGL((fv::paged_join_kernel<D, 16>), join, dim3(256), 0, st, p);
-            if (split && c.nt != 1) hipLaunchKernelGGL((fv::paged_join_kernel<D, 32>), join, dim3(256), 0, st, p);
+            if (split)
+                fv::paged_pick(c.nt == 1, [&](auto one) {
+                    fv::paged_pick(many, [&](auto m) {
+                        hipLaunchKernelGGL((fv::paged_join_kernel<D, one() ? 16 : 32, m() ? 8 : 1>), join, dim3(256), 0, st, p);
+                    });
+                });
         });
     });
     const hipError_t e = hipGetLastError();

@@ -328,3 +328,33 @@ def test_many_rows_over_long_walks(fv, four, d, page):
         for out16 in (True, False):
             got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=out16)
             w.check(q, got, f"long {lens} {mask} four={four} d={d} out16={out16}", *mask)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("rows", ["tokens", "prompt"])
+def test_scores_of_any_size(fv, four, rows):
+    """Rows whose scores grow by hundreds after their first keys, whose first keys are hidden while all that they see is far below
+    zero, and whose scores are all alike: no overflow, nothing vanishes."""
+    announce(f"paged: scores of any size four={four} {rows}")
+    d, kvh, heads, n = 128, 1, 4, 700
+    for mask in ((1, 0, 0), (1, 90, 0), (1, 90, 3)):
+        for grow in ("up", "down", "low", "flat"):
+            counts = [1, 1] if rows == "tokens" else [300, 64]
+            lens = [n, 130]
+            w = World(fv, 71, lens, counts, kvh, d, 16, four)
+            # keys along one direction: score = size(j) * |q| / sqrt(d)
+            for s, length in enumerate(lens):
+                j = np.arange(length)
+                size = {"up": j / 8, "down": (length - j) / 8, "low": np.full(length, -40.0) + 0.5 * np.sin(j), "flat": np.full(length, 20.0)}[grow]
+                k = np.zeros((length, kvh, d), dtype=np.float32)
+                k[:, 0, :32] = size[:, None]
+                p, t = w.table[s, j // 16], j % 16
+                if four:
+                    w.host["k"][p, :, t], w.scales["k"][p, :, t] = pu.quantize4(k)
+                else:
+                    w.host["k"][p, :, t] = pu.bf16(k)
+            w.push()
+            q = np.zeros((w.rows(), heads, d), dtype=np.float32)
+            q[:, :, :32] = np.array([1.0, 2.0, 0.25, 4.0], dtype=np.float32)[None, :, None]
+            got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False)
+            w.check(q, got, f"scores {rows} {mask} {grow} four={four}", *mask)
