@@ -61,6 +61,11 @@ FV_DEV u32x4 fp4_eight(unsigned w, float scale) {
     return u32x4{fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale)};
 }
 
+// NaN where one of the two bf16 of a word is not finite, else `x`: for testing many.
+FV_DEV float not_finite(unsigned w, float x) {
+    return __builtin_fmaf(__builtin_bit_cast(float, w & 0xffff0000u), 0.f, __builtin_fmaf(__builtin_bit_cast(float, w << 16), 0.f, x));
+}
+
 // f(std::true_type) or f(std::false_type): host values as template arguments.
 template <class F>
 inline void paged_pick(bool v, F&& f) {

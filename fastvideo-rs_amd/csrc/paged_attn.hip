@@ -204,6 +204,25 @@ FV_DEV void v_words(const PagedStage<D, FOUR>& s, const VScales<D, FOUR>& scales
     }
 }
 
+// N channels from `c` of row `row` of the values as they stand in the pool.
+template <int D, bool FOUR, int N, class Pool>
+FV_DEV void pool_values(const Pool& pool, unsigned row, int c, float (&v)[N]) {
+    if constexpr (FOUR) {
+        const uint8_t* at = (const uint8_t*)pool.v + (size_t)row * (D / 2) + c / 2;
+        const float scale = e8m0_scale(pool.vs[(size_t)row * (D / 32) + c / 32]);   // (N channels lie in one block)
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const unsigned w = fp4_pair<0>(at[i / 2], scale);
+            v[i] = __builtin_bit_cast(float, w << 16);
+            v[i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
+        }
+    } else {
+        const uint16_t* at = (const uint16_t*)pool.v + (size_t)row * D + c;
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = bf16_bits_to_f32(at[i]);
+    }
+}
+
 // One workgroup: a share of the walk of a tile of 16 NT rows of one (sequence, key head); its four waves take the share's
 // steps in turn, each with a running maximum of its own, and join through LDS. One tile of rows: a whole step is loaded ahead.
 // Two: the keys of the next step go into the registers of this one's as soon as their scores are there, its values likewise
@@ -327,11 +346,58 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
             pr[n] = __builtin_convertvector(e, bf16x8);
         }
     };
-    auto add_values = [&](const PagedStage<D, FOUR>& s, const bf16x8 (&pr)[NT], int k0, unsigned good) {
+    auto add_values = [&](const PagedStage<D, FOUR>& s, const bf16x8 (&pr)[NT], int k0, unsigned good, unsigned row_a, unsigned row_b) {
         const VScales<D, FOUR> scales(s, lane);
         const bool whole = paged_whole(all_see, k0, k0 + kStep) && good == 3;
         // values that no row sees are zeros, whatever they are
-        const unsigned used = whole ? 0xffu : w.any.eight(k0 + 8 * g) & ((good >> (g >> 1)) & 1 ? 0xffu : 0u);
+        unsigned used = whole ? 0xffu : w.any.eight(k0 + 8 * g) & ((good >> (g >> 1)) & 1 ? 0xffu : 0u);
+        if (!whole && t0 != t1) {
+            // A value that is not finite belongs to the rows that see it: a probability of zero does not keep it from the others.
+            // Its key leaves the product, and the rows that have a share in it add theirs one by one. (Rare.)
+            float bad[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            auto look = [&](auto x) {
+                unsigned vw[8];
+                v_words<x()>(s, scales, vw);
+#pragma unroll
+                for (int j = 0; j < 8; j++) bad[j] = not_finite(vw[j], bad[j]);
+            };
+            look(std::integral_constant<int, 0>{});
+            look(std::integral_constant<int, 1>{});
+            if constexpr (D == 128) {
+                look(std::integral_constant<int, 2>{});
+                look(std::integral_constant<int, 3>{});
+            }
+            unsigned out_of_it = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) out_of_it |= bad[j] != 0.f ? 1u << j : 0u;
+            out_of_it &= used;
+            if (__builtin_amdgcn_ballot_w64(out_of_it != 0) != 0) {
+#pragma unroll 1
+                for (int x = 0; x < 32; x++) {   // key x of the step: bit x % 8 of lanes 16 (x / 8) ..
+                    const int j = x & 7, h = x >> 3;
+                    if (((__builtin_amdgcn_ballot_w64((out_of_it >> j) & 1) >> (16 * h)) & 0xffff) == 0) continue;
+                    if (g == h) out_of_it |= 1u << j;   // (of all lanes that hold the key)
+                    const unsigned row = (h < 2 ? row_a : row_b) + 8 * (h & 1) + j;
+                    float pj[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const u32x4 all = __builtin_bit_cast(u32x4, pr[n]);
+                        const unsigned pair = j < 4 ? (j < 2 ? all[0] : all[1]) : (j < 6 ? all[2] : all[3]);
+                        pj[n] = __shfl(__builtin_bit_cast(float, j & 1 ? pair & 0xffff0000u : pair << 16), 16 * h + col, 64);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float v[kNO];
+                        pool_values<D, FOUR>(p.pool, row, (D / 4) * g + kNO * i, v);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int c = 0; c < kNO; c++) o[n][c][i] += pj[n] == 0.f ? 0.f : pj[n] * v[c];
+                    }
+                }
+            }
+            used &= ~out_of_it;
+        }
         auto word = [&](auto x) {
             unsigned vw[8];
             v_words<x()>(s, scales, vw);
@@ -404,7 +470,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 softmax(sc, pr, now.key, now.good);
-                add_values(s, pr, now.key, now.good);
+                add_values(s, pr, now.key, now.good, now.row[0], now.row[1]);
                 if constexpr (kDepth == 1) {
                     __builtin_amdgcn_sched_barrier(0);
                     paged_load_v<D, FOUR>(s, at, next.row[0], next.row[1], lane);
@@ -493,7 +559,8 @@ constexpr int kBigRows = 128, kTileKeys = 64;
 // FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop:
 // 8 % of one frame against 21, 9 % of three over 4 bits, 7 % of prompts under a window). Exact as long as nothing overflows or
 // vanishes, which is checked before anything is stored: the sum of every row that sees a key of the walk within 2^-60 .. 2^100 and
-// its values finite, or the workgroup makes the pass again with the running maximum (returns false).
+// its values finite, or the workgroup makes the pass again with the running maximum and an eye on values that are not finite
+// (returns false).
 template <int D, bool FOUR, bool FIXED, class Params>
 FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, const int block) {
     using G = TileGeo<D>;
@@ -641,6 +708,60 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     st.init();
     ProbTile pb;
 
+    // The second pass, a tile that some of the workgroup's rows see a part of: a value that is not finite belongs to the rows that see
+    // it, and a probability of zero does not keep it from the others. Such keys leave the V tile, and the rows that have a share
+    // in one add theirs from the pool. (The first pass ends in the check where there is such a value.)
+    const PagedSight wg_see = paged_all(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
+    auto set_apart = [&](int m, int k, const ProbTile& pb, f32x4 (&o)[kNO][2]) {
+        lds_u8* mine_v = vbuf(m) + 16 * wave * G::kRow;
+        unsigned bad_rows = 0;   // of the wave's 16
+#pragma unroll
+        for (int i = 0; i < 16 * G::kRow / 1024; i++) {
+            lds_u8* at = mine_v + i * 1024 + lane * 16;
+            const u32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(at);
+            float bad = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) bad = not_finite(v[x], bad);
+            const unsigned long long lanes = __builtin_amdgcn_ballot_w64(bad != 0.f);
+#pragma unroll
+            for (int r = 0; r < G::kRowsPerDma; r++)
+                if ((lanes >> (r * G::kChunks)) & ((1ull << G::kChunks) - 1)) bad_rows |= 1u << (i * G::kRowsPerDma + r);
+            if ((bad_rows >> (i * G::kRowsPerDma + lane / G::kChunks)) & 1) lds_write_b128(at, u32x4{0u, 0u, 0u, 0u});
+        }
+        auto* said = (__attribute__((address_space(3))) unsigned*)kbuf(m);   // (read by every wave, not yet loaded anew)
+        if (lane == 0) said[wave] = bad_rows;
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        block_barrier();
+        const u32x4 of = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(said);
+        unsigned long long keys = 0;
+#pragma unroll
+        for (int x = 0; x < 4; x++) keys |= (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane(of[x]) << (16 * x);
+#pragma unroll 1
+        for (; keys != 0; keys &= keys - 1) {
+            const int x = __builtin_ctzll(keys), key = k + x;
+            const int id = table[min(key >> lg, columns - 1)];
+            const unsigned row = (((unsigned)max(id, 0) * (unsigned)p.pool.kv_heads + (unsigned)kvh) << lg) + (unsigned)(key & slots);
+            float pj[2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) {   // key x: the (x & 3)-th of its four of block (x >> 4) & 1 in lanes 16 ((x >> 2) & 3) ..
+                const u32x4 lo = __builtin_bit_cast(u32x4, pb[0][g]), hi = __builtin_bit_cast(u32x4, pb[1][g]);
+                const u32x4 half = x < 32 ? lo : hi;
+                const unsigned pair = (x & 16) ? ((x & 2) ? half[3] : half[2]) : ((x & 2) ? half[1] : half[0]);
+                pj[g] = __shfl(__builtin_bit_cast(float, x & 1 ? pair & 0xffff0000u : pair << 16), 16 * ((x >> 2) & 3) + i16, 64);
+            }
+#pragma unroll
+            for (int db = 0; db < kNO; db++) {
+                float v[4];
+                pool_values<D, FOUR>(p.pool, row, 16 * db + 4 * q4, v);
+#pragma unroll
+                for (int g = 0; g < 2; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[db][g][i] += pj[g] == 0.f ? 0.f : pj[g] * v[i];
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0), lgkmcnt(0)
+        block_barrier();
+    };
     auto mask_tile = [&](ScoreTile& s, int e) {
         if ((e < whole0 || (e >= whole1 && e < whole2)) && clean) return;
         const int k = w.key(e), ok = __builtin_amdgcn_readlane(good, e - ids_at);
@@ -731,6 +852,10 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
             next = after;
             block_barrier();   // K(m + 1), V(m) resident; this phase's tiles read by every wave
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!FIXED) {
+                const int k = w.key(e);
+                if (!paged_whole(wg_see, k, k + kTileKeys)) set_apart(m, k, pb, o);
+            }
         };
         phase(0, std::true_type{});
 #pragma unroll 1
@@ -974,6 +1099,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
                        size_t d, const int32_t* q_start, const int32_t* lens, const int32_t* table, size_t table_stride, size_t table_pages,
                        size_t seqs, size_t tokens, size_t max_q, size_t max_len, float scale, size_t block_tokens, size_t window,
                        size_t sink, void* workspace, size_t workspace_bytes, void* stream) {
+    if (seqs == 0 || tokens == 0 || max_q == 0) return FV_OK;   // (empty arrays may have no address)
     fv::PagedAttnParams p;
     const int rc = fv_paged_args("paged attention", k_pages, v_pages, k_scales, v_scales, pages, page_tokens, kv_heads, d, q_start, lens,
                                  table, table_stride, table_pages, seqs, tokens, &max_len, &p.pool, &p.b);
@@ -989,7 +1115,6 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     if (block_tokens > (size_t)INT_MAX / 2 || window > (size_t)INT_MAX / 2 || sink > (size_t)INT_MAX / 2)
         return fv_decline("paged attention: mask too large");
     if (max_q > tokens) max_q = tokens;
-    if (seqs == 0 || tokens == 0 || max_q == 0) return FV_OK;
     const bool four = k_scales != nullptr;
     fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, max_q, max_len, block_tokens, window, sink);
     const size_t need = fv::part_bytes(c.chunks(), tokens, heads, d);

@@ -147,6 +147,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p)
     for (int i = 0; i < TOKENS; i++) {
         const int t = blockIdx.x * TOKENS + i;
         if (t >= p.b.tokens || t >= p.b.q_start[p.b.seqs]) return;
+        if (t < p.b.q_start[0]) continue;
         const PagedPlace at = paged_place(p.b, p.pool, t);
         const int row = p.rope_at ? p.rope_at[t] : at.pos;
         const bool turn = p.cos_t != nullptr;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const PagedPool pool, c
     const int piece = blockIdx.y * 256 + threadIdx.x, t = blockIdx.x;
     const int head = piece / kPer, c = piece % kPer, kvh = pool.kv_heads;
     if (head >= 2 * kvh) return;
-    if (t >= b.q_start[b.seqs]) return;   // behind the last sequence: left as it was
+    if (t < b.q_start[0] || t >= b.q_start[b.seqs]) return;   // of no sequence: left as it was
     const PagedPlace at = paged_place(b, pool, t);
     const bool is_v = head >= kvh;
     const int h = is_v ? head - kvh : head;
@@ -268,6 +269,7 @@ int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stri
                     int halves, void* k_pages, void* v_pages, void* k_scales, void* v_scales, size_t pages, size_t page_tokens,
                     size_t kv_heads, size_t d, const int32_t* q_start, const int32_t* lens, const int32_t* table, size_t table_stride,
                     size_t table_pages, size_t seqs, size_t tokens, void* stream) {
+    if (seqs == 0 || tokens == 0) return FV_OK;   // (empty arrays may have no address)
     fv::AppendParams p;
     const int rc = fv_paged_args("paged append", k_pages, v_pages, k_scales, v_scales, pages, page_tokens, kv_heads, d, q_start, lens, table,
                                  table_stride, table_pages, seqs, tokens, nullptr, &p.pool, &p.b);
@@ -285,7 +287,6 @@ int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stri
     if (!fv::aligned16(k) || !fv::aligned16(v) || !fv::aligned16(q) || !fv::aligned16(q_out) || !fv::aligned16(cos_t) || !fv::aligned16(sin_t))
         return fv_invalid("paged append: operands must be 16-byte aligned");
     if (rope_rows > (size_t)INT_MAX) return fv_decline("paged append: rope tables too long");
-    if (seqs == 0 || tokens == 0) return FV_OK;
     p.k = k, p.v = v, p.q = q, p.q_out = q_out;
     p.k_stride = (long)k_stride, p.v_stride = (long)v_stride, p.q_stride = (long)q_stride;
     p.cos_t = cos_t, p.sin_t = sin_t, p.rope_at = rope_at, p.rope_rows = (int)rope_rows, p.heads = (int)heads;
@@ -311,6 +312,7 @@ int fv_paged_read(void* k_out, void* v_out, int out_is_bf16, const void* k_pages
                   const void* v_scales, size_t pages, size_t page_tokens, size_t kv_heads, size_t d, const int32_t* q_start,
                   const int32_t* lens, const int32_t* table, size_t table_stride, size_t table_pages, size_t seqs, size_t tokens,
                   void* stream) {
+    if (seqs == 0 || tokens == 0) return FV_OK;
     fv::PagedPool pool;
     fv::PagedBatch b;
     const int rc = fv_paged_args("paged read", k_pages, v_pages, k_scales, v_scales, pages, page_tokens, kv_heads, d, q_start, lens, table,
@@ -318,7 +320,6 @@ int fv_paged_read(void* k_out, void* v_out, int out_is_bf16, const void* k_pages
     if (rc != FV_OK) return rc;
     if (!k_out || !v_out) return fv_invalid("paged read: null operand");
     if (!fv::aligned16(k_out) || !fv::aligned16(v_out)) return fv_invalid("paged read: operands must be 16-byte aligned");
-    if (seqs == 0 || tokens == 0) return FV_OK;
     const dim3 grid((unsigned)tokens, (unsigned)((2 * kv_heads * (d / 8) + 255) / 256));
     if ((size_t)grid.x * grid.y >= (size_t)1 << 24) return fv_decline("paged read: too large for one launch");
     const bool four = k_scales != nullptr;

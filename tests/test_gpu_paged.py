@@ -358,3 +358,50 @@ def test_scores_of_any_size(fv, four, rows):
             q[:, :, :32] = np.array([1.0, 2.0, 0.25, 4.0], dtype=np.float32)[None, :, None]
             got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False)
             w.check(q, got, f"scores {rows} {mask} {grow} four={four}", *mask)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 64)])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(fv, four, d, page):
+    """NaN and infinities in keys and values at positions that some rows of a tile see and their neighbours do not."""
+    announce(f"paged: NaN and infinities four={four} d={d}")
+    for lens, counts, mask in (([70, 9], [5, 3], (1, 0, 0)), ([200, 150], [200, 90], (1, 0, 0)), ([300, 260], [120, 260], (1, 40, 3)),
+                               ([40, 40], [12, 6], (1, 9, 2)), ([240, 96], [240, 48], (48, 1, 0))):
+        kvh, heads = 2, 6
+        for what in ("v", "k", "both"):
+            w = World(fv, 81 + d, lens, counts, kvh, d, page, four)
+            for s, n in enumerate(lens):
+                for j in (n - counts[s] // 2, n - 3, n - counts[s] - 1 if counts[s] < n else n // 3, 1):
+                    p, t = w.table[s, j // page], j % page
+                    for name in ("kv" if what == "both" else what):
+                        if four:
+                            w.scales[name][p, 1, t, -1] = 255          # one head, its last 32 channels
+                        else:
+                            w.host[name][p, 1, t, 5] = np.nan if j % 2 or name == "k" else np.inf
+            w.push()
+            q = w.queries(heads)
+            got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False)
+            got = got.cpu().numpy()
+            for s, n in enumerate(counts):
+                part = slice(w.starts[s], w.starts[s] + n)
+                k, v = w.held("k", s), w.held("v", s)
+                seen = pu.sees(np.arange(n) + w.lens[s] - n, np.arange(w.lens[s]), *mask)
+                for h in range(heads):
+                    kk, vv = k[:, h // 3], v[:, h // 3]
+                    bad_k = ~np.isfinite(kk).all(1)
+                    bad_row = (seen & bad_k[None, :]).any(1)
+                    bad = bad_row[:, None] | ((seen[:, :, None] & ~np.isfinite(vv)[None, :, :]).any(1))
+                    x = got[part, h]
+                    assert (np.isfinite(x) == ~bad).all(), f"{lens} {mask} {what}: sequence {s} head {h}: {int((np.isfinite(x) != ~bad).sum())} values"
+                fine = [w.held(name, s) for name in "kv"]
+                clean = [np.nan_to_num(x, nan=0.0, posinf=0.0) for x in fine]
+                out, mag = pu.attention(q[part], *clean, w.lens[s] - n, d ** -0.5, *mask)
+                x = got[part]
+                ok = np.isfinite(x)
+                # rows that see nothing of the kind are as always (a row whose sum holds no such key, in every channel)
+                whole = ok.all(-1)
+                for h in range(heads):
+                    some = (seen & (~np.isfinite(fine[0][:, h // 3]).all(1) | ~np.isfinite(fine[1][:, h // 3]).all(1))[None, :]).any(1)
+                    whole[some, h] = False
+                off = np.abs(x - out)[whole] - pu.attention_bound(out, mag, False, 60.0)[whole]
+                assert off.size == 0 or off.max() <= 0
