@@ -37,9 +37,13 @@ struct PagedAttnParams {
         int tiles;              // row tiles of a (sequence, key head)
         int chunk, chunks;      // steps of the walk that a workgroup takes, workgroups a walk
     } rows, big;
-    int big_total, big_per_xcd; // workgroups of paged_tiles_kernel, an eighth of them
-    float* part_o;              // [chunks][tokens * heads][d], each normalised, and the base-2 logarithm of its sum
-    float* part_lse;            // [chunks][tokens * heads]
+    // paged_tiles_kernel: the first big_full tiles (a multiple of 8), counted key head by key head, have a workgroup each, the
+    // others big.chunks; big_rest: those others' workgroups, big_per_xcd an eighth of them
+    int big_full, big_rest, big_per_xcd;
+    // Shares: values, each normalised, and the base-2 logarithm of its sum. Of paged_rows_kernel [chunks][tokens * heads][d] and
+    // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
+    float *rows_o, *rows_lse, *big_o, *big_lse;
+    long big_rows;              // the latter's rows
 };
 
 // The keys that a row at position p of a sequence of `len` tokens sees: [0, a) and [lo, hi), a <= hi.
@@ -526,10 +530,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
                 }
                 if (split) {
                     const size_t all = (size_t)p.b.tokens * p.heads;
-                    float* po = p.part_o + ((size_t)chunk * all + dst) * D + cc;
+                    float* po = p.rows_o + ((size_t)chunk * all + dst) * D + cc;
 #pragma unroll
                     for (int c = 0; c < kPer; c += 4) *reinterpret_cast<f32x4*>(po + c) = f32x4{val[c], val[c + 1], val[c + 2], val[c + 3]};
-                    if (cc == 0) p.part_lse[(size_t)chunk * all + dst] = lds_row[rr][1];
+                    if (cc == 0) p.rows_lse[(size_t)chunk * all + dst] = lds_row[rr][1];
                 } else if (p.out_is_bf16) {
                     __attribute__((ext_vector_type(kPer))) float f;
 #pragma unroll
@@ -570,20 +574,25 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     const int q4 = lane >> 4, i16 = lane & 15;
     // XCD x takes a contiguous eighth of the items, key head by key head, so that an L2 holds few heads' keys; the last rows,
     // whose walks are the longest, first
-    int item = (block & 7) * p.big_per_xcd + (block >> 3);
-    if (item >= p.big_total) return true;
+    const bool full = block < p.big_full;
+    const int at = full ? block : block - p.big_full;
+    int item = (at & 7) * (full ? p.big_full >> 3 : p.big_per_xcd) + (at >> 3), chunk = 0;
+    if (!full) {
+        if (item >= p.big_rest) return true;
+        chunk = item % p.big.chunks;
+        item = p.big_full + item / p.big.chunks;
+    }
+    const int cut_tile = item - p.big_full;   // (where it is cut)
     const int tile = p.big.tiles - 1 - item % p.big.tiles;
     item /= p.big.tiles;
-    const int chunk = item % p.big.chunks;
-    item /= p.big.chunks;
     const int seq = item % p.b.seqs, kvh = item / p.b.seqs;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group, row0 = tile * kBigRows;
     if (row0 >= rows || rows <= p.few) return true;
     const PagedWalk<kTileKeys> w = paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
-    const int e0 = chunk * p.big.chunk, e1 = min(w.n, e0 + p.big.chunk);
+    const int e0 = chunk * p.big.chunk, e1 = full ? w.n : min(w.n, e0 + p.big.chunk);
     if (chunk > 0 && e0 >= e1) return true;
-    const bool split = w.n > p.big.chunk;
+    const bool split = !full && w.n > p.big.chunk;
     const float sl2 = p.sl2;
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
@@ -895,7 +904,7 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         const u32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(votes);
         if (__builtin_amdgcn_readfirstlane(v[0] | v[1] | v[2] | v[3]) != 0) return false;
     }
-    const size_t all = (size_t)p.b.tokens * p.heads;
+    const size_t shares = (size_t)chunk * p.big_rows + (size_t)cut_tile * kBigRows;
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         const float l = quad_sum(st.l_acc[g]);
@@ -903,14 +912,15 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         const int r = wrow + 16 * g + i16, t = r / p.group;
         if (r >= rows) continue;
         const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
-        if (split && q4 == 0) p.part_lse[(size_t)chunk * all + dst] = l == 0.f ? neg_inf() : st.log2_offset<true>(g, sl2) + __log2f(l);
+        const size_t share = shares + (r - row0);
+        if (split && q4 == 0) p.big_lse[share] = l == 0.f ? neg_inf() : st.log2_offset<true>(g, sl2) + __log2f(l);
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
             f32x4 x;
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = o[db][g][i] * inv;
             const size_t at = dst * D + 16 * db + 4 * q4;
-            if (split) *reinterpret_cast<f32x4*>(p.part_o + (size_t)chunk * all * D + at) = x;
+            if (split) *reinterpret_cast<f32x4*>(p.big_o + share * D + 16 * db + 4 * q4) = x;
             else if (p.out_is_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.out + at) = __builtin_convertvector(x, bf16x4);
             else *reinterpret_cast<f32x4*>((float*)p.out + at) = x;
         }
@@ -943,21 +953,28 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     const PagedSeq sq = paged_seq(p.b, seq);
     const int slot = threadIdx.x / (kPer * G), gi = threadIdx.x / kPer % G, c = threadIdx.x % kPer;
     const int rows = sq.count * p.group, r = blockIdx.y * kRows + slot;
+    const int t = r / p.group;
+    const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
     int chunks = 0;
+    const bool few = rows <= p.few;
+    size_t first = dst, step = (size_t)p.b.tokens * p.heads;   // the row's place in the first share, rows to the next
     if (r < rows) {
-        if (rows <= p.few) {
+        if (few) {
             const int row0 = r / ROWS * ROWS;
             if (r < p.rows.tiles * ROWS)
                 chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
         } else {
             const int row0 = r / kBigRows * kBigRows;
-            if (r < p.big.tiles * kBigRows)
+            const int tile = r / kBigRows, item = (kvh * p.b.seqs + seq) * p.big.tiles + p.big.tiles - 1 - tile;   // (as paged_tiles_item counts)
+            if (tile < p.big.tiles && item >= p.big_full)
                 chunks = (paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + p.big.chunk - 1) / p.big.chunk;
+            first = (size_t)(item - p.big_full) * kBigRows + (r - row0);
+            step = (size_t)p.big_rows;
         }
     }
     if (G == 1 && chunks <= 1) return;
-    const int t = r / p.group;
-    const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group), all = (size_t)p.b.tokens * p.heads;
+    const float* part_o = few ? p.rows_o : p.big_o;
+    const float* part_lse = few ? p.rows_lse : p.big_lse;
     float top = neg_inf(), total = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (chunks > 1) {
@@ -966,9 +983,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
             f32x4 x[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const size_t at = (size_t)min(s + u * G, chunks - 1) * all + dst;
-                lse[u] = p.part_lse[at];
-                x[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * c);
+                const size_t at = (size_t)min(s + u * G, chunks - 1) * step + first;
+                lse[u] = part_lse[at];
+                x[u] = *reinterpret_cast<const f32x4*>(part_o + at * D + 4 * c);
             }
             float m = top;
 #pragma unroll
@@ -1031,7 +1048,7 @@ struct PagedCut {
     size_t few = 0;                         // rows a key head up to which a sequence is paged_rows_kernel's
     size_t nt = 0;                          // its tiles of 16 rows; 0: not launched
     size_t rows_tiles = 1, rows_chunk = 1, rows_chunks = 1;
-    size_t big_tiles = 0, big_chunk = 1, big_chunks = 1;   // of paged_tiles_kernel; no tiles: not launched
+    size_t big_tiles = 0, big_full = 0, big_chunk = 1, big_chunks = 1;   // of paged_tiles_kernel; no tiles: not launched
     size_t chunks() const { return std::max(nt ? rows_chunks : 1, big_tiles ? big_chunks : 1); }
 };
 constexpr size_t kFewRows = 64;
@@ -1042,17 +1059,32 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
     if (rows > kFewRows) {
         c.big_tiles = (rows + kBigRows - 1) / kBigRows;
         const size_t steps = walk_bound(kTileKeys, kBigRows, group, max_len, block_tokens, window, sink);
-        // tiles that hold rows: those of the longest sequence alone where one has them all
-        const size_t base = kv_heads * std::min(seqs * c.big_tiles, tokens * group / kBigRows + seqs);
-        // shares of the walk: rounds of two workgroups a unit, a fixed part of 4 steps each, against what joining moves
+        // Shares of the walk: rounds of as many workgroups as there is room for, 4 steps' time besides their own each, against a
+        // launch and the bytes that joining moves. Where the last round is far from full, the tiles of the rounds before keep
+        // their walk whole and only the rest are cut. (Tiles whose walks differ, causal or of ragged prompts, fill the
+        // rounds by themselves: no count of rounds, and all or none are cut.)
+        const size_t items = seqs * kv_heads * c.big_tiles, held = kv_heads * std::min(seqs * c.big_tiles, tokens * group / kBigRows + seqs);
+        const size_t slots = (d == 64 ? 3 : 2) * units / 8 * 8;
+        const bool varied = 10 * held < 9 * items || (window == 0 && 4 * block_tokens < max_q && 2 * max_q > max_len);
+        const double step = d == 64 ? 1.3 : 2.0;   // us
         double best = 0;
-        for (size_t k = 1; k <= 32 && k <= steps; k++) {
-            const size_t chunk = (steps + k - 1) / k, rounds = (base * k + 2 * units - 1) / (2 * units);
-            const double cost = (double)rounds * (double)(chunk + 4) * 2.0 + (k > 1 ? 5.0 + (double)(k * tokens * heads) * 8.0 * (double)d / 4e6 : 0.0);
-            if (k == 1 || cost < 0.97 * best) best = cost, c.big_chunk = chunk, c.big_chunks = (steps + chunk - 1) / chunk;
+        const size_t rounds_before = varied ? 0 : held / slots;
+        for (size_t keep = 0; keep <= std::min<size_t>(rounds_before, 2); keep++) {
+            const size_t full = keep == 0 ? 0 : (rounds_before - (keep - 1)) * slots, rest = held - full;
+            if (rest == 0) continue;
+            for (size_t k = 1; k <= 32 && k <= steps; k++) {
+                const size_t chunk = (steps + k - 1) / k, wgs = rest * k;
+                const double rounds = varied ? std::max(1.0, (double)wgs / (double)slots) + 0.5 : (double)((wgs + slots - 1) / slots);
+                const double cost = (double)(full / slots) * (double)(steps + 4) * step + rounds * ((varied ? 0.6 : 1.0) * (double)chunk + 4.0) * step +
+                                    (k > 1 ? 5.0 + (double)(k * rest * kBigRows) * 8.0 * (double)d / 4e6 : 0.0);
+                if ((keep == 0 && k == 1) || cost < 0.97 * best) best = cost, c.big_full = full, c.big_chunk = chunk, c.big_chunks = (steps + chunk - 1) / chunk;
+            }
         }
+        if (c.big_chunks == 1) c.big_full = 0;
     }
-    if (rows <= kFewRows || seqs > 1) {   // (the one sequence of a long call is the tiles' whatever its rows)
+    // (Sequences of few rows beside longer ones: a launch of their own where they may be many, by the mean; else they are the tiles', which
+    // take any, and the launch, 5 us, is saved.)
+    if (rows <= kFewRows || 2 * tokens < seqs * max_q) {
         const size_t most = std::min(rows, kFewRows);
         c.few = rows <= kFewRows ? rows : kFewRows;
         c.nt = most <= 16 ? 1 : 2;
@@ -1072,11 +1104,22 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
     }
     return c;
 }
-size_t part_bytes(size_t chunks, size_t tokens, size_t heads, size_t d) {
-    if (chunks <= 1) return 0;
-    const size_t rows = chunks * tokens * heads, lse = (rows * 4 + 255) / 256 * 256;
-    return rows * d * 4 + lse;
-}
+// The shares' places in the workspace.
+struct PagedParts {
+    size_t rows_o = 0, rows_lse = 0, big_o = 0, big_lse = 0, big_rows = 0, bytes = 0;   // rows_o ..: bytes from its start
+    PagedParts(const PagedCut& c, size_t tokens, size_t heads, size_t kv_heads, size_t d, size_t seqs) {
+        auto take = [this](size_t n) {
+            const size_t at = bytes;
+            bytes += (n + 255) / 256 * 256;
+            return at;
+        };
+        if (c.nt && c.rows_chunks > 1) rows_o = take(c.rows_chunks * tokens * heads * d * 4), rows_lse = take(c.rows_chunks * tokens * heads * 4);
+        if (c.big_tiles && c.big_chunks > 1) {
+            big_rows = (seqs * kv_heads * c.big_tiles - c.big_full) * kBigRows;
+            big_o = take(c.big_chunks * big_rows * d * 4), big_lse = take(c.big_chunks * big_rows * 4);
+        }
+    }
+};
 
 }  // namespace
 }  // namespace fv
@@ -1089,7 +1132,7 @@ size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t 
     size_t most = 0;   // of both kinds of pages
     for (const bool four : {false, true}) {
         const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
-        most = std::max(most, fv::part_bytes(c.chunks(), tokens, heads, d));
+        most = std::max(most, fv::PagedParts(c, tokens, heads, kv_heads, d, seqs).bytes);
     }
     return most;
 }
@@ -1117,18 +1160,20 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     if (max_q > tokens) max_q = tokens;
     const bool four = k_scales != nullptr;
     fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, max_q, max_len, block_tokens, window, sink);
-    const size_t need = fv::part_bytes(c.chunks(), tokens, heads, d);
-    if (need > 0 && (!workspace || workspace_bytes < need)) {   // a share is the whole walk
+    fv::PagedParts parts(c, tokens, heads, kv_heads, d, seqs);
+    if (parts.bytes > 0 && (!workspace || workspace_bytes < parts.bytes)) {   // a share is the whole walk
         c.rows_chunk *= c.rows_chunks, c.big_chunk *= c.big_chunks;
-        c.rows_chunks = c.big_chunks = 1;
+        c.rows_chunks = c.big_chunks = 1, c.big_full = 0;
+        parts = fv::PagedParts(c, tokens, heads, kv_heads, d, seqs);
+        workspace = nullptr;
     }
     const bool split = c.chunks() > 1;
     if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
     const bool many = (c.big_tiles ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
     const dim3 join((unsigned)(seqs * kv_heads), (unsigned)((max_q * (heads / kv_heads) * (d / 4) * (many ? 8 : 1) + 255) / 256));
-    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_blocks = seqs * kv_heads * c.big_tiles * c.big_chunks;
+    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (seqs * kv_heads * c.big_tiles - c.big_full) * c.big_chunks;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
-    if (row_blocks >= kMost || big_blocks + 8 >= kMost || seqs * kv_heads * join.y >= kMost)
+    if (row_blocks >= kMost || c.big_full + big_rest + 8 >= kMost || seqs * kv_heads * join.y >= kMost)
         return fv_decline("paged attention: too large for one launch");
     p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
     p.heads = (int)heads, p.group = (int)(heads / kv_heads);
@@ -1137,15 +1182,16 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     p.few = (int)c.few;
     p.rows = {(int)c.rows_tiles, (int)c.rows_chunk, (int)c.rows_chunks};
     p.big = {(int)c.big_tiles, (int)c.big_chunk, (int)c.big_chunks};
-    p.big_total = (int)big_blocks, p.big_per_xcd = (int)((big_blocks + 7) / 8);
-    p.part_o = (float*)workspace;
-    p.part_lse = split ? p.part_o + c.chunks() * tokens * heads * d : nullptr;
+    p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.big_per_xcd = (int)((big_rest + 7) / 8);
+    uint8_t* ws = (uint8_t*)workspace;
+    p.rows_o = (float*)(ws + parts.rows_o), p.rows_lse = (float*)(ws + parts.rows_lse);
+    p.big_o = (float*)(ws + parts.big_o), p.big_lse = (float*)(ws + parts.big_lse), p.big_rows = (long)parts.big_rows;
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(d == 128, [&](auto d128) {
         fv::paged_pick(four, [&](auto f) {
             constexpr int D = d128() ? 128 : 64;
             if (c.big_tiles)
-                hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3(8 * p.big_per_xcd), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
+                hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3(p.big_full + 8 * p.big_per_xcd), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
             if (c.nt == 1) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 1>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if (split)

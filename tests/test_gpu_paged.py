@@ -405,3 +405,29 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(fv, four, 
                     whole[some, h] = False
                 off = np.abs(x - out)[whole] - pu.attention_bound(out, mag, False, 60.0)[whole]
                 assert off.size == 0 or off.max() <= 0
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("heads,kvh,d,rows,length,block", [(40, 40, 128, 1560, 3120, 1560), (32, 2, 64, 1500, 2000, 1500), (48, 16, 128, 500, 900, 1)])
+def test_calls_of_more_than_a_round(fv, four, heads, kvh, d, rows, length, block):
+    """More tiles than the chip holds at once: those of full rounds keep their walk, the rest are cut and joined. Against sums in 64
+    bits (made on the device, head by head)."""
+    import torch
+
+    announce(f"paged: more than a round four={four} {heads}/{kvh} d={d}")
+    w = World(fv, 91, [length], [rows], kvh, d, 64, four)
+    q = w.queries(heads, 1.5)
+    dq = w.dev(q).bfloat16()
+    need = fv.lib().fv_paged_attention_workspace_bytes(heads, kvh, d, 1, rows, rows, length, block, 0, 0)
+    got = fv.paged_attention(dq, w.pool, w.batch, fv.BlockCausal(block), out_bf16=False)
+    k, v = (w.dev(w.held(n, 0)) for n in "kv")
+    seen = w.dev(pu.sees(np.arange(rows) + length - rows, np.arange(length), block, 0, 0))
+    for h in range(heads):
+        s = (dq[:, h].double() @ k[:, h * kvh // heads].T) * d ** -0.5
+        p = torch.softmax(s.masked_fill(~seen, -float("inf")), -1)
+        out, mag = p @ v[:, h * kvh // heads], p @ v[:, h * kvh // heads].abs()
+        # (the bound of attention_bound, with scores of up to 60)
+        bound = (2.0 ** -8 + 2.0 * 130 * 2.0 ** -24 * 60 + 2.0 ** -12) * mag + 2.0 ** -24 * out.abs() + 1e-30
+        off = float(((got[:, h].double() - out).abs() - bound).max())
+        assert off <= 0, (h, off)
+    print(f"[paged] {heads}/{kvh} d={d}: workspace {need} bytes", flush=True)
