@@ -554,12 +554,14 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
 // Sequences of many rows: a workgroup takes 128 rows of one (sequence, key head), 32 a wave, over tiles of 64 keys that pass
 // through LDS as in the dense kernels (attn_core.h): two buffers for K, two for V. A phase is one key tile: the matrix part
 // (O += P V of the tile before, S = K Q^T) with the next K and this V on their way in, the softmax, one barrier. A wave brings
-// 16 keys of each tile, which lie in one page whatever its size, so a page costs a tile one lookup:
+// 16 keys of each tile, which lie in one page whatever its size, so a page costs a tile one lookup; a tile is any four parts of 16 in
+// the walk's order, so a few sink tokens and a window that begins anywhere cost no tile of their own (prompts of 6001 tokens, 32 / 8
+// heads, a window of 1024 with 4 sinks: 228 us; in tiles of 64 neighbouring keys 240):
 //   bf16 pages: loads straight to LDS through a buffer descriptor of the wave's 16 rows, whose length cuts off what lies
 //     behind the sequence's last key (zeros in LDS, whatever the page holds);
 //   4-bit pages: a lane has a quarter of a row in registers a phase ahead and writes it to LDS as bf16 between the matrix
 //     instructions, 4 conversions and a write at a time.
-constexpr int kBigRows = 128, kTileKeys = 64;
+constexpr int kBigRows = 128, kPart = 16;   // keys that a wave brings of a tile
 // FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop:
 // 8 % of one frame against 21, 9 % of three over 4 bits, 7 % of prompts under a window). Exact as long as nothing overflows or
 // vanishes, which is checked before anything is stored: the sum of every row that sees a key of the walk within 2^-60 .. 2^100 and
@@ -589,10 +591,10 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group, row0 = tile * kBigRows;
     if (row0 >= rows || rows <= p.few) return true;
-    const PagedWalk<kTileKeys> w = paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
-    const int e0 = chunk * p.big.chunk, e1 = full ? w.n : min(w.n, e0 + p.big.chunk);
+    const PagedWalk<kPart> w = paged_walk<kPart>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
+    const int tiles = (w.n + 3) >> 2, e0 = chunk * p.big.chunk, e1 = full ? tiles : min(tiles, e0 + p.big.chunk);
     if (chunk > 0 && e0 >= e1) return true;
-    const bool split = !full && w.n > p.big.chunk;
+    const bool split = !full && tiles > p.big.chunk;
     const float sl2 = p.sl2;
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
@@ -603,10 +605,16 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         const int r = wrow + (lane & 31);
         mine = paged_sight(p, sq.first_pos() + min(r, rows - 1) / p.group, sq.len);
     }
-    // the walk's positions whose tiles the wave's rows see whole: [0, whole0) and [whole1, whole2)
-    auto before = [&](int t) { return min(t, w.ns) + min(max(t - w.b0, 0), w.n - w.ns); };   // positions of tiles before tile t
-    const int whole0 = before(all_see.a / kTileKeys), whole1 = all_see.a >= all_see.lo ? 0 : before((all_see.lo + kTileKeys - 1) / kTileKeys),
-              whole2 = before(all_see.hi / kTileKeys);
+    // the parts of the walk that rows which all see `all` see whole: those before `a` and [b, c)
+    struct Whole {
+        int a, b, c;
+        FV_DEV bool tile(int e) const { return 4 * e + 4 <= a || (4 * e >= b && 4 * e + 4 <= c); }
+    };
+    auto whole_parts = [&](const PagedSight& all) {
+        auto before = [&](int t) { return min(t, w.ns) + min(max(t - w.b0, 0), w.n - w.ns); };   // of the parts before key 16 t
+        return Whole{before(all.a / kPart), all.a >= all.lo ? 0 : before((all.lo + kPart - 1) / kPart), before(all.hi / kPart)};
+    };
+    const Whole whole = whole_parts(all_see);
     bf16x8 qf[D / 32][2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
@@ -622,20 +630,21 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0) here: the compiler's own wait for them would stand among the tile loads
 
     const int* table = p.b.table + (size_t)seq * p.b.table_stride;
-    const int lg = p.pool.lg, slots = (1 << lg) - 1, columns = (p.b.max_len + slots) >> lg;
+    const int lg = p.pool.lg, slots = (1 << lg) - 1;
     // page numbers of 64 tiles of the walk, a tile a lane: that of the wave's 16 keys, and which of the tile's four 16 are in the pool
     int ids = 0, good = 0, ids_at = e0;
     bool clean = true;   // whether all of them are
     auto look_up = [&](int e) {
         ids_at = e;
-        const int k = w.key(min(e + lane, max(e1 - 1, 0)));
+        const int tile = min(e + lane, e1 - 1);
         good = 0;
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-            const int id = table[min((k + 16 * x) >> lg, columns - 1)];
+            const int part = 4 * tile + x;
+            const int id = table[w.key(min(part, w.n - 1)) >> lg];
             const bool ok = (unsigned)id < (unsigned)p.pool.pages;
-            good |= ok ? 1 << x : 0;
-            if (x == wave) ids = ok ? id : -1;
+            good |= ok || part >= w.n ? 1 << x : 0;   // (parts past the walk's end hold no key: none is seen)
+            if (x == wave) ids = ok && part < w.n ? id : -1;
         }
         clean = __builtin_amdgcn_ballot_w64(good != 15) == 0;
     };
@@ -651,8 +660,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     };
     auto part_of = [&](int e) {
         Part x;
-        x.key = w.key(min(e, e1 - 1)) + 16 * wave;
-        const int id = __builtin_amdgcn_readlane(ids, min(e, e1 - 1) - ids_at);
+        const int tile = min(e, e1 - 1), id = __builtin_amdgcn_readlane(ids, tile - ids_at);
+        x.key = w.key(4 * tile + wave);   // (past the walk's end: no page, no key)
         x.row = (((unsigned)max(id, 0) * (unsigned)p.pool.kv_heads + (unsigned)kvh) << lg) + (unsigned)(x.key & slots);
         x.count = id < 0 ? 0 : min(max(w.any.hi - x.key, 0), 16);
         return x;
@@ -720,8 +729,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     // The second pass, a tile that some of the workgroup's rows see a part of: a value that is not finite belongs to the rows that see
     // it, and a probability of zero does not keep it from the others. Such keys leave the V tile, and the rows that have a share
     // in one add theirs from the pool. (The first pass ends in the check where there is such a value.)
-    const PagedSight wg_see = paged_all(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
-    auto set_apart = [&](int m, int k, const ProbTile& pb, f32x4 (&o)[kNO][2]) {
+    const Whole wg_whole = whole_parts(paged_all(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group));
+    auto set_apart = [&](int m, int e, const ProbTile& pb, f32x4 (&o)[kNO][2]) {
         lds_u8* mine_v = vbuf(m) + 16 * wave * G::kRow;
         unsigned bad_rows = 0;   // of the wave's 16
 #pragma unroll
@@ -747,8 +756,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         for (int x = 0; x < 4; x++) keys |= (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane(of[x]) << (16 * x);
 #pragma unroll 1
         for (; keys != 0; keys &= keys - 1) {
-            const int x = __builtin_ctzll(keys), key = k + x;
-            const int id = table[min(key >> lg, columns - 1)];
+            const int x = __builtin_ctzll(keys), key = w.key(min(4 * e + (x >> 4), w.n - 1)) + (x & 15);
+            const int id = table[key >> lg];
             const unsigned row = (((unsigned)max(id, 0) * (unsigned)p.pool.kv_heads + (unsigned)kvh) << lg) + (unsigned)(key & slots);
             float pj[2];
 #pragma unroll
@@ -772,8 +781,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         block_barrier();
     };
     auto mask_tile = [&](ScoreTile& s, int e) {
-        if ((e < whole0 || (e >= whole1 && e < whole2)) && clean) return;
-        const int k = w.key(e), ok = __builtin_amdgcn_readlane(good, e - ids_at);
+        if (whole.tile(e) && clean) return;
+        const int ok = __builtin_amdgcn_readlane(good, e - ids_at);
         const unsigned m[3] = {(unsigned)mine.a, (unsigned)mine.lo, (unsigned)mine.hi};
         int both[3][2];   // the even rows of 16 lanes hold block 0's, the odd ones block 1's
 #pragma unroll
@@ -782,14 +791,14 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
             both[x][0] = (int)r[0];
             both[x][1] = (int)r[1];
         }
-        const int at = k + 4 * q4;
+        auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };   // bits of the first n of 4 keys
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const unsigned long long seen = first_bits(both[0][g] - at) | (first_bits(both[2][g] - at) & ~first_bits(both[1][g] - at));
-            const unsigned half[2] = {(unsigned)seen, (unsigned)(seen >> 32)};
+        for (int kb = 0; kb < 4; kb++) {
+            const bool none = 4 * e + kb >= w.n || !((ok >> kb) & 1);
+            const int at = (none ? 0x40000000 : w.key(4 * e + kb)) + 4 * q4;
 #pragma unroll
-            for (int kb = 0; kb < 4; kb++) {
-                const unsigned bits = (ok >> kb) & 1 ? half[kb >> 1] >> (16 * (kb & 1)) : 0u;
+            for (int g = 0; g < 2; g++) {
+                const unsigned bits = below(both[0][g] - at) | (below(both[2][g] - at) & ~below(both[1][g] - at));
 #pragma unroll
                 for (int i = 0; i < 4; i++) s[kb][g][i] = (bits >> i) & 1 ? s[kb][g][i] : neg_inf();
             }
@@ -862,8 +871,7 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
             block_barrier();   // K(m + 1), V(m) resident; this phase's tiles read by every wave
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!FIXED) {
-                const int k = w.key(e);
-                if (!paged_whole(wg_see, k, k + kTileKeys)) set_apart(m, k, pb, o);
+                if (!wg_whole.tile(e)) set_apart(m, e, pb, o);
             }
         };
         phase(0, std::true_type{});
@@ -880,9 +888,10 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
 
     if constexpr (FIXED) {
         // the lane's part of its rows' check; a row without a key in the walk has a sum of zero by right
-        const int from = w.key(max(e0, w.ns)), to = e1 > e0 ? w.key(e1 - 1) + kTileKeys : 0;   // of the walk past the sink
-        const bool any = e1 > e0 && wrow + (lane & 31) < rows &&
-                         ((e0 < w.ns && e0 * kTileKeys < mine.a) || (e1 > w.ns && max(mine.lo, from) < min(mine.hi, to)) || (e1 > w.ns && from < mine.a));
+        const int p0 = 4 * e0, p1 = min(4 * e1, w.n);   // the parts; those past the sink hold keys [from, to)
+        const int from = w.key(max(p0, w.ns)), to = w.key(max(p1 - 1, 0)) + kPart;
+        const bool any = p0 < p1 && wrow + (lane & 31) < rows &&
+                         ((p0 < w.ns && p0 * kPart < mine.a) || (p1 > w.ns && (max(mine.lo, from) < min(mine.hi, to) || from < mine.a)));
         const auto sees = __builtin_amdgcn_permlane16_swap((unsigned)any, (unsigned)any, false, false);   // (exchanged as in mask_tile)
         float chk = 0.f;
         bool fine = true;
@@ -967,7 +976,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
             const int row0 = r / kBigRows * kBigRows;
             const int tile = r / kBigRows, item = (kvh * p.b.seqs + seq) * p.big.tiles + p.big.tiles - 1 - tile;   // (as paged_tiles_item counts)
             if (tile < p.big.tiles && item >= p.big_full)
-                chunks = (paged_walk<kTileKeys>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + p.big.chunk - 1) / p.big.chunk;
+                chunks = ((paged_walk<kPart>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + 3) / 4 + p.big.chunk - 1) / p.big.chunk;
             first = (size_t)(item - p.big_full) * kBigRows + (r - row0);
             step = (size_t)p.big_rows;
         }
@@ -1058,7 +1067,7 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
     const size_t group = heads / kv_heads, rows = max_q * group, units = (size_t)fv_compute_units();
     if (rows > kFewRows) {
         c.big_tiles = (rows + kBigRows - 1) / kBigRows;
-        const size_t steps = walk_bound(kTileKeys, kBigRows, group, max_len, block_tokens, window, sink);
+        const size_t steps = (walk_bound(kPart, kBigRows, group, max_len, block_tokens, window, sink) + 3) / 4;
         // Shares of the walk: rounds of as many workgroups as there is room for, 4 steps' time besides their own each, against a
         // launch and the bytes that joining moves. Where the last round is far from full, the tiles of the rounds before keep
         // their walk whole and only the rest are cut. (Tiles whose walks differ, causal or of ragged prompts, fill the
