@@ -615,20 +615,6 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         return Whole{before(all.a / kPart), all.a >= all.lo ? 0 : before((all.lo + kPart - 1) / kPart), before(all.hi / kPart)};
     };
     const Whole whole = whole_parts(all_see);
-    bf16x8 qf[D / 32][2];
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-        const int r = wrow + 16 * g + i16, t = r / p.group;
-        const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + (kvh * p.group + r - t * p.group) * D + 8 * q4;
-#pragma unroll
-        for (int dk = 0; dk < D / 32; dk++) {
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (r < rows) x = *reinterpret_cast<const u32x4*>(q + 32 * dk);
-            qf[dk][g] = __builtin_bit_cast(bf16x8, x);
-        }
-    }
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0) here: the compiler's own wait for them would stand among the tile loads
-
     const int* table = p.b.table + (size_t)seq * p.b.table_stride;
     const int lg = p.pool.lg, slots = (1 << lg) - 1;
     // page numbers of 64 tiles of the walk, a tile a lane: that of the wave's 16 keys, and which of the tile's four 16 are in the pool
@@ -648,6 +634,20 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
         }
         clean = __builtin_amdgcn_ballot_w64(good != 15) == 0;
     };
+    // (the table, the queries and the first keys on their way together: short walks are mostly this wait)
+    if (e0 < e1) look_up(e0);
+    bf16x8 qf[D / 32][2];
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const int r = wrow + 16 * g + i16, t = r / p.group;
+        const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + (kvh * p.group + r - t * p.group) * D + 8 * q4;
+#pragma unroll
+        for (int dk = 0; dk < D / 32; dk++) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (r < rows) x = *reinterpret_cast<const u32x4*>(q + 32 * dk);
+            qf[dk][g] = __builtin_bit_cast(bf16x8, x);
+        }
+    }
     const TileReadBases rb = tile_read_bases<D>(lane);
     auto kbuf = [&](int m) -> lds_u8* { return smem + (m & 1) * kTile; };
     auto vbuf = [&](int m) -> lds_u8* { return smem + (2 + (m & 1)) * kTile; };
@@ -806,7 +806,6 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     };
 
     if (e0 < e1) {
-        look_up(e0);
         Part cur = part_of(e0), next = part_of(e0 + 1);   // of the tile whose V is loaded next, whose K is
         if constexpr (FOUR) {
             fetch(p.pool.k, p.pool.ks, cur, kq, kqs);
@@ -815,11 +814,14 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
             fetch(p.pool.v, p.pool.vs, cur, vq, vqs);
             fetch(p.pool.k, p.pool.ks, next, kq, kqs);
             __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+            __builtin_amdgcn_sched_barrier(0);
         } else {
 #pragma unroll
             for (int u = 0; u < kUnits; u++) issue(p.pool.k, cur, kbuf(0), koff, u);
-            wait_vmcnt<0>();
         }
+#pragma unroll
+        for (int dk = 0; dk < D / 32; dk++) asm volatile("" : "+v"(qf[dk][0]), "+v"(qf[dk][1]));   // (waited for here, not among the tile loads)
+        if constexpr (!FOUR) wait_vmcnt<0>();
         block_barrier();
         constexpr int kAhead = 3;
         auto phase = [&](int m, auto first) {
