@@ -32,7 +32,7 @@ struct PagedAttnParams {
     int block_tokens, window, sink;   // blocks; window 0: all
     // Two kernels share a call: sequences of up to `few` rows a key head go to paged_rows_kernel, the others to
     // paged_tiles_kernel. How each cuts its part:
-    int few;
+    int few, rows_m;            // (rows_m: rows a tile of paged_rows_kernel)
     struct Cut {
         int tiles;              // row tiles of a (sequence, key head)
         int chunk, chunks;      // steps of the walk that a workgroup takes, workgroups a walk
@@ -954,8 +954,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
 
 // The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). G groups of D / 4 threads share a
 // row's shares out, four at a time each, with a running maximum, and meet in LDS; rows whose walk one workgroup made have
-// their result already. ROWS: of a tile of paged_rows_kernel.
-template <int D, int ROWS, int G>
+// their result already.
+template <int D, int G>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
     constexpr int kPer = D / 4, kRows = 256 / (kPer * G);
     __shared__ float lds_top[kRows][G], lds_sum[kRows][G];
@@ -971,9 +971,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     size_t first = dst, step = (size_t)p.b.tokens * p.heads;   // the row's place in the first share, rows to the next
     if (r < rows) {
         if (few) {
-            const int row0 = r / ROWS * ROWS;
-            if (r < p.rows.tiles * ROWS)
-                chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + ROWS, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
+            const int tile = r / p.rows_m, row0 = tile * p.rows_m;
+            if (tile < p.rows.tiles)
+                chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + p.rows_m, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
         } else {
             const int row0 = r / kBigRows * kBigRows;
             const int tile = r / kBigRows, item = (kvh * p.b.seqs + seq) * p.big.tiles + p.big.tiles - 1 - tile;   // (as paged_tiles_item counts)
@@ -1062,32 +1062,43 @@ struct PagedCut {
     size_t big_tiles = 0, big_full = 0, big_chunk = 1, big_chunks = 1;   // of paged_tiles_kernel; no tiles: not launched
     size_t chunks() const { return std::max(nt ? rows_chunks : 1, big_tiles ? big_chunks : 1); }
 };
-constexpr size_t kFewRows = 64;
+// bf16: two tiles of 16 rows cost paged_rows_kernel a second pass over the keys' operands, or a second walk, and paged_tiles_kernel, which
+// pads to 128, streams the keys as fast (48 sessions of 5 drafts x 4 heads, a window of 2048: 86 us by rows, 77.5 by tiles; 16 x 8 x 5
+// heads, 8000 tokens: 160, 108; single tokens of 5 heads: 240, 242). 4 bits: the tiles' arithmetic is the bound (single tokens 177 us by
+// rows, 492 by tiles; 40 rows the same, 73).
+constexpr size_t few_rows(bool four) { return four ? 64 : 16; }
 PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t seqs, size_t tokens, size_t max_q, size_t max_len, size_t block_tokens,
                    size_t window, size_t sink) {
     PagedCut c;
-    const size_t group = heads / kv_heads, rows = max_q * group, units = (size_t)fv_compute_units();
-    if (rows > kFewRows) {
+    const size_t group = heads / kv_heads, rows = max_q * group, units = (size_t)fv_compute_units(), most_few = few_rows(four);
+    if (rows > most_few) {
         c.big_tiles = (rows + kBigRows - 1) / kBigRows;
         const size_t steps = (walk_bound(kPart, kBigRows, group, max_len, block_tokens, window, sink) + 3) / 4;
-        // Shares of the walk: rounds of as many workgroups as there is room for, 4 steps' time besides their own each, against a
+        // Shares of the walk, by microseconds: rounds of as many workgroups as there is room for, 4 each besides their steps (1.05 and 1.75 a
+        // step of one and of two workgroups a unit, or what the memory takes where few tiles share their keys), against a
         // launch and the bytes that joining moves. Where the last round is far from full, the tiles of the rounds before keep
         // their walk whole and only the rest are cut. (Tiles whose walks differ, causal or of ragged prompts, fill the
-        // rounds by themselves: no count of rounds, and all or none are cut.)
+        // rounds by themselves: no count of rounds, and all or none are cut.) One frame of 1560 against 32760, 12 heads: in 1, 2, 3, 4
+        // shares 538, 427, 293, 362 us.
         const size_t items = seqs * kv_heads * c.big_tiles, held = kv_heads * std::min(seqs * c.big_tiles, tokens * group / kBigRows + seqs);
         const size_t slots = (d == 64 ? 3 : 2) * units / 8 * 8;
         const bool varied = 10 * held < 9 * items || (window == 0 && 4 * block_tokens < max_q && 2 * max_q > max_len);
-        const double step = d == 64 ? 1.3 : 2.0;   // us
+        auto step_us = [&](size_t wgs) {
+            const size_t at_once = std::min(wgs, slots);
+            const double bytes = 64.0 * (double)(four ? d + d / 16 : 4 * d);
+            return std::max((at_once <= units ? 1.05 : 1.75) * (d == 64 ? 0.75 : 1.0), (double)at_once / (double)c.big_tiles * bytes / (at_once <= units ? 4.3e6 : 5.2e6));
+        };
         double best = 0;
         const size_t rounds_before = varied ? 0 : held / slots;
         for (size_t keep = 0; keep <= std::min<size_t>(rounds_before, 2); keep++) {
             const size_t full = keep == 0 ? 0 : (rounds_before - (keep - 1)) * slots, rest = held - full;
             if (rest == 0) continue;
-            for (size_t k = 1; k <= 32 && k <= steps; k++) {
+            for (size_t k = 1; k <= 64 && k <= steps; k++) {
                 const size_t chunk = (steps + k - 1) / k, wgs = rest * k;
                 const double rounds = varied ? std::max(1.0, (double)wgs / (double)slots) + 0.5 : (double)((wgs + slots - 1) / slots);
-                const double cost = (double)(full / slots) * (double)(steps + 4) * step + rounds * ((varied ? 0.6 : 1.0) * (double)chunk + 4.0) * step +
-                                    (k > 1 ? 5.0 + (double)(k * rest * kBigRows) * 8.0 * (double)d / 4e6 : 0.0);
+                const double cost = (double)(full / slots) * (4.0 + (double)steps * step_us(slots)) +
+                                    rounds * (4.0 + (varied ? 0.6 : 1.0) * (double)chunk * step_us(wgs)) +
+                                    (k > 1 ? 7.0 + (double)(k * std::min(rest * kBigRows, tokens * heads)) * 8.0 * (double)d / 6e6 : 0.0);
                 if ((keep == 0 && k == 1) || cost < 0.97 * best) best = cost, c.big_full = full, c.big_chunk = chunk, c.big_chunks = (steps + chunk - 1) / chunk;
             }
         }
@@ -1095,9 +1106,9 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
     }
     // (Sequences of few rows beside longer ones: a launch of their own where they may be many, by the mean; else they are the tiles', which
     // take any, and the launch, 5 us, is saved.)
-    if (rows <= kFewRows || 2 * tokens < seqs * max_q) {
-        const size_t most = std::min(rows, kFewRows);
-        c.few = rows <= kFewRows ? rows : kFewRows;
+    if (rows <= most_few || 2 * tokens < seqs * max_q) {
+        const size_t most = std::min(rows, most_few);
+        c.few = most;
         c.nt = most <= 16 ? 1 : 2;
         c.rows_tiles = (most + 16 * c.nt - 1) / (16 * c.nt);
         const size_t steps = walk_bound(kStep, 16 * c.nt, group, max_len, block_tokens, window, sink);
@@ -1190,7 +1201,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     p.heads = (int)heads, p.group = (int)(heads / kv_heads);
     p.sl2 = (float)((double)scale * 1.4426950408889634);
     p.block_tokens = (int)block_tokens, p.window = (int)window, p.sink = (int)sink;
-    p.few = (int)c.few;
+    p.few = (int)c.few, p.rows_m = (int)(16 * c.nt);
     p.rows = {(int)c.rows_tiles, (int)c.rows_chunk, (int)c.rows_chunks};
     p.big = {(int)c.big_tiles, (int)c.big_chunk, (int)c.big_chunks};
     p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.big_per_xcd = (int)((big_rest + 7) / 8);
@@ -1204,13 +1215,10 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
             if (c.big_tiles)
                 hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3(p.big_full + 8 * p.big_per_xcd), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
             if (c.nt == 1) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 1>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
-            if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
+            if constexpr (f())   // (the only pages whose calls have two tiles of rows, few_rows)
+                if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, true, 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if (split)
-                fv::paged_pick(c.nt == 1, [&](auto one) {
-                    fv::paged_pick(many, [&](auto m) {
-                        hipLaunchKernelGGL((fv::paged_join_kernel<D, one() ? 16 : 32, m() ? 8 : 1>), join, dim3(256), 0, st, p);
-                    });
-                });
+                fv::paged_pick(many, [&](auto m) { hipLaunchKernelGGL((fv::paged_join_kernel<D, m() ? 8 : 1>), join, dim3(256), 0, st, p); });
         });
     });
     const hipError_t e = hipGetLastError();
