@@ -141,12 +141,6 @@ struct TileDma {
     }
 };
 
-// The first n of 64 bits.
-FV_DEV unsigned long long first_bits(int n) {
-    const unsigned long long m = ~0ull >> ((64 - n) & 63);
-    return n <= 0 ? 0ull : n >= 64 ? ~0ull : m;
-}
-
 // Per-lane read bases into a swizzled tile.
 struct TileReadBases {
     int k;   // K A-operand (16 keys x 32 d): ^ (dk << 6), + kb * 16 rows

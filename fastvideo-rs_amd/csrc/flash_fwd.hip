@@ -112,6 +112,11 @@ FV_DEV ConstParams* params_again() {
     asm volatile("" : "+s"(again));
     return again;
 }
+// The first n of 64 bits.
+FV_DEV unsigned long long first_bits(int n) {
+    const unsigned long long m = ~0ull >> ((64 - n) & 63);
+    return n <= 0 ? 0ull : n >= 64 ? ~0ull : m;
+}
 // Scores of query block g that the lane's query may not see to -inf, and those of keys `left` (counted from the tile's first)
 // and on; `at`: the tile's first key. The bounds make one word of 64 keys, and a score costs a test of its bit and a
 // select: 3 vector instructions where four comparisons and their scalar joins took 9, and no path apart for tiles that are whole

@@ -44,6 +44,7 @@ struct PagedAttnParams {
     // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
     float *rows_o, *rows_lse, *big_o, *big_lse;
     long big_rows;              // the latter's rows
+    int join_blocks;            // of paged_join_kernel, for each (sequence, key head)
 };
 
 // The keys that a row at position p of a sequence of `len` tokens sees: [0, a) and [lo, hi), a <= hi.
@@ -228,9 +229,12 @@ FV_DEV void pool_values(const Pool& pool, unsigned row, int c, float (&v)[N]) {
 }
 
 // One workgroup: a share of the walk of a tile of 16 NT rows of one (sequence, key head); its four waves take the share's
-// steps in turn, each with a running maximum of its own, and join through LDS. One tile of rows: a whole step is loaded ahead.
-// Two: the keys of the next step go into the registers of this one's as soon as their scores are there, its values likewise
-// (a whole step ahead spilled 270 bytes a lane: 48 drafts of 5 tokens, 32 heads, a window of 2048, 136 us instead of 83).
+// steps in turn, each with a running maximum of its own, and join through LDS. A step reads its keys and values once, for all of
+// the tile's rows, straight into registers in the order of the matrix operands, so that nothing but the memory bounds it: 128
+// single tokens of 40 / 8 heads over 1.24 GB of bf16 pages 240 us, 5.15 TB/s; 40 of 64 / 8 heads over 0.85 GB of 4 bits 176 us, 4.8. Calls
+// too short for that are bound by their few waits in a row: 16 tokens over 300 keys 9.5 us.
+// One tile of rows: a whole step is loaded ahead. Two (4-bit pages, few_rows): the keys of the next step go into the registers of
+// this one's as soon as their scores are there, its values likewise; a whole step ahead spilled 270 bytes a lane.
 template <int D, bool FOUR, int NT>
 __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParams p) {
     constexpr int kNO = D / 16, kPad = D + 4, kDepth = NT == 1 ? 2 : 1;
@@ -555,13 +559,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
 // through LDS as in the dense kernels (attn_core.h): two buffers for K, two for V. A phase is one key tile: the matrix part
 // (O += P V of the tile before, S = K Q^T) with the next K and this V on their way in, the softmax, one barrier. A wave brings
 // 16 keys of each tile, which lie in one page whatever its size, so a page costs a tile one lookup; a tile is any four parts of 16 in
-// the walk's order, so a few sink tokens and a window that begins anywhere cost no tile of their own (prompts of 6001 tokens, 32 / 8
-// heads, a window of 1024 with 4 sinks: 228 us; in tiles of 64 neighbouring keys 240):
+// the walk's order, so a few sink tokens and a window that begins anywhere cost no tile of their own (prompts of up to 6001 tokens, 32 / 8
+// heads, a window of 1024 with 4 sinks: 227 us; in tiles of 64 neighbouring keys 240):
 //   bf16 pages: loads straight to LDS through a buffer descriptor of the wave's 16 rows, whose length cuts off what lies
 //     behind the sequence's last key (zeros in LDS, whatever the page holds);
 //   4-bit pages: a lane has a quarter of a row in registers a phase ahead and writes it to LDS as bf16 between the matrix
 //     instructions, 4 conversions and a write at a time.
 constexpr int kBigRows = 128, kPart = 16;   // keys that a wave brings of a tile
+// The softmax's vector work, about two thirds of a phase's matrix time, and the matrix work bound it together, and only in part
+// overlap between a unit's two workgroups: one frame of 1560 rows x 12 heads against 32760 293 us, 1.07 PFLOP/s of the large product's
+// 1.35, the matrix cores busy 60 % of the time while all units have work; three over 4 bits 1.51 ms, 1.25. (Tried and slower: 8 waves in
+// two groups that take turns, 333 us; priority to the softmax, 336; priority by the wave's slot, 331.)
 // FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop:
 // 8 % of one frame against 21, 9 % of three over 4 bits, 7 % of prompts under a window). Exact as long as nothing overflows or
 // vanishes, which is checked before anything is stored: the sum of every row that sees a key of the walk within 2^-60 .. 2^100 and
@@ -954,16 +962,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
 
 // The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). G groups of D / 4 threads share a
 // row's shares out, four at a time each, with a running maximum, and meet in LDS; rows whose walk one workgroup made have
-// their result already.
+// their result already. A row with many shares is a chain of waits, so G = 8 then (64 shares of one token's 64 heads: 5 us; with G = 1
+// 17); few shares are the memory's to bound, and G = 1 keeps them out of LDS.
 template <int D, int G>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
     constexpr int kPer = D / 4, kRows = 256 / (kPer * G);
     __shared__ float lds_top[kRows][G], lds_sum[kRows][G];
     __shared__ f32x4 lds_acc[kRows][G][kPer];
-    const int seq = blockIdx.x / p.pool.kv_heads, kvh = blockIdx.x % p.pool.kv_heads;
+    const int item = blockIdx.x / p.join_blocks, block = blockIdx.x - item * p.join_blocks;
+    const int seq = item / p.pool.kv_heads, kvh = item % p.pool.kv_heads;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int slot = threadIdx.x / (kPer * G), gi = threadIdx.x / kPer % G, c = threadIdx.x % kPer;
-    const int rows = sq.count * p.group, r = blockIdx.y * kRows + slot;
+    const int rows = sq.count * p.group, r = block * kRows + slot;
     const int t = r / p.group;
     const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
     int chunks = 0;
@@ -976,10 +986,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
                 chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + p.rows_m, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
         } else {
             const int row0 = r / kBigRows * kBigRows;
-            const int tile = r / kBigRows, item = (kvh * p.b.seqs + seq) * p.big.tiles + p.big.tiles - 1 - tile;   // (as paged_tiles_item counts)
-            if (tile < p.big.tiles && item >= p.big_full)
+            const int tile = r / kBigRows, at = (kvh * p.b.seqs + seq) * p.big.tiles + p.big.tiles - 1 - tile;   // (as paged_tiles_item counts)
+            if (tile < p.big.tiles && at >= p.big_full)
                 chunks = ((paged_walk<kPart>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + 3) / 4 + p.big.chunk - 1) / p.big.chunk;
-            first = (size_t)(item - p.big_full) * kBigRows + (r - row0);
+            first = (size_t)(at - p.big_full) * kBigRows + (r - row0);
             step = (size_t)p.big_rows;
         }
     }
@@ -1192,10 +1202,10 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     const bool split = c.chunks() > 1;
     if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
     const bool many = (c.big_tiles ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
-    const dim3 join((unsigned)(seqs * kv_heads), (unsigned)((max_q * (heads / kv_heads) * (d / 4) * (many ? 8 : 1) + 255) / 256));
+    const size_t join_blocks = (max_q * (heads / kv_heads) * (d / 4) * (many ? 8 : 1) + 255) / 256, join = seqs * kv_heads * join_blocks;
     const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (seqs * kv_heads * c.big_tiles - c.big_full) * c.big_chunks;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
-    if (row_blocks >= kMost || c.big_full + big_rest + 8 >= kMost || seqs * kv_heads * join.y >= kMost)
+    if (row_blocks >= kMost || c.big_full + big_rest + 8 >= kMost || (split && join >= kMost))
         return fv_decline("paged attention: too large for one launch");
     p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
     p.heads = (int)heads, p.group = (int)(heads / kv_heads);
@@ -1208,6 +1218,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     uint8_t* ws = (uint8_t*)workspace;
     p.rows_o = (float*)(ws + parts.rows_o), p.rows_lse = (float*)(ws + parts.rows_lse);
     p.big_o = (float*)(ws + parts.big_o), p.big_lse = (float*)(ws + parts.big_lse), p.big_rows = (long)parts.big_rows;
+    p.join_blocks = (int)join_blocks;
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(d == 128, [&](auto d128) {
         fv::paged_pick(four, [&](auto f) {
@@ -1218,7 +1229,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
             if constexpr (f())   // (the only pages whose calls have two tiles of rows, few_rows)
                 if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, true, 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if (split)
-                fv::paged_pick(many, [&](auto m) { hipLaunchKernelGGL((fv::paged_join_kernel<D, m() ? 8 : 1>), join, dim3(256), 0, st, p); });
+                fv::paged_pick(many, [&](auto m) { hipLaunchKernelGGL((fv::paged_join_kernel<D, m() ? 8 : 1>), dim3((unsigned)join), dim3(256), 0, st, p); });
         });
     });
     const hipError_t e = hipGetLastError();

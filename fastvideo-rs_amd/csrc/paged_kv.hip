@@ -2,8 +2,8 @@
 // in with the rotation of their positions applied on the way, as bf16 or as 4-bit codes, and come out again as rows.
 //
 // Both are HBM-bound scans: a thread moves 8 channels of one head of a token in one 16-byte piece (two for f32), a workgroup
-// takes 256 such pieces of one token (so that the sequence, the page and the slot are scalars), or of kTokens tokens where
-// the batch is long.
+// takes 256 such pieces of one token, so that the sequence, the page and the slot are scalars, computed once, and every load
+// and store of a wave is a run of neighbouring pieces.
 #include <limits.h>
 #include <stdio.h>
 
@@ -135,52 +135,50 @@ FV_DEV unsigned to_fp4x8(const float (&r)[8], unsigned& scale_byte) {
     return w;
 }
 
-// Block (x, y): pieces [256 y, 256 y + 256) of tokens [x TOKENS, (x + 1) TOKENS): the query heads' first (if any), then the
-// key heads', then the value heads'.
-template <bool IN16, int D, bool FOUR, bool HALVES, int TOKENS>
+// Block (x, y): pieces [256 y, 256 y + 256) of token x: the query heads' first (if any), then the key heads', then the value
+// heads'. 20011 tokens of 40 / 8 heads, their tables and queries: 1.42 GB in 271 us, 5.2 TB/s (a large copy: 4.9); 4680 of 12 heads
+// to 4 bits: 0.21 GB in 49 us, 4.2 TB/s.
+template <bool IN16, int D, bool FOUR, bool HALVES>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p) {
     constexpr int kPer = D / 8;
     const int piece = blockIdx.y * 256 + threadIdx.x;
     const int head = piece / kPer, c = piece % kPer, nq = p.q ? p.heads : 0, kvh = p.pool.kv_heads;
     if (head >= nq + 2 * kvh) return;
-#pragma unroll
-    for (int i = 0; i < TOKENS; i++) {
-        const int t = blockIdx.x * TOKENS + i;
-        if (t >= p.b.tokens || t >= p.b.q_start[p.b.seqs]) return;
-        if (t < p.b.q_start[0]) continue;
-        const PagedPlace at = paged_place(p.b, p.pool, t);
-        const int row = p.rope_at ? p.rope_at[t] : at.pos;
-        const bool turn = p.cos_t != nullptr;
-        const bool ok = at.pos >= 0 && (!turn || (unsigned)row < (unsigned)p.rope_rows);
-        float r[8];
-        if (!ok || (head >= nq && at.page < 0)) {   // lies nowhere: nothing is stored, a query is zeros
-            if (head < nq) *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = u32x4{0u, 0u, 0u, 0u};
-            continue;
+    const int t = blockIdx.x;
+    if (t >= p.b.tokens || t >= p.b.q_start[p.b.seqs]) return;
+    if (t < p.b.q_start[0]) return;
+    const PagedPlace at = paged_place(p.b, p.pool, t);
+    const int row = p.rope_at ? p.rope_at[t] : at.pos;
+    const bool turn = p.cos_t != nullptr;
+    const bool ok = at.pos >= 0 && (!turn || (unsigned)row < (unsigned)p.rope_rows);
+    float r[8];
+    if (!ok || (head >= nq && at.page < 0)) {   // lies nowhere: nothing is stored, a query is zeros
+        if (head < nq) *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = u32x4{0u, 0u, 0u, 0u};
+        return;
+    }
+    if (head < nq + kvh) {
+        const bool is_q = head < nq;
+        const void* x = is_q ? p.q : p.k;
+        const size_t from = is_q ? (size_t)t * p.q_stride + head * D : (size_t)t * p.k_stride + (head - nq) * D;
+        if (turn) load_turned<IN16, D, HALVES>(x, from, c, p.cos_t, p.sin_t, row, r);
+        else load8<IN16>(x, from + 8 * c, r);
+        if (is_q) {
+            *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = to_bf16x8(r);
+            return;
         }
-        if (head < nq + kvh) {
-            const bool is_q = head < nq;
-            const void* x = is_q ? p.q : p.k;
-            const size_t from = is_q ? (size_t)t * p.q_stride + head * D : (size_t)t * p.k_stride + (head - nq) * D;
-            if (turn) load_turned<IN16, D, HALVES>(x, from, c, p.cos_t, p.sin_t, row, r);
-            else load8<IN16>(x, from + 8 * c, r);
-            if (is_q) {
-                *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = to_bf16x8(r);
-                continue;
-            }
-        } else {
-            load8<IN16>(p.v, (size_t)t * p.v_stride + (head - nq - kvh) * D + 8 * c, r);
-        }
-        const bool is_v = head >= nq + kvh;
-        const size_t at_row = (((size_t)at.page * kvh + (head - nq - (is_v ? kvh : 0))) << p.pool.lg) + at.slot;
-        uint8_t* base = (uint8_t*)(is_v ? p.pool.v : p.pool.k);
-        if constexpr (FOUR) {
-            unsigned scale;
-            const unsigned w = to_fp4x8(r, scale);
-            *reinterpret_cast<unsigned*>(base + at_row * (D / 2) + 4 * c) = w;
-            if (c % 4 == 0) (is_v ? p.pool.vs : p.pool.ks)[at_row * (D / 32) + c / 4] = (uint8_t)scale;
-        } else {
-            *reinterpret_cast<u32x4*>(base + at_row * (2 * D) + 16 * c) = to_bf16x8(r);
-        }
+    } else {
+        load8<IN16>(p.v, (size_t)t * p.v_stride + (head - nq - kvh) * D + 8 * c, r);
+    }
+    const bool is_v = head >= nq + kvh;
+    const size_t at_row = (((size_t)at.page * kvh + (head - nq - (is_v ? kvh : 0))) << p.pool.lg) + at.slot;
+    uint8_t* base = (uint8_t*)(is_v ? p.pool.v : p.pool.k);
+    if constexpr (FOUR) {
+        unsigned scale;
+        const unsigned w = to_fp4x8(r, scale);
+        *reinterpret_cast<unsigned*>(base + at_row * (D / 2) + 4 * c) = w;
+        if (c % 4 == 0) (is_v ? p.pool.vs : p.pool.ks)[at_row * (D / 32) + c / 4] = (uint8_t)scale;
+    } else {
+        *reinterpret_cast<u32x4*>(base + at_row * (2 * D) + 16 * c) = to_bf16x8(r);
     }
 }
 
@@ -299,7 +297,7 @@ int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stri
         fv::paged_pick(d == 128, [&](auto d128) {
             fv::paged_pick(four, [&](auto f) {
                 fv::paged_pick(halves != 0, [&](auto h) {
-                    hipLaunchKernelGGL((fv::paged_append_kernel<i16(), d128() ? 128 : 64, f(), h(), 1>), grid, dim3(256), 0, st, p);
+                    hipLaunchKernelGGL((fv::paged_append_kernel<i16(), d128() ? 128 : 64, f(), h()>), grid, dim3(256), 0, st, p);
                 });
             });
         });
