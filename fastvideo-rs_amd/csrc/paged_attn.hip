@@ -7,6 +7,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <numeric>
 
 #include "../../include/fv_sdpa_hip.h"
 #include "attn_core.h"
@@ -19,6 +20,36 @@ namespace {
 
 constexpr int kStep = 32;       // keys a wave takes at a time
 constexpr int kWaves = 4;
+
+// Pieces of up to R rows of the (token, head of the group) rows of a batch, for one key head. Where the sequences are as long as
+// the longest, piece t of sequence s is number s tiles + t. Where they are not (tiles 0), it is number first(s) + t with
+// first(s) = (group q_start[s] + (R - 1) s) / R, which leaves each its ceil(rows / R) numbers and no more than one for each sequence
+// unused, whatever the longest is. (A prompt of 8192 tokens among 255 single ones: 6.8 ms with the longest's pieces for all.)
+struct PagedPieces {
+    int n, tiles;               // numbers, of a sequence
+};
+struct PagedPiece {
+    int seq, tile;              // (of an unused number: a tile that the sequence does not have)
+};
+template <int R, class Pieces, class Batch>
+FV_DEV long paged_first_piece(const Pieces& x, const Batch& b, int group, int seq) {
+    return x.tiles ? (long)seq * x.tiles : ((long)b.q_start[seq] * group + (long)(R - 1) * seq) / R;
+}
+template <int R, class Pieces, class Batch>
+FV_DEV PagedPiece paged_piece(const Pieces& x, const Batch& b, int group, int number) {   // (of a whole wave)
+    if (x.tiles) return {number / x.tiles, number % x.tiles};
+    const int lane = threadIdx.x & 63;
+    int seq = 0, n = b.seqs;    // the last of sequences seq .. seq + n - 1 whose first piece is no later: 64 of them at a time
+    while (n > 1) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const bool le = at < n && paged_first_piece<R>(x, b, group, seq + min(at, n - 1)) <= number;
+        const int k = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)), 1) - 1;
+        seq += k * step;
+        n = min(step, n - k * step);
+    }
+    const long tile = number - paged_first_piece<R>(x, b, group, seq);
+    return {seq, tile < 0 || tile > 0x1000000 ? 0x1000000 : (int)tile};
+}
 
 struct PagedAttnParams {
     PagedPool pool;
@@ -33,18 +64,20 @@ struct PagedAttnParams {
     // Two kernels share a call: sequences of up to `few` rows a key head go to paged_rows_kernel, the others to
     // paged_tiles_kernel. How each cuts its part:
     int few, rows_m;            // (rows_m: rows a tile of paged_rows_kernel)
+    int rows_tiles;             // (tiles of a (sequence, key head) there)
     struct Cut {
-        int tiles;              // row tiles of a (sequence, key head)
         int chunk, chunks;      // steps of the walk that a workgroup takes, workgroups a walk
     } rows, big;
-    // paged_tiles_kernel: the first big_full tiles (a multiple of 8), counted key head by key head, have a workgroup each, the
-    // others big.chunks; big_rest: those others' workgroups, big_per_xcd an eighth of them
-    int big_full, big_rest, big_per_xcd;
+    // paged_tiles_kernel: the first big_full tiles (a multiple of 8), counted key head by key head and the last rows first, have a
+    // workgroup each, the others big.chunks; big_rest: those others' workgroups.
+    PagedPieces big_pieces;
+    int big_full, big_rest;
+    int xcds;                   // XCDs that share a run of items (1, 2, 4, 8)
     // Shares: values, each normalised, and the base-2 logarithm of its sum. Of paged_rows_kernel [chunks][tokens * heads][d] and
     // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
     float *rows_o, *rows_lse, *big_o, *big_lse;
     long big_rows;              // the latter's rows
-    int join_blocks;            // of paged_join_kernel, for each (sequence, key head)
+    PagedPieces join_pieces;    // of paged_join_kernel
 };
 
 // The keys that a row at position p of a sequence of `len` tokens sees: [0, a) and [lo, hi), a <= hi.
@@ -243,8 +276,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     int item = blockIdx.x;
-    const int tile = item % p.rows.tiles;
-    item /= p.rows.tiles;
+    const int tile = item % p.rows_tiles;
+    item /= p.rows_tiles;
     const int kvh = item % p.pool.kv_heads;
     item /= p.pool.kv_heads;
     const int chunk = item % p.rows.chunks, seq = item / p.rows.chunks;
@@ -582,20 +615,22 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int q4 = lane >> 4, i16 = lane & 15;
-    // XCD x takes a contiguous eighth of the items, key head by key head, so that an L2 holds few heads' keys; the last rows,
-    // whose walks are the longest, first
+    // The items lie in 8 / xcds runs, key head by key head, so that an L2 holds few heads' keys; the XCDs of a run take its items in
+    // turn, so that each has as many of the long walks as the others. (One prompt of 16 heads on one key head: XCDs with an eighth
+    // each took as long as the one with the last rows.)
     const bool full = block < p.big_full;
-    const int at = full ? block : block - p.big_full;
-    int item = (at & 7) * (full ? p.big_full >> 3 : p.big_per_xcd) + (at >> 3), chunk = 0;
+    const int at = full ? block : block - p.big_full, of = full ? p.big_full : p.big_rest;
+    const int run = (of * p.xcds + 7) / 8, in_run = (at >> 3) * p.xcds + (at & (p.xcds - 1));
+    int item = (at & 7) / p.xcds * run + in_run, chunk = 0;
+    if (in_run >= run || item >= of) return true;
     if (!full) {
-        if (item >= p.big_rest) return true;
         chunk = item % p.big.chunks;
         item = p.big_full + item / p.big.chunks;
     }
     const int cut_tile = item - p.big_full;   // (where it is cut)
-    const int tile = p.big.tiles - 1 - item % p.big.tiles;
-    item /= p.big.tiles;
-    const int seq = item % p.b.seqs, kvh = item / p.b.seqs;
+    const int kvh = item / p.big_pieces.n;
+    const PagedPiece piece = paged_piece<kBigRows>(p.big_pieces, p.b, p.group, p.big_pieces.n - 1 - item % p.big_pieces.n);
+    const int seq = piece.seq, tile = piece.tile;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group, row0 = tile * kBigRows;
     if (row0 >= rows || rows <= p.few) return true;
@@ -969,11 +1004,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     constexpr int kPer = D / 4, kRows = 256 / (kPer * G);
     __shared__ float lds_top[kRows][G], lds_sum[kRows][G];
     __shared__ f32x4 lds_acc[kRows][G][kPer];
-    const int item = blockIdx.x / p.join_blocks, block = blockIdx.x - item * p.join_blocks;
-    const int seq = item / p.pool.kv_heads, kvh = item % p.pool.kv_heads;
+    const int kvh = blockIdx.x / p.join_pieces.n;
+    const PagedPiece piece = paged_piece<kRows>(p.join_pieces, p.b, p.group, blockIdx.x % p.join_pieces.n);
+    const int seq = piece.seq;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int slot = threadIdx.x / (kPer * G), gi = threadIdx.x / kPer % G, c = threadIdx.x % kPer;
-    const int rows = sq.count * p.group, r = block * kRows + slot;
+    const int rows = sq.count * p.group, r = piece.tile * kRows + slot;
     const int t = r / p.group;
     const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
     int chunks = 0;
@@ -982,12 +1018,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     if (r < rows) {
         if (few) {
             const int tile = r / p.rows_m, row0 = tile * p.rows_m;
-            if (tile < p.rows.tiles)
+            if (tile < p.rows_tiles)
                 chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + p.rows_m, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
         } else {
             const int row0 = r / kBigRows * kBigRows;
-            const int tile = r / kBigRows, at = (kvh * p.b.seqs + seq) * p.big.tiles + p.big.tiles - 1 - tile;   // (as paged_tiles_item counts)
-            if (tile < p.big.tiles && at >= p.big_full)
+            // (as paged_tiles_item counts)
+            const long number = paged_first_piece<kBigRows>(p.big_pieces, p.b, p.group, seq) + r / kBigRows;
+            const long at = (long)(kvh + 1) * p.big_pieces.n - 1 - number;
+            if (number < p.big_pieces.n && at >= p.big_full)
                 chunks = ((paged_walk<kPart>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + 3) / 4 + p.big.chunk - 1) / p.big.chunk;
             first = (size_t)(at - p.big_full) * kBigRows + (r - row0);
             step = (size_t)p.big_rows;
@@ -1064,13 +1102,19 @@ size_t walk_bound(size_t step, size_t rows, size_t group, size_t max_len, size_t
     return std::max<size_t>(steps, 1);
 }
 
+PagedPieces paged_pieces(size_t r, size_t seqs, size_t tokens, size_t max_q, size_t group) {
+    const size_t tiles = (max_q * group + r - 1) / r, like = seqs * tiles, ragged = (tokens * group + (r - 1) * seqs) / r;
+    const size_t most = INT_MAX;   // (past it no launch holds them)
+    return like <= ragged ? PagedPieces{(int)std::min(like, most), (int)std::min(tiles, most)} : PagedPieces{(int)std::min(ragged, most), 0};
+}
 // How a call is cut.
 struct PagedCut {
     size_t few = 0;                         // rows a key head up to which a sequence is paged_rows_kernel's
     size_t nt = 0;                          // its tiles of 16 rows; 0: not launched
     size_t rows_tiles = 1, rows_chunk = 1, rows_chunks = 1;
-    size_t big_tiles = 0, big_full = 0, big_chunk = 1, big_chunks = 1;   // of paged_tiles_kernel; no tiles: not launched
-    size_t chunks() const { return std::max(nt ? rows_chunks : 1, big_tiles ? big_chunks : 1); }
+    PagedPieces big = {0, 0};               // of paged_tiles_kernel, a key head; none: not launched
+    size_t big_full = 0, big_chunk = 1, big_chunks = 1;
+    size_t chunks() const { return std::max(nt ? rows_chunks : 1, big.n ? big_chunks : 1); }
 };
 // bf16: two tiles of 16 rows cost paged_rows_kernel a second pass over the keys' operands, or a second walk, and paged_tiles_kernel, which
 // pads to 128, streams the keys as fast (48 sessions of 5 drafts x 4 heads, a window of 2048: 86 us by rows, 77.5 by tiles; 16 x 8 x 5
@@ -1082,7 +1126,8 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
     PagedCut c;
     const size_t group = heads / kv_heads, rows = max_q * group, units = (size_t)fv_compute_units(), most_few = few_rows(four);
     if (rows > most_few) {
-        c.big_tiles = (rows + kBigRows - 1) / kBigRows;
+        const size_t tiles = (rows + kBigRows - 1) / kBigRows;   // (of the longest)
+        c.big = paged_pieces(kBigRows, seqs, tokens, max_q, group);
         const size_t steps = (walk_bound(kPart, kBigRows, group, max_len, block_tokens, window, sink) + 3) / 4;
         // Shares of the walk, by microseconds: rounds of as many workgroups as there is room for, 4 each besides their steps (1.05 and 1.75 a
         // step of one and of two workgroups a unit, or what the memory takes where few tiles share their keys), against a
@@ -1090,13 +1135,13 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         // their walk whole and only the rest are cut. (Tiles whose walks differ, causal or of ragged prompts, fill the
         // rounds by themselves: no count of rounds, and all or none are cut.) One frame of 1560 against 32760, 12 heads: in 1, 2, 3, 4
         // shares 538, 427, 293, 362 us.
-        const size_t items = seqs * kv_heads * c.big_tiles, held = kv_heads * std::min(seqs * c.big_tiles, tokens * group / kBigRows + seqs);
+        const size_t items = seqs * kv_heads * tiles, held = kv_heads * (size_t)c.big.n;
         const size_t slots = (d == 64 ? 3 : 2) * units / 8 * 8;
         const bool varied = 10 * held < 9 * items || (window == 0 && 4 * block_tokens < max_q && 2 * max_q > max_len);
         auto step_us = [&](size_t wgs) {
             const size_t at_once = std::min(wgs, slots);
             const double bytes = 64.0 * (double)(four ? d + d / 16 : 4 * d);
-            return std::max((at_once <= units ? 1.05 : 1.75) * (d == 64 ? 0.75 : 1.0), (double)at_once / (double)c.big_tiles * bytes / (at_once <= units ? 4.3e6 : 5.2e6));
+            return std::max((at_once <= units ? 1.05 : 1.75) * (d == 64 ? 0.75 : 1.0), (double)at_once / (double)tiles * bytes / (at_once <= units ? 4.3e6 : 5.2e6));
         };
         double best = 0;
         const size_t rounds_before = varied ? 0 : held / slots;
@@ -1114,10 +1159,10 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         }
         if (c.big_chunks == 1) c.big_full = 0;
     }
-    // (Sequences of few rows beside longer ones: a launch of their own where they may be many, by the mean; else they are the tiles', which
-    // take any, and the launch, 5 us, is saved.)
+    // (Sequences of few rows beside longer ones: a launch of their own where they may be many, by the mean, and then for those of one
+    // tile of rows; else they are the tiles', which take any, and the launch, 5 us, is saved.)
     if (rows <= most_few || 2 * tokens < seqs * max_q) {
-        const size_t most = std::min(rows, most_few);
+        const size_t most = rows <= most_few ? rows : 16;
         c.few = most;
         c.nt = most <= 16 ? 1 : 2;
         c.rows_tiles = (most + 16 * c.nt - 1) / (16 * c.nt);
@@ -1139,15 +1184,15 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
 // The shares' places in the workspace.
 struct PagedParts {
     size_t rows_o = 0, rows_lse = 0, big_o = 0, big_lse = 0, big_rows = 0, bytes = 0;   // rows_o ..: bytes from its start
-    PagedParts(const PagedCut& c, size_t tokens, size_t heads, size_t kv_heads, size_t d, size_t seqs) {
+    PagedParts(const PagedCut& c, size_t tokens, size_t heads, size_t kv_heads, size_t d) {
         auto take = [this](size_t n) {
             const size_t at = bytes;
             bytes += (n + 255) / 256 * 256;
             return at;
         };
         if (c.nt && c.rows_chunks > 1) rows_o = take(c.rows_chunks * tokens * heads * d * 4), rows_lse = take(c.rows_chunks * tokens * heads * 4);
-        if (c.big_tiles && c.big_chunks > 1) {
-            big_rows = (seqs * kv_heads * c.big_tiles - c.big_full) * kBigRows;
+        if (c.big.n && c.big_chunks > 1) {
+            big_rows = (kv_heads * (size_t)c.big.n - c.big_full) * kBigRows;
             big_o = take(c.big_chunks * big_rows * d * 4), big_lse = take(c.big_chunks * big_rows * 4);
         }
     }
@@ -1164,7 +1209,7 @@ size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t 
     size_t most = 0;   // of both kinds of pages
     for (const bool four : {false, true}) {
         const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
-        most = std::max(most, fv::PagedParts(c, tokens, heads, kv_heads, d, seqs).bytes);
+        most = std::max(most, fv::PagedParts(c, tokens, heads, kv_heads, d).bytes);
     }
     return most;
 }
@@ -1192,44 +1237,47 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     if (max_q > tokens) max_q = tokens;
     const bool four = k_scales != nullptr;
     fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, max_q, max_len, block_tokens, window, sink);
-    fv::PagedParts parts(c, tokens, heads, kv_heads, d, seqs);
+    fv::PagedParts parts(c, tokens, heads, kv_heads, d);
     if (parts.bytes > 0 && (!workspace || workspace_bytes < parts.bytes)) {   // a share is the whole walk
         c.rows_chunk *= c.rows_chunks, c.big_chunk *= c.big_chunks;
         c.rows_chunks = c.big_chunks = 1, c.big_full = 0;
-        parts = fv::PagedParts(c, tokens, heads, kv_heads, d, seqs);
+        parts = fv::PagedParts(c, tokens, heads, kv_heads, d);
         workspace = nullptr;
     }
     const bool split = c.chunks() > 1;
     if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
-    const bool many = (c.big_tiles ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
-    const size_t join_blocks = (max_q * (heads / kv_heads) * (d / 4) * (many ? 8 : 1) + 255) / 256, join = seqs * kv_heads * join_blocks;
-    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (seqs * kv_heads * c.big_tiles - c.big_full) * c.big_chunks;
+    const bool many = (c.big_chunks > 1 ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
+    const size_t group = heads / kv_heads, xcds = 8 / std::gcd(kv_heads, (size_t)8);
+    // (rows a workgroup of the join; where paged_tiles_kernel cuts nothing, of the sequences of few rows)
+    const size_t join_rows = 256 / (d / 4 * (many ? 8 : 1)), join_few = (c.few + join_rows - 1) / join_rows;
+    const fv::PagedPieces join = c.big.n && c.big_chunks == 1 ? fv::PagedPieces{(int)(seqs * join_few), (int)join_few}
+                                                              : fv::paged_pieces(join_rows, seqs, tokens, max_q, group);
+    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (kv_heads * (size_t)c.big.n - c.big_full) * c.big_chunks;
+    const size_t big_blocks = c.big_full + 8 * (((big_rest * xcds + 7) / 8 + xcds - 1) / xcds), join_blocks = kv_heads * (size_t)join.n;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
-    if (row_blocks >= kMost || c.big_full + big_rest + 8 >= kMost || (split && join >= kMost))
-        return fv_decline("paged attention: too large for one launch");
+    if (row_blocks >= kMost || big_blocks >= kMost || (split && join_blocks >= kMost)) return fv_decline("paged attention: too large for one launch");
     p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
-    p.heads = (int)heads, p.group = (int)(heads / kv_heads);
+    p.heads = (int)heads, p.group = (int)group;
     p.sl2 = (float)((double)scale * 1.4426950408889634);
     p.block_tokens = (int)block_tokens, p.window = (int)window, p.sink = (int)sink;
     p.few = (int)c.few, p.rows_m = (int)(16 * c.nt);
-    p.rows = {(int)c.rows_tiles, (int)c.rows_chunk, (int)c.rows_chunks};
-    p.big = {(int)c.big_tiles, (int)c.big_chunk, (int)c.big_chunks};
-    p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.big_per_xcd = (int)((big_rest + 7) / 8);
+    p.rows_tiles = (int)c.rows_tiles, p.rows = {(int)c.rows_chunk, (int)c.rows_chunks};
+    p.big = {(int)c.big_chunk, (int)c.big_chunks}, p.big_pieces = c.big, p.join_pieces = join;
+    p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.xcds = (int)xcds;
     uint8_t* ws = (uint8_t*)workspace;
     p.rows_o = (float*)(ws + parts.rows_o), p.rows_lse = (float*)(ws + parts.rows_lse);
     p.big_o = (float*)(ws + parts.big_o), p.big_lse = (float*)(ws + parts.big_lse), p.big_rows = (long)parts.big_rows;
-    p.join_blocks = (int)join_blocks;
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(d == 128, [&](auto d128) {
         fv::paged_pick(four, [&](auto f) {
             constexpr int D = d128() ? 128 : 64;
-            if (c.big_tiles)
-                hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3(p.big_full + 8 * p.big_per_xcd), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
+            if (c.big.n)
+                hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3((unsigned)big_blocks), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
             if (c.nt == 1) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 1>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if constexpr (f())   // (the only pages whose calls have two tiles of rows, few_rows)
                 if (c.nt == 2) hipLaunchKernelGGL((fv::paged_rows_kernel<D, true, 2>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if (split)
-                fv::paged_pick(many, [&](auto m) { hipLaunchKernelGGL((fv::paged_join_kernel<D, m() ? 8 : 1>), dim3((unsigned)join), dim3(256), 0, st, p); });
+                fv::paged_pick(many, [&](auto m) { hipLaunchKernelGGL((fv::paged_join_kernel<D, m() ? 8 : 1>), dim3((unsigned)join_blocks), dim3(256), 0, st, p); });
         });
     });
     const hipError_t e = hipGetLastError();
