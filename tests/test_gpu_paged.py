@@ -431,3 +431,23 @@ def test_calls_of_more_than_a_round(fv, four, heads, kvh, d, rows, length, block
         off = float(((got[:, h].double() - out).abs() - bound).max())
         assert off <= 0, (h, off)
     print(f"[paged] {heads}/{kvh} d={d}: workspace {need} bytes", flush=True)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("seqs,heads,kvh,d,window,long", [
+    (2, 10, 2, 128, 0, (300,)), (64, 5, 1, 128, 0, (90, 700)), (65, 12, 12, 64, 50, (130,)), (200, 16, 1, 64, 0, (257, 64)),
+    (33, 24, 3, 128, 0, (40,)), (4200, 5, 1, 64, 33, (1000, 128))])
+def test_long_and_short_sequences_of_a_batch(fv, four, seqs, heads, kvh, d, window, long):
+    """Sequences of no row, of one, of a few and of many, in any order, few of them long; the longest by itself says how much a
+    sequence may have."""
+    announce(f"paged: long and short four={four} {seqs} sequences {heads}/{kvh} d={d}")
+    rng = np.random.Generator(np.random.PCG64(seqs))
+    counts = rng.choice([0, 1, 1, 1, 2, 7], seqs)
+    counts[rng.permutation(seqs)[:len(long)]] = long
+    lens = counts + rng.integers(0, 90, seqs)
+    if seqs in (33, 65):                         # (a walk that is cut)
+        lens[counts.argmax()] += 9000
+    w = World(fv, 700 + seqs, lens.tolist(), counts.tolist(), kvh, d, 16, four, fill="nan" if seqs < 1000 else "normal")
+    q = w.queries(heads, 1.5)
+    got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(1, window, 3 if window else 0), out_bf16=False)
+    w.check(q, got, f"{seqs} sequences four={four}", 1, window, 3 if window else 0)
