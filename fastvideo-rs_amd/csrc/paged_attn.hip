@@ -838,7 +838,7 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) {
             const bool none = 4 * e + kb >= w.n || !((ok >> kb) & 1);
-            const int at = (none ? 0x40000000 : w.key(4 * e + kb)) + 4 * q4;
+            const int at = (none ? 0x7fffff00 : w.key(4 * e + kb)) + 4 * q4;   // (past every key: a table holds fewer than 2^31)
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 const unsigned bits = below(both[0][g] - at) | (below(both[2][g] - at) & ~below(both[1][g] - at));

@@ -360,7 +360,7 @@ int fv_kv_cache_update(fv_kv_cache* c, size_t layer, const fv_tensor* k, const f
  * q_start[s] .. q_start[s + 1] (ascending, q_start[0] is the first row's number) of the ragged tensors [tokens, heads, d]: the last
  * tokens of the sequence, in order. Token j lies in slot j % page_tokens of page table[s * table_stride + j / page_tokens],
  * of table_pages columns. Entries of pages that a call does not reach are not read; sequences may share pages that none of
- * them appends to (two tokens of one call in one slot: either is kept). A page number outside the pool is no fault: nothing is
+ * them appends to (two tokens of one call in one slot leave a mixture of both). A page number outside the pool is no fault: nothing is
  * written there, it reads as zeros, and its keys are seen by no query. Rows at q_start[seqs] and behind are left as they were, so
  * a padded batch may be captured into a graph and replayed with other lengths, tables and counts. The arrays are read when the
  * call's work runs.
@@ -380,8 +380,8 @@ int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stri
                     size_t pages, size_t page_tokens, size_t kv_heads, size_t d, const int32_t* q_start, const int32_t* lens,
                     const int32_t* table, size_t table_stride, size_t table_pages, size_t seqs, size_t tokens, void* stream);
 /* The batch's tokens out of the cache: k_out, v_out [tokens, kv_heads, d], contiguous, f32 or bf16 bits (both exact; a
- * 4-bit value of 2^128 or more is infinite). With
- * q_start the running sums of lens, whole sequences (a contiguous copy for the dense entries, for keeping elsewhere). */
+ * 4-bit value of 2^128 or more is infinite). With q_start the running sums of lens, whole sequences (a contiguous copy for the dense
+ * entries, for keeping elsewhere). */
 int fv_paged_read(void* k_out, void* v_out, int out_is_bf16, const void* k_pages, const void* v_pages, const void* k_scales,
                   const void* v_scales, size_t pages, size_t page_tokens, size_t kv_heads, size_t d, const int32_t* q_start,
                   const int32_t* lens, const int32_t* table, size_t table_stride, size_t table_pages, size_t seqs,

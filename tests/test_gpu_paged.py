@@ -218,6 +218,23 @@ def test_4_bit_blocks_of_every_kind(fv):
         assert np.array_equal(back, want, equal_nan=True), name
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_every_4_bit_value_reads_as_what_it_stands_for(fv, d):
+    """All codes under all 256 scales (f32 and bf16 hold every one of them, subnormal ones too, up to 2^128)."""
+    announce(f"paged read: every 4-bit value d={d}")
+    w = World(fv, 4, [256], [256], 1, d, 16, four=True)
+    p, t = w.table[0, np.arange(256) // 16], np.arange(256) % 16
+    for n, both in (("k", 0x10), ("v", 0x01)):
+        w.host[n][p, 0, t] = (np.arange(d // 2) % 16 * both + 7 * (0x11 - both)).astype(np.uint8)
+        w.scales[n][p, 0, t] = (np.arange(256)[:, None] + np.arange(d // 32)) % 256
+    w.push()
+    with np.errstate(over="ignore"):
+        want = [w.held(n, 0).astype(np.float32) for n in "kv"]
+    for out16 in (False, True):
+        for x, y in zip(fv.paged_read(w.pool, w.batch, 256, out_bf16=out16), want):
+            assert np.array_equal(x.float().cpu().numpy(), y, equal_nan=True), out16
+
+
 def test_tokens_that_lie_nowhere_are_left_out(fv):
     """Page numbers outside the pool, table rows outside the tables, more rows than tokens: the others are as always, the
     pool's other slots keep their bits, queries without a place are zeros."""
