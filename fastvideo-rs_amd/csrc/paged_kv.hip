@@ -55,21 +55,30 @@ FV_DEV PagedPlace paged_place(const PagedBatch& b, const PagedPool& pool, int t)
     return {pos, (unsigned)page < (unsigned)pool.pages ? page : -1, pos & ((1 << pool.lg) - 1)};
 }
 
+// Eight values as they stand in memory, and as f32.
 template <bool IN16>
-FV_DEV void load8(const void* x, size_t at, float (&v)[8]) {
-    if constexpr (IN16) {
-        const u32x4 t = *reinterpret_cast<const u32x4*>((const uint16_t*)x + at);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = __builtin_bit_cast(float, t[i] << 16);
-            v[2 * i + 1] = __builtin_bit_cast(float, t[i] & 0xffff0000u);
-        }
-    } else {
-        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)x + at), b = *reinterpret_cast<const f32x4*>((const float*)x + at + 4);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+struct Eight {
+    u32x4 w[IN16 ? 1 : 2];
+    FV_DEV void load(const void* x, size_t at) {
+        const u32x4* p = reinterpret_cast<const u32x4*>((const uint8_t*)x + at * (IN16 ? 2 : 4));
+        w[0] = p[0];
+        if constexpr (!IN16) w[1] = p[1];
     }
-}
+    FV_DEV void get(float (&v)[8]) const {
+        if constexpr (IN16) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[2 * i] = __builtin_bit_cast(float, w[0][i] << 16);
+                v[2 * i + 1] = __builtin_bit_cast(float, w[0][i] & 0xffff0000u);
+            }
+        } else {
+            // (not [i / 4][i % 4]: in one loop of eight the compiler took element 0 for 2 and 1 for 3)
+            const f32x4 lo = __builtin_bit_cast(f32x4, w[0]), hi = __builtin_bit_cast(f32x4, w[1]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = lo[i], v[4 + i] = hi[i];
+        }
+    }
+};
 FV_DEV u32x4 to_bf16x8(const float (&r)[8]) {
     f32x8 f;
 #pragma unroll
@@ -77,29 +86,31 @@ FV_DEV u32x4 to_bf16x8(const float (&r)[8]) {
     return __builtin_bit_cast(u32x4, __builtin_convertvector(f, bf16x8));
 }
 
-// Channels [8 c, 8 c + 8) of a head, turned by row `row` of the tables, f32 with unfused products (the rounding of the
-// plain formula, so that the value to be stored is the same number whoever computes it).
+// The piece of eight channels that piece c of a head is turned with: its own, or (halves) that half a head away.
+template <int D, bool HALVES>
+FV_DEV int partner(int c) { return HALVES ? c ^ (D / 16) : c; }
+// Piece `v` (the c-th) of a head and its partner `w`, turned by row `row` of the tables, f32 with unfused products (the rounding of
+// the plain formula, so that the value to be stored is the same number whoever computes it).
 template <bool IN16, int D, bool HALVES>
-FV_DEV void load_turned(const void* x, size_t head_at, int c, const float* cos_t, const float* sin_t, int row, float (&r)[8]) {
+FV_DEV void turn8(const Eight<IN16>& own, const Eight<IN16>& other, int c, const float* cos_t, const float* sin_t, int row, float (&r)[8]) {
 #pragma clang fp contract(off)
-    float v[8], cs[8], sn[8];
-    load8<IN16>(x, head_at + 8 * c, v);
+    const bool upper = HALVES && c >= D / 16;
+    const size_t slot = (size_t)row * D + 8 * (upper ? c - D / 16 : c);
+    Eight<false> ct, st;
+    ct.load(cos_t, slot);
+    st.load(sin_t, slot);
+    float v[8], w[8], cs[8], sn[8];
+    own.get(v);
+    ct.get(cs);
+    st.get(sn);
     if constexpr (HALVES) {   // pairs (i, i + D / 2), the angle in slot i
-        constexpr int kHalf = D / 16;
-        const bool upper = c >= kHalf;
-        const int slot = upper ? c - kHalf : c;
-        float w[8];
-        load8<IN16>(x, head_at + 8 * (upper ? slot : c + kHalf), w);
-        load8<false>(cos_t, (size_t)row * D + 8 * slot, cs);
-        load8<false>(sin_t, (size_t)row * D + 8 * slot, sn);
+        other.get(w);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float x1 = upper ? w[i] : v[i], x2 = upper ? v[i] : w[i];
             r[i] = upper ? x1 * sn[i] + x2 * cs[i] : x1 * cs[i] - x2 * sn[i];
         }
     } else {                  // pairs (2 i, 2 i + 1), the angle in slot 2 i
-        load8<false>(cos_t, (size_t)row * D + 8 * c, cs);
-        load8<false>(sin_t, (size_t)row * D + 8 * c, sn);
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             r[i] = v[i] * cs[i] - v[i + 1] * sn[i];
@@ -137,7 +148,7 @@ FV_DEV unsigned to_fp4x8(const float (&r)[8], unsigned& scale_byte) {
 
 // Block (x, y): pieces [256 y, 256 y + 256) of token x: the query heads' first (if any), then the key heads', then the value
 // heads'. 20011 tokens of 40 / 8 heads, their tables and queries: 1.42 GB in 271 us, 5.2 TB/s (a large copy: 4.9); 4680 of 12 heads
-// to 4 bits: 0.21 GB in 49 us, 4.2 TB/s.
+// to 4 bits: 0.21 GB in 46 us, 4.5 TB/s.
 template <bool IN16, int D, bool FOUR, bool HALVES>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p) {
     constexpr int kPer = D / 8;
@@ -145,30 +156,25 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p)
     const int head = piece / kPer, c = piece % kPer, nq = p.q ? p.heads : 0, kvh = p.pool.kv_heads;
     if (head >= nq + 2 * kvh) return;
     const int t = blockIdx.x;
-    if (t >= p.b.tokens || t >= p.b.q_start[p.b.seqs]) return;
-    if (t < p.b.q_start[0]) return;
+    const bool is_q = head < nq, turn = p.cos_t != nullptr && head < nq + kvh;
+    // the values first, which wait for nothing; where they go takes four or more loads in a row
+    const void* x = is_q ? p.q : head < nq + kvh ? p.k : p.v;
+    const size_t from = (size_t)t * (is_q ? p.q_stride : head < nq + kvh ? p.k_stride : p.v_stride) + (is_q ? head : (head - nq) % kvh) * D;
+    Eight<IN16> own, other;
+    own.load(x, from + 8 * c);
+    if (HALVES && turn) other.load(x, from + 8 * partner<D, HALVES>(c));
+    if (t < p.b.q_start[0] || t >= p.b.q_start[p.b.seqs]) return;   // of no sequence
     const PagedPlace at = paged_place(p.b, p.pool, t);
     const int row = p.rope_at ? p.rope_at[t] : at.pos;
-    const bool turn = p.cos_t != nullptr;
-    const bool ok = at.pos >= 0 && (!turn || (unsigned)row < (unsigned)p.rope_rows);
+    const bool ok = at.pos >= 0 && (!p.cos_t || (unsigned)row < (unsigned)p.rope_rows);
     float r[8];
-    if (!ok || (head >= nq && at.page < 0)) {   // lies nowhere: nothing is stored, a query is zeros
-        if (head < nq) *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = u32x4{0u, 0u, 0u, 0u};
+    if (ok && turn) turn8<IN16, D, HALVES>(own, other, c, p.cos_t, p.sin_t, row, r);
+    else own.get(r);
+    if (is_q) {   // (one that lies nowhere is zeros)
+        *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = ok ? to_bf16x8(r) : u32x4{0u, 0u, 0u, 0u};
         return;
     }
-    if (head < nq + kvh) {
-        const bool is_q = head < nq;
-        const void* x = is_q ? p.q : p.k;
-        const size_t from = is_q ? (size_t)t * p.q_stride + head * D : (size_t)t * p.k_stride + (head - nq) * D;
-        if (turn) load_turned<IN16, D, HALVES>(x, from, c, p.cos_t, p.sin_t, row, r);
-        else load8<IN16>(x, from + 8 * c, r);
-        if (is_q) {
-            *reinterpret_cast<u32x4*>(p.q_out + ((size_t)t * p.heads + head) * D + 8 * c) = to_bf16x8(r);
-            return;
-        }
-    } else {
-        load8<IN16>(p.v, (size_t)t * p.v_stride + (head - nq - kvh) * D + 8 * c, r);
-    }
+    if (!ok || at.page < 0) return;
     const bool is_v = head >= nq + kvh;
     const size_t at_row = (((size_t)at.page * kvh + (head - nq - (is_v ? kvh : 0))) << p.pool.lg) + at.slot;
     uint8_t* base = (uint8_t*)(is_v ? p.pool.v : p.pool.k);
