@@ -147,8 +147,8 @@ FV_DEV unsigned to_fp4x8(const float (&r)[8], unsigned& scale_byte) {
 }
 
 // Block (x, y): pieces [256 y, 256 y + 256) of token x: the query heads' first (if any), then the key heads', then the value
-// heads'. 20011 tokens of 40 / 8 heads, their tables and queries: 1.42 GB in 271 us, 5.2 TB/s (a large copy: 4.9); 4680 of 12 heads
-// to 4 bits: 0.21 GB in 46 us, 4.5 TB/s.
+// heads'. 20011 tokens of 40 / 8 heads, their tables and queries: 1.42 GB in 265 us, 5.4 TB/s (a large copy: 4.9; 299 with the values
+// loaded behind the look-ups); 4680 of 12 heads to 4 bits: 0.21 GB in 46 us, 4.5 TB/s.
 template <bool IN16, int D, bool FOUR, bool HALVES>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p) {
     constexpr int kPer = D / 8;
