@@ -263,9 +263,9 @@ FV_DEV void pool_values(const Pool& pool, unsigned row, int c, float (&v)[N]) {
 
 // One workgroup: a share of the walk of a tile of 16 NT rows of one (sequence, key head); its four waves take the share's
 // steps in turn, each with a running maximum of its own, and join through LDS. A step reads its keys and values once, for all of
-// the tile's rows, straight into registers in the order of the matrix operands, so that nothing but the memory bounds it: 128
-// single tokens of 40 / 8 heads over 1.24 GB of bf16 pages 240 us, 5.15 TB/s; 40 of 64 / 8 heads over 0.85 GB of 4 bits 176 us, 4.8. Calls
-// too short for that are bound by their few waits in a row: 16 tokens over 300 keys 9.5 us.
+// the tile's rows, straight into registers in the order of the matrix operands, so that nothing but the memory bounds it: 64
+// single tokens of 40 / 8 heads over 1.24 GB of bf16 pages 237 us, 5.2 TB/s; 40 such over 0.85 GB of 4 bits 173 us, 4.9. Calls too
+// short for that are bound by their few waits in a row: 4 tokens of 24 heads over up to 777 keys of 64 channels 9.2 us.
 // One tile of rows: a whole step is loaded ahead. Two (4-bit pages, few_rows): the keys of the next step go into the registers of
 // this one's as soon as their scores are there, its values likewise; a whole step ahead spilled 270 bytes a lane.
 template <int D, bool FOUR, int NT>
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
 constexpr int kBigRows = 128, kPart = 16;   // keys that a wave brings of a tile
 // The softmax's vector work, about two thirds of a phase's matrix time, and the matrix work bound it together, and only in part
 // overlap between a unit's two workgroups: one frame of 1560 rows x 12 heads against 32760 293 us, 1.07 PFLOP/s of the large product's
-// 1.35, the matrix cores busy 60 % of the time while all units have work; three over 4 bits 1.51 ms, 1.25. (Tried and slower: 8 waves in
+// 1.35, the matrix cores busy 60 % of the time while all units have work; three frames of two sequences over 4 bits 1.51 ms, 1.25. (Tried and slower: 8 waves in
 // two groups that take turns, 333 us; priority to the softmax, 336; priority by the wave's slot, 331.)
 // FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop:
 // 8 % of one frame against 21, 9 % of three over 4 bits, 7 % of prompts under a window). Exact as long as nothing overflows or
@@ -997,8 +997,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const
 
 // The shares of a split walk joined: out = sum_c w_c O_c / sum_c w_c, w_c = 2^(lse_c - max lse). G groups of D / 4 threads share a
 // row's shares out, four at a time each, with a running maximum, and meet in LDS; rows whose walk one workgroup made have
-// their result already. A row with many shares is a chain of waits, so G = 8 then (64 shares of one token's 64 heads: 5 us; with G = 1
-// 17); few shares are the memory's to bound, and G = 1 keeps them out of LDS.
+// their result already. A row with many shares is a chain of waits, so G = 8 then (61 shares of one token's 40 heads: 4.0
+// us); few shares are the memory's to bound, and G = 1 keeps them out of LDS (three of 1560 rows x 12 heads: 8.5 us).
 template <int D, int G>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
     constexpr int kPer = D / 4, kRows = 256 / (kPer * G);

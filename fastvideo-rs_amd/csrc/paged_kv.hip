@@ -147,8 +147,8 @@ FV_DEV unsigned to_fp4x8(const float (&r)[8], unsigned& scale_byte) {
 }
 
 // Block (x, y): pieces [256 y, 256 y + 256) of token x: the query heads' first (if any), then the key heads', then the value
-// heads'. 20011 tokens of 40 / 8 heads, their tables and queries: 1.42 GB in 265 us, 5.4 TB/s (a large copy: 4.9; 299 with the values
-// loaded behind the look-ups); 4680 of 12 heads to 4 bits: 0.21 GB in 46 us, 4.5 TB/s.
+// heads'. 56637 tokens of 32 / 8 heads in 24 prompts, their tables and queries: 1.42 GB in 265 us, 5.4 TB/s (a large copy: 4.9; 299 with
+// the values loaded behind the look-ups); 9360 of 12 heads from f32 to 4 bits: 0.14 GB in 28 us, 5.0 TB/s. 32 single tokens: 3.1 us.
 template <bool IN16, int D, bool FOUR, bool HALVES>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p) {
     constexpr int kPer = D / 8;
@@ -188,7 +188,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p)
     }
 }
 
-// The same walk the other way: k_out, v_out [tokens, kv_heads, d], f32 or bf16 (both exact); rows that lie nowhere are zeros.
+// The same walk the other way: k_out, v_out [tokens, kv_heads, d], f32 or bf16 (both exact); rows that lie nowhere are zeros. 9360
+// tokens of 12 heads from 4 bits to bf16: 73 MB in 16.7 us, 4.4 TB/s.
 template <bool OUT16, int D, bool FOUR>
 __global__ __launch_bounds__(256) void paged_read_kernel(const PagedPool pool, const PagedBatch b, void* __restrict__ k_out, void* __restrict__ v_out) {
     constexpr int kPer = D / 8;
