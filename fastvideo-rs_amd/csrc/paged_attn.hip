@@ -3,7 +3,8 @@
 // window of blocks or among the sink blocks.
 //
 // Rows of one key head lie together (token by token, the heads of its group in turn), so a step over 32 keys serves all of
-// them with one load of K and V.
+// them with one load of K and V. Scores, offsets, sums and O are f32; the probabilities are rounded to bf16 for the second product (each
+// off by 2^-9 of itself at most, as much as a result in bf16 is), 4-bit keys and values become bf16 exactly.
 #include <limits.h>
 
 #include <algorithm>
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
                 e[j] = fast_exp2(x[n][j >> 2][j & 3] * p.sl2);
                 l[n] += e[j];
             }
-            pr[n] = __builtin_convertvector(e, bf16x8);
+            pr[n] = __builtin_convertvector(e, bf16x8);   // (the second product's operand; the sum keeps all of f32)
         }
     };
     auto add_values = [&](const PagedStage<D, FOUR>& s, const bf16x8 (&pr)[NT], int k0, unsigned good, unsigned row_a, unsigned row_b) {
