@@ -4,7 +4,7 @@
 //
 // Rows of one key head lie together (token by token, the heads of its group in turn), so a step over 32 keys serves all of
 // them with one load of K and V. Scores, offsets, sums and O are f32; the probabilities are rounded to bf16 for the second product (each
-// off by 2^-9 of itself at most, as much as a result in bf16 is), 4-bit keys and values become bf16 exactly.
+// off by 2^-8 of itself at most, as much as a result in bf16 is), 4-bit keys and values become bf16 exactly.
 #include <limits.h>
 
 #include <algorithm>

@@ -11,13 +11,14 @@ from . import _lib
 __all__ = ["PagedKv", "PagedBatch", "paged_append", "paged_read", "paged_attention"]
 
 _BF16, _F32, _U8, _I32 = torch.bfloat16, torch.float32, torch.uint8, torch.int32
+_ONLY_BF16 = (_BF16,)
 
 
 class PagedKv:
     """One layer's pool: k, v [pages, kv_heads, page_tokens, d] bf16, or 4-bit codes [.., d / 2] with k_scales, v_scales
     [.., d / 32] (uint8 all four). The tensors are the caller's, used in place."""
 
-    __slots__ = ("k", "v", "k_scales", "v_scales", "d", "_args")
+    __slots__ = ("k", "v", "k_scales", "v_scales", "d", "kv_heads", "_args", "_device")
 
     def __init__(self, k, v, k_scales=None, v_scales=None):
         four = k_scales is not None
@@ -29,11 +30,11 @@ class PagedKv:
             raise ValueError(f"PagedKv: want contiguous CUDA tensors of {dtype} on one device")
         d = shape[3] * 2 if four else shape[3]
         if four:
-            want = (*shape[:3], d // 32)
+            want = (shape[0], shape[1], shape[2], d // 32)
             for t in (k_scales, v_scales):
-                if t.dtype is not _U8 or tuple(t.shape) != want or not t.is_contiguous() or t.get_device() != dev:
+                if t.dtype is not _U8 or t.shape != want or not t.is_contiguous() or t.get_device() != dev:
                     raise ValueError(f"PagedKv: want contiguous uint8 scales {want} on the pages' device")
-        self.k, self.v, self.k_scales, self.v_scales, self.d = k, v, k_scales, v_scales, d
+        self.k, self.v, self.k_scales, self.v_scales, self.d, self.kv_heads, self._device = k, v, k_scales, v_scales, d, shape[1], dev
         self._args = (k.data_ptr(), v.data_ptr(), k_scales.data_ptr() if four else None, v_scales.data_ptr() if four else None,
                       shape[0], shape[2], shape[1], d)
 
@@ -52,10 +53,6 @@ class PagedKv:
     @property
     def page_tokens(self):
         return self.k.shape[2]
-
-    @property
-    def kv_heads(self):
-        return self.k.shape[1]
 
 
 class PagedBatch:
@@ -83,16 +80,19 @@ class PagedBatch:
 
 
 def _rows(t, name, heads, d, dtypes, device):
-    """Elements between the tokens of t [tokens, heads, d], whose heads are contiguous."""
-    if t.dim() != 3 or t.dtype not in dtypes or t.get_device() != device:
+    """(heads, elements between the tokens) of t [tokens, heads, d], whose heads are contiguous."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype not in dtypes or t.get_device() != device:
         raise ValueError(f"{name}: want a [tokens, heads, d] tensor of {' or '.join(str(x) for x in dtypes)} on the pool's device")
-    n, h, dd = t.shape
+    n, h, dd = shape
     if (heads and h != heads) or dd != d:
-        raise ValueError(f"{name}: want [tokens, {heads or 'heads'}, {d}], got {tuple(t.shape)}")
+        raise ValueError(f"{name}: want [tokens, {heads or 'heads'}, {d}], got {tuple(shape)}")
+    if t.is_contiguous():
+        return h, h * d
     a, b, c = t.stride()
     if c != 1 or (h > 1 and b != d):
         raise ValueError(f"{name}: the heads of a token must be contiguous")
-    return a if n > 1 else h * d
+    return h, a if n > 1 else h * d
 
 
 def _on(device, name):
@@ -104,19 +104,19 @@ def paged_append(pool, batch, k, v, rope=None, halves=False, rope_at=None, q=Non
     """The new tokens' k, v [tokens, kv_heads, d] (f32 or bf16) into the pool, the keys turned by their positions (rows of
     rope = (cos, sin), f32 [rows, d]; rope_at: int32 [tokens], rows in place of the positions). q [tokens, heads, d]: turned
     likewise and returned, bf16. halves: pairs (i, i + d / 2) instead of (2i, 2i + 1)."""
-    dev, kvh, d = pool.k.get_device(), pool.kv_heads, pool.d
+    dev, kvh, d = pool._device, pool.kv_heads, pool.d
     _on(dev, "paged_append")
-    tokens = k.shape[0]
-    dtypes = (k.dtype,) if k.dtype in (_F32, _BF16) else (_F32, _BF16)
-    ks, vs = _rows(k, "k", kvh, d, dtypes, dev), _rows(v, "v", kvh, d, dtypes, dev)
+    tokens, dtype = k.shape[0], k.dtype
+    dtypes = (dtype,) if dtype is _BF16 or dtype is _F32 else (_F32, _BF16)
+    ks, vs = _rows(k, "k", kvh, d, dtypes, dev)[1], _rows(v, "v", kvh, d, dtypes, dev)[1]
     if v.shape[0] != tokens or batch._device != dev:
         raise ValueError("paged_append: k and v differ in tokens, or the batch is on another device")
     qs, heads, q_out = 0, 0, None
     if q is not None:
-        qs, heads = _rows(q, "q", 0, d, dtypes, dev), q.shape[1]
+        heads, qs = _rows(q, "q", 0, d, dtypes, dev)
         if q.shape[0] != tokens:
             raise ValueError("paged_append: q and k differ in tokens")
-        q_out = torch.empty_like(q) if q.dtype is _BF16 and q.is_contiguous() else torch.empty((tokens, heads, d), device=q.device, dtype=_BF16)
+        q_out = torch.empty_like(q) if dtype is _BF16 and q.is_contiguous() else torch.empty((tokens, heads, d), device=q.device, dtype=_BF16)
     cos = sin = None
     rows = 0
     if rope is not None:
@@ -131,18 +131,19 @@ def paged_append(pool, batch, k, v, rope=None, halves=False, rope_at=None, q=Non
         raise ValueError("paged_append: rope_at without tables")
     _lib.check(_lib.lib().fv_paged_append(
         k.data_ptr(), ks, v.data_ptr(), vs, q.data_ptr() if q is not None else None, qs, q_out.data_ptr() if q is not None else None,
-        1 if k.dtype is _BF16 else 0, heads, cos.data_ptr() if rows else None, sin.data_ptr() if rows else None, rows,
+        1 if dtype is _BF16 else 0, heads, cos.data_ptr() if rows else None, sin.data_ptr() if rows else None, rows,
         rope_at.data_ptr() if rope_at is not None else None, 1 if halves else 0, *pool._args, *batch._args, tokens, _lib.stream()))
     return q_out
 
 
 def paged_read(pool, batch, tokens, out_bf16=True):
     """(k, v) [tokens, kv_heads, d] of the batch's tokens; rows behind the last sequence are not written."""
-    dev = pool.k.get_device()
+    dev = pool._device
     _on(dev, "paged_read")
     if batch._device != dev:
         raise ValueError("paged_read: the batch is on another device")
-    k, v = (torch.empty((tokens, pool.kv_heads, pool.d), device=pool.k.device, dtype=_BF16 if out_bf16 else _F32) for _ in range(2))
+    k = torch.empty((tokens, pool.kv_heads, pool.d), device=pool.k.device, dtype=_BF16 if out_bf16 else _F32)
+    v = torch.empty_like(k)
     _lib.check(_lib.lib().fv_paged_read(k.data_ptr(), v.data_ptr(), 1 if out_bf16 else 0, *pool._args, *batch._args, tokens, _lib.stream()))
     return k, v
 
@@ -151,12 +152,12 @@ def paged_attention(q, pool, batch, mask=None, scale=None, out_bf16=True, out=No
     """softmax(scale q k^T) v of the rows q [tokens, heads, d] (bf16) over the cached keys of their sequences, [tokens, heads, d].
     mask: a BlockCausal; None: causal by token. A sink block is not seen before its time (BlockCausal.allows has it always
     seen). Rows behind the last sequence are not written."""
-    dev, kvh, d = pool.k.get_device(), pool.kv_heads, pool.d
+    dev, kvh, d = pool._device, pool.kv_heads, pool.d
     _on(dev, "paged_attention")
-    qs = _rows(q, "q", 0, d, (_BF16,), dev)
+    heads, qs = _rows(q, "q", 0, d, _ONLY_BF16, dev)
     if batch._device != dev:
         raise ValueError("paged_attention: the batch is on another device")
-    tokens, heads, _ = q.shape
+    tokens = q.shape[0]
     dtype = _BF16 if out_bf16 else _F32
     if out is None:   # (half the time of an empty() by shape)
         out = torch.empty_like(q) if out_bf16 and q.is_contiguous() else torch.empty((tokens, heads, d), device=q.device, dtype=dtype)
