@@ -1170,12 +1170,14 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         const size_t steps = walk_bound(kStep, 16 * c.nt, group, max_len, block_tokens, window, sink);
         // Shares of up to 128 steps, so that long sequences among short ones are cut (40 sessions of 15 to 100 % of 32760 tokens, 8
         // key heads, 4 bits: whole 270 us, 256 steps 211, 128 180, 64 184), a walk of up to 192 whole (128 sessions under a
-        // window of 4096: 100 us, in two 115). Where the workgroups then hold too little to fill the memory's pipe, about 2.2 MB of
-        // steps, as many shares as do: one session of 131000 tokens over 4 bits in 32 shares 38.7 us, in 64 36.9, in 128 41.2, in
-        // 16 66; 40 heads of 13270 tokens in bf16 in 4 shares 61, in 13 68. Short walks are not worth a second launch.
-        const size_t base = seqs * kv_heads * c.rows_tiles, step_bytes = kStep * (four ? d + d / 16 : 4 * d);
+        // window of 4096: 100 us, in two 115). Where that leaves units idle, as many shares as give each unit one workgroup, two over 4
+        // bits: 8 sessions of 12 heads x 6000 tokens in bf16, 96 workgroups 71 us, 192 49; 2 of 20000 x 12, 240 workgroups 42, 264 50 (some
+        // units have two). A share costs its launch and its join some 4 us where a step of each wave costs 1, so short walks are cut in three
+        // or more (one of 1500 tokens, 40 / 8 heads: whole 17.7, 11 shares 10.4; 30 of 1400 over 4 bits whole 15.2, in two 17.0) or not at all.
+        const size_t base = seqs * kv_heads * c.rows_tiles;
         size_t shares = steps <= 192 ? 1 : (steps + 127) / 128;
-        if (steps >= 48) shares = std::max(shares, std::min(std::min(2 * units, (size_t)2200000 / step_bytes) / base, steps / 8));
+        const size_t fill = std::min((four ? 2 : 1) * units / base, std::max(steps / 8, std::min<size_t>(steps / 4, 16)));
+        if (steps >= 36 && fill >= (steps < 96 ? 3 : 2)) shares = std::max(shares, fill);
         size_t chunk = ((steps + shares - 1) / shares + kWaves - 1) / kWaves * kWaves;
         c.rows_chunk = chunk;
         c.rows_chunks = (steps + chunk - 1) / chunk;
