@@ -30,11 +30,11 @@ struct PagedPieces {
     int n, tiles;               // numbers, of a sequence
 };
 struct PagedPiece {
-    int seq, tile;              // (of an unused number: a tile that the sequence does not have)
+    int seq, tile;              // (of an unused number: a tile that the sequence does not have, R tile below 2^31)
 };
 template <int R, class Pieces, class Batch>
 FV_DEV long paged_first_piece(const Pieces& x, const Batch& b, int group, int seq) {
-    return x.tiles ? (long)seq * x.tiles : ((long)b.q_start[seq] * group + (long)(R - 1) * seq) / R;
+    return x.tiles ? (long)seq * x.tiles : ((long)min(max(b.q_start[seq], 0), b.tokens) * group + (long)(R - 1) * seq) / R;
 }
 template <int R, class Pieces, class Batch>
 FV_DEV PagedPiece paged_piece(const Pieces& x, const Batch& b, int group, int number) {   // (of a whole wave)
@@ -48,8 +48,9 @@ FV_DEV PagedPiece paged_piece(const Pieces& x, const Batch& b, int group, int nu
         seq += k * step;
         n = min(step, n - k * step);
     }
-    const long tile = number - paged_first_piece<R>(x, b, group, seq);
-    return {seq, tile < 0 || tile > 0x1000000 ? 0x1000000 : (int)tile};
+    const long tile = number - paged_first_piece<R>(x, b, group, seq);   // (negative: of rows before the first sequence)
+    constexpr int kNone = 0x7fffffff / R;
+    return {seq, tile < 0 || tile > kNone ? kNone : (int)tile};
 }
 
 struct PagedAttnParams {

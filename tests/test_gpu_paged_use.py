@@ -229,6 +229,25 @@ def test_rows_outside_the_sequences_are_left(fv):
     w.check(q[part], marked[3][part].contiguous(), "rows outside")
 
 
+@pytest.mark.parametrize("heads,kvh", [(4, 4), (10, 2)])
+def test_many_rows_before_the_first_sequence(fv, heads, kvh):
+    """A batch of long and short sequences whose first row is far behind the tensors' first: pieces of rows that belong to nobody."""
+    import torch
+
+    announce(f"paged: rows before the first sequence {heads}/{kvh}")
+    lens, counts, before = [700, 3, 50, 9000, 2, 1, 1, 1], [300, 1, 0, 130, 1, 1, 1, 1], 1000
+    w = World(fv, 41, lens, counts, kvh, 64, 16)
+    n, rows = w.rows(), before + w.rows() + 200
+    q = w.queries(heads, 1.5)
+    dq = torch.zeros((rows, heads, 64), device="cuda", dtype=torch.bfloat16)
+    dq[before:before + n] = w.dev(q).bfloat16()
+    batch = fv.PagedBatch(w.dev(w.starts + np.int32(before)), w.dev(np.array(lens, dtype=np.int32)), w.dev(w.table), max(counts), max(lens))
+    out = torch.full((rows, heads, 64), 5.0, device="cuda", dtype=torch.float32)
+    fv.paged_attention(dq, w.pool, batch, out_bf16=False, out=out)
+    w.check(q, out[before:before + n], f"rows before {heads}/{kvh}")
+    assert (out[:before] == 5.0).all() and (out[before + n:] == 5.0).all()
+
+
 def test_sequences_may_share_pages(fv):
     """A prefix kept once: both sequences read it, each appends to pages of its own."""
     announce("paged: a shared prefix")
