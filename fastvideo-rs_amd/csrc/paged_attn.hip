@@ -8,7 +8,6 @@
 #include <limits.h>
 
 #include <algorithm>
-#include <numeric>
 
 #include "../../include/fv_sdpa_hip.h"
 #include "attn_core.h"
@@ -22,23 +21,42 @@ namespace {
 constexpr int kStep = 32;       // keys a wave takes at a time
 constexpr int kWaves = 4;
 
+// Division of a number below 2^31 by one that the host knows, as a product and a shift: with 2^l >= by, mul = 2^(31 + l) / by rounded up is
+// too large by less than 1, so n mul / 2^(31 + l) by less than 1 / by. (The compiler's own takes 20 instructions and waits for a
+// reciprocal; a workgroup makes ten of them before its first load.)
+struct PagedDiv {
+    unsigned mul;
+    int shift, by;
+};
+template <class Div>
+FV_DEV int paged_quot(int n, const Div& d) { return (int)(((unsigned long long)(unsigned)n * d.mul) >> d.shift); }
+PagedDiv paged_div(size_t by) {   // below 2^31 (0: never used)
+    if (by == 0) return {0, 0, 0};
+    int l = 0;
+    while (((size_t)1 << l) < by) l++;
+    return {(unsigned)((1ull << (31 + l)) / by + 1), 31 + l, (int)by};
+}
+
 // Pieces of up to R rows of the (token, head of the group) rows of a batch, for one key head. Where the sequences are as long as
 // the longest, piece t of sequence s is number s tiles + t. Where they are not (tiles 0), it is number first(s) + t with
 // first(s) = (group q_start[s] + (R - 1) s) / R, which leaves each its ceil(rows / R) numbers and no more than one for each sequence
 // unused, whatever the longest is. (A prompt of 8192 tokens among 255 single ones: 6.8 ms with the longest's pieces for all.)
 struct PagedPieces {
-    int n, tiles;               // numbers, of a sequence
+    PagedDiv n, tiles;          // numbers, of a sequence
 };
 struct PagedPiece {
     int seq, tile;              // (of an unused number: a tile that the sequence does not have, R tile below 2^31)
 };
 template <int R, class Pieces, class Batch>
 FV_DEV long paged_first_piece(const Pieces& x, const Batch& b, int group, int seq) {
-    return x.tiles ? (long)seq * x.tiles : ((long)min(max(b.q_start[seq], 0), b.tokens) * group + (long)(R - 1) * seq) / R;
+    return x.tiles.by ? (long)seq * x.tiles.by : ((long)min(max(b.q_start[seq], 0), b.tokens) * group + (long)(R - 1) * seq) / R;
 }
 template <int R, class Pieces, class Batch>
 FV_DEV PagedPiece paged_piece(const Pieces& x, const Batch& b, int group, int number) {   // (of a whole wave)
-    if (x.tiles) return {number / x.tiles, number % x.tiles};
+    if (x.tiles.by) {
+        const int seq = paged_quot(number, x.tiles);
+        return {seq, number - seq * x.tiles.by};
+    }
     const int lane = threadIdx.x & 63;
     int seq = 0, n = b.seqs;    // the last of sequences seq .. seq + n - 1 whose first piece is no later: 64 of them at a time
     while (n > 1) {
@@ -60,21 +78,24 @@ struct PagedAttnParams {
     long q_stride;              // elements between tokens
     void* out;                  // [tokens, heads, d]
     int out_is_bf16;
-    int heads, group;           // query heads, of which `group` share a key head
+    int heads;
+    PagedDiv group;             // query heads that share a key head
     float sl2;                  // scale * log2(e)
-    int block_tokens, window, sink;   // blocks; window 0: all
+    PagedDiv block_tokens;
+    int window, sink;           // blocks; window 0: all
     // Two kernels share a call: sequences of up to `few` rows a key head go to paged_rows_kernel, the others to
     // paged_tiles_kernel. How each cuts its part:
-    int few, rows_m;            // (rows_m: rows a tile of paged_rows_kernel)
-    int rows_tiles;             // (tiles of a (sequence, key head) there)
+    int few;
+    int rows_m;                 // rows a tile of paged_rows_kernel
+    PagedDiv rows_tiles, kv_heads;   // (tiles of a (sequence, key head) there)
     struct Cut {
-        int chunk, chunks;      // steps of the walk that a workgroup takes, workgroups a walk
+        PagedDiv chunk, chunks; // steps of the walk that a workgroup takes, workgroups a walk
     } rows, big;
     // paged_tiles_kernel: the first big_full tiles (a multiple of 8), counted key head by key head and the last rows first, have a
     // workgroup each, the others big.chunks; big_rest: those others' workgroups.
     PagedPieces big_pieces;
     int big_full, big_rest;
-    int xcds;                   // XCDs that share a run of items (1, 2, 4, 8)
+    int xcds;                   // 2^xcds XCDs share a run of items
     // Shares: values, each normalised, and the base-2 logarithm of its sum. Of paged_rows_kernel [chunks][tokens * heads][d] and
     // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
     float *rows_o, *rows_lse, *big_o, *big_lse;
@@ -95,7 +116,7 @@ struct PagedSight {
 template <class Params>
 FV_DEV PagedSight paged_sight(const Params& p, int pos, int len) {
     if (pos < 0) return {0, 0, 0};
-    const int bt = p.block_tokens, block = bt == 1 ? pos : pos / bt;
+    const int bt = p.block_tokens.by, block = paged_quot(pos, p.block_tokens);
     const long hi = (long)(block + 1) * bt, sink = (long)p.sink * bt;
     PagedSight s;
     s.hi = (int)min(hi, (long)len);
@@ -278,25 +299,26 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     int item = blockIdx.x;
-    const int tile = item % p.rows_tiles;
-    item /= p.rows_tiles;
-    const int kvh = item % p.pool.kv_heads;
-    item /= p.pool.kv_heads;
-    const int chunk = item % p.rows.chunks, seq = item / p.rows.chunks;
+    auto digit = [&](const PagedDiv& d) {   // of the workgroup's number, the last one
+        const int q = paged_quot(item, d), r = item - q * d.by;
+        item = q;
+        return r;
+    };
+    const int tile = digit(p.rows_tiles), kvh = digit(p.kv_heads), chunk = digit(p.rows.chunks), seq = item;
     const PagedSeq sq = paged_seq(p.b, seq);
-    const int rows = sq.count * p.group, row0 = tile * 16 * NT;
+    const int rows = sq.count * p.group.by, row0 = tile * 16 * NT;
     if (row0 >= rows || rows > p.few) return;
-    const int t0 = row0 / p.group, t1 = (min(row0 + 16 * NT, rows) - 1) / p.group;
+    const int t0 = paged_quot(row0, p.group), t1 = paged_quot(min(row0 + 16 * NT, rows) - 1, p.group);
     const PagedWalk<kStep> w = paged_walk<kStep>(p, sq, t0, t1);
     const PagedSight all_see = paged_all(p, sq, t0, t1);
-    const int e0 = chunk * p.rows.chunk, e1 = min(w.n, e0 + p.rows.chunk);
+    const int e0 = chunk * p.rows.chunk.by, e1 = min(w.n, e0 + p.rows.chunk.by);
     if (chunk > 0 && e0 >= e1) return;
 
     PagedSight see[NT];
     bf16x8 qf[NT][D / 32];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int r = row0 + 16 * n + col, t = r / p.group, h = kvh * p.group + r - t * p.group;
+        const int r = row0 + 16 * n + col, t = paged_quot(r, p.group), h = kvh * p.group.by + r - t * p.group.by;
         const bool ok = r < rows;
         see[n] = paged_sight(p, ok ? sq.first_pos() + t : -1, sq.len);
         const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + h * D + (FOUR ? (D / 4) * g : 8 * g);
@@ -525,7 +547,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     }
 
     // join the waves: each brings its rows' offsets and sums, and its O scaled to the common offset
-    const bool split = w.n > p.rows.chunk;
+    const bool split = w.n > p.rows.chunk.by;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const float sum = quad_sum(l[n]);
@@ -556,8 +578,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
             const int rr = threadIdx.x >> 4, cc = (threadIdx.x & 15) * kPer;
             const int r = row0 + 16 * n + rr;
             if (r < rows) {
-                const int t = r / p.group;
-                const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
+                const int t = paged_quot(r, p.group);
+                const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
                 const float k = lds_row[rr][0];
                 float val[kPer];
 #pragma unroll
@@ -617,38 +639,39 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int q4 = lane >> 4, i16 = lane & 15;
-    // The items lie in 8 / xcds runs, key head by key head, so that an L2 holds few heads' keys; the XCDs of a run take its items in
+    // The items lie in runs of 2^xcds XCDs, key head by key head, so that an L2 holds few heads' keys; the XCDs of a run take its items in
     // turn, so that each has as many of the long walks as the others. (One prompt of 16 heads on one key head: XCDs with an eighth
     // each took as long as the one with the last rows.)
     const bool full = block < p.big_full;
     const int at = full ? block : block - p.big_full, of = full ? p.big_full : p.big_rest;
-    const int run = (of * p.xcds + 7) / 8, in_run = (at >> 3) * p.xcds + (at & (p.xcds - 1));
-    int item = (at & 7) / p.xcds * run + in_run, chunk = 0;
+    const int run = ((of << p.xcds) + 7) >> 3, in_run = ((at >> 3) << p.xcds) + (at & ((1 << p.xcds) - 1));
+    int item = ((at & 7) >> p.xcds) * run + in_run, chunk = 0;
     if (in_run >= run || item >= of) return true;
     if (!full) {
-        chunk = item % p.big.chunks;
-        item = p.big_full + item / p.big.chunks;
+        const int q = paged_quot(item, p.big.chunks);
+        chunk = item - q * p.big.chunks.by;
+        item = p.big_full + q;
     }
     const int cut_tile = item - p.big_full;   // (where it is cut)
-    const int kvh = item / p.big_pieces.n;
-    const PagedPiece piece = paged_piece<kBigRows>(p.big_pieces, p.b, p.group, p.big_pieces.n - 1 - item % p.big_pieces.n);
+    const int kvh = paged_quot(item, p.big_pieces.n);
+    const PagedPiece piece = paged_piece<kBigRows>(p.big_pieces, p.b, p.group.by, (kvh + 1) * p.big_pieces.n.by - 1 - item);
     const int seq = piece.seq, tile = piece.tile;
     const PagedSeq sq = paged_seq(p.b, seq);
-    const int rows = sq.count * p.group, row0 = tile * kBigRows;
+    const int rows = sq.count * p.group.by, row0 = tile * kBigRows;
     if (row0 >= rows || rows <= p.few) return true;
-    const PagedWalk<kPart> w = paged_walk<kPart>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group);
-    const int tiles = (w.n + 3) >> 2, e0 = chunk * p.big.chunk, e1 = full ? tiles : min(tiles, e0 + p.big.chunk);
+    const PagedWalk<kPart> w = paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group));
+    const int tiles = (w.n + 3) >> 2, e0 = chunk * p.big.chunk.by, e1 = full ? tiles : min(tiles, e0 + p.big.chunk.by);
     if (chunk > 0 && e0 >= e1) return true;
-    const bool split = !full && tiles > p.big.chunk;
+    const bool split = !full && tiles > p.big.chunk.by;
     const float sl2 = p.sl2;
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
     const int wrow = row0 + 32 * wave;
     PagedSight all_see = {0x7fffffff, 0, 0x7fffffff}, mine = {0, 0, 0};
     if (wrow < rows) {
-        all_see = paged_all(p, sq, wrow / p.group, (min(wrow + 32, rows) - 1) / p.group);
+        all_see = paged_all(p, sq, paged_quot(wrow, p.group), paged_quot(min(wrow + 32, rows) - 1, p.group));
         const int r = wrow + (lane & 31);
-        mine = paged_sight(p, sq.first_pos() + min(r, rows - 1) / p.group, sq.len);
+        mine = paged_sight(p, sq.first_pos() + paged_quot(min(r, rows - 1), p.group), sq.len);
     }
     // the parts of the walk that rows which all see `all` see whole: those before `a` and [b, c)
     struct Whole {
@@ -684,8 +707,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     bf16x8 qf[D / 32][2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        const int r = wrow + 16 * g + i16, t = r / p.group;
-        const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + (kvh * p.group + r - t * p.group) * D + 8 * q4;
+        const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
+        const uint16_t* q = p.q + (size_t)(sq.start + t) * p.q_stride + (kvh * p.group.by + r - t * p.group.by) * D + 8 * q4;
 #pragma unroll
         for (int dk = 0; dk < D / 32; dk++) {
             u32x4 x = {0u, 0u, 0u, 0u};
@@ -774,7 +797,7 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     // The second pass, a tile that some of the workgroup's rows see a part of: a value that is not finite belongs to the rows that see
     // it, and a probability of zero does not keep it from the others. Such keys leave the V tile, and the rows that have a share
     // in one add theirs from the pool. (The first pass ends in the check where there is such a value.)
-    const Whole wg_whole = whole_parts(paged_all(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group));
+    const Whole wg_whole = whole_parts(paged_all(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)));
     auto set_apart = [&](int m, int e, const ProbTile& pb, f32x4 (&o)[kNO][2]) {
         lds_u8* mine_v = vbuf(m) + 16 * wave * G::kRow;
         unsigned bad_rows = 0;   // of the wave's 16
@@ -965,9 +988,9 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     for (int g = 0; g < 2; g++) {
         const float l = quad_sum(st.l_acc[g]);
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int r = wrow + 16 * g + i16, t = r / p.group;
+        const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
         if (r >= rows) continue;
-        const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
+        const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
         const size_t share = shares + (r - row0);
         if (split && q4 == 0) p.big_lse[share] = l == 0.f ? neg_inf() : st.log2_offset<true>(g, sl2) + __log2f(l);
 #pragma unroll
@@ -1006,29 +1029,29 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     constexpr int kPer = D / 4, kRows = 256 / (kPer * G);
     __shared__ float lds_top[kRows][G], lds_sum[kRows][G];
     __shared__ f32x4 lds_acc[kRows][G][kPer];
-    const int kvh = blockIdx.x / p.join_pieces.n;
-    const PagedPiece piece = paged_piece<kRows>(p.join_pieces, p.b, p.group, blockIdx.x % p.join_pieces.n);
+    const int kvh = paged_quot(blockIdx.x, p.join_pieces.n);
+    const PagedPiece piece = paged_piece<kRows>(p.join_pieces, p.b, p.group.by, blockIdx.x - kvh * p.join_pieces.n.by);
     const int seq = piece.seq;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int slot = threadIdx.x / (kPer * G), gi = threadIdx.x / kPer % G, c = threadIdx.x % kPer;
-    const int rows = sq.count * p.group, r = piece.tile * kRows + slot;
-    const int t = r / p.group;
-    const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group + (r - t * p.group);
+    const int rows = sq.count * p.group.by, r = piece.tile * kRows + slot;
+    const int t = paged_quot(r, p.group);
+    const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
     int chunks = 0;
     const bool few = rows <= p.few;
     size_t first = dst, step = (size_t)p.b.tokens * p.heads;   // the row's place in the first share, rows to the next
     if (r < rows) {
         if (few) {
-            const int tile = r / p.rows_m, row0 = tile * p.rows_m;
-            if (tile < p.rows_tiles)
-                chunks = (paged_walk<kStep>(p, sq, row0 / p.group, (min(row0 + p.rows_m, rows) - 1) / p.group).n + p.rows.chunk - 1) / p.rows.chunk;
+            const int tile = p.rows_m == 16 ? r >> 4 : r >> 5, row0 = tile * p.rows_m;
+            if (tile < p.rows_tiles.by)
+                chunks = paged_quot(paged_walk<kStep>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + p.rows_m, rows) - 1, p.group)).n + p.rows.chunk.by - 1, p.rows.chunk);
         } else {
             const int row0 = r / kBigRows * kBigRows;
             // (as paged_tiles_item counts)
-            const long number = paged_first_piece<kBigRows>(p.big_pieces, p.b, p.group, seq) + r / kBigRows;
-            const long at = (long)(kvh + 1) * p.big_pieces.n - 1 - number;
-            if (number < p.big_pieces.n && at >= p.big_full)
-                chunks = ((paged_walk<kPart>(p, sq, row0 / p.group, (min(row0 + kBigRows, rows) - 1) / p.group).n + 3) / 4 + p.big.chunk - 1) / p.big.chunk;
+            const long number = paged_first_piece<kBigRows>(p.big_pieces, p.b, p.group.by, seq) + r / kBigRows;
+            const long at = (long)(kvh + 1) * p.big_pieces.n.by - 1 - number;
+            if (number < p.big_pieces.n.by && at >= p.big_full)
+                chunks = paged_quot((paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)).n + 3) / 4 + p.big.chunk.by - 1, p.big.chunk);
             first = (size_t)(at - p.big_full) * kBigRows + (r - row0);
             step = (size_t)p.big_rows;
         }
@@ -1107,16 +1130,17 @@ size_t walk_bound(size_t step, size_t rows, size_t group, size_t max_len, size_t
 PagedPieces paged_pieces(size_t r, size_t seqs, size_t tokens, size_t max_q, size_t group) {
     const size_t tiles = (max_q * group + r - 1) / r, like = seqs * tiles, ragged = (tokens * group + (r - 1) * seqs) / r;
     const size_t most = INT_MAX;   // (past it no launch holds them)
-    return like <= ragged ? PagedPieces{(int)std::min(like, most), (int)std::min(tiles, most)} : PagedPieces{(int)std::min(ragged, most), 0};
+    return like <= ragged ? PagedPieces{paged_div(std::min(like, most)), paged_div(std::min(tiles, most))}
+                          : PagedPieces{paged_div(std::min(ragged, most)), paged_div(0)};
 }
 // How a call is cut.
 struct PagedCut {
     size_t few = 0;                         // rows a key head up to which a sequence is paged_rows_kernel's
     size_t nt = 0;                          // its tiles of 16 rows; 0: not launched
     size_t rows_tiles = 1, rows_chunk = 1, rows_chunks = 1;
-    PagedPieces big = {0, 0};               // of paged_tiles_kernel, a key head; none: not launched
+    PagedPieces big = {};                   // of paged_tiles_kernel, a key head; none: not launched
     size_t big_full = 0, big_chunk = 1, big_chunks = 1;
-    size_t chunks() const { return std::max(nt ? rows_chunks : 1, big.n ? big_chunks : 1); }
+    size_t chunks() const { return std::max(nt ? rows_chunks : 1, big.n.by ? big_chunks : 1); }
 };
 // bf16: two tiles of 16 rows cost paged_rows_kernel a second pass over the keys' operands, or a second walk, and paged_tiles_kernel, which
 // pads to 128, streams the keys as fast (48 sessions of 5 drafts x 4 heads, a window of 2048: 86 us by rows, 77.5 by tiles; 16 x 8 x 5
@@ -1137,7 +1161,7 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         // their walk whole and only the rest are cut. (Tiles whose walks differ, causal or of ragged prompts, fill the
         // rounds by themselves: no count of rounds, and all or none are cut.) One frame of 1560 against 32760, 12 heads: in 1, 2, 3, 4
         // shares 538, 427, 293, 362 us.
-        const size_t items = seqs * kv_heads * tiles, held = kv_heads * (size_t)c.big.n;
+        const size_t items = seqs * kv_heads * tiles, held = kv_heads * (size_t)c.big.n.by;
         const size_t slots = (d == 64 ? 3 : 2) * units / 8 * 8;
         const bool varied = 10 * held < 9 * items || (window == 0 && 4 * block_tokens < max_q && 2 * max_q > max_len);
         auto step_us = [&](size_t wgs) {
@@ -1195,8 +1219,8 @@ struct PagedParts {
             return at;
         };
         if (c.nt && c.rows_chunks > 1) rows_o = take(c.rows_chunks * tokens * heads * d * 4), rows_lse = take(c.rows_chunks * tokens * heads * 4);
-        if (c.big.n && c.big_chunks > 1) {
-            big_rows = (kv_heads * (size_t)c.big.n - c.big_full) * kBigRows;
+        if (c.big.n.by && c.big_chunks > 1) {
+            big_rows = (kv_heads * (size_t)c.big.n.by - c.big_full) * kBigRows;
             big_o = take(c.big_chunks * big_rows * d * 4), big_lse = take(c.big_chunks * big_rows * 4);
         }
     }
@@ -1251,23 +1275,24 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     const bool split = c.chunks() > 1;
     if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
     const bool many = (c.big_chunks > 1 ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
-    const size_t group = heads / kv_heads, xcds = 8 / std::gcd(kv_heads, (size_t)8);
+    const size_t group = heads / kv_heads;
+    const int xcds = kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3;   // (a run has whole key heads)
     // (rows a workgroup of the join; where paged_tiles_kernel cuts nothing, of the sequences of few rows)
     const size_t join_rows = 256 / (d / 4 * (many ? 8 : 1)), join_few = (c.few + join_rows - 1) / join_rows;
-    const fv::PagedPieces join = c.big.n && c.big_chunks == 1 ? fv::PagedPieces{(int)(seqs * join_few), (int)join_few}
+    const fv::PagedPieces join = c.big.n.by && c.big_chunks == 1 ? fv::PagedPieces{fv::paged_div(seqs * join_few), fv::paged_div(join_few)}
                                                               : fv::paged_pieces(join_rows, seqs, tokens, max_q, group);
-    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (kv_heads * (size_t)c.big.n - c.big_full) * c.big_chunks;
-    const size_t big_blocks = c.big_full + 8 * (((big_rest * xcds + 7) / 8 + xcds - 1) / xcds), join_blocks = kv_heads * (size_t)join.n;
+    const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (kv_heads * (size_t)c.big.n.by - c.big_full) * c.big_chunks;
+    const size_t big_blocks = c.big_full + 8 * ((((big_rest << xcds) + 7) / 8 + ((size_t)1 << xcds) - 1) >> xcds), join_blocks = kv_heads * (size_t)join.n.by;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     if (row_blocks >= kMost || big_blocks >= kMost || (split && join_blocks >= kMost)) return fv_decline("paged attention: too large for one launch");
     p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
-    p.heads = (int)heads, p.group = (int)group;
+    p.heads = (int)heads, p.group = fv::paged_div(group), p.kv_heads = fv::paged_div(kv_heads);
     p.sl2 = (float)((double)scale * 1.4426950408889634);
-    p.block_tokens = (int)block_tokens, p.window = (int)window, p.sink = (int)sink;
+    p.block_tokens = fv::paged_div(block_tokens), p.window = (int)window, p.sink = (int)sink;
     p.few = (int)c.few, p.rows_m = (int)(16 * c.nt);
-    p.rows_tiles = (int)c.rows_tiles, p.rows = {(int)c.rows_chunk, (int)c.rows_chunks};
-    p.big = {(int)c.big_chunk, (int)c.big_chunks}, p.big_pieces = c.big, p.join_pieces = join;
-    p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.xcds = (int)xcds;
+    p.rows_tiles = fv::paged_div(c.rows_tiles), p.rows = {fv::paged_div(c.rows_chunk), fv::paged_div(c.rows_chunks)};
+    p.big = {fv::paged_div(c.big_chunk), fv::paged_div(c.big_chunks)}, p.big_pieces = c.big, p.join_pieces = join;
+    p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.xcds = xcds;
     uint8_t* ws = (uint8_t*)workspace;
     p.rows_o = (float*)(ws + parts.rows_o), p.rows_lse = (float*)(ws + parts.rows_lse);
     p.big_o = (float*)(ws + parts.big_o), p.big_lse = (float*)(ws + parts.big_lse), p.big_rows = (long)parts.big_rows;
@@ -1275,7 +1300,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     fv::paged_pick(d == 128, [&](auto d128) {
         fv::paged_pick(four, [&](auto f) {
             constexpr int D = d128() ? 128 : 64;
-            if (c.big.n)
+            if (c.big.n.by)
                 hipLaunchKernelGGL((fv::paged_tiles_kernel<D, f()>), dim3((unsigned)big_blocks), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
             if (c.nt == 1) hipLaunchKernelGGL((fv::paged_rows_kernel<D, f(), 1>), dim3((unsigned)row_blocks), dim3(256), 0, st, p);
             if constexpr (f())   // (the only pages whose calls have two tiles of rows, few_rows)

@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p)
     const bool is_q = head < nq, turn = p.cos_t != nullptr && head < nq + kvh;
     // the values first, which wait for nothing; where they go takes four or more loads in a row
     const void* x = is_q ? p.q : head < nq + kvh ? p.k : p.v;
-    const size_t from = (size_t)t * (is_q ? p.q_stride : head < nq + kvh ? p.k_stride : p.v_stride) + (is_q ? head : (head - nq) % kvh) * D;
+    const size_t from = (size_t)t * (is_q ? p.q_stride : head < nq + kvh ? p.k_stride : p.v_stride) + (is_q ? head : head < nq + kvh ? head - nq : head - nq - kvh) * D;
     Eight<IN16> own, other;
     own.load(x, from + 8 * c);
     if (HALVES && turn) other.load(x, from + 8 * partner<D, HALVES>(c));
