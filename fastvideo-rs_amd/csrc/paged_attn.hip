@@ -88,13 +88,13 @@ struct PagedAttnParams {
     int few;
     int rows_m;                 // rows a tile of paged_rows_kernel
     PagedDiv rows_tiles, kv_heads;   // (tiles of a (sequence, key head) there)
-    struct Cut {
-        PagedDiv chunk, chunks; // steps of the walk that a workgroup takes, workgroups a walk
-    } rows, big;
+    PagedDiv rows_chunk, rows_chunks;   // steps of the walk that a workgroup takes, workgroups a walk
+    PagedDiv big_chunk;         // (steps)
     // paged_tiles_kernel: the first big_full tiles (a multiple of 8), counted key head by key head and the last rows first, have a
-    // workgroup each, the others big.chunks; big_rest: those others' workgroups.
+    // workgroup each, the others as many as they have shares: big_rest workgroups, in sets of big_set tiles and big_set_shares shares.
     PagedPieces big_pieces;
     int big_full, big_rest;
+    PagedDiv big_set, big_set_shares;
     int xcds;                   // 2^xcds XCDs share a run of items
     // Shares: values, each normalised, and the base-2 logarithm of its sum. Of paged_rows_kernel [chunks][tokens * heads][d] and
     // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
@@ -304,14 +304,14 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
         item = q;
         return r;
     };
-    const int tile = digit(p.rows_tiles), kvh = digit(p.kv_heads), chunk = digit(p.rows.chunks), seq = item;
+    const int tile = digit(p.rows_tiles), kvh = digit(p.kv_heads), chunk = digit(p.rows_chunks), seq = item;
     const PagedSeq sq = paged_seq(p.b, seq);
     const int rows = sq.count * p.group.by, row0 = tile * 16 * NT;
     if (row0 >= rows || rows > p.few) return;
     const int t0 = paged_quot(row0, p.group), t1 = paged_quot(min(row0 + 16 * NT, rows) - 1, p.group);
     const PagedWalk<kStep> w = paged_walk<kStep>(p, sq, t0, t1);
     const PagedSight all_see = paged_all(p, sq, t0, t1);
-    const int e0 = chunk * p.rows.chunk.by, e1 = min(w.n, e0 + p.rows.chunk.by);
+    const int e0 = chunk * p.rows_chunk.by, e1 = min(w.n, e0 + p.rows_chunk.by);
     if (chunk > 0 && e0 >= e1) return;
 
     PagedSight see[NT];
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
     }
 
     // join the waves: each brings its rows' offsets and sums, and its O scaled to the common offset
-    const bool split = w.n > p.rows.chunk.by;
+    const bool split = w.n > p.rows_chunk.by;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const float sum = quad_sum(l[n]);
@@ -648,9 +648,11 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     int item = ((at & 7) >> p.xcds) * run + in_run, chunk = 0;
     if (in_run >= run || item >= of) return true;
     if (!full) {
-        const int q = paged_quot(item, p.big.chunks);
-        chunk = item - q * p.big.chunks.by;
-        item = p.big_full + q;
+        // all tiles of a key head in their first share, then all in their second: neighbours walk the same keys, and the shares that
+        // short walks do not have lie together (tile by tile they came to the same units again and again)
+        const int set = paged_quot(item, p.big_set_shares), rest = item - set * p.big_set_shares.by;
+        chunk = paged_quot(rest, p.big_set);
+        item = p.big_full + set * p.big_set.by + rest - chunk * p.big_set.by;
     }
     const int cut_tile = item - p.big_full;   // (where it is cut)
     const int kvh = paged_quot(item, p.big_pieces.n);
@@ -660,9 +662,9 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     const int rows = sq.count * p.group.by, row0 = tile * kBigRows;
     if (row0 >= rows || rows <= p.few) return true;
     const PagedWalk<kPart> w = paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group));
-    const int tiles = (w.n + 3) >> 2, e0 = chunk * p.big.chunk.by, e1 = full ? tiles : min(tiles, e0 + p.big.chunk.by);
+    const int tiles = (w.n + 3) >> 2, e0 = chunk * p.big_chunk.by, e1 = full ? tiles : min(tiles, e0 + p.big_chunk.by);
     if (chunk > 0 && e0 >= e1) return true;
-    const bool split = !full && tiles > p.big.chunk.by;
+    const bool split = !full && tiles > p.big_chunk.by;
     const float sl2 = p.sl2;
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
@@ -1044,14 +1046,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
         if (few) {
             const int tile = p.rows_m == 16 ? r >> 4 : r >> 5, row0 = tile * p.rows_m;
             if (tile < p.rows_tiles.by)
-                chunks = paged_quot(paged_walk<kStep>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + p.rows_m, rows) - 1, p.group)).n + p.rows.chunk.by - 1, p.rows.chunk);
+                chunks = paged_quot(paged_walk<kStep>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + p.rows_m, rows) - 1, p.group)).n + p.rows_chunk.by - 1, p.rows_chunk);
         } else {
             const int row0 = r / kBigRows * kBigRows;
             // (as paged_tiles_item counts)
             const long number = paged_first_piece<kBigRows>(p.big_pieces, p.b, p.group.by, seq) + r / kBigRows;
             const long at = (long)(kvh + 1) * p.big_pieces.n.by - 1 - number;
             if (number < p.big_pieces.n.by && at >= p.big_full)
-                chunks = paged_quot((paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)).n + 3) / 4 + p.big.chunk.by - 1, p.big.chunk);
+                chunks = paged_quot((paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)).n + 3) / 4 + p.big_chunk.by - 1, p.big_chunk);
             first = (size_t)(at - p.big_full) * kBigRows + (r - row0);
             step = (size_t)p.big_rows;
         }
@@ -1274,7 +1276,9 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     }
     const bool split = c.chunks() > 1;
     if (split && ((uintptr_t)workspace & 255) != 0) return fv_invalid("paged attention: the workspace must be 256-byte aligned");
-    const bool many = (c.big_chunks > 1 ? c.big_chunks : c.rows_chunks) > 4;   // shares: eight groups of threads a row, or one
+    // eight groups of threads a row of the join, or one: where rows are few for their shares
+    const size_t most_shares = c.big_chunks > 1 ? c.big_chunks : c.rows_chunks;
+    const bool many = most_shares > 4 && tokens * heads < 128 * most_shares;
     const size_t group = heads / kv_heads;
     const int xcds = kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3;   // (a run has whole key heads)
     // (rows a workgroup of the join; where paged_tiles_kernel cuts nothing, of the sequences of few rows)
@@ -1290,8 +1294,10 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     p.sl2 = (float)((double)scale * 1.4426950408889634);
     p.block_tokens = fv::paged_div(block_tokens), p.window = (int)window, p.sink = (int)sink;
     p.few = (int)c.few, p.rows_m = (int)(16 * c.nt);
-    p.rows_tiles = fv::paged_div(c.rows_tiles), p.rows = {fv::paged_div(c.rows_chunk), fv::paged_div(c.rows_chunks)};
-    p.big = {fv::paged_div(c.big_chunk), fv::paged_div(c.big_chunks)}, p.big_pieces = c.big, p.join_pieces = join;
+    p.rows_tiles = fv::paged_div(c.rows_tiles), p.rows_chunk = fv::paged_div(c.rows_chunk), p.rows_chunks = fv::paged_div(c.rows_chunks);
+    const size_t set = c.big_full ? kv_heads * (size_t)c.big.n.by - c.big_full : (size_t)c.big.n.by;   // (a key head's; else all)
+    p.big_set = fv::paged_div(set), p.big_set_shares = fv::paged_div(set * c.big_chunks);
+    p.big_chunk = fv::paged_div(c.big_chunk), p.big_pieces = c.big, p.join_pieces = join;
     p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.xcds = xcds;
     uint8_t* ws = (uint8_t*)workspace;
     p.rows_o = (float*)(ws + parts.rows_o), p.rows_lse = (float*)(ws + parts.rows_lse);
