@@ -100,7 +100,9 @@ struct PagedAttnParams {
     // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
     float *rows_o, *rows_lse, *big_o, *big_lse;
     long big_rows;              // the latter's rows
-    PagedPieces join_pieces;    // of paged_join_kernel
+    // paged_join_kernel: the first join_tiles workgroups those of the cut tiles, then join_few each of a (sequence, key head) of few rows
+    int join_tiles;
+    PagedDiv join_few;
 };
 
 // The keys that a row at position p of a sequence of `len` tokens sees: [0, a) and [lo, hi), a <= hi.
@@ -644,7 +646,9 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     // each took as long as the one with the last rows.)
     const bool full = block < p.big_full;
     const int at = full ? block : block - p.big_full, of = full ? p.big_full : p.big_rest;
-    const int run = ((of << p.xcds) + 7) >> 3, in_run = ((at >> 3) << p.xcds) + (at & ((1 << p.xcds) - 1));
+    // (Every other 32 of an XCD's items backwards: its 32 units take them in turn, and the first would have the longest each time.)
+    const int nth = (at >> 3) ^ ((at >> 8 & 1) * 31);
+    const int run = ((of << p.xcds) + 7) >> 3, in_run = (nth << p.xcds) + (at & ((1 << p.xcds) - 1));
     int item = ((at & 7) >> p.xcds) * run + in_run, chunk = 0;
     if (in_run >= run || item >= of) return true;
     if (!full) {
@@ -1031,30 +1035,36 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     constexpr int kPer = D / 4, kRows = 256 / (kPer * G);
     __shared__ float lds_top[kRows][G], lds_sum[kRows][G];
     __shared__ f32x4 lds_acc[kRows][G][kPer];
-    const int kvh = paged_quot(blockIdx.x, p.join_pieces.n);
-    const PagedPiece piece = paged_piece<kRows>(p.join_pieces, p.b, p.group.by, blockIdx.x - kvh * p.join_pieces.n.by);
-    const int seq = piece.seq;
-    const PagedSeq sq = paged_seq(p.b, seq);
+    constexpr int kPerTile = kBigRows / kRows;
     const int slot = threadIdx.x / (kPer * G), gi = threadIdx.x / kPer % G, c = threadIdx.x % kPer;
-    const int rows = sq.count * p.group.by, r = piece.tile * kRows + slot;
-    const int t = paged_quot(r, p.group);
+    const bool few = (int)blockIdx.x >= p.join_tiles;
+    int kvh, seq, r, item = 0;
+    if (few) {
+        const int at = blockIdx.x - p.join_tiles, q = paged_quot(at, p.join_few);
+        seq = paged_quot(q, p.kv_heads);
+        kvh = q - seq * p.kv_heads.by;
+        r = (at - q * p.join_few.by) * kRows + slot;
+    } else {
+        item = p.big_full + blockIdx.x / kPerTile;   // (as paged_tiles_item counts)
+        kvh = paged_quot(item, p.big_pieces.n);
+        const PagedPiece piece = paged_piece<kBigRows>(p.big_pieces, p.b, p.group.by, (kvh + 1) * p.big_pieces.n.by - 1 - item);
+        seq = piece.seq;
+        r = piece.tile * kBigRows + (blockIdx.x % kPerTile) * kRows + slot;
+    }
+    const PagedSeq sq = paged_seq(p.b, seq);
+    const int rows = sq.count * p.group.by, t = paged_quot(r, p.group);
     const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
     int chunks = 0;
-    const bool few = rows <= p.few;
     size_t first = dst, step = (size_t)p.b.tokens * p.heads;   // the row's place in the first share, rows to the next
-    if (r < rows) {
+    if (r < rows && few == (rows <= p.few)) {
+        auto shares = [&](const auto& walk, int parts, const PagedDiv& chunk) { return paged_quot((walk.n + parts - 1) / parts + chunk.by - 1, chunk); };
         if (few) {
-            const int tile = p.rows_m == 16 ? r >> 4 : r >> 5, row0 = tile * p.rows_m;
-            if (tile < p.rows_tiles.by)
-                chunks = paged_quot(paged_walk<kStep>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + p.rows_m, rows) - 1, p.group)).n + p.rows_chunk.by - 1, p.rows_chunk);
+            const int row0 = r & -p.rows_m;
+            chunks = shares(paged_walk<kStep>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + p.rows_m, rows) - 1, p.group)), 1, p.rows_chunk);
         } else {
-            const int row0 = r / kBigRows * kBigRows;
-            // (as paged_tiles_item counts)
-            const long number = paged_first_piece<kBigRows>(p.big_pieces, p.b, p.group.by, seq) + r / kBigRows;
-            const long at = (long)(kvh + 1) * p.big_pieces.n.by - 1 - number;
-            if (number < p.big_pieces.n.by && at >= p.big_full)
-                chunks = paged_quot((paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)).n + 3) / 4 + p.big_chunk.by - 1, p.big_chunk);
-            first = (size_t)(at - p.big_full) * kBigRows + (r - row0);
+            const int row0 = r & -kBigRows;
+            chunks = shares(paged_walk<kPart>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)), 4, p.big_chunk);
+            first = (size_t)(item - p.big_full) * kBigRows + (r - row0);
             step = (size_t)p.big_rows;
         }
     }
@@ -1157,32 +1167,41 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         const size_t tiles = (rows + kBigRows - 1) / kBigRows;   // (of the longest)
         c.big = paged_pieces(kBigRows, seqs, tokens, max_q, group);
         const size_t steps = (walk_bound(kPart, kBigRows, group, max_len, block_tokens, window, sink) + 3) / 4;
-        // Shares of the walk, by microseconds: rounds of as many workgroups as there is room for, 4 each besides their steps (1.05 and 1.75 a
-        // step of one and of two workgroups a unit, or what the memory takes where few tiles share their keys), against a
+        // Shares of the walk, by microseconds (fitted to 446 calls in 1 to 24 shares, within 7 %; the number it takes is 1 % slower than the best of them on average): rounds of as many workgroups as there is
+        // room for, each step by how many a unit has at once, or by what the memory takes where few tiles share their keys; against a
         // launch and the bytes that joining moves. Where the last round is far from full, the tiles of the rounds before keep
-        // their walk whole and only the rest are cut. (Tiles whose walks differ, causal or of ragged prompts, fill the
-        // rounds by themselves: no count of rounds, and all or none are cut.) One frame of 1560 against 32760, 12 heads: in 1, 2, 3, 4
-        // shares 538, 427, 293, 362 us.
-        const size_t items = seqs * kv_heads * tiles, held = kv_heads * (size_t)c.big.n.by;
-        const size_t slots = (d == 64 ? 3 : 2) * units / 8 * 8;
-        const bool varied = 10 * held < 9 * items || (window == 0 && 4 * block_tokens < max_q && 2 * max_q > max_len);
-        auto step_us = [&](size_t wgs) {
-            const size_t at_once = std::min(wgs, slots);
-            const double bytes = 64.0 * (double)(four ? d + d / 16 : 4 * d);
-            return std::max((at_once <= units ? 1.05 : 1.75) * (d == 64 ? 0.75 : 1.0), (double)at_once / (double)tiles * bytes / (at_once <= units ? 4.3e6 : 5.2e6));
+        // their walk whole and only the rest are cut. Tiles whose walks differ (causal, or of ragged prompts) fill the rounds by
+        // themselves: their steps in all, and the longest at the end. One frame of 1560 against 32760, 12 heads: in 1, 2, 3, 4 shares
+        // 538, 427, 290, 362 us.
+        const size_t numbers = kv_heads * (size_t)c.big.n.by;
+        const size_t slots = (d == 64 ? 3 : 2) * (units / 8 * 8);
+        const bool ragged = c.big.tiles.by == 0;
+        const size_t held = ragged ? kv_heads * (tokens * group / kBigRows + 1) : numbers;   // (the numbers without those that may be unused)
+        const double mean = ragged ? 0.6 : window > 0 || block_tokens >= max_q || max_q > max_len ? 1.0   // of the longest walk
+                                                                                               : 1.0 - 0.5 * (double)(max_q - block_tokens) / (double)max_len;
+        const bool varied = mean < 0.8;
+        auto steps_us = [&](double n, double wgs) {
+            const int at_once = wgs <= (double)units ? 0 : wgs <= 2.0 * (double)units ? 1 : 2;
+            const double wide[] = {1.07, 1.49, 1.49}, narrow[] = {0.67, 0.97, 1.26}, bytes = 64.0 * (double)(four ? d + d / 16 : 4 * d);
+            return n * std::max((d == 64 ? narrow : wide)[at_once] * (four ? 1.08 : 1.0), wgs / (double)tiles * bytes / (at_once == 0 ? 5e6 : 6.1e6));
         };
         double best = 0;
         const size_t rounds_before = varied ? 0 : held / slots;
         for (size_t keep = 0; keep <= std::min<size_t>(rounds_before, 2); keep++) {
             const size_t full = keep == 0 ? 0 : (rounds_before - (keep - 1)) * slots, rest = held - full;
-            if (rest == 0) continue;
+            if (rest == 0) continue;   // (full only where walks are alike: held is numbers)
             for (size_t k = 1; k <= 64 && k <= steps; k++) {
-                const size_t chunk = (steps + k - 1) / k, wgs = rest * k;
-                const double rounds = varied ? std::max(1.0, (double)wgs / (double)slots) + 0.5 : (double)((wgs + slots - 1) / slots);
-                const double cost = (double)(full / slots) * (4.0 + (double)steps * step_us(slots)) +
-                                    rounds * (4.0 + (varied ? 0.6 : 1.0) * (double)chunk * step_us(wgs)) +
-                                    (k > 1 ? 7.0 + (double)(k * std::min(rest * kBigRows, tokens * heads)) * 8.0 * (double)d / 6e6 : 0.0);
-                if ((keep == 0 && k == 1) || cost < 0.97 * best) best = cost, c.big_full = full, c.big_chunk = chunk, c.big_chunks = (steps + chunk - 1) / chunk;
+                const size_t chunk = (steps + k - 1) / k, shares = (steps + chunk - 1) / chunk, wgs = rest * shares;
+                double cost = (double)(full / slots) * steps_us((double)steps, (double)slots);
+                if (varied) {
+                    const double each = std::max(1.0, (double)shares * mean), all = (double)rest * each, at_once = std::min(all, (double)slots);
+                    cost += std::max(all / (double)slots * steps_us((double)steps * mean / each, at_once) + steps_us(0.43 * (double)chunk, at_once) * at_once / (double)slots,
+                                     steps_us(0.92 * (double)chunk, at_once));
+                } else {
+                    cost += (double)(wgs / slots) * steps_us((double)chunk * mean, (double)slots) + steps_us((double)chunk * mean, (double)(wgs % slots)) * (wgs % slots != 0);
+                }
+                if (shares > 1) cost += 2.0 + (double)(shares * std::min(rest * kBigRows, tokens * heads)) * std::min(1.0, mean + 0.1) * 8.0 * (double)d / 5.5e6 + 0.01 * (double)(numbers - full);
+                if ((keep == 0 && k == 1) || cost < 0.97 * best) best = cost, c.big_full = full, c.big_chunk = chunk, c.big_chunks = shares;
             }
         }
         if (c.big_chunks == 1) c.big_full = 0;
@@ -1281,12 +1300,13 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     const bool many = most_shares > 4 && tokens * heads < 128 * most_shares;
     const size_t group = heads / kv_heads;
     const int xcds = kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3;   // (a run has whole key heads)
-    // (rows a workgroup of the join; where paged_tiles_kernel cuts nothing, of the sequences of few rows)
-    const size_t join_rows = 256 / (d / 4 * (many ? 8 : 1)), join_few = (c.few + join_rows - 1) / join_rows;
-    const fv::PagedPieces join = c.big.n.by && c.big_chunks == 1 ? fv::PagedPieces{fv::paged_div(seqs * join_few), fv::paged_div(join_few)}
-                                                              : fv::paged_pieces(join_rows, seqs, tokens, max_q, group);
+    const size_t join_rows = 256 / (d / 4 * (many ? 8 : 1));   // a workgroup
+    const size_t cut_tiles = c.big.n.by && c.big_chunks > 1 ? kv_heads * (size_t)c.big.n.by - c.big_full : 0;
+    const size_t join_tiles = cut_tiles * (fv::kBigRows / join_rows), join_few = c.rows_chunks > 1 ? (c.few + join_rows - 1) / join_rows : 0;
     const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (kv_heads * (size_t)c.big.n.by - c.big_full) * c.big_chunks;
-    const size_t big_blocks = c.big_full + 8 * ((((big_rest << xcds) + 7) / 8 + ((size_t)1 << xcds) - 1) >> xcds), join_blocks = kv_heads * (size_t)join.n.by;
+    size_t an_xcd = (((big_rest << xcds) + 7) / 8 + ((size_t)1 << xcds) - 1) >> xcds;
+    if (an_xcd > 32) an_xcd = (an_xcd + 31) / 32 * 32;   // (the last 32 may be taken backwards)
+    const size_t big_blocks = c.big_full + 8 * an_xcd, join_blocks = join_tiles + seqs * kv_heads * join_few;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     if (row_blocks >= kMost || big_blocks >= kMost || (split && join_blocks >= kMost)) return fv_decline("paged attention: too large for one launch");
     p.q = q, p.q_stride = (long)q_stride, p.out = out, p.out_is_bf16 = out_is_bf16 != 0;
@@ -1297,7 +1317,8 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     p.rows_tiles = fv::paged_div(c.rows_tiles), p.rows_chunk = fv::paged_div(c.rows_chunk), p.rows_chunks = fv::paged_div(c.rows_chunks);
     const size_t set = c.big_full ? kv_heads * (size_t)c.big.n.by - c.big_full : (size_t)c.big.n.by;   // (a key head's; else all)
     p.big_set = fv::paged_div(set), p.big_set_shares = fv::paged_div(set * c.big_chunks);
-    p.big_chunk = fv::paged_div(c.big_chunk), p.big_pieces = c.big, p.join_pieces = join;
+    p.big_chunk = fv::paged_div(c.big_chunk), p.big_pieces = c.big;
+    p.join_tiles = (int)join_tiles, p.join_few = fv::paged_div(join_few);
     p.big_full = (int)c.big_full, p.big_rest = (int)big_rest, p.xcds = xcds;
     uint8_t* ws = (uint8_t*)workspace;
     p.rows_o = (float*)(ws + parts.rows_o), p.rows_lse = (float*)(ws + parts.rows_lse);
