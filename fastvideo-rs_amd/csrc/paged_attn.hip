@@ -646,8 +646,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     // each took as long as the one with the last rows.)
     const bool full = block < p.big_full;
     const int at = full ? block : block - p.big_full, of = full ? p.big_full : p.big_rest;
-    // (Every other 32 of an XCD's items backwards: its 32 units take them in turn, and the first would have the longest each time.)
-    const int nth = (at >> 3) ^ ((at >> 8 & 1) * 31);
+    // (The second 32 of an XCD's items backwards: its 32 units take the first ones in turn, and the same would have the longest each time.)
+    const int nth = (at >> 3) ^ (at >> 8 == 1 ? 31 : 0);
     const int run = ((of << p.xcds) + 7) >> 3, in_run = (nth << p.xcds) + (at & ((1 << p.xcds) - 1));
     int item = ((at & 7) >> p.xcds) * run + in_run, chunk = 0;
     if (in_run >= run || item >= of) return true;
@@ -1305,7 +1305,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     const size_t join_tiles = cut_tiles * (fv::kBigRows / join_rows), join_few = c.rows_chunks > 1 ? (c.few + join_rows - 1) / join_rows : 0;
     const size_t row_blocks = seqs * kv_heads * c.rows_tiles * c.rows_chunks, big_rest = (kv_heads * (size_t)c.big.n.by - c.big_full) * c.big_chunks;
     size_t an_xcd = (((big_rest << xcds) + 7) / 8 + ((size_t)1 << xcds) - 1) >> xcds;
-    if (an_xcd > 32) an_xcd = (an_xcd + 31) / 32 * 32;   // (the last 32 may be taken backwards)
+    if (an_xcd > 32) an_xcd = std::max<size_t>(an_xcd, 64);   // (the second 32 are taken backwards)
     const size_t big_blocks = c.big_full + 8 * an_xcd, join_blocks = join_tiles + seqs * kv_heads * join_few;
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     if (row_blocks >= kMost || big_blocks >= kMost || (split && join_blocks >= kMost)) return fv_decline("paged attention: too large for one launch");
