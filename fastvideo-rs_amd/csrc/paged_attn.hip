@@ -647,7 +647,7 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     const bool full = block < p.big_full;
     const int at = full ? block : block - p.big_full, of = full ? p.big_full : p.big_rest;
     // (The second 32 of an XCD's items backwards: its 32 units take the first ones in turn, and the same would have the longest each time.)
-    const int nth = (at >> 3) ^ (at >> 8 == 1 ? 31 : 0);
+    const int nth = (at >> 3) ^ (!full && at >> 8 == 1 ? 31 : 0);
     const int run = ((of << p.xcds) + 7) >> 3, in_run = (nth << p.xcds) + (at & ((1 << p.xcds) - 1));
     int item = ((at & 7) >> p.xcds) * run + in_run, chunk = 0;
     if (in_run >= run || item >= of) return true;
@@ -1131,8 +1131,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
 // themselves are the device's.)
 size_t walk_bound(size_t step, size_t rows, size_t group, size_t max_len, size_t block_tokens, size_t window, size_t sink) {
     size_t steps = (max_len + step - 1) / step;
-    if (window > 0) {   // the window, the tile's tokens (which lie in as many blocks, or fewer), a step at either end; the sink
-        const size_t blocks = window + (rows + group - 1) / group + 1, far = (size_t)1 << 31;
+    if (window > 0) {   // the first token's window and the blocks to the last token's, a step more (they begin anywhere in one); the sink
+        const size_t apart = (rows + group - 2) / group, blocks = window + (apart + block_tokens - 1) / block_tokens, far = (size_t)1 << 31;
         const size_t band = blocks < far / block_tokens ? blocks * block_tokens : far, keep = sink < far / block_tokens ? sink * block_tokens : far;
         steps = std::min(steps, (band + step - 1) / step + 1 + (keep + step - 1) / step);
     }
@@ -1167,19 +1167,20 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         const size_t tiles = (rows + kBigRows - 1) / kBigRows;   // (of the longest)
         c.big = paged_pieces(kBigRows, seqs, tokens, max_q, group);
         const size_t steps = (walk_bound(kPart, kBigRows, group, max_len, block_tokens, window, sink) + 3) / 4;
-        // Shares of the walk, by microseconds (fitted to 446 calls in 1 to 24 shares, within 7 %; the number it takes is 1 % slower than the best of them on average): rounds of as many workgroups as there is
-        // room for, each step by how many a unit has at once, or by what the memory takes where few tiles share their keys; against a
-        // launch and the bytes that joining moves. Where the last round is far from full, the tiles of the rounds before keep
-        // their walk whole and only the rest are cut. Tiles whose walks differ (causal, or of ragged prompts) fill the rounds by
-        // themselves: their steps in all, and the longest at the end. One frame of 1560 against 32760, 12 heads: in 1, 2, 3, 4 shares
-        // 538, 427, 290, 362 us.
+        // Shares of the walk, by microseconds (fitted to 446 calls in 1 to 24 shares, within 7 %; the number that it takes is 1 % slower than
+        // the best of them on average): rounds of as many workgroups as there is room for, each step by how many a unit has at once, or
+        // by what the memory takes where few tiles share their keys; against a launch and the bytes that joining moves. Where the last
+        // round is far from full, the tiles of the rounds before keep their walk whole and only the rest are cut. Tiles whose walks
+        // differ (causal, or of ragged prompts) fill the rounds by themselves: their steps in all, and the longest at the end. One frame
+        // of 1560 against 32760, 12 heads: in 1, 2, 3, 4 shares 538, 427, 290, 362 us.
         const size_t numbers = kv_heads * (size_t)c.big.n.by;
         const size_t slots = (d == 64 ? 3 : 2) * (units / 8 * 8);
         const bool ragged = c.big.tiles.by == 0;
         const size_t held = ragged ? kv_heads * (tokens * group / kBigRows + 1) : numbers;   // (the numbers without those that may be unused)
-        const double mean = ragged ? 0.6 : window > 0 || block_tokens >= max_q || max_q > max_len ? 1.0   // of the longest walk
-                                                                                               : 1.0 - 0.5 * (double)(max_q - block_tokens) / (double)max_len;
-        const bool varied = mean < 0.8;
+        const bool in_window = steps < (max_len / kPart + 3) / 4;
+        const double later = block_tokens < max_q && max_q <= max_len ? (double)(max_q - block_tokens) : 0.0;   // rows behind the first block's
+        const double mean = in_window ? 1.0 : ragged ? 0.6 : 1.0 - 0.5 * later / (double)max_len;   // of the longest walk
+        const bool varied = ragged || mean < 0.8;
         auto steps_us = [&](double n, double wgs) {
             const int at_once = wgs <= (double)units ? 0 : wgs <= 2.0 * (double)units ? 1 : 2;
             const double wide[] = {1.07, 1.49, 1.49}, narrow[] = {0.67, 0.97, 1.26}, bytes = 64.0 * (double)(four ? d + d / 16 : 4 * d);
@@ -1188,8 +1189,8 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         double best = 0;
         const size_t rounds_before = varied ? 0 : held / slots;
         for (size_t keep = 0; keep <= std::min<size_t>(rounds_before, 2); keep++) {
-            const size_t full = keep == 0 ? 0 : (rounds_before - (keep - 1)) * slots, rest = held - full;
-            if (rest == 0) continue;   // (full only where walks are alike: held is numbers)
+            const size_t full = keep == 0 ? 0 : (rounds_before - (keep - 1)) * slots, rest = held - full;   // (full only where walks are alike: held is numbers)
+            if (rest == 0) continue;
             for (size_t k = 1; k <= 64 && k <= steps; k++) {
                 const size_t chunk = (steps + k - 1) / k, shares = (steps + chunk - 1) / chunk, wgs = rest * shares;
                 double cost = (double)(full / slots) * steps_us((double)steps, (double)slots);
@@ -1200,7 +1201,8 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
                 } else {
                     cost += (double)(wgs / slots) * steps_us((double)chunk * mean, (double)slots) + steps_us((double)chunk * mean, (double)(wgs % slots)) * (wgs % slots != 0);
                 }
-                if (shares > 1) cost += 2.0 + (double)(shares * std::min(rest * kBigRows, tokens * heads)) * std::min(1.0, mean + 0.1) * 8.0 * (double)d / 5.5e6 + 0.01 * (double)(numbers - full);
+                if (shares > 1)
+                    cost += 2.0 + (double)(shares * std::min(rest * kBigRows, tokens * heads)) * std::min(1.0, mean + 0.1) * 8.0 * (double)d / 5.5e6 + 0.01 * (double)(numbers - full);
                 if ((keep == 0 && k == 1) || cost < 0.97 * best) best = cost, c.big_full = full, c.big_chunk = chunk, c.big_chunks = shares;
             }
         }
