@@ -171,6 +171,45 @@ def test_append_stores_the_plain_values_bit_for_bit(fv, four, d, page, halves, i
             assert np.array_equal(x.float().cpu().numpy().astype(np.float64), want), (name, out16)
 
 
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("in16", [False, True])
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_append_in_every_form(fv, d, halves, in16, four):
+    """Each kind of pages, inputs, pairs and head sizes: keys and queries turned, values as they are, bit for bit; with queries and
+    without."""
+    import torch
+
+    announce(f"paged append: every form d={d} halves={halves} in16={in16} four={four}")
+    kvh, heads = 5, 15
+    for with_q in (True, False):
+        w = World(fv, 500 + d, [40, 7, 100], [33, 7, 3], kvh, d, 32, four)
+        n = w.rows()
+        k, v, q = (w.rng.standard_normal((n, h, d)).astype(np.float32) * 3 for h in (kvh, kvh, heads))
+        if in16:
+            k, v, q = pu.bf16(k), pu.bf16(v), pu.bf16(q)
+        cos, sin = tables(100, d, halves)
+        pos = np.concatenate([np.arange(w.lens[s] - c, w.lens[s]) for s, c in enumerate(w.counts)])
+        to = lambda x: w.dev(x).to(torch.bfloat16 if in16 else torch.float32)  # noqa: E731
+        got_q = fv.paged_append(w.pool, w.batch, to(k), to(v), rope=(w.dev(cos), w.dev(sin)), halves=halves, q=to(q) if with_q else None)
+        got, got_s = w.pull()
+        if with_q:
+            assert np.array_equal(got_q.float().cpu().numpy(), pu.bf16(pu.rotate(q, cos, sin, pos, halves)))
+        else:
+            assert got_q is None
+        for name, x in (("k", pu.rotate(k, cos, sin, pos, halves)), ("v", v)):
+            for s, c in enumerate(w.counts):
+                part = slice(w.starts[s], w.starts[s] + c)
+                p, t = w.table[s, pos[part] // 32], pos[part] % 32
+                if four:
+                    w.host[name][p, :, t], w.scales[name][p, :, t] = pu.quantize4(x[part])
+                else:
+                    w.host[name][p, :, t] = pu.bf16(x[part])
+            assert np.array_equal(got[name], w.host[name]), name
+            if four:
+                assert np.array_equal(got_s[name], w.scales[name]), name
+
+
 def test_append_without_tables_and_with_rows_of_its_own(fv):
     """No rotation; then a table row for each token (tokens of a frame that share an angle, a token twice)."""
     import torch
