@@ -96,8 +96,8 @@ struct PagedAttnParams {
     int big_full, big_rest;
     PagedDiv big_set, big_set_shares;
     int xcds;                   // 2^xcds XCDs share a run of items
-    // Shares: values, each normalised, and the base-2 logarithm of its sum. Of paged_rows_kernel [chunks][tokens * heads][d] and
-    // [chunks][tokens * heads], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
+    // Shares: values, each normalised, and the base-2 logarithm of its sum. Of paged_rows_kernel [chunks][`few` rows of each (sequence, key head)][d] and
+    // [chunks][these rows], of paged_tiles_kernel [chunks][128 rows of each tile that is cut] likewise.
     float *rows_o, *rows_lse, *big_o, *big_lse;
     long big_rows;              // the latter's rows
     // paged_join_kernel: the first join_tiles workgroups those of the cut tiles, then join_few each of a (sequence, key head) of few rows
@@ -592,11 +592,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
                     val[c] = a * k;
                 }
                 if (split) {
-                    const size_t all = (size_t)p.b.tokens * p.heads;
-                    float* po = p.rows_o + ((size_t)chunk * all + dst) * D + cc;
+                    const size_t share = ((size_t)chunk * p.b.seqs * p.kv_heads.by + (size_t)seq * p.kv_heads.by + kvh) * p.few + r;
+                    float* po = p.rows_o + share * D + cc;
 #pragma unroll
                     for (int c = 0; c < kPer; c += 4) *reinterpret_cast<f32x4*>(po + c) = f32x4{val[c], val[c + 1], val[c + 2], val[c + 3]};
-                    if (cc == 0) p.rows_lse[(size_t)chunk * all + dst] = lds_row[rr][1];
+                    if (cc == 0) p.rows_lse[share] = lds_row[rr][1];
                 } else if (p.out_is_bf16) {
                     __attribute__((ext_vector_type(kPer))) float f;
 #pragma unroll
@@ -1055,11 +1055,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     const int rows = sq.count * p.group.by, t = paged_quot(r, p.group);
     const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
     int chunks = 0;
-    size_t first = dst, step = (size_t)p.b.tokens * p.heads;   // the row's place in the first share, rows to the next
+    size_t first = 0, step = 0;   // the row's place in the first share, rows to the next
     if (r < rows && few == (rows <= p.few)) {
         auto shares = [&](const auto& walk, int parts, const PagedDiv& chunk) { return paged_quot((walk.n + parts - 1) / parts + chunk.by - 1, chunk); };
         if (few) {
             const int row0 = r & -p.rows_m;
+            first = ((size_t)seq * p.kv_heads.by + kvh) * p.few + r;
+            step = (size_t)p.b.seqs * p.kv_heads.by * p.few;
             chunks = shares(paged_walk<kStep>(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + p.rows_m, rows) - 1, p.group)), 1, p.rows_chunk);
         } else {
             const int row0 = r & -kBigRows;
@@ -1193,6 +1195,7 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
             if (rest == 0) continue;
             for (size_t k = 1; k <= 64 && k <= steps; k++) {
                 const size_t chunk = (steps + k - 1) / k, shares = (steps + chunk - 1) / chunk, wgs = rest * shares;
+                if (k > 1 && shares * (numbers - full) * kBigRows * d * 4 > (size_t)1 << 30) break;   // (shares of a gigabyte at most)
                 double cost = (double)(full / slots) * steps_us((double)steps, (double)slots);
                 if (varied) {
                     const double each = std::max(1.0, (double)shares * mean), all = (double)rest * each, at_once = std::min(all, (double)slots);
@@ -1235,13 +1238,16 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
 // The shares' places in the workspace.
 struct PagedParts {
     size_t rows_o = 0, rows_lse = 0, big_o = 0, big_lse = 0, big_rows = 0, bytes = 0;   // rows_o ..: bytes from its start
-    PagedParts(const PagedCut& c, size_t tokens, size_t heads, size_t kv_heads, size_t d) {
+    PagedParts(const PagedCut& c, size_t seqs, size_t kv_heads, size_t d) {
         auto take = [this](size_t n) {
             const size_t at = bytes;
             bytes += (n + 255) / 256 * 256;
             return at;
         };
-        if (c.nt && c.rows_chunks > 1) rows_o = take(c.rows_chunks * tokens * heads * d * 4), rows_lse = take(c.rows_chunks * tokens * heads * 4);
+        if (c.nt && c.rows_chunks > 1) {
+            const size_t rows = seqs * kv_heads * c.few;
+            rows_o = take(c.rows_chunks * rows * d * 4), rows_lse = take(c.rows_chunks * rows * 4);
+        }
         if (c.big.n.by && c.big_chunks > 1) {
             big_rows = (kv_heads * (size_t)c.big.n.by - c.big_full) * kBigRows;
             big_o = take(c.big_chunks * big_rows * d * 4), big_lse = take(c.big_chunks * big_rows * 4);
@@ -1260,7 +1266,7 @@ size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t 
     size_t most = 0;   // of both kinds of pages
     for (const bool four : {false, true}) {
         const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
-        most = std::max(most, fv::PagedParts(c, tokens, heads, kv_heads, d).bytes);
+        most = std::max(most, fv::PagedParts(c, seqs, kv_heads, d).bytes);
     }
     return most;
 }
@@ -1288,11 +1294,11 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     if (max_q > tokens) max_q = tokens;
     const bool four = k_scales != nullptr;
     fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, max_q, max_len, block_tokens, window, sink);
-    fv::PagedParts parts(c, tokens, heads, kv_heads, d);
+    fv::PagedParts parts(c, seqs, kv_heads, d);
     if (parts.bytes > 0 && (!workspace || workspace_bytes < parts.bytes)) {   // a share is the whole walk
         c.rows_chunk *= c.rows_chunks, c.big_chunk *= c.big_chunks;
         c.rows_chunks = c.big_chunks = 1, c.big_full = 0;
-        parts = fv::PagedParts(c, tokens, heads, kv_heads, d);
+        parts = fv::PagedParts(c, seqs, kv_heads, d);
         workspace = nullptr;
     }
     const bool split = c.chunks() > 1;

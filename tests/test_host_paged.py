@@ -133,3 +133,12 @@ def test_signatures_name_every_argument():
     assert len(_lib.SIGNATURES["fv_paged_append"][1]) == len(ORDER["fv_paged_append"]) + 1
     assert len(_lib.SIGNATURES["fv_paged_attention"][1]) == len(ORDER["fv_paged_attention"]) + 1
     assert all(t in (C.c_void_p, C.c_size_t, C.c_int, C.c_float) for t in _lib.SIGNATURES["fv_paged_attention"][1])
+
+
+def test_workspace_of_long_and_short_sequences(lib):
+    """256 single tokens on up to 131072 keys (32 shares of their 16 rows a key head at most) beside a longer one: the shares take no more
+    than that and a gigabyte for the longer one, whose length does not count for the others."""
+    few = 32 * 256 * 8 * 16 * (128 * 4 + 4)
+    for longest in (1, 4, 100, 2048, 8192):
+        need = lib.fv_paged_attention_workspace_bytes(40, 8, 128, 256, 255 + longest, longest, 131072, 1, 0, 0)
+        assert 0 < need <= few + (1 << 30) * 129 // 128 + 1024, longest
