@@ -42,16 +42,17 @@ FV_DEV int paged_seq_of(const PagedBatch& b, int t) {
 }
 
 // Where row t of the batch lies in the cache: its position (-1: in no sequence, or before one's first token), page (-1 where the
-// pool has no such page) and slot.
+// table or the pool has no such page) and slot. The position is counted from the sequence's whole length: cut to what the table
+// holds, the tokens past it would take the slots, and the angles, of the newest that fit.
 struct PagedPlace {
     int pos, page, slot;
 };
 FV_DEV PagedPlace paged_place(const PagedBatch& b, const PagedPool& pool, int t) {
     const int s = paged_seq_of(b, t);
     const PagedSeq q = paged_seq(b, s);
-    const int pos = q.first_pos() + (t - q.start);
+    const int pos = max(b.lens[s], 0) - q.count + (t - q.start);
     if (t < q.start || t >= q.start + q.count || pos < 0) return {-1, -1, 0};
-    const int page = b.table[(size_t)s * b.table_stride + (pos >> pool.lg)];
+    const int page = pos < b.max_len ? b.table[(size_t)s * b.table_stride + (pos >> pool.lg)] : -1;   // (max_len: the table's slots)
     return {pos, (unsigned)page < (unsigned)pool.pages ? page : -1, pos & ((1 << pool.lg) - 1)};
 }
 

@@ -103,7 +103,8 @@ def _on(device, name):
 def paged_append(pool, batch, k, v, rope=None, halves=False, rope_at=None, q=None):
     """The new tokens' k, v [tokens, kv_heads, d] (f32 or bf16) into the pool, the keys turned by their positions (rows of
     rope = (cos, sin), f32 [rows, d]; rope_at: int32 [tokens], rows in place of the positions). q [tokens, heads, d]: turned
-    likewise and returned, bf16. halves: pairs (i, i + d / 2) instead of (2i, 2i + 1)."""
+    likewise and returned, bf16. halves: pairs (i, i + d / 2) instead of (2i, 2i + 1). A token past the table's columns is not
+    stored; positions are counted from lens, whatever max_len says."""
     dev, kvh, d = pool._device, pool.kv_heads, pool.d
     _on(dev, "paged_append")
     tokens, dtype = k.shape[0], k.dtype

@@ -360,8 +360,8 @@ int fv_kv_cache_update(fv_kv_cache* c, size_t layer, const fv_tensor* k, const f
  * q_start[s] .. q_start[s + 1] (ascending, q_start[0] is the first row's number) of the ragged tensors [tokens, heads, d]: the last
  * tokens of the sequence, in order. Token j lies in slot j % page_tokens of page table[s * table_stride + j / page_tokens],
  * of table_pages columns. Entries of pages that a call does not reach are not read; sequences may share pages that none of
- * them appends to (two tokens of one call in one slot leave a mixture of both). A page number outside the pool is no fault: nothing is
- * written there, it reads as zeros, and its keys are seen by no query. Rows at q_start[seqs] and behind are left as they were, so
+ * them appends to (two tokens of one call in one slot leave a mixture of both). A page number outside the pool is no fault, nor is a
+ * token past the table's columns: nothing is written there, it reads as zeros, and its keys are seen by no query. Rows at q_start[seqs] and behind are left as they were, so
  * a padded batch may be captured into a graph and replayed with other lengths, tables and counts. The arrays are read when the
  * call's work runs.
  *
@@ -373,7 +373,8 @@ int fv_kv_cache_update(fv_kv_cache* c, size_t layer, const fv_tensor* k, const f
  * unfused, one rounding: to bf16, or to 4 bits with the smallest power of two for each 32 channels that takes none of them past
  * the largest code (ties to the even code; a value that is not finite makes its 32 channels not a number). A token whose
  * table row lies outside the tables, or that lies before the first token of its sequence (more rows than tokens), is not
- * stored and its query is zeros. */
+ * stored and its query is zeros. Positions are counted from lens as it is; fv_paged_attention counts its rows' from lens cut to its
+ * max_len, so the two agree where max_len bounds lens, as it should. */
 int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q, size_t q_stride,
                     uint16_t* q_out, int in_is_bf16, size_t heads, const float* cos_t, const float* sin_t, size_t rope_rows,
                     const int32_t* rope_at, int halves, void* k_pages, void* v_pages, void* k_scales, void* v_scales,

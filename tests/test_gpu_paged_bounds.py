@@ -1,0 +1,69 @@
+"""The paged KV cache at the borders of what a call describes."""
+import numpy as np
+import pytest
+
+import paged_util as pu
+from test_gpu_paged import World, tables
+from util import announce
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fv():
+    import torch
+
+    assert torch.cuda.is_available()
+    import fv_sdpa
+
+    fv_sdpa.lib()
+    return fv_sdpa
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("d,page,halves", [(128, 16, False), (64, 32, True)])
+def test_tokens_past_the_table_are_not_stored(fv, four, d, page, halves):
+    """Sequences of more tokens than their table has slots for: the new tokens that fit go to their places under their own
+    angles, the others nowhere (the newest that fits keeps its slot), whose queries are turned like any; all read as zeros."""
+    import torch
+
+    announce(f"paged append: past the table four={four} d={d}")
+    kvh, heads, columns = 2, 4, 2
+    held = columns * page
+    counts = [5, 3, 20, 2, 4]
+    w = World(fv, 51, [held, held, 20, held, held], counts, kvh, d, page, four)
+    lens = [held + 3, held + 8, 20, 2 ** 31 - 1, held]           # 3 tokens past it, all of them, none, all at the far end, none
+    w.batch = fv.PagedBatch(w.batch.q_start, w.dev(np.array(lens, dtype=np.int32)), w.batch.table, 20)
+    n = w.rows()
+    k, v = (pu.bf16(w.rng.standard_normal((n, kvh, d))) for _ in range(2))
+    q = w.queries(heads)
+    rows = held + 20
+    cos, sin = tables(rows, d, halves)
+    to = lambda x: w.dev(x).to(torch.bfloat16)  # noqa: E731
+    got_q = fv.paged_append(w.pool, w.batch, to(k), to(v), rope=(w.dev(cos), w.dev(sin)), halves=halves, q=to(q))
+    pos = np.concatenate([np.arange(m - c, m, dtype=np.int64) for m, c in zip(lens, counts)])
+    at = np.clip(pos, 0, rows - 1)
+    want_q = pu.bf16(pu.rotate(q, cos, sin, at, halves))
+    want_q[pos >= rows] = 0                                      # (no row of the tables)
+    turned = pu.rotate(k, cos, sin, at, halves)
+    fits = pos < held
+    assert fits.sum() == 2 + 0 + 20 + 0 + 4
+    want = {name: np.zeros((n, kvh, d)) for name in "kv"}
+    for s, c in enumerate(counts):
+        for i in range(w.starts[s], w.starts[s] + c):
+            if not fits[i]:
+                continue
+            p, t = w.table[s, pos[i] // page], pos[i] % page
+            for name, x in (("k", turned[i]), ("v", v[i])):
+                if four:
+                    w.host[name][p, :, t], w.scales[name][p, :, t] = pu.quantize4(x)
+                    want[name][i] = pu.values4(w.host[name][p, :, t], w.scales[name][p, :, t])
+                else:
+                    want[name][i] = w.host[name][p, :, t] = pu.bf16(x)
+    got, got_s = w.pull()
+    assert np.array_equal(got_q.float().cpu().numpy(), want_q)
+    for name in "kv":
+        assert np.array_equal(got[name], w.host[name]), name
+        assert not four or np.array_equal(got_s[name], w.scales[name]), name
+    for x, name in zip(fv.paged_read(w.pool, w.batch, n, out_bf16=False), "kv"):
+        assert np.array_equal(x.cpu().numpy().astype(np.float64), want[name]), name
