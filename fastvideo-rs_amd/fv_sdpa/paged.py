@@ -123,6 +123,8 @@ def paged_append(pool, batch, k, v, rope=None, halves=False, rope_at=None, q=Non
     if rope is not None:
         cos, sin = rope
         rows = cos.shape[0]
+        if rows == 0 and tokens:   # (no address: the entry would take them for none, and turn nothing)
+            raise ValueError("paged_append: rope tables without rows")
         for t in rope:
             if t.dtype is not _F32 or t.shape != (rows, d) or not t.is_contiguous() or t.get_device() != dev:
                 raise ValueError(f"paged_append: rope tables must be contiguous f32 [rows, {d}] on the pool's device")

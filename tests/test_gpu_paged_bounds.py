@@ -67,3 +67,20 @@ def test_tokens_past_the_table_are_not_stored(fv, four, d, page, halves):
         assert not four or np.array_equal(got_s[name], w.scales[name]), name
     for x, name in zip(fv.paged_read(w.pool, w.batch, n, out_bf16=False), "kv"):
         assert np.array_equal(x.cpu().numpy().astype(np.float64), want[name]), name
+
+
+def test_rope_tables_without_rows_are_refused(fv):
+    """Every token's row lies outside them: storing the keys unturned is not what was asked."""
+    import torch
+
+    announce("paged append: empty rope tables")
+    w = World(fv, 53, [20], [2], 2, 64, 16)
+    x = torch.zeros((2, 2, 64), device="cuda", dtype=torch.bfloat16)
+    none = torch.empty((0, 64), device="cuda")
+    before = w.pull()[0]
+    with pytest.raises(ValueError, match="rope"):
+        fv.paged_append(w.pool, w.batch, x, x, rope=(none, none))
+    with pytest.raises(ValueError, match="rope"):
+        fv.paged_append(w.pool, w.batch, x, x, rope=(none, none), rope_at=torch.zeros(2, device="cuda", dtype=torch.int32))
+    after = w.pull()[0]
+    assert all(np.array_equal(before[n], after[n]) for n in "kv")
