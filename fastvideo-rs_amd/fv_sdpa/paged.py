@@ -3,6 +3,7 @@ sequences of different lengths in one pool of pages of bf16 or of 4 bits, new to
 positions applied on the way, attention under the block mask with a window and sinks, single tokens to long prompts.
 """
 import math
+from operator import attrgetter
 
 import torch
 
@@ -16,9 +17,11 @@ _ONLY_BF16 = (_BF16,)
 
 class PagedKv:
     """One layer's pool: k, v [pages, kv_heads, page_tokens, d] bf16, or 4-bit codes [.., d / 2] with k_scales, v_scales
-    [.., d / 32] (uint8 all four). The tensors are the caller's, used in place."""
+    [.., d / 32] (uint8 all four). The tensors are the caller's, used in place; their addresses are taken here, so that the
+    fields cannot be set (other tensors are another PagedKv)."""
 
-    __slots__ = ("k", "v", "k_scales", "v_scales", "d", "kv_heads", "_args", "_device")
+    __slots__ = ("_k", "_v", "_k_scales", "_v_scales", "_d", "_kv_heads", "_args", "_device")
+    k, v, k_scales, v_scales, d, kv_heads = (property(attrgetter(n)) for n in __slots__[:6])
 
     def __init__(self, k, v, k_scales=None, v_scales=None):
         four = k_scales is not None
@@ -34,7 +37,7 @@ class PagedKv:
             for t in (k_scales, v_scales):
                 if t.dtype is not _U8 or t.shape != want or not t.is_contiguous() or t.get_device() != dev:
                     raise ValueError(f"PagedKv: want contiguous uint8 scales {want} on the pages' device")
-        self.k, self.v, self.k_scales, self.v_scales, self.d, self.kv_heads, self._device = k, v, k_scales, v_scales, d, shape[1], dev
+        self._k, self._v, self._k_scales, self._v_scales, self._d, self._kv_heads, self._device = k, v, k_scales, v_scales, d, shape[1], dev
         self._args = (k.data_ptr(), v.data_ptr(), k_scales.data_ptr() if four else None, v_scales.data_ptr() if four else None,
                       shape[0], shape[2], shape[1], d)
 
@@ -48,19 +51,21 @@ class PagedKv:
 
     @property
     def four_bits(self):
-        return self.k_scales is not None
+        return self._k_scales is not None
 
     @property
     def page_tokens(self):
-        return self.k.shape[2]
+        return self._k.shape[2]
 
 
 class PagedBatch:
     """The sequences of a call: int32 CUDA tensors q_start [n + 1] (rows of sequence s: q_start[s] .. q_start[s + 1]), lens [n]
     (tokens in the cache, the new ones among them) and table [n, columns] (page numbers); max_q and max_len bound the rows of
-    a sequence and its length (host numbers: the launches are sized by them; max_len None: what the table's columns hold)."""
+    a sequence and its length (host numbers: the launches are sized by them; max_len None: what the table's columns hold). The
+    tensors' addresses are taken here: other numbers go into them, other tensors are another PagedBatch."""
 
-    __slots__ = ("q_start", "lens", "table", "max_q", "max_len", "_args", "_device")
+    __slots__ = ("_q_start", "_lens", "_table", "max_q", "max_len", "_args", "_device")
+    q_start, lens, table = (property(attrgetter(n)) for n in __slots__[:3])
 
     def __init__(self, q_start, lens, table, max_q, max_len=None):
         dev = lens.get_device()
@@ -75,7 +80,7 @@ class PagedBatch:
             raise ValueError("PagedBatch: want contiguous arrays (of the table: rows)")
         if max_q < 0 or (max_len is not None and max_len < 0):
             raise ValueError("PagedBatch: bounds must not be negative")
-        self.q_start, self.lens, self.table, self.max_q, self.max_len, self._device = q_start, lens, table, max_q, max_len, dev
+        self._q_start, self._lens, self._table, self.max_q, self.max_len, self._device = q_start, lens, table, max_q, max_len, dev
         self._args = (q_start.data_ptr(), lens.data_ptr(), table.data_ptr(), step if n > 1 else columns, columns, n)
 
 
@@ -105,7 +110,7 @@ def paged_append(pool, batch, k, v, rope=None, halves=False, rope_at=None, q=Non
     rope = (cos, sin), f32 [rows, d]; rope_at: int32 [tokens], rows in place of the positions). q [tokens, heads, d]: turned
     likewise and returned, bf16. halves: pairs (i, i + d / 2) instead of (2i, 2i + 1). A token past the table's columns is not
     stored; positions are counted from lens, whatever max_len says."""
-    dev, kvh, d = pool._device, pool.kv_heads, pool.d
+    dev, kvh, d = pool._device, pool._kv_heads, pool._d
     _on(dev, "paged_append")
     tokens, dtype = k.shape[0], k.dtype
     dtypes = (dtype,) if dtype is _BF16 or dtype is _F32 else (_F32, _BF16)
@@ -145,7 +150,7 @@ def paged_read(pool, batch, tokens, out_bf16=True):
     _on(dev, "paged_read")
     if batch._device != dev:
         raise ValueError("paged_read: the batch is on another device")
-    k = torch.empty((tokens, pool.kv_heads, pool.d), device=pool.k.device, dtype=_BF16 if out_bf16 else _F32)
+    k = torch.empty((tokens, pool._kv_heads, pool._d), device=pool._k.device, dtype=_BF16 if out_bf16 else _F32)
     v = torch.empty_like(k)
     _lib.check(_lib.lib().fv_paged_read(k.data_ptr(), v.data_ptr(), 1 if out_bf16 else 0, *pool._args, *batch._args, tokens, _lib.stream()))
     return k, v
@@ -155,7 +160,7 @@ def paged_attention(q, pool, batch, mask=None, scale=None, out_bf16=True, out=No
     """softmax(scale q k^T) v of the rows q [tokens, heads, d] (bf16) over the cached keys of their sequences, [tokens, heads, d].
     mask: a BlockCausal; None: causal by token. A sink block is not seen before its time (BlockCausal.allows has it always
     seen). Rows behind the last sequence are not written."""
-    dev, kvh, d = pool._device, pool.kv_heads, pool.d
+    dev, kvh, d = pool._device, pool._kv_heads, pool._d
     _on(dev, "paged_attention")
     heads, qs = _rows(q, "q", 0, d, _ONLY_BF16, dev)
     if batch._device != dev:
@@ -166,7 +171,7 @@ def paged_attention(q, pool, batch, mask=None, scale=None, out_bf16=True, out=No
         out = torch.empty_like(q) if out_bf16 and q.is_contiguous() else torch.empty((tokens, heads, d), device=q.device, dtype=dtype)
     elif out.dtype is not dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(q.shape)} on {q.device}")
-    max_len = batch.max_len if batch.max_len is not None else batch.table.shape[1] * pool.page_tokens
+    max_len = batch.max_len if batch.max_len is not None else batch._table.shape[1] * pool._k.shape[2]
     bt, window, sink = (mask.block_tokens, mask.window, mask.sink) if mask is not None else (1, 0, 0)
     n = batch._args[5]
     lib = _lib.lib()
