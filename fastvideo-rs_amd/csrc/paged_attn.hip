@@ -1260,14 +1260,17 @@ struct PagedParts {
 
 extern "C" {
 
+size_t fv_paged_attention_workspace_bytes_for(int four_bits, size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q,
+                                              size_t max_len, size_t block_tokens, size_t window, size_t sink) {
+    if (kv_heads == 0 || heads < kv_heads || heads % kv_heads != 0 || block_tokens == 0 || seqs == 0 || tokens == 0 || max_q == 0) return 0;
+    const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four_bits != 0, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
+    return fv::PagedParts(c, seqs, kv_heads, d).bytes;
+}
 size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q, size_t max_len,
                                           size_t block_tokens, size_t window, size_t sink) {
-    if (kv_heads == 0 || heads < kv_heads || heads % kv_heads != 0 || block_tokens == 0 || seqs == 0 || tokens == 0 || max_q == 0) return 0;
-    size_t most = 0;   // of both kinds of pages
-    for (const bool four : {false, true}) {
-        const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
-        most = std::max(most, fv::PagedParts(c, seqs, kv_heads, d).bytes);
-    }
+    size_t most = 0;
+    for (const int four : {0, 1})
+        most = std::max(most, fv_paged_attention_workspace_bytes_for(four, heads, kv_heads, d, seqs, tokens, max_q, max_len, block_tokens, window, sink));
     return most;
 }
 

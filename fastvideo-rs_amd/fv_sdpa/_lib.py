@@ -57,6 +57,7 @@ SIGNATURES = {
                                   _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
     "fv_paged_read": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _sz,
                                 _vp]),
+    "fv_paged_attention_workspace_bytes_for": (_sz, [C.c_int] + [_sz] * 10),
     "fv_paged_attention_workspace_bytes": (_sz, [_sz] * 10),
     "fv_paged_attention": (C.c_int, [_vp, _sz, _vp, C.c_int, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz,
                                      _sz, _sz, _sz, _sz, _sz, C.c_float, _sz, _sz, _sz, _vp, _sz, _vp]),

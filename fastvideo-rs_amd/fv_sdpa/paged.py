@@ -175,7 +175,7 @@ def paged_attention(q, pool, batch, mask=None, scale=None, out_bf16=True, out=No
     bt, window, sink = (mask.block_tokens, mask.window, mask.sink) if mask is not None else (1, 0, 0)
     n = batch._args[5]
     lib = _lib.lib()
-    nbytes = lib.fv_paged_attention_workspace_bytes(heads, kvh, d, n, tokens, batch.max_q, max_len, bt, window, sink)
+    nbytes = lib.fv_paged_attention_workspace_bytes_for(pool._k_scales is not None, heads, kvh, d, n, tokens, batch.max_q, max_len, bt, window, sink)
     work = torch.empty(nbytes, device=q.device, dtype=_U8) if nbytes else None
     _lib.check(lib.fv_paged_attention(
         q.data_ptr(), qs, out.data_ptr(), 1 if out_bf16 else 0, heads, *pool._args, *batch._args, tokens, batch.max_q, max_len,

@@ -393,9 +393,12 @@ int fv_paged_read(void* k_out, void* v_out, int out_is_bf16, const void* k_pages
  * tj <= ti && (window == 0 || ti - tj < window || tj < sink): a sink block is not seen before its time. block_tokens == 1: causal by
  * token, a window of tokens, sink tokens. A row that sees no key is zeros. max_q / max_len: bounds of the rows of a sequence and of
  * lens, host numbers that the launch is sized by (longer lengths are cut to max_len, rows past max_q may not be written).
- * workspace: fv_paged_attention_workspace_bytes of the same numbers (0: none), 256-byte aligned, this call's alone until its work
- * is done; where it is too small or NULL long walks are not split, which costs time only (and bits: shares are
- * normalised before they are joined). The results of a call with the same bounds and workspace are the same bits. */
+ * workspace: fv_paged_attention_workspace_bytes_for the pool's kind of pages (four_bits: with scales) and the same numbers (0: none;
+ * fv_paged_attention_workspace_bytes: enough for either kind), 256-byte aligned, this call's alone until its work is done; where
+ * it is too small or NULL long walks are not split, which costs time only (and bits: shares are normalised before they are
+ * joined). The results of a call with the same bounds and workspace are the same bits. */
+size_t fv_paged_attention_workspace_bytes_for(int four_bits, size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens,
+                                              size_t max_q, size_t max_len, size_t block_tokens, size_t window, size_t sink);
 size_t fv_paged_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q,
                                           size_t max_len, size_t block_tokens, size_t window, size_t sink);
 int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is_bf16, size_t heads, const void* k_pages,

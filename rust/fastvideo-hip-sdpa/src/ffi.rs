@@ -117,6 +117,7 @@ extern "C" {
     pub fn fv_kv_cache_update(c: *mut FvKvCache, layer: usize, k: *const FvTensor, v: *const FvTensor, current_start: usize, k_window: *mut FvTensor, v_window: *mut FvTensor, stream: *mut c_void) -> c_int;
     pub fn fv_paged_append(k: *const c_void, k_stride: usize, v: *const c_void, v_stride: usize, q: *const c_void, q_stride: usize, q_out: *mut u16, in_is_bf16: c_int, heads: usize, cos_t: *const f32, sin_t: *const f32, rope_rows: usize, rope_at: *const i32, halves: c_int, k_pages: *mut c_void, v_pages: *mut c_void, k_scales: *mut c_void, v_scales: *mut c_void, pages: usize, page_tokens: usize, kv_heads: usize, d: usize, q_start: *const i32, lens: *const i32, table: *const i32, table_stride: usize, table_pages: usize, seqs: usize, tokens: usize, stream: *mut c_void) -> c_int;
     pub fn fv_paged_read(k_out: *mut c_void, v_out: *mut c_void, out_is_bf16: c_int, k_pages: *const c_void, v_pages: *const c_void, k_scales: *const c_void, v_scales: *const c_void, pages: usize, page_tokens: usize, kv_heads: usize, d: usize, q_start: *const i32, lens: *const i32, table: *const i32, table_stride: usize, table_pages: usize, seqs: usize, tokens: usize, stream: *mut c_void) -> c_int;
+    pub fn fv_paged_attention_workspace_bytes_for(four_bits: c_int, heads: usize, kv_heads: usize, d: usize, seqs: usize, tokens: usize, max_q: usize, max_len: usize, block_tokens: usize, window: usize, sink: usize) -> usize;
     pub fn fv_paged_attention_workspace_bytes(heads: usize, kv_heads: usize, d: usize, seqs: usize, tokens: usize, max_q: usize, max_len: usize, block_tokens: usize, window: usize, sink: usize) -> usize;
     pub fn fv_paged_attention(q: *const u16, q_stride: usize, out: *mut c_void, out_is_bf16: c_int, heads: usize, k_pages: *const c_void, v_pages: *const c_void, k_scales: *const c_void, v_scales: *const c_void, pages: usize, page_tokens: usize, kv_heads: usize, d: usize, q_start: *const i32, lens: *const i32, table: *const i32, table_stride: usize, table_pages: usize, seqs: usize, tokens: usize, max_q: usize, max_len: usize, scale: f32, block_tokens: usize, window: usize, sink: usize, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn fv_vsa_topk_for(sparsity: f64, num_tiles: usize) -> usize;

@@ -84,3 +84,26 @@ def test_rope_tables_without_rows_are_refused(fv):
         fv.paged_append(w.pool, w.batch, x, x, rope=(none, none), rope_at=torch.zeros(2, device="cuda", dtype=torch.int32))
     after = w.pull()[0]
     assert all(np.array_equal(before[n], after[n]) for n in "kv")
+
+
+def test_drafts_over_bf16_pages_allocate_their_result_alone(fv):
+    """64 sequences of 9 drafts, a bound of 131072 keys: no shares (over 4 bits there are, 380 MB)."""
+    import torch
+
+    announce("paged attention: memory of a call of drafts")
+    seqs, rows, heads, kvh, d, page = 64, 9, 40, 8, 128, 64
+    pool = fv.PagedKv.new(seqs, page, kvh, d)
+    columns = 131072 // page
+    table = torch.full((seqs, columns), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(seqs, device="cuda")
+    start = torch.arange(seqs + 1, device="cuda", dtype=torch.int32) * rows
+    batch = fv.PagedBatch(start, torch.full((seqs,), 50, dtype=torch.int32, device="cuda"), table, rows)
+    q = torch.zeros((seqs * rows, heads, d), device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = fv.paged_attention(q, pool, batch)
+    torch.cuda.synchronize()
+    assert not out.any()
+    more = torch.cuda.max_memory_allocated() - before
+    assert more <= out.numel() * 2 + (1 << 20), more
