@@ -1147,6 +1147,7 @@ PagedPieces paged_pieces(size_t r, size_t seqs, size_t tokens, size_t max_q, siz
     return like <= ragged ? PagedPieces{paged_div(std::min(like, most)), paged_div(std::min(tiles, most))}
                           : PagedPieces{paged_div(std::min(ragged, most)), paged_div(0)};
 }
+constexpr size_t kMostShares = (size_t)1 << 30;   // bytes of a kernel's shares: past it its walks are cut less
 // How a call is cut.
 struct PagedCut {
     size_t few = 0;                         // rows a key head up to which a sequence is paged_rows_kernel's
@@ -1195,7 +1196,7 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
             if (rest == 0) continue;
             for (size_t k = 1; k <= 64 && k <= steps; k++) {
                 const size_t chunk = (steps + k - 1) / k, shares = (steps + chunk - 1) / chunk, wgs = rest * shares;
-                if (k > 1 && shares * (numbers - full) * kBigRows * d * 4 > (size_t)1 << 30) break;   // (shares of a gigabyte at most)
+                if (k > 1 && shares * (numbers - full) * kBigRows * d * 4 > kMostShares) break;
                 double cost = (double)(full / slots) * steps_us((double)steps, (double)slots);
                 if (varied) {
                     const double each = std::max(1.0, (double)shares * mean), all = (double)rest * each, at_once = std::min(all, (double)slots);
@@ -1229,6 +1230,10 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
         size_t shares = steps <= 192 ? 1 : (steps + 127) / 128;
         const size_t fill = std::min((four ? 2 : 1) * units / base, std::max(steps / 8, std::min<size_t>(steps / 4, 16)));
         if (steps >= 36 && fill >= (steps < 96 ? 3 : 2)) shares = std::max(shares, fill);
+        // (max_len is a bound that lengths may be far below. 256 sequences of 9 drafts, 32 / 8 heads, over 4 bits, 500 to 30000 keys: under
+        // a bound of 2^20 9.7 GB of shares of 128 steps 2.89 ms, a gigabyte 3.31, its walks being whole; of 12 drafts, 40 / 8 heads, under 2^17
+        // 2.03 GB 2.20 ms, a gigabyte 1.98.)
+        shares = std::min(shares, std::max<size_t>(kMostShares / (seqs * kv_heads * c.few * d * 4), 1));
         size_t chunk = ((steps + shares - 1) / shares + kWaves - 1) / kWaves * kWaves;
         c.rows_chunk = chunk;
         c.rows_chunks = (steps + chunk - 1) / chunk;

@@ -1,4 +1,4 @@
-"""The workspace of attention over pages: of the call's own kind of pages. Host arithmetic, no GPU."""
+"""The workspace of attention over pages: of the call's own kind of pages, and limited. Host arithmetic, no GPU."""
 import itertools
 
 import pytest
@@ -35,3 +35,18 @@ def test_nothing_for_numbers_that_no_call_takes(lib):
         for bad in (dict(heads=3), dict(kv_heads=0), dict(seqs=0), dict(tokens=0), dict(max_q=0), dict(block=0)):
             n = {"heads": 4, "kv_heads": 2, "d": 128, "seqs": 3, "tokens": 5, "max_q": 2, "max_len": 1 << 20, "block": 1, "window": 0, "sink": 0, **bad}
             assert need(kind, *n.values()) == 0, bad
+
+
+def test_shares_are_limited(lib):
+    """Whatever the bounds: a gigabyte of shares for each of the two kernels, a sum beside every row of them (1 / d of that), and
+    what rounding to 256 bytes adds."""
+    worst = 0
+    for kind, d, (heads, kvh) in itertools.product((0, 1), (64, 128), ((40, 8), (64, 8), (12, 12), (16, 1), (32, 2))):
+        for seqs, rows, most in itertools.product((1, 16, 256, 1024, 20000), (1, 2, 12, 60), (None, 700, 8192)):
+            for longest, window in itertools.product((4096, 131072, 1 << 20, (1 << 31) - 64), (0, 100000)):
+                tokens, max_q = (seqs * rows, rows) if most is None else (seqs - 1 + most, most)
+                worst = max(worst, lib.fv_paged_attention_workspace_bytes_for(kind, heads, kvh, d, seqs, tokens, max_q, longest, 1, window, 4))
+    assert worst <= 2 * ((1 << 30) * 65 // 64 + 512), worst
+    # (9.7 GB for 19 MB of results without the limit; these are cut as far as it lets them)
+    drafts = lib.fv_paged_attention_workspace_bytes_for(1, 32, 8, 128, 256, 256 * 9, 9, 1 << 20, 1, 0, 0)
+    assert (1 << 29) < drafts <= (1 << 30) * 129 // 128 + 512
