@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kStep = 32;       // keys a wave takes at a time
 constexpr int kWaves = 4;
+constexpr float kLeast = 0x1p-149f;   // the weight of a seen key that vanished, where its value is not finite
 
 // Division of a number below 2^31 by one that the host knows, as a product and a shift: with 2^l >= by, mul = 2^(31 + l) / by rounded up is
 // too large by less than 1, so n mul / 2^(31 + l) by less than 1 / by. (The compiler's own takes 20 instructions and waits for a
@@ -114,6 +115,7 @@ struct PagedSight {
         return below(a - k) | (below(hi - k) & ~below(lo - k));
     }
     static FV_DEV unsigned below(int n) { return (1u << min(max(n, 0), 8)) - 1u; }
+    FV_DEV bool one(int k) const { return k < a || (k >= lo && k < hi); }
 };
 template <class Params>
 FV_DEV PagedSight paged_sight(const Params& p, int pos, int len) {
@@ -419,8 +421,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
         // values that no row sees are zeros, whatever they are
         unsigned used = whole ? 0xffu : w.any.eight(k0 + 8 * g) & ((good >> (g >> 1)) & 1 ? 0xffu : 0u);
         if (!whole && t0 != t1) {
-            // A value that is not finite belongs to the rows that see it: a probability of zero does not keep it from the others.
-            // Its key leaves the product, and the rows that have a share in it add theirs one by one. (Rare.)
+            // A value that is not finite belongs to the rows that see it, whatever its weight: a probability of zero does not keep it
+            // from the others. Its key leaves the product, and the rows that see it add their shares one by one. (Rare.)
             float bad[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             auto look = [&](auto x) {
                 unsigned vw[8];
@@ -451,6 +453,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttnParam
                         const u32x4 all = __builtin_bit_cast(u32x4, pr[n]);
                         const unsigned pair = j < 4 ? (j < 2 ? all[0] : all[1]) : (j < 6 ? all[2] : all[3]);
                         pj[n] = __shfl(__builtin_bit_cast(float, j & 1 ? pair & 0xffff0000u : pair << 16), 16 * h + col, 64);
+                        if (pj[n] == 0.f && see[n].one(k0 + x)) pj[n] = kLeast;
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -801,8 +804,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     ProbTile pb;
 
     // The second pass, a tile that some of the workgroup's rows see a part of: a value that is not finite belongs to the rows that see
-    // it, and a probability of zero does not keep it from the others. Such keys leave the V tile, and the rows that have a share
-    // in one add theirs from the pool. (The first pass ends in the check where there is such a value.)
+    // it, whatever its weight, and a probability of zero does not keep it from the others. Such keys leave the V tile, and the rows
+    // that see one add their share of it from the pool. (The first pass ends in the check where there is such a value.)
     const Whole wg_whole = whole_parts(paged_all(p, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kBigRows, rows) - 1, p.group)));
     auto set_apart = [&](int m, int e, const ProbTile& pb, f32x4 (&o)[kNO][2]) {
         lds_u8* mine_v = vbuf(m) + 16 * wave * G::kRow;
@@ -840,6 +843,8 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
                 const u32x4 half = x < 32 ? lo : hi;
                 const unsigned pair = (x & 16) ? ((x & 2) ? half[3] : half[2]) : ((x & 2) ? half[1] : half[0]);
                 pj[g] = __shfl(__builtin_bit_cast(float, x & 1 ? pair & 0xffff0000u : pair << 16), 16 * ((x >> 2) & 3) + i16, 64);
+                const PagedSight row_sees = {__shfl(mine.a, 16 * g + i16, 64), __shfl(mine.lo, 16 * g + i16, 64), __shfl(mine.hi, 16 * g + i16, 64)};
+                if (pj[g] == 0.f && row_sees.one(key)) pj[g] = kLeast;
             }
 #pragma unroll
             for (int db = 0; db < kNO; db++) {

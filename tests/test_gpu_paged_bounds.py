@@ -107,3 +107,49 @@ def test_drafts_over_bf16_pages_allocate_their_result_alone(fv):
     assert not out.any()
     more = torch.cuda.max_memory_allocated() - before
     assert more <= out.numel() * 2 + (1 << 20), more
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("lens,counts,heads,mask", [([45, 20], [3, 2], 2, (1, 0, 0)), ([45, 200], [7, 9], 4, (1, 12, 2)), ([300], [150], 2, (1, 0, 0)),
+                                                    ([260, 90], [140, 70], 4, (1, 40, 3)), ([240], [96], 4, (48, 0, 0))])
+def test_a_value_that_is_not_finite_reaches_rows_whose_weight_for_it_vanishes(fv, four, lens, counts, heads, mask):
+    """Its key scores 300 below the others, so that its weight is less than any f32; a row that sees it is not a number all the
+    same (as where every row of the tile sees it), a row that does not is as always."""
+    import torch
+
+    d, kvh, page = 128, 2, 16
+    announce(f"paged: a vanishing weight on NaN four={four} {lens} {mask}")
+    for back in (1, 5, 20):                                      # the planted key, from the first new token back
+        w = World(fv, 57, lens, counts, kvh, d, page, four)
+        for s, n in enumerate(lens):
+            j = np.arange(n)
+            keys = np.zeros((n, kvh, d), dtype=np.float32)
+            bad = [x for x in (n - counts[s] - back, n - counts[s] + counts[s] // 2) if x >= 0]
+            keys[bad] = -6.0
+            p, t = w.table[s, j // page], j % page
+            if four:
+                w.host["k"][p, :, t], w.scales["k"][p, :, t] = pu.quantize4(keys)
+            else:
+                w.host["k"][p, :, t] = keys
+            for x in bad:
+                if four:
+                    w.scales["v"][w.table[s, x // page], 1, x % page, -1] = 255
+                else:
+                    w.host["v"][w.table[s, x // page], 1, x % page, 5] = np.nan
+        w.push()
+        q = np.full((w.rows(), heads, d), 4.5, dtype=np.float32)   # -6 x 4.5 x 128 / sqrt(128) = -305
+        got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False).cpu().numpy()
+        some = False
+        for s, n in enumerate(counts):
+            part = slice(w.starts[s], w.starts[s] + n)
+            k, v = w.held("k", s), w.held("v", s)
+            seen = pu.sees(np.arange(n) + lens[s] - n, np.arange(lens[s]), *mask)
+            finite = np.stack([~(seen[:, :, None] & ~np.isfinite(v[:, h * kvh // heads])[None]).any(1) for h in range(heads)], 1)
+            x = got[part]
+            wrong = int((np.isfinite(x) != finite).sum())
+            assert wrong == 0, f"back={back}: sequence {s}: {wrong} of {x.size} values are numbers where they are none, or the reverse"
+            out, mag = pu.attention(q[part], k, np.nan_to_num(v, nan=0.0), lens[s] - n, d ** -0.5, *mask)
+            off = np.where(finite, np.abs(x - out) - pu.attention_bound(out, mag, False, 1.45 * 306), -1.0)
+            assert off.max() <= 0, (back, s, off.max())
+            some |= bool((~finite).any() and finite[:, -1].any())
+        assert some or back > 1
