@@ -153,3 +153,31 @@ def test_a_value_that_is_not_finite_reaches_rows_whose_weight_for_it_vanishes(fv
             assert off.max() <= 0, (back, s, off.max())
             some |= bool((~finite).any() and finite[:, -1].any())
         assert some or back > 1
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("counts", [[1, 1, 2], [90, 1, 150]])
+def test_entries_that_no_row_reaches_may_hold_anything(fv, four, page, counts):
+    """Pages that lie wholly outside a window and its sinks, or behind the last token: numbers outside the pool, and of a page of
+    NaN that is another's (a window's pages given away)."""
+    announce(f"paged: entries out of reach four={four} page={page} {counts}")
+    lens, mask = [1003, 37, 777], (1, 70, 5)
+    w = World(fv, 61, lens, counts, 2, 128, page, four, columns=-(-1003 // page) + 2)
+    other = next(p for p in range(w.pages) if not (w.table == p).any())   # (a spare page, no sequence's)
+    for name in "kv":
+        if four:
+            w.scales[name][other] = 255
+        else:
+            w.host[name][other] = np.nan
+    w.push()
+    reached = np.zeros(w.table.shape, dtype=bool)
+    for s, (n, c) in enumerate(zip(lens, counts)):
+        seen = pu.sees(np.arange(c) + n - c, np.arange(n), *mask).any(0)
+        reached[s, np.unique(np.nonzero(seen)[0] // page)] = True
+    assert (~reached).sum() > 5
+    q = w.queries(4)
+    for stale in (other, -1, w.pages, 2 ** 31 - 1, -2 ** 31):
+        w.batch = fv.PagedBatch(w.batch.q_start, w.batch.lens, w.dev(np.where(reached, w.table, np.int32(stale))), max(counts), max(lens))
+        got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False)
+        w.check(q, got, f"stale {stale} page={page} {counts}", *mask)
