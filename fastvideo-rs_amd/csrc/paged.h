@@ -31,13 +31,16 @@ struct PagedBatch {
 
 struct PagedSeq {
     int start, count, len;   // first row, rows, tokens in the cache
-    FV_DEV int first_pos() const { return len - count; }   // of row `start`; negative where there are more rows than tokens
+    int behind;              // the row behind its last token, which the call's tensors need not have
+    FV_DEV int first_pos() const { return pos_of(len); }   // of row `start`; negative where there are more rows than tokens
+    FV_DEV int pos_of(int length) const { return length - (behind - start); }
 };
 template <class Batch>   // (PagedBatch, or the same struct read through another address space)
 FV_DEV PagedSeq paged_seq(const Batch& b, int s) {
     PagedSeq q;
     q.start = min(max(b.q_start[s], 0), b.tokens);
-    q.count = min(max(b.q_start[s + 1], q.start), b.tokens) - q.start;
+    q.behind = max(b.q_start[s + 1], q.start);
+    q.count = min(q.behind, b.tokens) - q.start;
     q.len = min(max(b.lens[s], 0), b.max_len);
     return q;
 }

@@ -50,7 +50,7 @@ struct PagedPlace {
 FV_DEV PagedPlace paged_place(const PagedBatch& b, const PagedPool& pool, int t) {
     const int s = paged_seq_of(b, t);
     const PagedSeq q = paged_seq(b, s);
-    const int pos = max(b.lens[s], 0) - q.count + (t - q.start);
+    const int pos = q.pos_of(max(b.lens[s], 0)) + (t - q.start);
     if (t < q.start || t >= q.start + q.count || pos < 0) return {-1, -1, 0};
     const int page = pos < b.max_len ? b.table[(size_t)s * b.table_stride + (pos >> pool.lg)] : -1;   // (max_len: the table's slots)
     return {pos, (unsigned)page < (unsigned)pool.pages ? page : -1, pos & ((1 << pool.lg) - 1)};

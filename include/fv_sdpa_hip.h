@@ -362,8 +362,9 @@ int fv_kv_cache_update(fv_kv_cache* c, size_t layer, const fv_tensor* k, const f
  * of table_pages columns. Entries of pages that a call does not reach (no row sees a token there, none is appended or read) may
  * hold anything; sequences may share pages that none of them appends to (two tokens of one call in one slot leave a mixture of
  * both). A page number outside the pool is no fault, nor is a token past the table's columns: nothing is written there, it reads as
- * zeros, and its keys are seen by no query. Rows at q_start[seqs] and behind are left as they were, so a padded batch may be captured
- * into a graph and replayed with other lengths, tables and counts. The arrays are read when the call's work runs.
+ * zeros, and its keys are seen by no query; nor are rows that the tensors do not have, before their first or behind their last.
+ * Rows at q_start[seqs] and behind are left as they were, so a padded batch may be captured into a graph and replayed with other
+ * lengths, tables and counts. The arrays are read when the call's work runs.
  *
  * fv_paged_append: the new tokens' keys k and values v [tokens, kv_heads, d] into the cache, the keys (and the queries q
  * [tokens, heads, d], into q_out, contiguous bf16 bits; both NULL: none) turned by row rope_at[token] (NULL: by the token's

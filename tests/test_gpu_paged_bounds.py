@@ -181,3 +181,46 @@ def test_entries_that_no_row_reaches_may_hold_anything(fv, four, page, counts):
         w.batch = fv.PagedBatch(w.batch.q_start, w.batch.lens, w.dev(np.where(reached, w.table, np.int32(stale))), max(counts), max(lens))
         got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False)
         w.check(q, got, f"stale {stale} page={page} {counts}", *mask)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("lens,counts,first,rows", [([40, 50], [10, 20], 0, 22), ([40, 50], [3, 2], -2, 20), ([300, 260], [150, 160], -7, 200)])
+def test_rows_that_the_tensors_do_not_have(fv, four, lens, counts, first, rows):
+    """q_start from before the tensors' first row, or to behind their last: the rows that are there are the tokens that q_start says."""
+    import torch
+
+    announce(f"paged: rows past the tensors four={four} {counts} {first} {rows}")
+    kvh, heads, d, page = 2, 4, 64, 16
+    w = World(fv, 67, lens, counts, kvh, d, page, four)
+    starts = w.starts + np.int32(first)
+    batch = fv.PagedBatch(w.dev(starts), w.batch.lens, w.batch.table, max(counts), max(lens))
+    k, v, q = (pu.bf16(w.rng.standard_normal((rows, h, d))) for h in (kvh, kvh, heads))
+    cos, sin = tables(max(lens), d, False)
+    to = lambda x: w.dev(x).to(torch.bfloat16)  # noqa: E731
+    rq = fv.paged_append(w.pool, batch, to(k), to(v), rope=(w.dev(cos), w.dev(sin)), q=to(q))
+    there = []
+    for s, (n, c) in enumerate(zip(lens, counts)):
+        t = np.arange(max(starts[s], 0), min(starts[s] + c, rows))
+        pos = n - c + t - starts[s]
+        there.append((t, pos))
+        p, slot = w.table[s, pos // page], pos % page
+        for name, x in (("k", pu.rotate(k[t], cos, sin, pos, False)), ("v", v[t])):
+            if four:
+                w.host[name][p, :, slot], w.scales[name][p, :, slot] = pu.quantize4(x)
+            else:
+                w.host[name][p, :, slot] = pu.bf16(x)
+    got, _ = w.pull()
+    fine = all(np.array_equal(got[name], w.host[name]) for name in "kv")
+    assert fine
+    back = fv.paged_read(w.pool, batch, rows, out_bf16=False)
+    out = fv.paged_attention(rq, w.pool, batch, out_bf16=False).cpu().numpy()
+    for s, (t, pos) in enumerate(there):
+        turned = pu.bf16(pu.rotate(q[t], cos, sin, pos, False))
+        fine = np.array_equal(rq[t].float().cpu().numpy(), turned)
+        assert fine, s
+        for x, name in zip(back, "kv"):
+            fine = np.array_equal(x[t].cpu().numpy().astype(np.float64), w.held(name, s)[pos])
+            assert fine, (s, name)
+        want, mag = pu.attention(turned, w.held("k", s), w.held("v", s), pos[0], d ** -0.5)
+        off = float((np.abs(out[t] - want) - pu.attention_bound(want, mag, False, 60.0)).max())
+        assert off <= 0, (s, off)
