@@ -78,6 +78,7 @@ inline void paged_pick(bool v, F&& f) {
 
 }  // namespace fv
 
+constexpr size_t kMostSeqs = (size_t)1 << 24, kMostRows = (size_t)1 << 26;   // of a call
 int fv_paged_args(const char* who, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, size_t pages,
                   size_t page_tokens, size_t kv_heads, size_t d, const int32_t* q_start, const int32_t* lens, const int32_t* table,
                   size_t table_stride, size_t table_pages, size_t seqs, size_t tokens, const size_t* max_len, fv::PagedPool* pool,

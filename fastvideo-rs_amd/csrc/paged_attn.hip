@@ -1201,7 +1201,7 @@ PagedCut paged_cut(size_t heads, size_t kv_heads, size_t d, bool four, size_t se
             if (rest == 0) continue;
             for (size_t k = 1; k <= 64 && k <= steps; k++) {
                 const size_t chunk = (steps + k - 1) / k, shares = (steps + chunk - 1) / chunk, wgs = rest * shares;
-                if (k > 1 && shares * (numbers - full) * kBigRows * d * 4 > kMostShares) break;
+                if (k > 1 && shares > kMostShares / ((numbers - full) * kBigRows * d * 4)) break;
                 double cost = (double)(full / slots) * steps_us((double)steps, (double)slots);
                 if (varied) {
                     const double each = std::max(1.0, (double)shares * mean), all = (double)rest * each, at_once = std::min(all, (double)slots);
@@ -1268,11 +1268,18 @@ struct PagedParts {
 }  // namespace
 }  // namespace fv
 
+static bool mask_fits(size_t block_tokens, size_t window, size_t sink) {
+    return std::max({block_tokens, window, sink}) <= (size_t)INT_MAX / 2;
+}
+
 extern "C" {
 
 size_t fv_paged_attention_workspace_bytes_for(int four_bits, size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t tokens, size_t max_q,
                                               size_t max_len, size_t block_tokens, size_t window, size_t sink) {
     if (kv_heads == 0 || heads < kv_heads || heads % kv_heads != 0 || block_tokens == 0 || seqs == 0 || tokens == 0 || max_q == 0) return 0;
+    // (what fv_paged_attention refuses: products of these numbers would pass 64 bits)
+    if ((d != 64 && d != 128) || heads > 65535 || seqs > kMostSeqs || tokens > kMostRows || max_len > (size_t)INT_MAX || !mask_fits(block_tokens, window, sink))
+        return 0;
     const fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four_bits != 0, seqs, tokens, std::min(max_q, tokens), max_len, block_tokens, window, sink);
     return fv::PagedParts(c, seqs, kv_heads, d).bytes;
 }
@@ -1302,8 +1309,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
     if (((uintptr_t)q & 15) != 0 || ((uintptr_t)out & 15) != 0) return fv_invalid("paged attention: operands must be 16-byte aligned");
     if (!(scale > 0.f) || !(scale <= 2e38f)) return fv_decline("paged attention: scale must be positive and finite");
     if (block_tokens == 0) return fv_invalid("paged attention: block_tokens must be positive");
-    if (block_tokens > (size_t)INT_MAX / 2 || window > (size_t)INT_MAX / 2 || sink > (size_t)INT_MAX / 2)
-        return fv_decline("paged attention: mask too large");
+    if (!mask_fits(block_tokens, window, sink)) return fv_decline("paged attention: mask too large");
     if (max_q > tokens) max_q = tokens;
     const bool four = k_scales != nullptr;
     fv::PagedCut c = fv::paged_cut(heads, kv_heads, d, four, seqs, tokens, max_q, max_len, block_tokens, window, sink);

@@ -257,7 +257,7 @@ int fv_paged_args(const char* who, const void* k_pages, const void* v_pages, con
         return say("pages and scales must be 16-byte aligned", false);
     if (table_pages > table_stride) return say("table rows shorter than their pages", false);
     if (table_pages > (size_t)INT_MAX / page_tokens) return say("table too wide", true);
-    if (seqs > (size_t)1 << 24 || tokens > (size_t)1 << 26) return say("too many sequences or rows for one launch", true);
+    if (seqs > kMostSeqs || tokens > kMostRows) return say("too many sequences or rows for one launch", true);
     if (max_len && *max_len > table_pages * page_tokens) return say("lengths past the table's pages", false);
     int lg = 0;
     while (((size_t)1 << lg) < page_tokens) lg++;

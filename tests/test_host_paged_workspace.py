@@ -30,11 +30,16 @@ def test_either_kind(lib):
 
 
 def test_nothing_for_numbers_that_no_call_takes(lib):
-    need = lib.fv_paged_attention_workspace_bytes_for
+    """Numbers among them whose products pass 64 bits."""
+    base = {"heads": 4, "kv_heads": 2, "d": 128, "seqs": 3, "tokens": 5, "max_q": 2, "max_len": 1 << 20, "block": 1, "window": 0, "sink": 0}
+    far = [{name: n} for name in ("heads", "seqs", "tokens", "max_len", "block", "window", "sink") for n in (1 << 31, 1 << 61, (1 << 64) - 2)]
     for kind in (0, 1):
-        for bad in (dict(heads=3), dict(kv_heads=0), dict(seqs=0), dict(tokens=0), dict(max_q=0), dict(block=0)):
-            n = {"heads": 4, "kv_heads": 2, "d": 128, "seqs": 3, "tokens": 5, "max_q": 2, "max_len": 1 << 20, "block": 1, "window": 0, "sink": 0, **bad}
-            assert need(kind, *n.values()) == 0, bad
+        assert lib.fv_paged_attention_workspace_bytes_for(kind, *base.values()) > 0
+        for bad in (dict(heads=3), dict(kv_heads=0), dict(seqs=0), dict(tokens=0), dict(max_q=0), dict(block=0), dict(d=0), dict(d=96), *far):
+            assert lib.fv_paged_attention_workspace_bytes_for(kind, *{**base, **bad}.values()) == 0, bad
+            assert lib.fv_paged_attention_workspace_bytes(*{**base, **bad}.values()) == 0, bad
+        every = lib.fv_paged_attention_workspace_bytes_for(kind, *{**base, "max_q": (1 << 64) - 1}.values())   # (cut to the rows)
+        assert every == lib.fv_paged_attention_workspace_bytes_for(kind, *{**base, "max_q": 5}.values())
 
 
 def test_shares_are_limited(lib):
@@ -50,3 +55,15 @@ def test_shares_are_limited(lib):
     # (9.7 GB for 19 MB of results without the limit; these are cut as far as it lets them)
     drafts = lib.fv_paged_attention_workspace_bytes_for(1, 32, 8, 128, 256, 256 * 9, 9, 1 << 20, 1, 0, 0)
     assert (1 << 29) < drafts <= (1 << 30) * 129 // 128 + 512
+
+
+def test_the_largest_numbers(lib):
+    """Each bound of a call at its largest, all at once too: a gigabyte a kernel, or none."""
+    most = {"heads": 65534, "kv_heads": 32767, "d": 128, "seqs": 1 << 24, "tokens": 1 << 26, "max_q": 1 << 26, "max_len": (1 << 31) - 1,
+            "block": (1 << 30) - 1, "window": (1 << 30) - 1, "sink": (1 << 30) - 1}
+    base = {"heads": 40, "kv_heads": 8, "d": 128, "seqs": 64, "tokens": 300, "max_q": 100, "max_len": 1 << 20, "block": 1, "window": 0, "sink": 0}
+    some = [dict(base, **{n: most[n]}) for n in most if n not in ("heads", "kv_heads")] + [dict(base, heads=65535, kv_heads=1), dict(base, heads=65535, kv_heads=65535)]
+    for kind in (0, 1):
+        for numbers in (*some, most, dict(most, block=1), dict(most, window=0), dict(most, window=0, heads=65535, kv_heads=1), dict(most, max_q=1)):
+            need = lib.fv_paged_attention_workspace_bytes_for(kind, *numbers.values())
+            assert need <= 2 * ((1 << 30) * 129 // 128 + 512), numbers
