@@ -224,3 +224,46 @@ def test_rows_that_the_tensors_do_not_have(fv, four, lens, counts, first, rows):
         want, mag = pu.attention(turned, w.held("k", s), w.held("v", s), pos[0], d ** -0.5)
         off = float((np.abs(out[t] - want) - pu.attention_bound(want, mag, False, 60.0)).max())
         assert off <= 0, (s, off)
+
+
+@pytest.mark.parametrize("lens,counts,heads,mask", [([70, 9], [5, 3], 6, (1, 0, 0)), ([9000, 300], [2, 1], 4, (1, 0, 0)), ([200, 150], [200, 90], 2, (1, 0, 0)),
+                                                    ([300, 260], [120, 260], 4, (1, 40, 3)), ([9000], [70], 4, (1, 0, 0))])
+def test_infinite_keys_and_queries_that_are_not_numbers(fv, lens, counts, heads, mask):
+    """A key of infinite entries scores infinity (the row is not a number) or minus infinity (its weight is zero) for a row that
+    sees it, by the sign of the query there; a query that is not a number is its own row's alone."""
+    d, kvh, page = 128, 2, 32
+    announce(f"paged: infinite keys {lens} {mask}")
+    w = World(fv, 71, lens, counts, kvh, d, page)
+    for s, n in enumerate(lens):
+        for j, x in ((n - counts[s] // 2 - 1, np.inf), (n - 2, -np.inf), (n // 2, np.inf), (3, -np.inf)):
+            w.host["k"][w.table[s, j // page], 1, j % page, 7] = x
+    w.push()
+    q = w.queries(heads)
+    q[:, heads // 2:, 7] = np.where(w.rng.random((w.rows(), heads - heads // 2)) < 0.5, 2.0, -2.0)
+    lost = [0, w.rows() - 2]
+    q[lost[0], 0, 3] = np.nan
+    q[lost[1], heads - 1, 100] = np.inf
+    got = fv.paged_attention(w.dev(q).bfloat16(), w.pool, w.batch, fv.BlockCausal(*mask), out_bf16=False).cpu().numpy()
+    nan = number = 0
+    for s, n in enumerate(counts):
+        part = slice(w.starts[s], w.starts[s] + n)
+        seen = pu.sees(np.arange(n) + lens[s] - n, np.arange(lens[s]), *mask)
+        k = w.held("k", s)
+        for h in range(heads):
+            kk = k[:, h * kvh // heads]
+            with np.errstate(invalid="ignore"):
+                scores = q[part, h].astype(np.float64) @ kk.T * d ** -0.5
+            scores[~seen] = -np.inf
+            bad = ~(scores < np.inf).all(1)
+            x = got[part, h]
+            wrong = int((np.isnan(x).all(1) != bad).sum() + (np.isfinite(x).all(1) == bad).sum())
+            assert wrong == 0, (s, h, wrong)
+            some = ~bad & np.isfinite(scores).any(1)
+            p = np.exp(scores[some] - scores[some].max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            v = w.held("v", s)[:, h * kvh // heads]
+            out, mag = p @ v, p @ np.abs(v)
+            off = np.abs(x[some] - out) - pu.attention_bound(out, mag, False, 1.45 * 40)
+            assert off.size == 0 or off.max() <= 0, (s, h, off.max())
+            nan, number = nan + int(bad.sum()), number + int(some.sum())
+    assert nan > 2 and number > 2
