@@ -1017,8 +1017,11 @@ FV_DEV bool paged_tiles_item(const Params& p, const int wave, const int lane, co
     }
     return true;
 }
-// The kernel's arguments read again from their segment, of which PagedAttnParams is the whole, and the lane counted anew: the second
-// pass, which runs once in a blue moon, keeps nothing of the first in registers.
+// The kernel's arguments read again from their segment, of which PagedAttnParams is the whole, and the lane counted anew, so that the
+// second pass keeps nothing of the first in registers. It spills (65 - 184 registers where both share the kernel's 256, or 168 at 64
+// channels) and the first does not in its loop. Where every workgroup needs it, a call takes 3 times as long over bf16 pages, 5 over
+// 4 bits (keys whose scores grow by 1000 and more along a sequence): a frame of 1560 rows x 12 heads on 32760 298 -> 929 us, prompts under a window
+// 229 -> 702, three frames of two sequences over 4 bits 1.75 -> 9.0 ms.
 template <int D, bool FOUR>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tiles_kernel(const PagedAttnParams p) {
     int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = blockIdx.x;
