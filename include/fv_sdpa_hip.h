@@ -375,7 +375,7 @@ int fv_kv_cache_update(fv_kv_cache* c, size_t layer, const fv_tensor* k, const f
  * the largest code (ties to the even code; a value that is not finite makes its 32 channels not a number). A token whose
  * table row lies outside the tables, or that lies before the first token of its sequence (more rows than tokens), is not
  * stored and its query is zeros. Positions are counted from lens as it is; fv_paged_attention counts its rows' from lens cut to its
- * max_len, so the two agree where max_len bounds lens, as it should. */
+ * max_len, so the two agree where max_len bounds lens, as it should. q_out may not overlap an input. */
 int fv_paged_append(const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q, size_t q_stride,
                     uint16_t* q_out, int in_is_bf16, size_t heads, const float* cos_t, const float* sin_t, size_t rope_rows,
                     const int32_t* rope_at, int halves, void* k_pages, void* v_pages, void* k_scales, void* v_scales,
@@ -389,11 +389,12 @@ int fv_paged_read(void* k_out, void* v_out, int out_is_bf16, const void* k_pages
                   const int32_t* lens, const int32_t* table, size_t table_stride, size_t table_pages, size_t seqs,
                   size_t tokens, void* stream);
 /* out [tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale * q k^T) v of the batch's rows over the cached keys of
- * their sequences; q bf16 bits, tokens q_stride elements apart; heads / kv_heads neighbouring heads share a key head. Under the
- * block mask of fv_sdpa_block_causal_bf16 with one difference: the query at position i sees key j iff, t = position / block_tokens,
- * tj <= ti && (window == 0 || ti - tj < window || tj < sink): a sink block is not seen before its time. block_tokens == 1: causal by
- * token, a window of tokens, sink tokens. A row that sees no key is zeros. max_q / max_len: bounds of the rows of a sequence and of
- * lens, host numbers that the launch is sized by (longer lengths are cut to max_len, rows past max_q may not be written).
+ * their sequences; q bf16 bits, tokens q_stride elements apart, not overlapping out; heads / kv_heads neighbouring heads share a
+ * key head. Under the block mask of fv_sdpa_block_causal_bf16 with one difference: the query at position i sees key j iff, t =
+ * position / block_tokens, tj <= ti && (window == 0 || ti - tj < window || tj < sink): a sink block is not seen before its time.
+ * block_tokens == 1: causal by token, a window of tokens, sink tokens. A row that sees no key is zeros. max_q / max_len: bounds of
+ * the rows of a sequence and of lens, host numbers that the launch is sized by (longer lengths are cut to max_len, rows past max_q
+ * may not be written).
  * workspace: fv_paged_attention_workspace_bytes_for the pool's kind of pages (four_bits: with scales) and the same numbers (0: none;
  * fv_paged_attention_workspace_bytes: enough for either kind), 256-byte aligned, this call's alone until its work is done; where
  * it is too small or NULL long walks are not split, which costs time only (and bits: shares are normalised before they are
