@@ -41,6 +41,9 @@ class PagedKv:
         self._args = (k.data_ptr(), v.data_ptr(), k_scales.data_ptr() if four else None, v_scales.data_ptr() if four else None,
                       shape[0], shape[2], shape[1], d)
 
+    def __reduce__(self):   # (copies take the addresses of their own tensors)
+        return PagedKv, (self._k, self._v, self._k_scales, self._v_scales)
+
     @staticmethod
     def new(pages, page_tokens, kv_heads, d, four_bits=False, device="cuda"):
         """A pool of zeros."""
@@ -82,6 +85,9 @@ class PagedBatch:
             raise ValueError("PagedBatch: bounds must not be negative")
         self._q_start, self._lens, self._table, self.max_q, self.max_len, self._device = q_start, lens, table, max_q, max_len, dev
         self._args = (q_start.data_ptr(), lens.data_ptr(), table.data_ptr(), step if n > 1 else columns, columns, n)
+
+    def __reduce__(self):
+        return PagedBatch, (self._q_start, self._lens, self._table, self.max_q, self.max_len)
 
 
 def _rows(t, name, heads, d, dtypes, device):

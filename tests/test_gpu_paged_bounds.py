@@ -267,3 +267,27 @@ def test_infinite_keys_and_queries_that_are_not_numbers(fv, lens, counts, heads,
             assert off.size == 0 or off.max() <= 0, (s, h, off.max())
             nan, number = nan + int(bad.sum()), number + int(some.sum())
     assert nan > 2 and number > 2
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_copies_of_the_handles_are_of_their_own_tensors(fv, four):
+    """A deep copy of a pool is another pool, of a batch another batch; a shallow one has the same tensors."""
+    import copy
+
+    import torch
+
+    announce(f"paged: copies four={four}")
+    w = World(fv, 73, [20, 9], [2, 1], 2, 64, 16, four)
+    before = [t.clone() for t in (w.pool.k, w.pool.v)]
+    other, batch = copy.deepcopy(w.pool), copy.deepcopy(w.batch)
+    assert other.k.data_ptr() != w.pool.k.data_ptr() and other.four_bits == four
+    x = torch.full((3, 2, 64), 3.0, device="cuda", dtype=torch.bfloat16)
+    batch.lens.fill_(1)                                          # (the copy's: the first token of a sequence, two rows of which one is it)
+    fv.paged_append(other, batch, x, x)
+    assert torch.equal(w.pool.k, before[0]) and torch.equal(w.pool.v, before[1])
+    back = fv.paged_read(other, batch, 3)[0]
+    assert not back[0].any() and (back[1:] == 3.0).all()
+    assert w.batch.lens.tolist() == [20, 9] and (batch.max_q, batch.max_len) == (w.batch.max_q, w.batch.max_len)
+    same = copy.copy(w.pool)
+    fv.paged_append(same, copy.copy(w.batch), x, x)
+    assert (fv.paged_read(w.pool, w.batch, 3)[0] == 3.0).all()
