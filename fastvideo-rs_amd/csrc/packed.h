@@ -1,0 +1,151 @@
+// Packed sequences: the tokens of sequences of different lengths one behind the other in [tokens, heads, d] tensors, queries and keys
+// with starts of their own. What the kernels of the attention (packed_attn.hip) and of its gradients (packed_back.hip) share.
+#pragma once
+#include "attn_core.h"
+#include "fv_internal.h"
+#include "paged.h"
+
+namespace fv {
+
+// Sequence s: rows q_start[s] .. q_start[s + 1] of the queries, k_start[s] .. k_start[s + 1] of the keys. Device memory that the host does
+// not see: bounded here to the tensors' rows.
+struct PackedBatch {
+    const int* q_start;
+    const int* k_start;
+    int seqs, tokens, k_tokens, max_q, max_k;   // (what lies past the bounds that the launch is sized by is left out)
+};
+// The keys' side alone, for numbering pieces of keys.
+struct PackedKeys {
+    const int* q_start;
+    int seqs, tokens;
+};
+
+struct PackedSeq {
+    int start, count;   // first row, rows
+    int k0, len;        // first key, keys
+    int pos0;           // position of the first row among the keys: the last row is at the last key; negative where rows are more than keys
+};
+template <class Batch>
+FV_DEV PackedSeq packed_seq(const Batch& b, int s) {
+    PackedSeq q;
+    q.start = min(max(b.q_start[s], 0), b.tokens);
+    const int behind = max(b.q_start[s + 1], q.start), k_behind = b.k_start[s + 1];
+    q.count = min(min(behind, b.tokens) - q.start, b.max_q);
+    q.k0 = min(max(b.k_start[s], 0), b.k_tokens);
+    q.len = min(min(max(k_behind, q.k0), b.k_tokens) - q.k0, b.max_k);
+    q.pos0 = q.len - (behind - q.start);
+    return q;
+}
+
+// The mask: without `causal` every row sees every key of its sequence; with it as in paged_sight.
+struct PackedMask {
+    int causal;
+    PagedDiv block_tokens;
+    int window, sink;
+};
+template <class Mask>
+FV_DEV PagedSight packed_sight(const Mask& m, int pos, int len) {
+    return m.causal ? paged_sight(m, pos, len) : PagedSight{0, 0, len};
+}
+template <class Mask>
+FV_DEV PagedSight packed_all(const Mask& m, const PackedSeq& s, int t0, int t1) {   // what the tokens t0 .. t1 all see
+    const PagedSight f = packed_sight(m, s.pos0 + t0, s.len), l = packed_sight(m, s.pos0 + t1, s.len);
+    return {f.a, l.lo, f.hi};
+}
+
+// The walk of a tile of rows (tokens t0 .. t1 of the sequence) over tiles of 64 keys: the first ns hold the sink, then from tile b0.
+struct PackedWalk {
+    int ns, b0, n;
+    PagedSight any;   // the keys that some row sees
+    FV_DEV int key(int e) const { return (e < ns ? e : b0 + e - ns) * kTileRows; }
+    // the tiles of the walk before key 64 t
+    FV_DEV int before(int t) const { return min(t, ns) + min(max(t - b0, 0), n - ns); }
+};
+template <class Mask>
+FV_DEV PackedWalk packed_walk(const Mask& m, const PackedSeq& s, int t0, int t1) {
+    PackedWalk w;
+    const PagedSight l = packed_sight(m, s.pos0 + t1, s.len);
+    w.any = {l.a, packed_sight(m, max(s.pos0 + t0, 0), s.len).lo, l.hi};
+    w.ns = (w.any.a + kTileRows - 1) / kTileRows;
+    w.b0 = max(w.any.lo / kTileRows, w.ns);
+    w.n = w.ns + max(0, (w.any.hi + kTileRows - 1) / kTileRows - w.b0);
+    return w;
+}
+// The tiles of the walk that rows which all see `all` see whole: those before `a` and [b, c).
+struct PackedWhole {
+    int a, b, c;
+    FV_DEV bool tile(int e) const { return e < a || (e >= b && e < c); }
+};
+FV_DEV PackedWhole packed_whole(const PackedWalk& w, const PagedSight& all) {
+    return {w.before(all.a / kTileRows), all.a >= all.lo ? 0 : w.before((all.lo + kTileRows - 1) / kTileRows), w.before(all.hi / kTileRows)};
+}
+
+// Items (pieces of rows or keys of a key head, in shares) to workgroups: key head by key head, 2^xcds XCDs to a run of items, so that an
+// L2 holds few heads' tensors; the XCDs of a run take its items in turn, so that each has as many of the long walks as the others.
+struct PackedItems {
+    PagedDiv n, shares_n;   // pieces of a key head, pieces times shares
+    int total, xcds;
+};
+struct PackedItem {
+    int head, piece, share;   // head < 0: none
+};
+template <class Items>
+FV_DEV PackedItem packed_item(const Items& x, int block) {
+    const int run = ((x.total << x.xcds) + 7) >> 3, in_run = ((block >> 3) << x.xcds) + (block & ((1 << x.xcds) - 1));
+    const int item = ((block & 7) >> x.xcds) * run + in_run;
+    if (in_run >= run || item >= x.total) return {-1, 0, 0};
+    const int head = paged_quot(item, x.shares_n), rest = item - head * x.shares_n.by, share = paged_quot(rest, x.n);
+    return {head, rest - share * x.n.by, share};
+}
+inline PackedItems packed_items(size_t kv_heads, size_t pieces, size_t shares) {
+    return {paged_div(pieces), paged_div(pieces * shares), (int)(kv_heads * pieces * shares),
+            kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3};   // (a run has whole key heads)
+}
+inline size_t packed_blocks(const PackedItems& x) {
+    const size_t run = (((size_t)x.total << x.xcds) + 7) / 8;
+    return ((run + ((size_t)1 << x.xcds) - 1) >> x.xcds) * 8;
+}
+
+// Per-lane source offsets of a wave's part of a 64-row tile whose rows lie `stride` bytes apart (ITER loads a wave of four, in the LDS
+// layout of attn_core.h). Second loads of a pair less the 1 KB that their immediate offset adds.
+template <int D, int ITER, class Swz>
+FV_DEV void packed_offsets(unsigned (&off)[ITER], unsigned stride, int wave, int lane, Swz&& swz) {
+    using G = TileGeo<D>;
+#pragma unroll
+    for (int it = 0; it < ITER; it++) {
+        const int r = (wave * ITER + it) * G::kRowsPerDma + lane / G::kChunks, c = lane % G::kChunks;
+        off[it] = (unsigned)r * stride + ((unsigned)(c ^ swz(r)) << 4) - (unsigned)(it & 1) * 1024u;
+    }
+}
+// Rows [first, first + count) of a head whose rows lie `stride` bytes apart, count <= 64, as a descriptor: rows behind them are zeros.
+FV_DEV u32x4 packed_rows(const uint16_t* base, long first, long stride, int count, int row_bytes) {
+    return plane_descriptor((const uint8_t*)base + first * stride, count > 0 ? (unsigned)((long)(count - 1) * stride) + (unsigned)row_bytes : 0u);
+}
+// Two loads of a wave into LDS at `lds` (wave-uniform).
+FV_DEV void packed_issue(const u32x4& rows, unsigned o0, unsigned o1, unsigned lds) {
+    const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                 "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds"
+                 :: "s"(m0), "v"(o0), "v"(o1), "s"(rows) : "memory");
+}
+
+}  // namespace fv
+
+// What the entries check alike; FV_OK, or what they return. Operands: bf16 bits [tokens, heads, d], tokens a stride apart.
+struct PackedOperand {
+    const void* at;
+    size_t stride, heads;
+};
+struct PackedCall {
+    size_t heads, kv_heads, d, seqs, tokens, k_tokens, max_q, max_k;
+    const int32_t *q_start, *k_start;
+    float scale;
+    int causal;
+    size_t block_tokens, window, sink;
+};
+int fv_packed_args(const char* who, const PackedCall& c, const PackedOperand* x, size_t operands, const void* workspace);
+fv::PackedMask fv_packed_mask(const PackedCall& c);
+// Numbers whose workspace is asked for, within what the entries take.
+bool fv_packed_sizes(const PackedCall& c);
+// Steps of `step` keys (or rows) that the walk of a piece may have, on the call's bounds.
+size_t fv_packed_key_steps(const PackedCall& c, size_t rows);

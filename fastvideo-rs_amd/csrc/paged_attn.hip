@@ -22,56 +22,6 @@ constexpr int kStep = 32;       // keys a wave takes at a time
 constexpr int kWaves = 4;
 constexpr float kLeast = 0x1p-149f;   // the weight of a seen key that vanished, where its value is not finite
 
-// Division of a number below 2^31 by one that the host knows, as a product and a shift: with 2^l >= by, mul = 2^(31 + l) / by rounded up is
-// too large by less than 1, so n mul / 2^(31 + l) by less than 1 / by. (The compiler's own takes 20 instructions and waits for a
-// reciprocal; a workgroup makes ten of them before its first load.)
-struct PagedDiv {
-    unsigned mul;
-    int shift, by;
-};
-template <class Div>
-FV_DEV int paged_quot(int n, const Div& d) { return (int)(((unsigned long long)(unsigned)n * d.mul) >> d.shift); }
-PagedDiv paged_div(size_t by) {   // below 2^31 (0: never used)
-    if (by == 0) return {0, 0, 0};
-    int l = 0;
-    while (((size_t)1 << l) < by) l++;
-    return {(unsigned)((1ull << (31 + l)) / by + 1), 31 + l, (int)by};
-}
-
-// Pieces of up to R rows of the (token, head of the group) rows of a batch, for one key head. Where the sequences are as long as
-// the longest, piece t of sequence s is number s tiles + t. Where they are not (tiles 0), it is number first(s) + t with
-// first(s) = (group q_start[s] + (R - 1) s) / R, which leaves each its ceil(rows / R) numbers and no more than one for each sequence
-// unused, whatever the longest is. (A prompt of 8192 tokens among 255 single ones: 6.8 ms with the longest's pieces for all.)
-struct PagedPieces {
-    PagedDiv n, tiles;          // numbers, of a sequence
-};
-struct PagedPiece {
-    int seq, tile;              // (of an unused number: a tile that the sequence does not have, R tile below 2^31)
-};
-template <int R, class Pieces, class Batch>
-FV_DEV long paged_first_piece(const Pieces& x, const Batch& b, int group, int seq) {
-    return x.tiles.by ? (long)seq * x.tiles.by : ((long)min(max(b.q_start[seq], 0), b.tokens) * group + (long)(R - 1) * seq) / R;
-}
-template <int R, class Pieces, class Batch>
-FV_DEV PagedPiece paged_piece(const Pieces& x, const Batch& b, int group, int number) {   // (of a whole wave)
-    if (x.tiles.by) {
-        const int seq = paged_quot(number, x.tiles);
-        return {seq, number - seq * x.tiles.by};
-    }
-    const int lane = threadIdx.x & 63;
-    int seq = 0, n = b.seqs;    // the last of sequences seq .. seq + n - 1 whose first piece is no later: 64 of them at a time
-    while (n > 1) {
-        const int step = (n + 63) / 64, at = lane * step;
-        const bool le = at < n && paged_first_piece<R>(x, b, group, seq + min(at, n - 1)) <= number;
-        const int k = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)), 1) - 1;
-        seq += k * step;
-        n = min(step, n - k * step);
-    }
-    const long tile = number - paged_first_piece<R>(x, b, group, seq);   // (negative: of rows before the first sequence)
-    constexpr int kNone = 0x7fffffff / R;
-    return {seq, tile < 0 || tile > kNone ? kNone : (int)tile};
-}
-
 struct PagedAttnParams {
     PagedPool pool;
     PagedBatch b;
@@ -105,29 +55,6 @@ struct PagedAttnParams {
     int join_tiles;
     PagedDiv join_few;
 };
-
-// The keys that a row at position p of a sequence of `len` tokens sees: [0, a) and [lo, hi), a <= hi.
-struct PagedSight {
-    int a, lo, hi;
-    // bit j: key k + j, j < 8. (Bits and selects: the comparisons key by key under divergent branches were compiled into
-    // code that lost the stores of -inf.)
-    FV_DEV unsigned eight(int k) const {
-        return below(a - k) | (below(hi - k) & ~below(lo - k));
-    }
-    static FV_DEV unsigned below(int n) { return (1u << min(max(n, 0), 8)) - 1u; }
-    FV_DEV bool one(int k) const { return k < a || (k >= lo && k < hi); }
-};
-template <class Params>
-FV_DEV PagedSight paged_sight(const Params& p, int pos, int len) {
-    if (pos < 0) return {0, 0, 0};
-    const int bt = p.block_tokens.by, block = paged_quot(pos, p.block_tokens);
-    const long hi = (long)(block + 1) * bt, sink = (long)p.sink * bt;
-    PagedSight s;
-    s.hi = (int)min(hi, (long)len);
-    s.lo = p.window > 0 ? max(0, block - p.window + 1) * bt : 0;
-    s.a = (int)min(sink, (long)s.hi);
-    return s;
-}
 
 // The walk of a tile of rows (tokens t0 .. t1 of the sequence) in steps of STEP keys: [0, ns) hold the sink, then
 // [b0, b0 + n - ns).
@@ -1149,12 +1076,6 @@ size_t walk_bound(size_t step, size_t rows, size_t group, size_t max_len, size_t
     return std::max<size_t>(steps, 1);
 }
 
-PagedPieces paged_pieces(size_t r, size_t seqs, size_t tokens, size_t max_q, size_t group) {
-    const size_t tiles = (max_q * group + r - 1) / r, like = seqs * tiles, ragged = (tokens * group + (r - 1) * seqs) / r;
-    const size_t most = INT_MAX;   // (past it no launch holds them)
-    return like <= ragged ? PagedPieces{paged_div(std::min(like, most)), paged_div(std::min(tiles, most))}
-                          : PagedPieces{paged_div(std::min(ragged, most)), paged_div(0)};
-}
 constexpr size_t kMostShares = (size_t)1 << 30;   // bytes of a kernel's shares: past it its walks are cut less
 // How a call is cut.
 struct PagedCut {

@@ -1,0 +1,227 @@
+// Rotary positions without tables (declarations: include/fv_sdpa_hip.h): pair (a, b) of token t becomes amplitude * (a c - b s, a s + b c) with
+// c, s = cos, sin of 2 pi times the turns position * freq, or, turned back, (a c + b s, b c - a s).
+//
+// freq counts turns a position in units of 2^-64, so that position * freq modulo 2^64 is the angle's fraction of a turn, exact in
+// integers but for freq's own rounding: 2^31 positions are 2^-33 turns off at most, where f32 (or a product in f32) loses the angle at some
+// ten thousand. Its nearest quarter turn is taken off and the rest, at most 1/8 turn, goes through the series of sin and cos, whose next
+// terms are below 2^-29 and 2^-33. Memory is the bound: a thread makes the angles of its channels once and turns them in all heads.
+#include <limits.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "../../include/fv_sdpa_hip.h"
+#include "fv_common.h"
+#include "fv_internal.h"
+#include "paged.h"
+
+namespace fv {
+namespace {
+
+struct RopeParams {
+    const void *q, *k;
+    void *q_out, *k_out;
+    long q_stride, k_stride, q_out_stride, k_out_stride;   // elements between tokens
+    int heads, kv_heads, d, pairs, axes;
+    const uint64_t* freq;
+    const int* pair_axis;
+    const int* positions;
+    long tokens;
+    float amplitude;
+    int inverse;
+    PagedDiv chunks;        // threads of a token in one piece of heads
+    PagedDiv pieces;        // pieces of a token's heads
+    int per;                // heads a piece
+};
+
+// sin and cos of a fraction of a turn in units of 2^-64.
+FV_DEV void turn_sincos(uint64_t turns, float& sin, float& cos) {
+    const uint32_t t = (uint32_t)(turns >> 32) + ((uint32_t)turns >> 31);   // to the nearest 2^-32
+    const uint32_t quarter = (t + 0x20000000u) >> 30;
+    const float x = (float)(int)(t - (quarter << 30)) * (6.28318530717958647692f * 0x1p-32f), y = x * x;
+    float s = __builtin_fmaf(y, 1.f / 362880.f, -1.f / 5040.f), c = __builtin_fmaf(y, -1.f / 3628800.f, 1.f / 40320.f);
+    s = __builtin_fmaf(y, s, 1.f / 120.f), c = __builtin_fmaf(y, c, -1.f / 720.f);
+    s = __builtin_fmaf(y, s, -1.f / 6.f), c = __builtin_fmaf(y, c, 1.f / 24.f);
+    s = __builtin_fmaf(x * y, s, x), c = __builtin_fmaf(y, c, -0.5f);
+    c = __builtin_fmaf(y, c, 1.f);
+    sin = quarter & 1 ? c : s, cos = quarter & 1 ? s : c;
+    sin = quarter & 2 ? -sin : sin, cos = (quarter + 1) & 2 ? -cos : cos;
+}
+
+template <bool IS16>
+FV_DEV void load_eight(const void* base, long at, float (&x)[8]) {
+    if constexpr (IS16) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)base + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[2 * i] = __builtin_bit_cast(float, w[i] << 16), x[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>((const float*)base + at + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[4 * h + i] = w[i];
+        }
+    }
+}
+template <bool IS16>
+FV_DEV void store_eight(void* base, long at, const float (&x)[8]) {
+    if constexpr (IS16) {
+        f32x8 v;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = x[i];
+        *reinterpret_cast<bf16x8*>((uint16_t*)base + at) = __builtin_convertvector(v, bf16x8);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4*>((float*)base + at + 4 * h) = f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
+    }
+}
+
+// A thread has 16 channels of a token: of the turned ones eight pairs (neighbours: 16 channels in a row; halves: eight and their partners), of the
+// others any, and goes through `per` heads of q and then k.
+template <bool IN16, bool OUT16, bool HALVES>
+__global__ __launch_bounds__(256) void rope_tokens_kernel(const RopeParams p) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    const long unit = id / p.chunks.by;   // (token, piece of heads)
+    const int chunk = (int)(id - unit * p.chunks.by);
+    const long token = unit / p.pieces.by;
+    if (token >= p.tokens) return;
+    const int piece = (int)(unit - token * p.pieces.by);
+    const int all = p.heads + p.kv_heads, h0 = piece * p.per, h1 = min(all, h0 + p.per);
+    const bool turns = 8 * chunk < p.pairs;
+    // the two runs of eight channels
+    const int c0 = !turns ? 2 * p.pairs + 16 * (chunk - p.pairs / 8) : HALVES ? 8 * chunk : 16 * chunk, c1 = turns && HALVES ? p.pairs + 8 * chunk : c0 + 8;
+    const bool two = c1 < p.d;   // (a last run of eight channels alone that are not turned)
+    float c[8], s[8];
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int pair = 8 * chunk + i;
+            int axis = p.pair_axis ? p.pair_axis[pair] : 0;
+            axis = (unsigned)axis < (unsigned)p.axes ? axis : 0;
+            turn_sincos((uint64_t)(int64_t)p.positions[token * p.axes + axis] * p.freq[pair], s[i], c[i]);
+            s[i] = (p.inverse ? -s[i] : s[i]) * p.amplitude;
+            c[i] *= p.amplitude;
+        }
+    }
+    for (int h = h0; h < h1; h++) {
+        const bool is_k = h >= p.heads;
+        const void* in = is_k ? p.k : p.q;
+        void* out = is_k ? p.k_out : p.q_out;
+        const long col = (long)(is_k ? h - p.heads : h) * p.d, from = token * (is_k ? p.k_stride : p.q_stride) + col,
+                   to = token * (is_k ? p.k_out_stride : p.q_out_stride) + col;
+        float x[8], y[8];
+        load_eight<IN16>(in, from + c0, x);
+        if (two) load_eight<IN16>(in, from + c1, y);
+        if (turns) {
+#pragma clang fp contract(off)
+            if constexpr (HALVES) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float a = x[i], b = y[i];
+                    x[i] = a * c[i] - b * s[i];
+                    y[i] = a * s[i] + b * c[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float a = x[2 * i], b = x[2 * i + 1];
+                    x[2 * i] = a * c[i] - b * s[i];
+                    x[2 * i + 1] = a * s[i] + b * c[i];
+                    a = y[2 * i], b = y[2 * i + 1];
+                    y[2 * i] = a * c[4 + i] - b * s[4 + i];
+                    y[2 * i + 1] = a * s[4 + i] + b * c[4 + i];
+                }
+            }
+        }
+        store_eight<OUT16>(out, to + c0, x);
+        if (two) store_eight<OUT16>(out, to + c1, y);
+    }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+}  // namespace fv
+
+extern "C" {
+
+int fv_rope_frequencies(size_t pairs, double base, int scaling, double factor, double original, double low, double high, uint64_t* out) {
+    if (!out) return fv_invalid("rope frequencies: null operand");
+    if (pairs == 0 || pairs > 65536) return fv_invalid("rope frequencies: pairs");
+    if (!(base >= 1.0) || !(base < 1e300)) return fv_invalid("rope frequencies: base must be 1 or more, and finite");
+    if (scaling < 0 || scaling > 3) return fv_invalid("rope frequencies: scaling is 0 to 3");
+    if (scaling != 0 && (!(factor >= 1.0) || !(factor < 1e9))) return fv_invalid("rope frequencies: factor must be 1 or more");
+    if (scaling == 2 && pairs < 2) return fv_invalid("rope frequencies: a scaled base needs two pairs");
+    if (scaling == 3 && (!(original > 0.0) || !(original < 1e18) || !(high > low) || !(high < 1e18) || !(low > -1e18)))
+        return fv_invalid("rope frequencies: original must be positive and low below high");
+    constexpr double kTurn = 6.283185307179586476925;
+    const double n = (double)pairs;
+    if (scaling == 2) base *= pow(factor, n / (n - 1.0));
+    for (size_t i = 0; i < pairs; i++) {
+        double theta = pow(base, -(double)i / n);
+        if (scaling == 1) theta /= factor;
+        if (scaling == 3) {
+            const double kept = std::min(1.0, std::max(0.0, (original * theta / kTurn - low) / (high - low)));
+            theta *= kept + (1.0 - kept) / factor;
+        }
+        out[i] = (uint64_t)llrint(ldexp(theta / kTurn, 64));   // (theta is 1 at most: below 2^62)
+    }
+    return FV_OK;
+}
+
+int fv_rope_tokens(const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t heads, const void* k, size_t k_stride, void* k_out,
+                   size_t k_out_stride, size_t kv_heads, size_t d, int in_is_bf16, int out_is_bf16, const uint64_t* freq, const int32_t* pair_axis,
+                   size_t pairs, const int32_t* positions, size_t axes, size_t tokens, float amplitude, int halves, int inverse, void* stream) {
+    if (tokens == 0) return FV_OK;   // (empty arrays may have no address)
+    if (!q || !q_out || !freq || !positions) return fv_invalid("rope tokens: null operand");
+    if ((k == nullptr) != (k_out == nullptr)) return fv_invalid("rope tokens: keys without a place for the turned ones, or the reverse");
+    if (heads == 0 || (k && kv_heads == 0)) return fv_invalid("rope tokens: no heads");
+    if (!k) kv_heads = 0;
+    if (d == 0 || d % 8 != 0 || d > 4096) return fv_decline("rope tokens: head dim must be a multiple of 8, 4096 at most");
+    if (pairs == 0 || pairs % 8 != 0) return fv_decline("rope tokens: pairs must be a multiple of 8");
+    if (2 * pairs > d) return fv_invalid("rope tokens: more pairs than channels");
+    if (axes == 0 || axes > 4) return fv_invalid("rope tokens: 1 to 4 position axes");
+    if (heads > 65535 || kv_heads > 65535) return fv_decline("rope tokens: too many heads");
+    if (tokens > kMostRows) return fv_decline("rope tokens: too many tokens for one launch");
+    if (!(amplitude > 0.f) || !(amplitude < 1e30f)) return fv_invalid("rope tokens: amplitude must be positive and finite");
+    const size_t most = (size_t)INT_MAX / 4;
+    struct {
+        const void* at;
+        size_t stride, heads;
+    } const x[] = {{q, q_stride, heads}, {q_out, q_out_stride, heads}, {k, k_stride, kv_heads}, {k_out, k_out_stride, kv_heads}};
+    for (size_t i = 0; i < (k ? 4 : 2); i++) {
+        if (!fv::aligned16(x[i].at)) return fv_invalid("rope tokens: operands must be 16-byte aligned");
+        if (x[i].stride < x[i].heads * d) return fv_invalid("rope tokens: tokens overlap (a stride below heads * d)");
+        if (x[i].stride % 8 != 0 || x[i].stride > most) return fv_decline("rope tokens: strides must be multiples of 8 elements");
+    }
+    const bool same = (in_is_bf16 != 0) == (out_is_bf16 != 0);
+    if ((q == q_out && (!same || q_stride != q_out_stride)) || (k && k == k_out && (!same || k_stride != k_out_stride)))
+        return fv_invalid("rope tokens: in place only with one type and stride");
+    fv::RopeParams p;
+    p.q = q, p.k = k, p.q_out = q_out, p.k_out = k_out;
+    p.q_stride = (long)q_stride, p.k_stride = (long)k_stride, p.q_out_stride = (long)q_out_stride, p.k_out_stride = (long)k_out_stride;
+    p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.d = (int)d, p.pairs = (int)pairs, p.axes = (int)axes;
+    p.freq = freq, p.pair_axis = pair_axis, p.positions = positions, p.tokens = (long)tokens;
+    p.amplitude = amplitude, p.inverse = inverse != 0;
+    const size_t chunks = pairs / 8 + (d - 2 * pairs + 15) / 16, all = heads + kv_heads;
+    // Heads of a thread: eight where tokens are many, so that the angles are a small part of its work; fewer tokens spread over the units.
+    const size_t wanted = (size_t)fv_compute_units() * 1024;   // threads
+    size_t per = std::min<size_t>(all, 8);
+    while (per > 1 && tokens * chunks * ((all + per - 1) / per) < wanted) per = (per + 1) / 2;
+    p.per = (int)per;
+    p.chunks = fv::paged_div(chunks), p.pieces = fv::paged_div((all + per - 1) / per);
+    const size_t blocks = (tokens * chunks * ((all + per - 1) / per) + 255) / 256;
+    if (blocks >= (size_t)1 << 24) return fv_decline("rope tokens: too large for one launch");
+    hipStream_t st = (hipStream_t)stream;
+    fv::paged_pick(in_is_bf16 != 0, [&](auto i16) {
+        fv::paged_pick(out_is_bf16 != 0, [&](auto o16) {
+            fv::paged_pick(halves != 0, [&](auto h) {
+                hipLaunchKernelGGL((fv::rope_tokens_kernel<i16(), o16(), h()>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+            });
+        });
+    });
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? FV_OK : fv_fail_hip(e, "rope_tokens");
+}
+
+}  // extern "C"

@@ -9,3 +9,4 @@ from .sdpa import *  # noqa: F401,F403
 from .prep import *  # noqa: F401,F403
 from .kv_cache import *  # noqa: F401,F403
 from .paged import *  # noqa: F401,F403
+from .packed import *  # noqa: F401,F403

@@ -61,6 +61,16 @@ SIGNATURES = {
     "fv_paged_attention_workspace_bytes": (_sz, [_sz] * 10),
     "fv_paged_attention": (C.c_int, [_vp, _sz, _vp, C.c_int, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz,
                                      _sz, _sz, _sz, _sz, _sz, C.c_float, _sz, _sz, _sz, _vp, _sz, _vp]),
+    "fv_packed_attention_workspace_bytes": (_sz, [_sz] * 8 + [C.c_int] + [_sz] * 3),
+    "fv_packed_attention": (C.c_int, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, C.c_int, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz,
+                                      C.c_float, C.c_int, _sz, _sz, _sz, _vp, _sz, _vp]),
+    "fv_packed_attention_backward_workspace_bytes": (_sz, [C.c_int] + [_sz] * 8 + [C.c_int] + [_sz] * 3),
+    "fv_packed_attention_backward": (C.c_int, [_vp, C.c_int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, C.c_int, _vp, _vp, _vp, _vp, C.c_int, _sz,
+                                               _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, C.c_int, _sz, _sz, _sz, _vp, _sz,
+                                               _vp]),
+    "fv_rope_frequencies": (C.c_int, [_sz, C.c_double, C.c_int] + [C.c_double] * 4 + [_vp]),
+    "fv_rope_tokens": (C.c_int, [_vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, C.c_int, C.c_int, _vp, _vp, _sz, _vp, _sz, _sz,
+                                 C.c_float, C.c_int, C.c_int, _vp]),
     "fv_sdpa_block_causal_bf16": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, _sz, _sz, _sz, _sz, C.c_float,
                                             _sz, _sz, _sz, _vp]),
     "fv_cast_f32_bf16": (C.c_int, [_vp, _vp, _sz, _vp]),

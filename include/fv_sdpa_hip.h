@@ -410,6 +410,64 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
                        float scale, size_t block_tokens, size_t window, size_t sink, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ---- packed sequences: attention, its gradients, rotary positions (no counterpart in the reference) --------------
+ * Sequences of different lengths one behind the other: queries q [q_tokens, heads, d] and keys and values k, v [k_tokens, kv_heads,
+ * d], bf16 bits, d = 64 or 128, the heads of a token contiguous, tokens *_stride elements apart (a multiple of 8, 2^24 at most: a slice of a
+ * fused projection), 16-byte aligned; heads / kv_heads neighbouring heads share a key head. Sequence s is rows q_start[s] .. q_start[s + 1]
+ * and keys k_start[s] .. k_start[s + 1] (int32 [seqs + 1] device arrays, ascending; self-attention passes one array for both). They are read when the
+ * call's work runs, and every index from them is bounded to the tensors, so a captured call may be replayed with other lengths. max_q / max_k bound the rows and
+ * keys of a sequence (host numbers that the launch is sized by; what lies past them may be left out). Rows at q_start[seqs] and
+ * behind, and keys' gradients likewise, are left as they were.
+ *
+ * causal == 0: every row sees every key of its sequence. Else a sequence's last row is at its last key's position, and the row at position i
+ * sees key j as in fv_paged_attention: ti = i / block_tokens, tj <= ti && (window == 0 || ti - tj < window || tj < sink). A row that sees no key
+ * (a sequence without keys, or with more rows than keys) is zeros, with lse -inf and no gradient. What a row does not see does not
+ * reach its result, whatever is stored there; the gradients of a sequence are numbers only where all its operands are.
+ *
+ * out [q_tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale q k^T) v; lse (NULL: not wanted) f32 [q_tokens, heads] = the natural
+ * logarithm of sum e^(scale q k^T). Results are the same bits from call to call with the same bounds and workspace.
+ * workspace: fv_packed_attention_workspace_bytes of the same numbers (0: none), 256-byte aligned, this call's alone until its work is done; too small or
+ * NULL: walks are not split among workgroups, which costs time only. */
+size_t fv_packed_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t q_tokens, size_t k_tokens,
+                                           size_t max_q, size_t max_k, int causal, size_t block_tokens, size_t window, size_t sink);
+int fv_packed_attention(const uint16_t* q, size_t q_stride, const uint16_t* k, size_t k_stride, const uint16_t* v,
+                        size_t v_stride, void* out, int out_is_bf16, float* lse, size_t heads, size_t kv_heads, size_t d,
+                        const int32_t* q_start, const int32_t* k_start, size_t seqs, size_t q_tokens, size_t k_tokens,
+                        size_t max_q, size_t max_k, float scale, int causal, size_t block_tokens, size_t window, size_t sink,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients dq [q_tokens, heads, d] and dk, dv [k_tokens, kv_heads, d] (contiguous, f32 or bf16 bits: grads_are_bf16) of a scalar from its gradient
+ * dout [q_tokens, heads, d] (contiguous, f32 or bf16 bits: dout_is_bf16; f32 is rounded to bf16 first) by the result of
+ * fv_packed_attention on the same operands and numbers, its out (contiguous, out_is_bf16) and lse: with P = e^(scale q k^T - lse), dv = P^T dout,
+ * dS = P (dout v^T - sum(dout out)), dq = scale dS k, dk = scale dS^T q, summed over the heads that share a key head, always in one order (no
+ * atomics). P and dS are rounded to bf16 for the second products. workspace: fv_packed_attention_backward_workspace_bytes, which it cannot do without. */
+size_t fv_packed_attention_backward_workspace_bytes(int dout_is_bf16, size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t q_tokens,
+                                                    size_t k_tokens, size_t max_q, size_t max_k, int causal, size_t block_tokens,
+                                                    size_t window, size_t sink);
+int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint16_t* q, size_t q_stride, const uint16_t* k,
+                                 size_t k_stride, const uint16_t* v, size_t v_stride, const void* out, int out_is_bf16,
+                                 const float* lse, void* dq, void* dk, void* dv, int grads_are_bf16, size_t heads, size_t kv_heads,
+                                 size_t d, const int32_t* q_start, const int32_t* k_start, size_t seqs, size_t q_tokens,
+                                 size_t k_tokens, size_t max_q, size_t max_k, float scale, int causal, size_t block_tokens,
+                                 size_t window, size_t sink, void* workspace, size_t workspace_bytes, void* stream);
+/* Rotary positions without tables. fv_rope_frequencies (host): for pair i of `pairs`, theta_i = base^(-i / pairs) radians a position, scaled for
+ * contexts `factor` times as long:
+ *   scaling 0: not (factor is not read); 1: theta / factor; 2: with base * factor^(pairs / (pairs - 1)) in place of base, which leaves the first
+ *   pair and slows the last by factor (pairs > 1); 3: by parts: theta (c + (1 - c) / factor), c = clamp((original theta / 2 pi - low) / (high - low), 0, 1), so
+ *   that pairs of more than `high` turns in the `original` context stay and those of fewer than `low` are slowed (original, low, high are read here alone);
+ * as turns a position in units of 2^-64: angles of any 32-bit position are exact to 2^-33 turns, with no table to make. */
+int fv_rope_frequencies(size_t pairs, double base, int scaling, double factor, double original, double low, double high,
+                        uint64_t* out);
+/* q [tokens, heads, d] (and k [tokens, kv_heads, d]; NULL: none) with the first 2 * pairs channels of each head turned by angles positions[token *
+ * axes + pair_axis[pair]] * freq[pair] and multiplied by `amplitude` (1.0f: a rotation), the others as they are, to q_out, k_out. inverse: turned back,
+ * which is the gradients' way (amplitude multiplies there too). halves == 0: pairs (2i, 2i + 1), else (i, i + pairs). All f32 or bf16 bits (in_is_bf16,
+ * out_is_bf16), the heads of a token contiguous, tokens a stride apart (multiples of 8 elements); d a multiple of 8, pairs of 8, 2 pairs <= d. An output may be
+ * its input (same address, stride and type) and may not overlap an input otherwise. freq: device [pairs] (fv_rope_frequencies); positions: device int32 [tokens, axes], axes 1
+ * to 4, any values; pair_axis: device int32 [pairs], values below axes (others count as 0), NULL: axis 0. Products in f32, unfused, one rounding. */
+int fv_rope_tokens(const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t heads, const void* k, size_t k_stride,
+                   void* k_out, size_t k_out_stride, size_t kv_heads, size_t d, int in_is_bf16, int out_is_bf16,
+                   const uint64_t* freq, const int32_t* pair_axis, size_t pairs, const int32_t* positions, size_t axes,
+                   size_t tokens, float amplitude, int halves, int inverse, void* stream);
+
 /* ---- Video Sparse Attention (rt/vsa.rs, rt/ops.rs:811-1619) --------------------------
  * Geometry: 64-token cubes (4x4x4 in t,h,w), TilePlan arrays as rt/vsa.rs:42-109:
  * slot_src [num_tiles*64] (token of each padded slot, -1 = padding), block_sizes

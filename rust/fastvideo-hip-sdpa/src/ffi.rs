@@ -120,6 +120,12 @@ extern "C" {
     pub fn fv_paged_attention_workspace_bytes_for(four_bits: c_int, heads: usize, kv_heads: usize, d: usize, seqs: usize, tokens: usize, max_q: usize, max_len: usize, block_tokens: usize, window: usize, sink: usize) -> usize;
     pub fn fv_paged_attention_workspace_bytes(heads: usize, kv_heads: usize, d: usize, seqs: usize, tokens: usize, max_q: usize, max_len: usize, block_tokens: usize, window: usize, sink: usize) -> usize;
     pub fn fv_paged_attention(q: *const u16, q_stride: usize, out: *mut c_void, out_is_bf16: c_int, heads: usize, k_pages: *const c_void, v_pages: *const c_void, k_scales: *const c_void, v_scales: *const c_void, pages: usize, page_tokens: usize, kv_heads: usize, d: usize, q_start: *const i32, lens: *const i32, table: *const i32, table_stride: usize, table_pages: usize, seqs: usize, tokens: usize, max_q: usize, max_len: usize, scale: f32, block_tokens: usize, window: usize, sink: usize, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn fv_packed_attention_workspace_bytes(heads: usize, kv_heads: usize, d: usize, seqs: usize, q_tokens: usize, k_tokens: usize, max_q: usize, max_k: usize, causal: c_int, block_tokens: usize, window: usize, sink: usize) -> usize;
+    pub fn fv_packed_attention(q: *const u16, q_stride: usize, k: *const u16, k_stride: usize, v: *const u16, v_stride: usize, out: *mut c_void, out_is_bf16: c_int, lse: *mut f32, heads: usize, kv_heads: usize, d: usize, q_start: *const i32, k_start: *const i32, seqs: usize, q_tokens: usize, k_tokens: usize, max_q: usize, max_k: usize, scale: f32, causal: c_int, block_tokens: usize, window: usize, sink: usize, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn fv_packed_attention_backward_workspace_bytes(dout_is_bf16: c_int, heads: usize, kv_heads: usize, d: usize, seqs: usize, q_tokens: usize, k_tokens: usize, max_q: usize, max_k: usize, causal: c_int, block_tokens: usize, window: usize, sink: usize) -> usize;
+    pub fn fv_packed_attention_backward(dout: *const c_void, dout_is_bf16: c_int, q: *const u16, q_stride: usize, k: *const u16, k_stride: usize, v: *const u16, v_stride: usize, out: *const c_void, out_is_bf16: c_int, lse: *const f32, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, grads_are_bf16: c_int, heads: usize, kv_heads: usize, d: usize, q_start: *const i32, k_start: *const i32, seqs: usize, q_tokens: usize, k_tokens: usize, max_q: usize, max_k: usize, scale: f32, causal: c_int, block_tokens: usize, window: usize, sink: usize, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn fv_rope_frequencies(pairs: usize, base: f64, scaling: c_int, factor: f64, original: f64, low: f64, high: f64, out: *mut u64) -> c_int;
+    pub fn fv_rope_tokens(q: *const c_void, q_stride: usize, q_out: *mut c_void, q_out_stride: usize, heads: usize, k: *const c_void, k_stride: usize, k_out: *mut c_void, k_out_stride: usize, kv_heads: usize, d: usize, in_is_bf16: c_int, out_is_bf16: c_int, freq: *const u64, pair_axis: *const i32, pairs: usize, positions: *const i32, axes: usize, tokens: usize, amplitude: f32, halves: c_int, inverse: c_int, stream: *mut c_void) -> c_int;
     pub fn fv_vsa_topk_for(sparsity: f64, num_tiles: usize) -> usize;
     pub fn fv_vsa_default_sparsity() -> f64;
     pub fn fv_vsa_tile_plan(t: usize, h: usize, w: usize, dims_out: *mut usize, slot_src: *mut i32, token_slot: *mut u32, block_sizes: *mut i32) -> c_int;
