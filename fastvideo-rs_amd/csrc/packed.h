@@ -1,6 +1,8 @@
 // Packed sequences: the tokens of sequences of different lengths one behind the other in [tokens, heads, d] tensors, queries and keys
 // with starts of their own. What the kernels of the attention (packed_attn.hip) and of its gradients (packed_back.hip) share.
 #pragma once
+#include <utility>
+
 #include "attn_core.h"
 #include "fv_internal.h"
 #include "paged.h"
@@ -35,6 +37,16 @@ FV_DEV PackedSeq packed_seq(const Batch& b, int s) {
     q.len = min(min(max(k_behind, q.k0), b.k_tokens) - q.k0, b.max_k);
     q.pos0 = q.len - (behind - q.start);
     return q;
+}
+
+// f(0), f(1), .., f(N - 1) with the numbers as types (loops that the compiler does not unroll in time).
+template <class F, int... I>
+FV_DEV void static_for_each(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+FV_DEV void static_for(F&& f) {
+    static_for_each(f, std::make_integer_sequence<int, N>{});
 }
 
 // The mask: without `causal` every row sees every key of its sequence; with it as in paged_sight.
@@ -121,6 +133,26 @@ FV_DEV void packed_offsets(unsigned (&off)[ITER], unsigned stride, int wave, int
 FV_DEV u32x4 packed_rows(const uint16_t* base, long first, long stride, int count, int row_bytes) {
     return plane_descriptor((const uint8_t*)base + first * stride, count > 0 ? (unsigned)((long)(count - 1) * stride) + (unsigned)row_bytes : 0u);
 }
+// The tiles of a walk over K or V, one after the other: where a tile lies goes on by one product that is made once.
+struct PackedRun {
+    const uint8_t* at;
+    long step, jump;   // to the next tile; from the sink's last to the band's first, besides
+    unsigned stride;
+    int left, gap;     // keys of the sequence from the tile's first; keys between the sink's tiles and the band's
+    int e, ns;
+    FV_DEV PackedRun(const uint16_t* base, long stride_, const PackedSeq& s, const PackedWalk& w, int e_) {
+        e = e_, ns = w.ns, stride = (unsigned)stride_;
+        const int key = w.key(e);
+        at = (const uint8_t*)base + (s.k0 + key) * stride_, left = s.len - key;
+        step = kTileRows * stride_, gap = (w.b0 - w.ns) * kTileRows, jump = gap * stride_;
+    }
+    FV_DEV u32x4 rows(int row_bytes) const { return plane_descriptor(at, (unsigned)(min(max(left, 1), kTileRows) - 1) * stride + (unsigned)row_bytes); }
+    FV_DEV void next() {
+        e++;
+        at += step, left -= kTileRows;
+        if (e == ns) at += jump, left -= gap;
+    }
+};
 // Two loads of a wave into LDS at `lds` (wave-uniform).
 FV_DEV void packed_issue(const u32x4& rows, unsigned o0, unsigned o1, unsigned lds) {
     const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds);

@@ -94,8 +94,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     packed_offsets<D>(voff, (unsigned)p.v_stride, wave, lane, [](int r) { return G::vswz(r); });
     const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
     const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
-    auto left_at = [&](int e) { return min(sq.len - w.key(min(e, e1 - 1)), kTileRows); };   // (past the walk: its last tile again)
-    auto rows_of = [&](const uint16_t* base, long stride, int e) { return packed_rows(base, sq.k0 + w.key(min(e, e1 - 1)), stride, left_at(e), G::kRow); };
+    PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
 
     f32x4 o[kNO][2], s_init[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     SoftmaxOffState st;
@@ -185,7 +184,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     for (int db = 0; db < kNO; db++) o[db][0] = o[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (e0 < e1) {
         {
-            const u32x4 kd = rows_of(kbase, p.k_stride, e0);
+            const u32x4 kd = krun.rows(G::kRow);
 #pragma unroll
             for (int u = 0; u < kUnits; u++) packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + u * 2048);
         }
@@ -194,7 +193,9 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
         wait_vmcnt<0>();
         block_barrier();
         constexpr int kAhead = 3;
-        u32x4 vd = rows_of(vbase, p.v_stride, e0), kd = rows_of(kbase, p.k_stride, e0 + 1);
+        // (past the walk: its last tile again)
+        if (e0 + 1 < e1) krun.next();
+        u32x4 vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow);
         auto phase = [&](int m, auto first) {
             const int e = e0 + m;
             ScoreTile s;
@@ -217,7 +218,9 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
                 else softmax_tile_off<true>(s, st, o, s_init, sl2, pb);
                 asm volatile("" ::"v"(pb[0][0]), "v"(pb[0][1]), "v"(pb[1][0]), "v"(pb[1][1]), "v"(st.l_acc[0]), "v"(st.l_acc[1]));
             }
-            vd = rows_of(vbase, p.v_stride, e + 1), kd = rows_of(kbase, p.k_stride, e + 2);
+            vrun.next();
+            if (e + 2 < e1) krun.next();
+            vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow);
             __builtin_amdgcn_sched_barrier(0);
             wait_vmcnt<0>();
             block_barrier();   // K(m + 1), V(m) resident; this phase's tiles read by every wave

@@ -18,15 +18,15 @@
 namespace fv {
 namespace {
 
-constexpr int kRows = 128;       // rows of a workgroup of packed_dq_kernel, keys of one of packed_dkv_kernel: 32 a wave
-constexpr int kStepRows = 32;    // rows a step of packed_dkv_kernel takes
+constexpr int kRows = 128;   // of a workgroup of packed_dq_kernel, 32 a wave
 
 struct PackedBackParams {
     PackedBatch b;
     PackedMask mask;
     const uint16_t *q, *k, *v, *dout;
     long q_stride, k_stride, v_stride, dout_stride;   // bytes between tokens
-    const f32x2* stats;                               // [kv_heads][tokens * group]: -lse / scale, -D
+    const float* stats;                               // [2][kv_heads][tokens * group]: -lse / scale; -D
+    long stat_rows;                                   // of a plane
     void *dq, *dk, *dv;
     int grads_are_bf16;
     int heads, kv_heads;
@@ -40,10 +40,14 @@ struct PackedBackParams {
     long part_rows, part_keys;
 };
 
-// Chunk c of row r of a tile lies at chunk c ^ both_swz(r): the 16 rows of a ds_read_b128 lie at 16 different chunks (64 channels: 8, in two halves
-// of a line) and the 8 rows of a transposed read at 8 different pairs of them, so a tile serves both kinds of operands without conflicts.
+// Chunk c of row r of a tile lies at chunk c ^ both_swz(r), so that a tile serves both kinds of operands without bank conflicts: the 8 rows of a
+// transposed read lie at 8 different pairs of chunks, and the 16 lanes that a ds_read_b128 serves at once, rows 0 .. 3 and 12 .. 15 of one chunk
+// and 4 .. 11 of its neighbour, at 16 different chunks (64 channels: 8, in two halves of a line): with the rows' pairs in order
+// rows 8 .. 15 take the other chunk of the pairs of rows 4 .. 7, 0 .. 3.
 template <int D>
-FV_DEV int both_swz(int r) { return D == 128 ? ((r & 7) << 1 | ((r >> 3) & 1)) : (((r >> 1) & 3) << 1 | ((r >> 3) & 1)); }
+FV_DEV int both_swz(int r) {
+    return D == 128 ? (((r & 7) ^ ((r >> 1) & 4)) << 1 | ((r >> 3) & 1)) : ((((r >> 1) & 3) ^ ((r >> 2) & 2)) << 1 | ((r >> 3) & 1));
+}
 template <int D>
 FV_DEV TileReadBases both_bases(int lane) {
     using G = TileGeo<D>;
@@ -53,7 +57,7 @@ FV_DEV TileReadBases both_bases(int lane) {
 
 // D / 8 threads a row (token, head); OUT16, DOUT16: bf16 bits. An f32 gradient is kept as bf16 bits in `rounded` [tokens, heads, d].
 template <int D, bool OUT16, bool DOUT16>
-__global__ __launch_bounds__(256) void packed_stats_kernel(const void* dout, const void* out, const float* lse, f32x2* stats, uint16_t* rounded, long rows,
+__global__ __launch_bounds__(256) void packed_stats_kernel(const void* dout, const void* out, const float* lse, float* stats, uint16_t* rounded, long rows,
                                                            long tokens, int heads, PagedDiv group, float inv_scale) {
     constexpr int kPer = D / 8;
     const int c = threadIdx.x % kPer;
@@ -94,7 +98,9 @@ __global__ __launch_bounds__(256) void packed_stats_kernel(const void* dout, con
         const long t = row / heads;
         const int h = (int)(row - t * heads), kvh = paged_quot(h, group);
         const float l = lse[row];
-        stats[((long)kvh * tokens + t) * group.by + (h - kvh * group.by)] = f32x2{l == neg_inf() ? l : -l * inv_scale, -sum};
+        float* at = stats + ((long)kvh * tokens + t) * group.by + (h - kvh * group.by);
+        at[0] = l == neg_inf() ? l : -l * inv_scale;
+        at[rows] = -sum;
     }
 }
 
@@ -114,7 +120,14 @@ FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group)
     k.hi = hi >= s.count ? 0x7fffffff : (int)max(hi, 0L) * group;
     return k;
 }
-// The steps [from, to) of kStepRows rows that some key of [first, last] is seen by.
+// packed_dkv_kernel: a workgroup's keys, the rows of a step, and its LDS: V's operands | 2 x (q, dout) | 2 x (-lse / scale, -D).
+constexpr int kKeys = 128, kStep = 32;
+template <int D>
+struct KeyForm {
+    static constexpr int kHalf = kStep * 2 * D;   // bytes of a step's q, or dout
+    static constexpr int kFrags = D / 16, kSteps = 4 * kFrags * 1024, kStats = kSteps + 4 * kHalf, kLds = kStats + 2 * 256;
+};
+// The steps [from, to) that some key of [first, last] is seen by.
 struct RowWalk {
     int from, to;
 };
@@ -122,33 +135,115 @@ template <class Mask>
 FV_DEV RowWalk row_walk(const Mask& m, const PackedSeq& s, int first, int last, int group) {
     const int rows = s.count * group;
     const KeySight a = key_sight(m, s, first, group), b = key_sight(m, s, last, group);
-    return {a.lo / kStepRows, (min(rows, max(a.hi, b.hi)) + kStepRows - 1) / kStepRows};
+    return {a.lo / kStep, (min(rows, max(a.hi, b.hi)) + kStep - 1) / kStep};
 }
 
-// 128 keys of one (sequence, key head), 32 a wave, over steps of 32 rows of q and dout that pass through LDS, two buffers each. A lane has
-// two keys (columns lane % 16 and 16 + lane % 16 of its wave's): S and dP [rows x keys] come out of the products in the layout that the second ones
-// take P and dS in, and dV^T, dK^T [d x keys] stay in 128 registers (64 at 64 channels). K's operands stay in registers, V's in LDS, which
-// has room for it: a product's operands are read once for two, and an LDS read a product costs nothing (at two waves a SIMD 1706
-// and 1715 TFLOP/s of 16x16x32 with half a ds_read_b128 each and one).
+// A wave's part in a step of 32 rows at `qt` and `gt` (q and dout), `cut`: with keys that rows do not see, whose scores become -inf. The products, two to a unit that shares an operand read: S = Q K^T - lse / scale, 16 rows after 16; dP = dO V^T - D; dV^T += dO^T P; dK^T += Q^T dS. The vector work lies
+// in their shadow: a 16x16x32 product holds the matrix pipe for four instructions' time, of which two others of the same wave cost
+// nothing (measured, with one wave a SIMD: 8.1 ns a product with none, 8.7 with two multiplications, 10.3 with three; an exponential counts for two). So the
+// exponentials of the first 16 rows run under the scores of the others and dP, dS under dV. With the softmax by itself between dP and dV: 5 to 6 %
+// slower. Operands are read three units ahead: one, 15 % slower; four need registers that are not there.
+template <int D>
+FV_DEV void key_step(const lds_u8* qt, const lds_u8* gt, const lds_u8* vt, const lds_u8* stat, const TileReadBases& rb, const bf16x8 (&kf)[D / 32][2],
+                     f32x4 (&dk)[D / 16][2], f32x4 (&dv)[D / 16][2], float sl2, bool cut, const KeySight (&mine)[2], int row0) {
+    using G = TileGeo<D>;
+    constexpr int kNK = D / 32, U = 2 * kNK, kUnits = 4 * U, kAhead = 3;
+    const int lane = threadIdx.x & 63, q4 = lane >> 4;
+    bf16x8 a[kUnits], b[kNK][2];        // a unit's operand; V's
+    int read_k = rb.k, read_v = rb.v;   // (pinned: the addresses made from them would take registers over the whole loop)
+    asm volatile("" : "+v"(read_k), "+v"(read_v));
+    auto issue = [&](int u) {
+        if (u < U) {              // Q, 16 rows u / kNK
+            a[u] = lds_read_b128(qt + (read_k ^ ((u % kNK) << 6)) + (u / kNK) * 16 * G::kRow);
+        } else if (u < 2 * U) {   // dO, 16 rows u % 2 of d chunk (u - U) / 2, and before the first V's
+            const int dc = (u - U) >> 1, x = u & 1;
+            if (x == 0) {
+#pragma unroll
+                for (int g = 0; g < 2; g++) b[dc][g] = lds_read_b128(vt + (2 * dc + g) * 1024 + lane * 16);
+            }
+            a[u] = lds_read_b128(gt + (read_k ^ (dc << 6)) + x * 16 * G::kRow);
+        } else {                  // dO^T, then Q^T, 16 channels u % U
+            a[u] = read_v_frag<D>((u < 3 * U ? gt : qt) + (read_v ^ ((u % U) << 5)));
+        }
+    };
+    f32x4 s[2][2], dp[2][2], init_s[2], init_d[2];   // [16 rows][16 keys]; what their sums start from
+    bf16x8 pb[2], ds[2];       // the second products' operands: of 32 rows, those of both blocks that the lane has
+    // Vector work k of 16 scores, of the first 16 rows first: the lane's rows i of keys g.
+    auto score = [&](int k) { s[k >> 3][(k >> 2) & 1][k & 3] = fast_exp2(s[k >> 3][(k >> 2) & 1][k & 3] * sl2); };
+    auto weigh = [&](int k) { dp[k >> 3][(k >> 2) & 1][k & 3] *= s[k >> 3][(k >> 2) & 1][k & 3]; };
+    auto round = [&](const f32x4 (&from)[2][2], bf16x8 (&to)[2], int c) {   // pair c of 8
+        const int g = c >> 2, x = (c >> 1) & 1, i = 2 * (c & 1);
+        const bf16x2 y = __builtin_convertvector((f32x2{from[x][g][i], from[x][g][i + 1]}), bf16x2);
+        to[g][4 * x + i] = y[0], to[g][4 * x + i + 1] = y[1];
+    };
+    auto stat_rows = [&](int x, int which) { return *reinterpret_cast<const __attribute__((address_space(3))) f32x4*>(stat + 128 * which + (16 * x + 4 * q4) * 4); };
+    auto hide = [&](int x) {
+        if (!cut) return;
+        auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int r = row0 + 16 * x + 4 * q4;
+            const unsigned bits = below(mine[g].hi - r) & ~below(mine[g].lo - r);
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[x][g][i] = (bits >> i) & 1 ? s[x][g][i] : neg_inf();
+        }
+    };
+    auto gap = [&](auto n) {   // behind product n
+        if constexpr (n() == 2 * U - 6 || n() == 2 * U - 4) {
+            constexpr int x = (n() - 2 * U + 6) / 2;
+            init_d[x] = stat_rows(x, 1);
+        }
+        if constexpr (n() == U + 1) hide(0);
+        if constexpr (n() == 2 * U + 1) hide(1);
+        static_for<16>([&](auto k) {
+            if constexpr (n() == U + 2 + k() * U / 8) score(k());
+            if constexpr (n() == 4 * U + 2 + k() * U / 16) weigh(k());
+            if constexpr (k() < 8 && n() == 3 * U + 2 + k() * U / 16) round(s, pb, k());
+            if constexpr (k() < 8 && n() == 5 * U + 2 + k() * U / 16) round(dp, ds, k());
+        });
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) issue(u);
+#pragma unroll
+    for (int x = 0; x < 2; x++) init_s[x] = stat_rows(x, 0);
+    __builtin_amdgcn_s_setprio(1);
+    static_for<2 * kUnits>([&](auto at) {
+        constexpr int u = at() / 2, g = at() & 1;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (u < U) s[u / kNK][g] = mfma16(a[u], kf[u % kNK][g], u % kNK == 0 ? init_s[u / kNK] : s[u / kNK][g]);
+        else if constexpr (u < 2 * U) dp[u & 1][g] = mfma16(a[u], b[(u - U) >> 1][g], u < U + 2 ? init_d[u & 1] : dp[u & 1][g]);
+        else if constexpr (u < 3 * U) dv[u % U][g] = mfma16(a[u], pb[g], dv[u % U][g]);
+        else dk[u % U][g] = mfma16(a[u], ds[g], dk[u % U][g]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (g == 0 && u + kAhead < kUnits) issue(u + kAhead);
+        gap(at);
+    });
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// 128 keys of one (sequence, key head), 32 a wave, over steps of 32 rows of q and dout that pass through LDS, two buffers each (three, a step's
+// rows on their way for two: 6 to 9 % slower). A lane has two keys (columns lane % 16 and 16 + lane % 16 of its wave's): S and dP [rows x keys] come out of the products in the layout that the second ones take P and dS in, and dV^T, dK^T [d x keys] stay in 128
+// registers (64 at 64 channels). K's operands stay in registers, V's in LDS as they are read: an operand is read once for two products, and an LDS
+// read a product costs nothing (at two waves a SIMD 1706 and 1715 TFLOP/s of 16x16x32 with half a ds_read_b128 each and one).
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const PackedBackParams p) {
     using G = TileGeo<D>;
-    constexpr int kNO = D / 16, kNK = D / 32, kHalf = kStepRows * G::kRow;   // bytes of a step's q, or dout
-    constexpr int kLoads = kHalf / 4096;                                       // of a wave: its part of a step's q
+    using F = KeyForm<D>;
+    constexpr int kNO = D / 16, kNK = D / 32, kHalf = F::kHalf;
+    constexpr int kLoads = kHalf / 4096;   // of a wave: its part of a step's q
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
-    // V | 2 x (q, dout) | 2 x stats
-    constexpr int kSteps = kRows * G::kRow, kStats = kSteps + 4 * kHalf;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
     const PackedItem item = packed_item(p.key_items, blockIdx.x);
     if (item.head < 0) return;
     const int kvh = item.head, group = p.group.by;
     const PackedKeys kb = {p.b.k_start, p.b.seqs, p.b.k_tokens};
-    const PagedPiece piece = paged_piece<kRows>(p.key_pieces, kb, 1, item.piece);   // (a sequence's first keys, which most rows see, first)
+    const PagedPiece piece = paged_piece<kKeys>(p.key_pieces, kb, 1, item.piece);   // (a sequence's first keys, which most rows see, first)
     const PackedSeq sq = packed_seq(p.b, piece.seq);
-    const int key0 = piece.tile * kRows;
+    const int key0 = piece.tile * kKeys;
     if (key0 >= sq.len) return;
-    const int rows = sq.count * group, last = min(key0 + kRows, sq.len) - 1;
+    const int rows = sq.count * group, last = min(key0 + kKeys, sq.len) - 1;
     const RowWalk walk = row_walk(p.mask, sq, key0, last, group);
     const int e0 = walk.from + item.share * p.key_chunk, e1 = min(walk.to, e0 + p.key_chunk);
     if (item.share > 0 && e0 >= e1) return;
@@ -166,23 +261,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
         some = {a.lo, max(a.hi, b.hi)}, all = {b.lo, key_sight(p.mask, sq, max(wkey, early), group).hi};
     }
     const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
-    // V: the wave's 32 rows into its part of LDS
     const unsigned lds0 = (unsigned)(size_t)smem;
+    // V: the wave's operands, 1 KB each: the lane's 16 bytes of key i16 (+ 16) and chunk 4 dc + q4
+    bf16x8 kf[kNK][2];
     {
-        constexpr int kIter = 32 * G::kRow / 1024;
         const u32x4 vd = packed_rows(vbase, sq.k0 + wkey, p.v_stride, min(sq.len - wkey, 32), G::kRow);
+        const unsigned at = (unsigned)i16 * (unsigned)p.v_stride + 16u * q4;
 #pragma unroll
-        for (int it = 0; it < kIter; it += 2) {
-            unsigned off[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int r = (it + x) * G::kRowsPerDma + lane / G::kChunks, c = lane % G::kChunks;
-                off[x] = (unsigned)r * (unsigned)p.v_stride + ((unsigned)(c ^ both_swz<D>(r)) << 4) - x * 1024u;
-            }
-            packed_issue(vd, off[0], off[1], lds0 + wave * 32 * G::kRow + it * 1024);
+        for (int f = 0; f < F::kFrags; f++) {
+            const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + (wave * F::kFrags + f) * 1024)), off = at + (f & 1) * 16u * (unsigned)p.v_stride + (f >> 1) * 64;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m0), "v"(off), "s"(vd) : "memory");
         }
     }
-    bf16x8 kf[kNK][2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         const int key = wkey + 16 * g + i16;
@@ -194,29 +284,54 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
             kf[dk][g] = __builtin_bit_cast(bf16x8, x);
         }
     }
-    // A step's rows into buffer `buf`: each wave loads 8 rows of q and of dout, the first one the statistics.
-    auto load = [&](int e, int buf) {
-        const int r0 = e * kStepRows, t0 = paged_quot(r0, p.group);
-        const uint8_t* qb = (const uint8_t*)p.q + (long)(sq.start + t0) * p.q_stride + (long)kvh * group * G::kRow;
-        const uint8_t* gb = (const uint8_t*)p.dout + (long)(sq.start + t0) * p.dout_stride + (long)kvh * group * G::kRow;
-        const u32x4 qd = plane_descriptor(qb, 0x80000000u), gd = plane_descriptor(gb, 0x80000000u);
-        const unsigned at = lds0 + kSteps + buf * 2 * kHalf + wave * (kHalf / 4);
+    // Steps are loaded from the walk's last to its first: their rows' tokens t0 .. and the h0 heads of t0 before them, and where t0 and the statistics lie, go
+    // back by 32 rows a step. (The same from the step's number, 50 scalar instructions in a row, cost 13 to 17 % of the time.) Row x of a step is token t0 + dt,
+    // dt = (h0 + x) / group, of numbers below group + 32. Rows lie in the order of their addresses, so those behind the last are cut off by the
+    // descriptor (zeros); only the walk's last step has any.
+    const int back = kStep / group, back_heads = kStep - back * group;   // tokens and heads of 32 rows
+    const unsigned mul = 65536u / (unsigned)group + 1, qstep = (unsigned)p.q_stride - (unsigned)(group * G::kRow), gstep = (unsigned)p.dout_stride - (unsigned)(group * G::kRow);
+    auto row_dt = [&](int x) { return group >= 32 ? (x >= group ? 1 : 0) : (int)((unsigned)x * mul >> 16); };
+    const int r_last = (e1 - 1) * kStep, t_last = paged_quot(r_last, p.group);
+    int h0 = r_last - t_last * group;
+    const uint8_t* qb = (const uint8_t*)p.q + (long)(sq.start + t_last) * p.q_stride + (long)kvh * group * G::kRow;
+    const uint8_t* gb = (const uint8_t*)p.dout + (long)(sq.start + t_last) * p.dout_stride + (long)kvh * group * G::kRow;
+    const float* sb = p.stats + (wave & 1) * p.stat_rows + ((long)kvh * p.b.tokens + sq.start) * group + r_last;
+    unsigned qo[kLoads], go[kLoads];
+    auto offsets = [&]() {
 #pragma unroll
         for (int it = 0; it < kLoads; it++) {
-            const int rr = (wave * kLoads + it) * G::kRowsPerDma + lane / G::kChunks, r = r0 + rr, t = paged_quot(r, p.group);
-            const unsigned in = (unsigned)((r - t * group) * G::kRow) + ((unsigned)((lane % G::kChunks) ^ both_swz<D>(rr)) << 4);
-            const bool none = r >= rows;   // (past the range: zeros)
-            const unsigned qo = none ? 0x80000000u : (unsigned)(t - t0) * (unsigned)p.q_stride + in, go = none ? 0x80000000u : (unsigned)(t - t0) * (unsigned)p.dout_stride + in;
+            const int rr = (wave * kLoads + it) * G::kRowsPerDma + lane / G::kChunks, x = h0 + rr, dt = row_dt(x);
+            const unsigned in = (unsigned)(x * G::kRow) + ((unsigned)((lane % G::kChunks) ^ both_swz<D>(rr)) << 4);
+            qo[it] = (unsigned)dt * qstep + in, go[it] = (unsigned)dt * gstep + in;
+        }
+    };
+    offsets();
+    unsigned q_bytes, g_bytes, s_bytes;
+    {
+        const int n = max(min(rows - r_last, kStep), 1), end = h0 + n - 1, dt_end = row_dt(end);   // the last row
+        q_bytes = (unsigned)dt_end * qstep + (unsigned)(end + 1) * G::kRow, g_bytes = (unsigned)dt_end * gstep + (unsigned)(end + 1) * G::kRow, s_bytes = n * 4u;
+    }
+    auto load = [&](int buf) {
+        const u32x4 qd = plane_descriptor(qb, q_bytes), gd = plane_descriptor(gb, g_bytes);
+        const unsigned at = lds0 + F::kSteps + buf * 2 * kHalf + wave * (kHalf / 4);
+#pragma unroll
+        for (int it = 0; it < kLoads; it++) {
             const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(at + it * 1024)), m1 = m0 + kHalf;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
                          "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds"
-                         :: "s"(m0), "s"(m1), "v"(qo), "v"(go), "s"(qd), "s"(gd) : "memory");
+                         :: "s"(m0), "s"(m1), "v"(qo[it]), "v"(go[it]), "s"(qd), "s"(gd) : "memory");
         }
-        if (wave == 0) {
-            const u32x4 sd = plane_descriptor(p.stats + ((long)kvh * p.b.tokens + sq.start) * group + r0, (unsigned)min(rows - r0, kStepRows) * 8u);
-            const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + kStats + buf * 256));
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(m0), "v"(lane * 4), "s"(sd) : "memory");
+        if (wave < 2) {   // (32 floats, -lse / scale or -D)
+            const u32x4 sd = plane_descriptor(sb, s_bytes);
+            const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + F::kStats + buf * 256 + wave * 128));
+            if (lane < 32) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(m0), "v"(lane * 4), "s"(sd) : "memory");
         }
+        q_bytes = g_bytes = 0x80000000u, s_bytes = 128;
+        h0 -= back_heads;
+        const bool more = h0 < 0;
+        h0 += more ? group : 0;
+        qb -= (long)(back + more) * p.q_stride, gb -= (long)(back + more) * p.dout_stride, sb -= kStep;
+        if (back_heads != 0) offsets();
     };
     const TileReadBases rb = both_bases<D>(lane);
     f32x4 dv[kNO][2], dk[kNO][2];
@@ -226,110 +341,27 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
         for (int g = 0; g < 2; g++) dv[db][g] = dk[db][g] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float sl2 = p.sl2;
 
+    // (The walk goes backwards: under a causal mask every piece ends at the sequence's last row, so that workgroups that begin together go through the same
+    // rows, which an L2 then holds.)
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): K's operands, on every path, or the compiler waits for them, and so for the steps' loads, in the loop
     if (e0 < e1) {
-        load(e0, 0);
-#pragma unroll
-        for (int x = 0; x < kNK; x++) asm volatile("" : "+v"(kf[x][0]), "+v"(kf[x][1]));   // (waited for here)
+        load(0);
         wait_vmcnt<0>();
         block_barrier();
     }
+    int buf = 0;
 #pragma unroll 1
-    for (int e = e0; e < e1; e++) {
-        const int buf = (e - e0) & 1, r0 = e * kStepRows;
-        if (e + 1 < e1) load(e + 1, buf ^ 1);
-        if (r0 + kStepRows > some.lo && r0 < some.hi && !idle) {
-            const lds_u8* qt = smem + kSteps + buf * 2 * kHalf;
-            const lds_u8* gt = qt + kHalf;
-            const lds_u8* vt = smem + wave * 32 * G::kRow;
-            const lds_u8* stat = smem + kStats + buf * 256;
-            f32x4 s[2][2], dp[2][2];   // [16 rows][16 keys]
-            // S = Q K^T - lse / scale and dP = dO V^T - D: a group is two operands of 16 rows (dP: and two of keys) for four products
-            constexpr int kN1 = 2 * kNK, kAhead = 2;
-            bf16x8 f[kN1][2], fv[kN1][2];
-            auto issue1 = [&](int i, int x) {
-                const int at = (rb.k ^ ((i >> 1) << 6)) + x * 16 * G::kRow;
-                if (i & 1) f[i][x] = lds_read_b128(gt + at), fv[i][x] = lds_read_b128(vt + at);
-                else f[i][x] = lds_read_b128(qt + at);
-            };
-            f32x4 init_s[2], init_d[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const auto* at = reinterpret_cast<const __attribute__((address_space(3))) f32x4*>(stat + (16 * x + 4 * q4) * 8);
-                const f32x4 a = at[0], b = at[1];
-                init_s[x] = f32x4{a[0], a[2], b[0], b[2]};
-                init_d[x] = f32x4{a[1], a[3], b[1], b[3]};
-            }
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) issue1(i, 0), issue1(i, 1);
-#pragma unroll
-            for (int i = 0; i < kN1; i++) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int x = j >> 1, g = j & 1;
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (i & 1) dp[x][g] = mfma16(f[i][x], fv[i][g], i < 2 ? init_d[x] : dp[x][g]);
-                    else s[x][g] = mfma16(f[i][x], kf[i >> 1][g], i < 2 ? init_s[x] : s[x][g]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (j < 2 && i + kAhead < kN1) issue1(i + kAhead, j);
-                }
-            }
-            __builtin_amdgcn_s_setprio(0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (r0 < all.lo || r0 + kStepRows > all.hi) {
-                auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const int at = r0 + 16 * x + 4 * q4;
-                        const unsigned bits = below(mine[g].hi - at) & ~below(mine[g].lo - at);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            s[x][g][i] = (bits >> i) & 1 ? s[x][g][i] : neg_inf();
-                            dp[x][g][i] = (bits >> i) & 1 ? dp[x][g][i] : 0.f;
-                        }
-                    }
-            }
-            // P and dS, the rows of both blocks the second products' eight
-            bf16x8 pb[2], db_[2];
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                f32x8 a, b;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    a[i] = fast_exp2(s[i >> 2][g][i & 3] * sl2);
-                    b[i] = a[i] * dp[i >> 2][g][i & 3];
-                }
-                pb[g] = __builtin_convertvector(a, bf16x8);
-                db_[g] = __builtin_convertvector(b, bf16x8);
-            }
-            asm volatile("" ::"v"(pb[0]), "v"(pb[1]), "v"(db_[0]), "v"(db_[1]));
-            __builtin_amdgcn_sched_barrier(0);
-            // dV^T += dO^T P, dK^T += Q^T dS
-            constexpr int kN2 = 2 * (kNO / 2), kAhead2 = 3;
-            bf16x8 h[kN2][2];
-            auto issue2 = [&](int i, int x) { h[i][x] = read_v_frag<D>((i < kNO / 2 ? gt : qt) + (rb.v ^ ((2 * (i % (kNO / 2)) + x) << 5))); };
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < kAhead2; i++) issue2(i, 0), issue2(i, 1);
-#pragma unroll
-            for (int i = 0; i < kN2; i++) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int x = j >> 1, g = j & 1, db = 2 * (i % (kNO / 2)) + x;
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (i < kNO / 2) dv[db][g] = mfma16(h[i][x], pb[g], dv[db][g]);
-                    else dk[db][g] = mfma16(h[i][x], db_[g], dk[db][g]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (j < 2 && i + kAhead2 < kN2) issue2(i + kAhead2, j);
-                }
-            }
-            __builtin_amdgcn_s_setprio(0);
+    for (int e = e1 - 1; e >= e0; e--) {
+        if (e - 1 >= e0) load(buf ^ 1);
+        if ((e + 1) * kStep > some.lo && e * kStep < some.hi && !idle) {
+            const lds_u8* step = smem + F::kSteps + buf * 2 * kHalf;
+            const bool cut = e * kStep < all.lo || (e + 1) * kStep > all.hi;
+            key_step<D>(step, step + kHalf, smem + wave * F::kFrags * 1024, smem + F::kStats + buf * 256, rb, kf, dk, dv, sl2, cut, mine, e * kStep);
         }
+        buf ^= 1;
         __builtin_amdgcn_sched_barrier(0);
         wait_vmcnt<0>();
-        block_barrier();
+        block_barrier();   // the next step resident; this one's read by every wave
         __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -337,7 +369,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
         const int key = wkey + 16 * g + i16;
         if (key >= sq.len) continue;
         const size_t dst = ((size_t)(sq.k0 + key) * p.kv_heads + kvh) * D;
-        float* part = p.part_dkv + ((size_t)item.share * p.part_keys + (size_t)(kvh * p.key_items.n.by + item.piece) * kRows + (key - key0)) * 2 * D;
+        float* part = p.part_dkv + ((size_t)item.share * p.part_keys + (size_t)(kvh * p.key_items.n.by + item.piece) * kKeys + (key - key0)) * 2 * D;
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
             const int at = 16 * db + 4 * q4;
@@ -359,6 +391,94 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
 }
 
 // ---- the queries' gradients ------------------------------------------------------------------------------------------
+
+// A wave's part in a tile of 64 keys at `kt` and `vt`, `cut`: with keys that rows do not see (key0: the tile's first). In halves of 32 keys, two
+// products to a unit: S^T = K Q^T - lse / scale and dP^T = V dO^T - D of the one, of the other, dQ^T += K^T dS of the one, of the other, with the vector work
+// in their shadow, as in key_step: the exponentials under dP, dS of a half under what follows it.
+template <int D>
+FV_DEV void row_step(const lds_u8* kt, const lds_u8* vt, const TileReadBases& rb, const bf16x8 (&qf)[D / 32][2], const bf16x8 (&gf)[D / 32][2],
+                     const f32x4 (&s_init)[2], const f32x4 (&d_init)[2], f32x4 (&dq)[D / 16][2], float sl2, bool cut, const PagedSight& mine, int key0) {
+    using G = TileGeo<D>;
+    constexpr int kNK = D / 32, U = 2 * kNK, kAll = 6 * U, kAhead = 3;
+    const int q4 = (threadIdx.x >> 4) & 3;
+    bf16x8 a[kAll];
+    int read_k = rb.k, read_v = rb.v;
+    asm volatile("" : "+v"(read_k), "+v"(read_v));
+    auto issue = [&](int n) {
+        if (n < 4 * U) {   // K, V of the first half, K, V of the second: 16 keys (n % U) / kNK, d chunk n % kNK
+            const int half = n / (2 * U), x = n % U / kNK;
+            a[n] = lds_read_b128((n / U & 1 ? vt : kt) + (read_k ^ ((n % kNK) << 6)) + (32 * half + 16 * x) * G::kRow);
+        } else {           // K^T, 16 channels n % U
+            a[n] = read_v_frag<D>(kt + (read_v ^ ((n % U) << 5)) + 32 * (n / U - 4) * G::kRow);
+        }
+    };
+    f32x4 s[2][2][2], dp[2][2][2];   // [half][16 keys][16 rows]
+    bf16x8 ds[2][2];
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int g = 0; g < 2; g++) s[half][x][g] = s_init[g];
+    if (cut) {
+        const unsigned m[3] = {(unsigned)mine.a, (unsigned)mine.lo, (unsigned)mine.hi};
+        int both[3][2];   // the even rows of 16 lanes hold block 0's, the odd ones block 1's
+#pragma unroll
+        for (int x = 0; x < 3; x++) {
+            const auto r = __builtin_amdgcn_permlane16_swap(m[x], m[x], false, false);
+            both[x][0] = (int)r[0];
+            both[x][1] = (int)r[1];
+        }
+        auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const int at = key0 + 32 * half + 16 * x + 4 * q4;
+                    const unsigned bits = below(both[0][g] - at) | (below(both[2][g] - at) & ~below(both[1][g] - at));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[half][x][g][i] = (bits >> i) & 1 ? s[half][x][g][i] : neg_inf();
+                }
+    }
+    auto score = [&](int half, int k) {   // k: of 16, the first 16 keys first
+        const int x = k >> 3, g = (k >> 2) & 1, i = k & 3;
+        s[half][x][g][i] = fast_exp2(s[half][x][g][i] * sl2);
+    };
+    auto weigh = [&](int half, int k) {
+        const int x = k >> 3, g = (k >> 2) & 1, i = k & 3;
+        dp[half][x][g][i] *= s[half][x][g][i];
+    };
+    auto round = [&](int half, int c) {   // pair c of 8
+        const int g = c >> 2, x = (c >> 1) & 1, i = 2 * (c & 1);
+        const bf16x2 y = __builtin_convertvector((f32x2{dp[half][x][g][i], dp[half][x][g][i + 1]}), bf16x2);
+        ds[half][g][4 * x + i] = y[0], ds[half][g][4 * x + i + 1] = y[1];
+    };
+    auto gap = [&](auto n) {   // behind product n
+        static_for<32>([&](auto i) {
+            constexpr int half = i() / 16, k = i() % 16, m = n() - 4 * U * half;
+            if constexpr (m == U + 2 + k * U / 8) score(half, k);
+            if constexpr (m == (k < 8 ? 3 * U + 2 + k * U / 16 : 4 * U + 2 + (k - 8) * U / 16)) weigh(half, k);
+            if constexpr (k < 8 && m == 4 * U + 2 + U / 2 + k * U / 16) round(half, k);
+        });
+    };
+#pragma unroll
+    for (int n = 0; n < kAhead; n++) issue(n);
+    __builtin_amdgcn_s_setprio(1);
+    static_for<2 * kAll>([&](auto at) {
+        constexpr int n = at() / 2, g = at() & 1, half = n / (2 * U), x = n % U / kNK, dc = n % kNK;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (n >= 4 * U) dq[n % U][g] = mfma16(a[n], ds[n / U - 4][g], dq[n % U][g]);
+        else if constexpr (n / U & 1) dp[half][x][g] = mfma16(a[n], gf[dc][g], dc == 0 ? d_init[g] : dp[half][x][g]);
+        else s[half][x][g] = mfma16(a[n], qf[dc][g], s[half][x][g]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (g == 0 && n + kAhead < kAll) issue(n + kAhead);
+        gap(at);
+    });
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // 128 rows of one (sequence, key head), 32 a wave, over tiles of 64 keys in LDS, two buffers for K and for V. Q and dO stay in registers; S^T =
 // K Q^T and dP^T = V dO^T leave the scores of two rows in a lane, dS the operand of dQ^T += K^T dS, whose K is the
@@ -406,10 +526,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
             qf[dk][g] = __builtin_bit_cast(bf16x8, x);
             gf[dk][g] = __builtin_bit_cast(bf16x8, y);
         }
-        f32x2 stat = {0.f, 0.f};
-        if (r < rows) stat = p.stats[((long)kvh * p.b.tokens + sq.start) * group + r];
+        float nlse = 0.f, nd = 0.f;
+        if (r < rows) {
+            const float* at = p.stats + ((long)kvh * p.b.tokens + sq.start) * group + r;
+            nlse = at[0], nd = at[p.stat_rows];
+        }
 #pragma unroll
-        for (int i = 0; i < 4; i++) s_init[g][i] = stat[0], d_init[g][i] = stat[1];
+        for (int i = 0; i < 4; i++) s_init[g][i] = nlse, d_init[g][i] = nd;
     }
     const TileReadBases rb = both_bases<D>(lane);
     unsigned koff[kIter], voff[kIter];
@@ -417,110 +540,32 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
     packed_offsets<D>(voff, (unsigned)p.v_stride, wave, lane, [](int r) { return both_swz<D>(r); });
     const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
     const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
-    auto load = [&](int e, int buf) {
-        const int key = w.key(e), left = min(sq.len - key, kTileRows);
-        const u32x4 kd = packed_rows(kbase, sq.k0 + key, p.k_stride, left, G::kRow), vd = packed_rows(vbase, sq.k0 + key, p.v_stride, left, G::kRow);
+    PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
+    auto load = [&](int buf) {
+        const u32x4 kd = krun.rows(G::kRow), vd = vrun.rows(G::kRow);
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
             packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + buf * kTile + u * 2048);
             packed_issue(vd, voff[2 * u], voff[2 * u + 1], slot + (2 + buf) * kTile + u * 2048);
         }
+        krun.next(), vrun.next();
     };
     f32x4 dq[kNO][2];
 #pragma unroll
     for (int db = 0; db < kNO; db++) dq[db][0] = dq[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the operands and statistics, on every path (as above)
     if (e0 < e1) {
-        load(e0, 0);
-#pragma unroll
-        for (int dk = 0; dk < kNK; dk++) asm volatile("" : "+v"(qf[dk][0]), "+v"(qf[dk][1]), "+v"(gf[dk][0]), "+v"(gf[dk][1]));
-        asm volatile("" : "+v"(s_init[0]), "+v"(s_init[1]), "+v"(d_init[0]), "+v"(d_init[1]));
+        load(0);
         wait_vmcnt<0>();
         block_barrier();
     }
 #pragma unroll 1
     for (int e = e0; e < e1; e++) {
         const int buf = (e - e0) & 1;
-        if (e + 1 < e1) load(e + 1, buf ^ 1);
+        if (e + 1 < e1) load(buf ^ 1);
         if (!idle) {
-            const bool cut = !whole.tile(e);
-#pragma unroll
-            for (int t = 0; t < 2; t++) {   // 32 keys at a time: the scores of 64 and their operands would not fit the registers
-                const lds_u8* kt = smem + buf * kTile + 32 * t * G::kRow;
-                const lds_u8* vt = kt + 2 * kTile;
-                f32x4 s[2][2], dp[2][2];   // [16 keys][16 rows]
-                constexpr int kN1 = 2 * kNK, kAhead = 3;   // groups: d chunk i / 2, K or V; two operands of 16 keys for four products
-                bf16x8 f[kN1][2];
-                auto issue1 = [&](int i, int x) { f[i][x] = lds_read_b128((i & 1 ? vt : kt) + (rb.k ^ ((i >> 1) << 6)) + x * 16 * G::kRow); };
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int i = 0; i < kAhead; i++) issue1(i, 0), issue1(i, 1);
-#pragma unroll
-                for (int i = 0; i < kN1; i++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int x = j >> 1, g = j & 1, dk = i >> 1;
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (i & 1) dp[x][g] = mfma16(f[i][x], gf[dk][g], dk == 0 ? d_init[g] : dp[x][g]);
-                        else s[x][g] = mfma16(f[i][x], qf[dk][g], dk == 0 ? s_init[g] : s[x][g]);
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (j < 2 && i + kAhead < kN1) issue1(i + kAhead, j);
-                    }
-                }
-                __builtin_amdgcn_s_setprio(0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (cut) {
-                    const unsigned m[3] = {(unsigned)mine.a, (unsigned)mine.lo, (unsigned)mine.hi};
-                    int both[3][2];   // the even rows of 16 lanes hold block 0's, the odd ones block 1's
-#pragma unroll
-                    for (int x = 0; x < 3; x++) {
-                        const auto r = __builtin_amdgcn_permlane16_swap(m[x], m[x], false, false);
-                        both[x][0] = (int)r[0];
-                        both[x][1] = (int)r[1];
-                    }
-                    auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int g = 0; g < 2; g++) {
-                            const int at = w.key(e) + 32 * t + 16 * x + 4 * q4;
-                            const unsigned bits = below(both[0][g] - at) | (below(both[2][g] - at) & ~below(both[1][g] - at));
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                s[x][g][i] = (bits >> i) & 1 ? s[x][g][i] : neg_inf();
-                                dp[x][g][i] = (bits >> i) & 1 ? dp[x][g][i] : 0.f;
-                            }
-                        }
-                }
-                bf16x8 ds[2];
-#pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    f32x8 a;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) a[i] = fast_exp2(s[i >> 2][g][i & 3] * sl2) * dp[i >> 2][g][i & 3];
-                    ds[g] = __builtin_convertvector(a, bf16x8);
-                }
-                asm volatile("" ::"v"(ds[0]), "v"(ds[1]));
-                __builtin_amdgcn_sched_barrier(0);
-                constexpr int kAhead2 = kNK < 3 ? kNK : 3;   // groups: d blocks 2 i + {0, 1}
-                bf16x8 h[kNK][2];
-                auto issue2 = [&](int i, int x) { h[i][x] = read_v_frag<D>(kt + (rb.v ^ ((2 * i + x) << 5))); };
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int i = 0; i < kAhead2; i++) issue2(i, 0), issue2(i, 1);
-#pragma unroll
-                for (int i = 0; i < kNK; i++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int x = j >> 1, g = j & 1;
-                        __builtin_amdgcn_sched_barrier(0);
-                        dq[2 * i + x][g] = mfma16(h[i][x], ds[g], dq[2 * i + x][g]);
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (j < 2 && i + kAhead2 < kNK) issue2(i + kAhead2, j);
-                    }
-                }
-                __builtin_amdgcn_s_setprio(0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            const lds_u8* kt = smem + buf * kTile;
+            row_step<D>(kt, kt + 2 * kTile, rb, qf, gf, s_init, d_init, dq, sl2, !whole.tile(e), mine, w.key(e));
         }
         __builtin_amdgcn_sched_barrier(0);
         wait_vmcnt<0>();
@@ -546,10 +591,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
     }
 }
 
-// The shares of split walks, added in their order: D / 4 threads a row (of dq) or key (twice as many: dk, dv).
+// The shares of split walks, added in their order: D / 4 threads a row of dq or (KEYS) twice as many a key, dk and dv.
 template <int D, bool KEYS>
 __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams p) {
-    constexpr int kWide = KEYS ? 2 * D : D, kPer = kWide / 4, kSum = 256 / kPer, kPerPiece = kRows / kSum;
+    constexpr int kPiece = KEYS ? kKeys : kRows, kWide = KEYS ? 2 * D : D, kPer = kWide / 4, kSum = 256 / kPer, kPerPiece = kPiece / kSum;
     const int c = threadIdx.x % kPer, in = (int)(blockIdx.x % kPerPiece) * kSum + threadIdx.x / kPer, item = blockIdx.x / kPerPiece;
     const PackedItems& items = KEYS ? p.key_items : p.row_items;
     const int kvh = paged_quot(item, items.n), number = item - kvh * items.n.by, group = p.group.by;
@@ -558,11 +603,11 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams 
     size_t dst;
     if constexpr (KEYS) {
         const PackedKeys kb = {p.b.k_start, p.b.seqs, p.b.k_tokens};
-        const PagedPiece piece = paged_piece<kRows>(p.key_pieces, kb, 1, number);
+        const PagedPiece piece = paged_piece<kPiece>(p.key_pieces, kb, 1, number);
         const PackedSeq sq = packed_seq(p.b, piece.seq);
-        const int key0 = piece.tile * kRows;
+        const int key0 = piece.tile * kPiece;
         if (key0 + in >= sq.len) return;
-        const RowWalk walk = row_walk(p.mask, sq, key0, min(key0 + kRows, sq.len) - 1, group);
+        const RowWalk walk = row_walk(p.mask, sq, key0, min(key0 + kPiece, sq.len) - 1, group);
         steps = walk.to - walk.from, chunk = p.key_chunk;
         out = 4 * c < D ? p.dk : p.dv;
         dst = ((size_t)(sq.k0 + key0 + in) * p.kv_heads + kvh) * D + 4 * c % D;
@@ -578,7 +623,7 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams 
     }
     if (steps <= chunk) return;   // (one workgroup's, written)
     const int shares = (steps + chunk - 1) / chunk;
-    const float* part = (KEYS ? p.part_dkv : p.part_dq) + ((size_t)item * kRows + in) * kWide + 4 * c;
+    const float* part = (KEYS ? p.part_dkv : p.part_dq) + ((size_t)item * kPiece + in) * kWide + 4 * c;
     const size_t next = (size_t)(KEYS ? p.part_keys : p.part_rows) * kWide;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < shares; s++) {
@@ -599,26 +644,27 @@ constexpr size_t kMostShares = (size_t)1 << 30;   // bytes of the shares of a ke
 BackCut back_cut(const PackedCall& c) {
     const size_t group = c.heads / c.kv_heads, units = (size_t)fv_compute_units(), slots = (c.d == 64 ? 3 : 2) * units;
     BackCut cut;
+    const size_t keys = kKeys, step = kStep;
     cut.rows = paged_pieces(kRows, c.seqs, c.tokens, c.max_q, group);
-    cut.keys = paged_pieces(kRows, c.seqs, c.k_tokens, c.max_k, 1);
-    auto shares_of = [&](const PagedPieces& x, size_t rows, size_t steps, size_t least, size_t bytes) {
+    cut.keys = paged_pieces(keys, c.seqs, c.k_tokens, c.max_k, 1);
+    auto shares_of = [&](const PagedPieces& x, size_t rows, size_t piece, size_t places, size_t steps, size_t least, size_t bytes) {
         const size_t items = c.kv_heads * (size_t)x.n.by;
         if (items == 0) return (size_t)1;
-        const size_t held = x.tiles.by ? items : std::max<size_t>(c.kv_heads * (rows / kRows + 1), items / 2);
-        const size_t shares = held < slots ? std::min(slots / held, std::max<size_t>(steps / least, 1)) : 1;
-        return std::min(shares, std::max<size_t>(kMostShares / (items * kRows * bytes), 1));
+        const size_t held = x.tiles.by ? items : std::max<size_t>(c.kv_heads * (rows / piece + 1), items / 2);
+        const size_t shares = held < places ? std::min(places / held, std::max<size_t>(steps / least, 1)) : 1;
+        return std::min(shares, std::max<size_t>(kMostShares / (items * piece * bytes), 1));
     };
     const size_t key_steps = fv_packed_key_steps(c, kRows), rows = c.max_q * group;
-    size_t row_steps = (rows + kStepRows - 1) / kStepRows;
+    size_t row_steps = (rows + step - 1) / step;
     if (c.causal && c.window > 0 && c.sink == 0) {   // rows of the window's blocks and of those of the piece's keys
-        const size_t blocks = c.window + (kRows + c.block_tokens - 1) / c.block_tokens, far = (size_t)1 << 31;
+        const size_t blocks = c.window + (keys + c.block_tokens - 1) / c.block_tokens, far = (size_t)1 << 31;
         const size_t band = blocks < far / c.block_tokens / group ? blocks * c.block_tokens * group : far;
-        row_steps = std::min(row_steps, (band + kStepRows - 1) / kStepRows + 1);
+        row_steps = std::min(row_steps, (band + step - 1) / step + 1);
     }
     row_steps = std::max<size_t>(row_steps, 1);
-    size_t n = shares_of(cut.rows, c.tokens * group, key_steps, 4, c.d * 4);
+    size_t n = shares_of(cut.rows, c.tokens * group, kRows, slots, key_steps, 4, c.d * 4);
     cut.row_chunk = (key_steps + n - 1) / n, cut.row_shares = (key_steps + cut.row_chunk - 1) / cut.row_chunk;
-    n = shares_of(cut.keys, c.k_tokens, row_steps, 8, c.d * 8);
+    n = shares_of(cut.keys, c.k_tokens, keys, slots, row_steps, 8, c.d * 8);
     cut.key_chunk = (row_steps + n - 1) / n, cut.key_shares = (row_steps + cut.key_chunk - 1) / cut.key_chunk;
     return cut;
 }
@@ -631,15 +677,14 @@ struct BackParts {
             bytes += (n + 255) / 256 * 256;
             return at;
         };
-        rows = c.kv_heads * (size_t)cut.rows.n.by * kRows, keys = c.kv_heads * (size_t)cut.keys.n.by * kRows;
+        rows = c.kv_heads * (size_t)cut.rows.n.by * kRows, keys = c.kv_heads * (size_t)cut.keys.n.by * kKeys;
         stats = take(c.tokens * c.heads * 8);
         if (round) rounded = take(c.tokens * c.heads * c.d * 2);
         if (cut.row_shares > 1) dq = take(cut.row_shares * rows * c.d * 4);
         if (cut.key_shares > 1) dkv = take(cut.key_shares * keys * c.d * 8);
     }
 };
-constexpr int dkv_lds(int d) { return kRows * d * 2 + 4 * kStepRows * d * 2 + 2 * 256; }
-std::atomic<unsigned long long> lds_done{0};
+std::atomic<unsigned long long> lds_done{0};   // (of the one kernel that takes more than 64 KB)
 
 }  // namespace
 }  // namespace fv
@@ -677,7 +722,7 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     if (parts.bytes > 0 && (!workspace || workspace_bytes < parts.bytes)) return fv_invalid("packed attention backward: workspace too small");
     const size_t row_items = kv_heads * (size_t)cut.rows.n.by, key_items = kv_heads * (size_t)cut.keys.n.by;
     const size_t rows = q_tokens * heads, stat_blocks = (rows + 2048 / d - 1) / (2048 / d);
-    const size_t sum_rows = row_items * fv::kRows / (1024 / d), sum_keys = key_items * fv::kRows / (512 / d);
+    const size_t sum_rows = row_items * fv::kRows / (1024 / d), sum_keys = key_items * fv::kKeys / (512 / d);
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     if (row_items * cut.row_shares >= kMost / 2 || key_items * cut.key_shares >= kMost / 2 || stat_blocks >= kMost ||
         (cut.row_shares > 1 && sum_rows >= kMost) || (cut.key_shares > 1 && sum_keys >= kMost))
@@ -688,7 +733,7 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     p.mask = fv_packed_mask(c);
     p.q = q, p.k = k, p.v = v, p.dout = dout_is_bf16 ? (const uint16_t*)dout : (const uint16_t*)(ws + parts.rounded);
     p.q_stride = (long)q_stride * 2, p.k_stride = (long)k_stride * 2, p.v_stride = (long)v_stride * 2, p.dout_stride = (long)(heads * d * 2);
-    p.stats = (const fv::f32x2*)(ws + parts.stats);
+    p.stats = (const float*)(ws + parts.stats), p.stat_rows = (long)(q_tokens * heads);
     p.dq = dq, p.dk = dk, p.dv = dv, p.grads_are_bf16 = grads_are_bf16 != 0;
     p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = fv::paged_div(heads / kv_heads);
     p.scale = scale, p.sl2 = (float)((double)scale * 1.4426950408889634);
@@ -701,18 +746,18 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     hipError_t e = hipSuccess;
     fv::paged_pick(d == 128, [&](auto d128) {
         constexpr int D = d128() ? 128 : 64;
-        if (D == 128) e = fv_set_max_lds_once((const void*)fv::packed_dkv_kernel<D>, fv::dkv_lds(D), fv::lds_done);
-        if (e != hipSuccess) return;
         if (q_tokens > 0)
             fv::paged_pick(out_is_bf16 != 0, [&](auto o16) {
                 fv::paged_pick(dout_is_bf16 != 0, [&](auto g16) {
                     hipLaunchKernelGGL((fv::packed_stats_kernel<D, o16(), g16()>), dim3((unsigned)stat_blocks), dim3(256), 0, st, dout, out, lse,
-                                       (fv::f32x2*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (long)q_tokens, (int)heads, p.group,
+                                       (float*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (long)q_tokens, (int)heads, p.group,
                                        (float)(1.0 / (double)scale));
                 });
             });
         if (key_items > 0) {
-            hipLaunchKernelGGL((fv::packed_dkv_kernel<D>), dim3((unsigned)fv::packed_blocks(p.key_items)), dim3(256), fv::dkv_lds(D), st, p);
+            if (fv::KeyForm<D>::kLds > 65536) e = fv_set_max_lds_once((const void*)fv::packed_dkv_kernel<D>, fv::KeyForm<D>::kLds, fv::lds_done);
+            if (e != hipSuccess) return;
+            hipLaunchKernelGGL((fv::packed_dkv_kernel<D>), dim3((unsigned)fv::packed_blocks(p.key_items)), dim3(256), fv::KeyForm<D>::kLds, st, p);
             if (cut.key_shares > 1) hipLaunchKernelGGL((fv::packed_sum_kernel<D, true>), dim3((unsigned)sum_keys), dim3(256), 0, st, p);
         }
         if (row_items > 0) {
