@@ -92,30 +92,26 @@ FV_DEV PackedWhole packed_whole(const PackedWalk& w, const PagedSight& all) {
     return {w.before(all.a / kTileRows), all.a >= all.lo ? 0 : w.before((all.lo + kTileRows - 1) / kTileRows), w.before(all.hi / kTileRows)};
 }
 
-// Items (pieces of rows or keys of a key head, in shares) to workgroups: key head by key head, 2^xcds XCDs to a run of items, so that an
-// L2 holds few heads' tensors; the XCDs of a run take its items in turn, so that each has as many of the long walks as the others.
-struct PackedItems {
-    PagedDiv n, shares_n;   // pieces of a key head, pieces times shares
-    int total, xcds;
+// Workgroups to pieces: 2^xcds XCDs take the pieces of a run of whole key heads, the heads' pieces in turn, so that an L2 holds few heads' tensors and
+// the longest walks of all heads come first; the XCDs of a run take them in turn.
+struct PackedRuns {
+    PagedDiv heads;   // of a run
+    int xcds;
 };
-struct PackedItem {
-    int head, piece, share;   // head < 0: none
+struct PackedSlot {
+    int head, number;   // of the key head's pieces; past the last: none
 };
-template <class Items>
-FV_DEV PackedItem packed_item(const Items& x, int block) {
-    const int run = ((x.total << x.xcds) + 7) >> 3, in_run = ((block >> 3) << x.xcds) + (block & ((1 << x.xcds) - 1));
-    const int item = ((block & 7) >> x.xcds) * run + in_run;
-    if (in_run >= run || item >= x.total) return {-1, 0, 0};
-    const int head = paged_quot(item, x.shares_n), rest = item - head * x.shares_n.by, share = paged_quot(rest, x.n);
-    return {head, rest - share * x.n.by, share};
+template <class Runs>
+FV_DEV PackedSlot packed_slot(const Runs& x, int block) {
+    const int in_run = ((block >> 3) << x.xcds) + (block & ((1 << x.xcds) - 1)), number = paged_quot(in_run, x.heads);
+    return {((block & 7) >> x.xcds) * x.heads.by + in_run - number * x.heads.by, number};
 }
-inline PackedItems packed_items(size_t kv_heads, size_t pieces, size_t shares) {
-    return {paged_div(pieces), paged_div(pieces * shares), (int)(kv_heads * pieces * shares),
-            kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3};   // (a run has whole key heads)
+inline PackedRuns packed_runs(size_t kv_heads) {
+    const int xcds = kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3;
+    return {paged_div(kv_heads >> (3 - xcds)), xcds};
 }
-inline size_t packed_blocks(const PackedItems& x) {
-    const size_t run = (((size_t)x.total << x.xcds) + 7) / 8;
-    return ((run + ((size_t)1 << x.xcds) - 1) >> x.xcds) * 8;
+inline size_t packed_blocks(const PackedRuns& x, size_t numbers) {
+    return (((size_t)x.heads.by * numbers + ((size_t)1 << x.xcds) - 1) >> x.xcds) * 8;
 }
 
 // Per-lane source offsets of a wave's part of a 64-row tile whose rows lie `stride` bytes apart (ITER loads a wave of four, in the LDS

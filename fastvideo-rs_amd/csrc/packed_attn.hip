@@ -31,8 +31,8 @@ struct PackedAttnParams {
     PagedDiv group;                      // query heads that share a key head
     float sl2;                           // scale * log2(e)
     PagedPieces pieces;
-    PackedItems items;
-    int chunk;                           // tiles of a walk that a workgroup takes
+    PackedRuns runs;
+    int shares, chunk;                   // workgroups a walk, tiles of it that each takes
     // shares of walks longer than that: values, each normalised, and the base-2 logarithm of its sum: [shares][128 rows of every piece]
     float *part_o, *part_lse;
     long part_rows;
@@ -52,16 +52,17 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int q4 = lane >> 4, i16 = lane & 15;
-    const PackedItem item = packed_item(p.items, block);
-    if (item.head < 0) return true;
-    const int kvh = item.head, number = p.items.n.by - 1 - item.piece;   // (a sequence's last rows, which see most, first)
+    const PackedSlot slot_at = packed_slot(p.runs, block);
+    const int kvh = slot_at.head, share = paged_quot(slot_at.number, p.pieces.n);
+    if (share >= p.shares) return true;
+    const int number = (share + 1) * p.pieces.n.by - 1 - slot_at.number;   // (a sequence's last rows, which see most, first)
     const PagedPiece piece = paged_piece<kRows>(p.pieces, p.b, p.group.by, number);
     const PackedSeq sq = packed_seq(p.b, piece.seq);
     const int rows = sq.count * p.group.by, row0 = piece.tile * kRows;
     if (row0 >= rows) return true;
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
-    const int e0 = item.share * p.chunk, e1 = min(w.n, e0 + p.chunk);
-    if (item.share > 0 && e0 >= e1) return true;
+    const int e0 = share * p.chunk, e1 = min(w.n, e0 + p.chunk);
+    if (share > 0 && e0 >= e1) return true;
     const bool split = w.n > p.chunk;
     const float sl2 = p.sl2;
 
@@ -277,7 +278,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
         const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
         if (r >= rows) continue;
         const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
-        const size_t part = (size_t)item.share * p.part_rows + (size_t)(kvh * p.items.n.by + number) * kRows + (r - row0);
+        const size_t part = (size_t)share * p.part_rows + (size_t)(kvh * p.pieces.n.by + number) * kRows + (r - row0);
         const float lse2 = l == 0.f ? neg_inf() : st.log2_offset<true>(g, sl2) + __log2f(l);
         if (q4 == 0) {
             if (split) p.part_lse[part] = lse2;
@@ -317,7 +318,7 @@ template <int D>
 __global__ __launch_bounds__(256) void packed_join_kernel(const PackedAttnParams p) {
     constexpr int kPer = D / 4, kJoin = 256 / kPer, kPerPiece = kRows / kJoin;
     const int c = threadIdx.x % kPer, slot = threadIdx.x / kPer;
-    const int item = blockIdx.x / kPerPiece, kvh = paged_quot(item, p.items.n), number = item - kvh * p.items.n.by;
+    const int item = blockIdx.x / kPerPiece, kvh = paged_quot(item, p.pieces.n), number = item - kvh * p.pieces.n.by;
     const PagedPiece piece = paged_piece<kRows>(p.pieces, p.b, p.group.by, number);
     const PackedSeq sq = packed_seq(p.b, piece.seq);
     const int rows = sq.count * p.group.by, row0 = piece.tile * kRows;
@@ -475,13 +476,13 @@ int fv_packed_attention(const uint16_t* q, size_t q_stride, const uint16_t* k, s
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     const size_t join_blocks = items * fv::kRows / (1024 / d);
     if (items * cut.shares >= kMost / 2 || (cut.shares > 1 && join_blocks >= kMost)) return fv_decline("packed attention: too large for one launch");
-    p.items = fv::packed_items(kv_heads, (size_t)cut.pieces.n.by, cut.shares);
+    p.runs = fv::packed_runs(kv_heads), p.shares = (int)cut.shares;
     p.part_rows = (long)cut.rows(kv_heads);
     p.part_o = (float*)workspace, p.part_lse = p.part_o + cut.shares * cut.rows(kv_heads) * d;
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(d == 128, [&](auto d128) {
         constexpr int D = d128() ? 128 : 64;
-        hipLaunchKernelGGL((fv::packed_attn_kernel<D>), dim3((unsigned)fv::packed_blocks(p.items)), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
+        hipLaunchKernelGGL((fv::packed_attn_kernel<D>), dim3((unsigned)fv::packed_blocks(p.runs, (size_t)cut.pieces.n.by * cut.shares)), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
         if (cut.shares > 1) hipLaunchKernelGGL((fv::packed_join_kernel<D>), dim3((unsigned)join_blocks), dim3(256), 0, st, p);
     });
     const hipError_t e = hipGetLastError();

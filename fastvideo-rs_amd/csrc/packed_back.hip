@@ -20,6 +20,21 @@ namespace {
 
 constexpr int kRows = 128;   // of a workgroup of packed_dq_kernel, 32 a wave
 
+// Which workgroup takes what, made on the device from the sequences' lengths (plan_pieces): the units of a key head, the longest first, each a
+// piece of 128 rows or keys and a part [from, to) of the steps of its walk: tiles of 64 keys; of 32 rows. A walk longer than a slot's mean load is cut into
+// shares, which leave f32 sums in places of 128 rows ([kv_heads][most_places][128][d or 2 d]) and are added by packed_sum_kernel.
+struct BackUnit {
+    int seq, tile, from, to, place, shares, unused[2];   // place < 0: a whole walk; of a share: its place
+};
+struct BackPlan {
+    PagedPieces pieces;
+    int* counts;         // units, cut pieces, places
+    BackUnit *units, *cuts;   // (of a cut piece: its first place)
+    int2* scratch;       // every piece number's sequence and steps
+    int most_units, most_cuts, most_places, least;   // of a key head; steps below which no walk is cut
+    float* places;
+};
+
 struct PackedBackParams {
     PackedBatch b;
     PackedMask mask;
@@ -32,12 +47,8 @@ struct PackedBackParams {
     int heads, kv_heads;
     PagedDiv group;
     float scale, sl2;                                 // sl2 = scale * log2(e)
-    PagedPieces row_pieces, key_pieces;
-    PackedItems row_items, key_items;
-    int row_chunk, key_chunk;                         // steps of a walk that a workgroup takes: tiles of 64 keys; of 32 rows
-    // shares of walks longer than that, f32: [shares][128 rows of every piece][d]; [shares][128 keys of every piece][2][d]
-    float *part_dq, *part_dkv;
-    long part_rows, part_keys;
+    PackedRuns runs;
+    BackPlan rows, keys;                              // of packed_dq_kernel, of packed_dkv_kernel
 };
 
 // Chunk c of row r of a tile lies at chunk c ^ both_swz(r), so that a tile serves both kinds of operands without bank conflicts: the 8 rows of a
@@ -55,13 +66,141 @@ FV_DEV TileReadBases both_bases(int lane) {
     return {i16 * G::kRow + ((both_swz<D>(i16) ^ q4) << 4), r * G::kRow + ((both_swz<D>(r) ^ ((i16 & 3) >> 1)) << 4) + 8 * (i16 & 1)};
 }
 
+// The rows of a sequence, counted (token, head of the group), that see a key: [lo, hi), hi INT_MAX where that is to the last.
+struct KeySight {
+    int lo, hi;
+};
+template <class Mask>
+FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group) {
+    if (!m.causal) return {0, 0x7fffffff};
+    const int bt = m.block_tokens.by, block = paged_quot(key, m.block_tokens);
+    const long lo = (long)block * bt - s.pos0, hi = m.window > 0 && block >= m.sink ? (long)block * bt + (long)m.window * bt - s.pos0 : s.count;
+    KeySight k;
+    k.lo = (int)min(max(lo, 0L), (long)s.count) * group;
+    k.hi = hi >= s.count ? 0x7fffffff : (int)max(hi, 0L) * group;
+    return k;
+}
+// packed_dkv_kernel: a workgroup's keys, the rows of a step, and its LDS: V's operands | 2 x (q, dout) | 2 x (-lse / scale, -D).
+constexpr int kKeys = 128, kStep = 32;
+template <int D>
+struct KeyForm {
+    static constexpr int kHalf = kStep * 2 * D;   // bytes of a step's q, or dout
+    static constexpr int kFrags = D / 16, kSteps = 4 * kFrags * 1024, kStats = kSteps + 4 * kHalf, kLds = kStats + 2 * 256;
+};
+// The steps [from, to) that some key of [first, last] is seen by.
+struct RowWalk {
+    int from, to;
+};
+template <class Mask>
+FV_DEV RowWalk row_walk(const Mask& m, const PackedSeq& s, int first, int last, int group) {
+    const int rows = s.count * group;
+    const KeySight a = key_sight(m, s, first, group), b = key_sight(m, s, last, group);
+    return {a.lo / kStep, (min(rows, max(a.hi, b.hi)) + kStep - 1) / kStep};
+}
+
+// The steps of a piece's walk.
+template <bool KEYS>
+FV_DEV int back_steps(const PackedBackParams& p, const PackedSeq& sq, int tile) {
+    if constexpr (KEYS) {
+        const int key0 = tile * kKeys;
+        if (key0 >= sq.len) return -1;
+        const RowWalk w = row_walk(p.mask, sq, key0, min(key0 + kKeys, sq.len) - 1, p.group.by);
+        return max(w.to - w.from, 0);
+    } else {
+        const int rows = sq.count * p.group.by, row0 = tile * kRows;
+        if (row0 >= rows) return -1;
+        return packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group)).n;
+    }
+}
+// One workgroup makes a plan: the walks' lengths; their sum, and from it the mean load of a slot, past which a walk is cut into equal shares; the units
+// sorted by their lengths into 64 classes, longest first (in a class in any order: it changes no result). By itself the order of the pieces left slots idle
+// for a third of the time (one clip of 7 frames, 12 heads, 1032 pieces on 512 slots) or for two thirds (a window with a sink, whose keys all rows see).
+template <bool KEYS>
+FV_DEV void plan_pieces(const PackedBackParams& p, const BackPlan& plan, int slots) {
+    constexpr int kClasses = 64;
+    __shared__ unsigned long long sum;
+    __shared__ int longest, units[kClasses], cuts, places;
+    const int tid = threadIdx.x, numbers = plan.pieces.n.by;
+    if (tid == 0) sum = 0, longest = 0, cuts = 0, places = 0;
+    if (tid < kClasses) units[tid] = 0;
+    __syncthreads();
+    const PackedKeys kb = {p.b.k_start, p.b.seqs, p.b.k_tokens};
+    const int group = KEYS ? 1 : p.group.by;
+    constexpr int R = KEYS ? kKeys : kRows;
+    auto first_of = [&](int seq) { return KEYS ? paged_first_piece<R>(plan.pieces, kb, group, seq) : paged_first_piece<R>(plan.pieces, p.b, group, seq); };
+    unsigned long long mine = 0;
+    int most = 0;
+    for (int n = tid; n < numbers; n += 256) {
+        int seq = 0;
+        if (plan.pieces.tiles.by) {
+            seq = paged_quot(n, plan.pieces.tiles);
+        } else {
+            int behind = p.b.seqs;   // the last of sequences seq .. behind - 1 whose first piece is no later
+            while (behind - seq > 1) {
+                const int mid = seq + (behind - seq) / 2;
+                if (first_of(mid) <= n) seq = mid;
+                else behind = mid;
+            }
+        }
+        const long tile = n - first_of(seq);
+        const int steps = tile < 0 || tile > 0x7fffffff / R ? -1 : back_steps<KEYS>(p, packed_seq(p.b, seq), (int)tile);
+        plan.scratch[n] = int2{seq, steps};
+        mine += (unsigned long long)max(steps, 0), most = max(most, steps);
+    }
+    atomicAdd(&sum, mine);
+    atomicMax(&longest, most);
+    __syncthreads();
+    const int load = max(plan.least, (int)min((sum * p.kv_heads + slots - 1) / slots, 0x7fffffffull));
+    auto shares_of = [&](int steps) { return steps > load ? (steps + load - 1) / load : 1; };
+    const int top = min(longest, load) + 1;
+    auto class_of = [&](int steps, int shares) { return kClasses - 1 - (int)((long)((steps + shares - 1) / shares) * kClasses / top); };   // 0: the longest
+    for (int n = tid; n < numbers; n += 256) {
+        const int steps = plan.scratch[n].y;
+        if (steps < 0) continue;
+        const int k = shares_of(steps);
+        atomicAdd(&units[class_of(steps, k)], k);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int at = 0;
+        for (int c = 0; c < kClasses; c++) {
+            const int n = units[c];
+            units[c] = at;
+            at += n;
+        }
+        plan.counts[0] = min(at, plan.most_units);
+    }
+    __syncthreads();
+    for (int n = tid; n < numbers; n += 256) {
+        const int2 x = plan.scratch[n];
+        if (x.y < 0) continue;
+        const int k = shares_of(x.y), chunk = (x.y + k - 1) / k, tile = (int)(n - first_of(x.x));
+        int u = atomicAdd(&units[class_of(x.y, k)], k), place = -1;
+        if (k > 1) {
+            const int c = atomicAdd(&cuts, 1);
+            place = atomicAdd(&places, k);
+            if (c < plan.most_cuts) plan.cuts[c] = BackUnit{x.x, tile, 0, x.y, place, k, {0, 0}};
+        }
+        for (int s = 0; s < k; s++, u++)
+            if (u < plan.most_units) plan.units[u] = BackUnit{x.x, tile, s * chunk, min(x.y, (s + 1) * chunk), place < 0 ? -1 : place + s, k, {0, 0}};
+    }
+    __syncthreads();
+    if (tid == 0) plan.counts[1] = min(cuts, plan.most_cuts);
+}
+
 // D / 8 threads a row (token, head); OUT16, DOUT16: bf16 bits. An f32 gradient is kept as bf16 bits in `rounded` [tokens, heads, d].
 template <int D, bool OUT16, bool DOUT16>
-__global__ __launch_bounds__(256) void packed_stats_kernel(const void* dout, const void* out, const float* lse, float* stats, uint16_t* rounded, long rows,
-                                                           long tokens, int heads, PagedDiv group, float inv_scale) {
+__global__ __launch_bounds__(256) void packed_stats_kernel(const PackedBackParams p, const void* dout, const void* out, const float* lse, float* stats, uint16_t* rounded,
+                                                           long rows, float inv_scale, int slots) {
+    if (blockIdx.x < 2) {   // (the first two: the plans)
+        if (blockIdx.x == 0) plan_pieces<true>(p, p.keys, slots);
+        else plan_pieces<false>(p, p.rows, slots);
+        return;
+    }
     constexpr int kPer = D / 8;
-    const int c = threadIdx.x % kPer;
-    const long row = (long)blockIdx.x * (256 / kPer) + threadIdx.x / kPer;
+    const int c = threadIdx.x % kPer, heads = p.heads;
+    const long row = (long)(blockIdx.x - 2) * (256 / kPer) + threadIdx.x / kPer, tokens = p.b.tokens;
+    const PagedDiv group = p.group;
     if (row >= rows) return;
     auto eight = [&](const void* at, auto is16, float (&x)[8]) {
         if constexpr (is16()) {
@@ -105,38 +244,6 @@ __global__ __launch_bounds__(256) void packed_stats_kernel(const void* dout, con
 }
 
 // ---- the keys' gradients ---------------------------------------------------------------------------------------------
-
-// The rows of a sequence, counted (token, head of the group), that see a key: [lo, hi), hi INT_MAX where that is to the last.
-struct KeySight {
-    int lo, hi;
-};
-template <class Mask>
-FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group) {
-    if (!m.causal) return {0, 0x7fffffff};
-    const int bt = m.block_tokens.by, block = paged_quot(key, m.block_tokens);
-    const long lo = (long)block * bt - s.pos0, hi = m.window > 0 && block >= m.sink ? (long)block * bt + (long)m.window * bt - s.pos0 : s.count;
-    KeySight k;
-    k.lo = (int)min(max(lo, 0L), (long)s.count) * group;
-    k.hi = hi >= s.count ? 0x7fffffff : (int)max(hi, 0L) * group;
-    return k;
-}
-// packed_dkv_kernel: a workgroup's keys, the rows of a step, and its LDS: V's operands | 2 x (q, dout) | 2 x (-lse / scale, -D).
-constexpr int kKeys = 128, kStep = 32;
-template <int D>
-struct KeyForm {
-    static constexpr int kHalf = kStep * 2 * D;   // bytes of a step's q, or dout
-    static constexpr int kFrags = D / 16, kSteps = 4 * kFrags * 1024, kStats = kSteps + 4 * kHalf, kLds = kStats + 2 * 256;
-};
-// The steps [from, to) that some key of [first, last] is seen by.
-struct RowWalk {
-    int from, to;
-};
-template <class Mask>
-FV_DEV RowWalk row_walk(const Mask& m, const PackedSeq& s, int first, int last, int group) {
-    const int rows = s.count * group;
-    const KeySight a = key_sight(m, s, first, group), b = key_sight(m, s, last, group);
-    return {a.lo / kStep, (min(rows, max(a.hi, b.hi)) + kStep - 1) / kStep};
-}
 
 // A wave's part in a step of 32 rows at `qt` and `gt` (q and dout), `cut`: with keys that rows do not see, whose scores become -inf. The products, two to a unit that shares an operand read: S = Q K^T - lse / scale, 16 rows after 16; dP = dO V^T - D; dV^T += dO^T P; dK^T += Q^T dS. The vector work lies
 // in their shadow: a 16x16x32 product holds the matrix pipe for four instructions' time, of which two others of the same wave cost
@@ -235,19 +342,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
-    const PackedItem item = packed_item(p.key_items, blockIdx.x);
-    if (item.head < 0) return;
-    const int kvh = item.head, group = p.group.by;
-    const PackedKeys kb = {p.b.k_start, p.b.seqs, p.b.k_tokens};
-    const PagedPiece piece = paged_piece<kKeys>(p.key_pieces, kb, 1, item.piece);   // (a sequence's first keys, which most rows see, first)
-    const PackedSeq sq = packed_seq(p.b, piece.seq);
-    const int key0 = piece.tile * kKeys;
-    if (key0 >= sq.len) return;
+    const PackedSlot at = packed_slot(p.runs, blockIdx.x);
+    if (at.number >= p.keys.counts[0]) return;
+    const BackUnit unit = p.keys.units[at.number];
+    const int kvh = at.head, group = p.group.by;
+    const PackedSeq sq = packed_seq(p.b, unit.seq);
+    const int key0 = unit.tile * kKeys;
+    if (key0 >= sq.len) return;   // (as the plan has it; lengths changed since make no address)
     const int rows = sq.count * group, last = min(key0 + kKeys, sq.len) - 1;
     const RowWalk walk = row_walk(p.mask, sq, key0, last, group);
-    const int e0 = walk.from + item.share * p.key_chunk, e1 = min(walk.to, e0 + p.key_chunk);
-    if (item.share > 0 && e0 >= e1) return;
-    const bool split = walk.to - walk.from > p.key_chunk;
+    const int e0 = walk.from + unit.from, e1 = min(walk.to, walk.from + unit.to);
 
     // the wave's keys: rows that see some of them, rows that see all; the lane's two
     const int wkey = key0 + 32 * wave;
@@ -369,14 +473,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
         const int key = wkey + 16 * g + i16;
         if (key >= sq.len) continue;
         const size_t dst = ((size_t)(sq.k0 + key) * p.kv_heads + kvh) * D;
-        float* part = p.part_dkv + ((size_t)item.share * p.part_keys + (size_t)(kvh * p.key_items.n.by + item.piece) * kKeys + (key - key0)) * 2 * D;
+        float* part = p.keys.places + (((size_t)kvh * p.keys.most_places + max(unit.place, 0)) * kKeys + (key - key0)) * 2 * D;
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
             const int at = 16 * db + 4 * q4;
             f32x4 x = dk[db][g];
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] *= p.scale;
-            if (split) {
+            if (unit.place >= 0) {
                 *reinterpret_cast<f32x4*>(part + at) = x;
                 *reinterpret_cast<f32x4*>(part + D + at) = dv[db][g];
             } else if (p.grads_are_bf16) {
@@ -490,17 +594,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
-    const PackedItem item = packed_item(p.row_items, blockIdx.x);
-    if (item.head < 0) return;
-    const int kvh = item.head, group = p.group.by, number = p.row_items.n.by - 1 - item.piece;
-    const PagedPiece piece = paged_piece<kRows>(p.row_pieces, p.b, group, number);
-    const PackedSeq sq = packed_seq(p.b, piece.seq);
-    const int rows = sq.count * group, row0 = piece.tile * kRows;
-    if (row0 >= rows) return;
+    const PackedSlot at = packed_slot(p.runs, blockIdx.x);
+    if (at.number >= p.rows.counts[0]) return;
+    const BackUnit unit = p.rows.units[at.number];
+    const int kvh = at.head, group = p.group.by;
+    const PackedSeq sq = packed_seq(p.b, unit.seq);
+    const int rows = sq.count * group, row0 = unit.tile * kRows;
+    if (row0 >= rows) return;   // (as above)
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
-    const int e0 = item.share * p.row_chunk, e1 = min(w.n, e0 + p.row_chunk);
-    if (item.share > 0 && e0 >= e1) return;
-    const bool split = w.n > p.row_chunk;
+    const int e0 = unit.from, e1 = min(w.n, unit.to);
     const float sl2 = p.sl2;
 
     const int wrow = row0 + 32 * wave;
@@ -577,57 +679,49 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
         const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
         if (r >= rows) continue;
         const size_t dst = ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D;
-        float* part = p.part_dq + ((size_t)item.share * p.part_rows + (size_t)(kvh * p.row_items.n.by + number) * kRows + (r - row0)) * D;
+        float* part = p.rows.places + (((size_t)kvh * p.rows.most_places + max(unit.place, 0)) * kRows + (r - row0)) * D;
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
             const int at = 16 * db + 4 * q4;
             f32x4 x = dq[db][g];
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] *= p.scale;
-            if (split) *reinterpret_cast<f32x4*>(part + at) = x;
+            if (unit.place >= 0) *reinterpret_cast<f32x4*>(part + at) = x;
             else if (p.grads_are_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.dq + dst + at) = __builtin_convertvector(x, bf16x4);
             else *reinterpret_cast<f32x4*>((float*)p.dq + dst + at) = x;
         }
     }
 }
 
-// The shares of split walks, added in their order: D / 4 threads a row of dq or (KEYS) twice as many a key, dk and dv.
+// The shares of cut walks, added in their order: D / 4 threads a row of dq or (KEYS) twice as many a key, dk and dv. (The grid is that of as many cut
+// pieces as there may be.)
 template <int D, bool KEYS>
 __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams p) {
     constexpr int kPiece = KEYS ? kKeys : kRows, kWide = KEYS ? 2 * D : D, kPer = kWide / 4, kSum = 256 / kPer, kPerPiece = kPiece / kSum;
+    const BackPlan& plan = KEYS ? p.keys : p.rows;
     const int c = threadIdx.x % kPer, in = (int)(blockIdx.x % kPerPiece) * kSum + threadIdx.x / kPer, item = blockIdx.x / kPerPiece;
-    const PackedItems& items = KEYS ? p.key_items : p.row_items;
-    const int kvh = paged_quot(item, items.n), number = item - kvh * items.n.by, group = p.group.by;
-    int steps, chunk;
+    const int number = item / p.kv_heads, kvh = item - number * p.kv_heads, group = p.group.by;
+    if (number >= plan.counts[1]) return;
+    const BackUnit cut = plan.cuts[number];
+    const PackedSeq sq = packed_seq(p.b, cut.seq);
     void* out;
     size_t dst;
     if constexpr (KEYS) {
-        const PackedKeys kb = {p.b.k_start, p.b.seqs, p.b.k_tokens};
-        const PagedPiece piece = paged_piece<kPiece>(p.key_pieces, kb, 1, number);
-        const PackedSeq sq = packed_seq(p.b, piece.seq);
-        const int key0 = piece.tile * kPiece;
-        if (key0 + in >= sq.len) return;
-        const RowWalk walk = row_walk(p.mask, sq, key0, min(key0 + kPiece, sq.len) - 1, group);
-        steps = walk.to - walk.from, chunk = p.key_chunk;
+        const int key = cut.tile * kKeys + in;
+        if (key >= sq.len) return;
         out = 4 * c < D ? p.dk : p.dv;
-        dst = ((size_t)(sq.k0 + key0 + in) * p.kv_heads + kvh) * D + 4 * c % D;
+        dst = ((size_t)(sq.k0 + key) * p.kv_heads + kvh) * D + 4 * c % D;
     } else {
-        const PagedPiece piece = paged_piece<kRows>(p.row_pieces, p.b, group, number);
-        const PackedSeq sq = packed_seq(p.b, piece.seq);
-        const int rows = sq.count * group, row0 = piece.tile * kRows, r = row0 + in;
-        if (r >= rows) return;
-        steps = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group)).n, chunk = p.row_chunk;
+        const int r = cut.tile * kRows + in;
+        if (r >= sq.count * group) return;
         const int t = paged_quot(r, p.group);
         out = p.dq;
         dst = ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D + 4 * c;
     }
-    if (steps <= chunk) return;   // (one workgroup's, written)
-    const int shares = (steps + chunk - 1) / chunk;
-    const float* part = (KEYS ? p.part_dkv : p.part_dq) + ((size_t)item * kPiece + in) * kWide + 4 * c;
-    const size_t next = (size_t)(KEYS ? p.part_keys : p.part_rows) * kWide;
+    const float* part = plan.places + (((size_t)kvh * plan.most_places + cut.place) * kPiece + in) * kWide + 4 * c;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < shares; s++) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(part + s * next);
+    for (int s = 0; s < cut.shares; s++) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(part + (size_t)s * kPiece * kWide);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] += y[i];
     }
@@ -635,53 +729,39 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams 
     else *reinterpret_cast<f32x4*>((float*)out + dst) = x;
 }
 
-// How a call is cut, and its workspace.
-struct BackCut {
-    PagedPieces rows, keys;
-    size_t row_chunk, row_shares, key_chunk, key_shares;
-};
-constexpr size_t kMostShares = (size_t)1 << 30;   // bytes of the shares of a kernel: past it its walks are cut less
-BackCut back_cut(const PackedCall& c) {
-    const size_t group = c.heads / c.kv_heads, units = (size_t)fv_compute_units(), slots = (c.d == 64 ? 3 : 2) * units;
-    BackCut cut;
-    const size_t keys = kKeys, step = kStep;
-    cut.rows = paged_pieces(kRows, c.seqs, c.tokens, c.max_q, group);
-    cut.keys = paged_pieces(keys, c.seqs, c.k_tokens, c.max_k, 1);
-    auto shares_of = [&](const PagedPieces& x, size_t rows, size_t piece, size_t places, size_t steps, size_t least, size_t bytes) {
-        const size_t items = c.kv_heads * (size_t)x.n.by;
-        if (items == 0) return (size_t)1;
-        const size_t held = x.tiles.by ? items : std::max<size_t>(c.kv_heads * (rows / piece + 1), items / 2);
-        const size_t shares = held < places ? std::min(places / held, std::max<size_t>(steps / least, 1)) : 1;
-        return std::min(shares, std::max<size_t>(kMostShares / (items * piece * bytes), 1));
-    };
-    const size_t key_steps = fv_packed_key_steps(c, kRows), rows = c.max_q * group;
-    size_t row_steps = (rows + step - 1) / step;
-    if (c.causal && c.window > 0 && c.sink == 0) {   // rows of the window's blocks and of those of the piece's keys
-        const size_t blocks = c.window + (keys + c.block_tokens - 1) / c.block_tokens, far = (size_t)1 << 31;
-        const size_t band = blocks < far / c.block_tokens / group ? blocks * c.block_tokens * group : far;
-        row_steps = std::min(row_steps, (band + step - 1) / step + 1);
-    }
-    row_steps = std::max<size_t>(row_steps, 1);
-    size_t n = shares_of(cut.rows, c.tokens * group, kRows, slots, key_steps, 4, c.d * 4);
-    cut.row_chunk = (key_steps + n - 1) / n, cut.row_shares = (key_steps + cut.row_chunk - 1) / cut.row_chunk;
-    n = shares_of(cut.keys, c.k_tokens, keys, slots, row_steps, 8, c.d * 8);
-    cut.key_chunk = (row_steps + n - 1) / n, cut.key_shares = (row_steps + cut.key_chunk - 1) / cut.key_chunk;
-    return cut;
-}
+// A call's plans and its workspace. With a walk cut where it passes the mean load of a slot there are no more shares past the first of a piece than slots, and
+// no more places than twice as many; walks of no more than `least` steps are not cut: a share costs its place's traffic (of 128 keys 256 KB, of 128 rows 128), some 18
+// steps of 32 rows or 8 tiles.
 struct BackParts {
-    size_t stats = 0, rounded = 0, dq = 0, dkv = 0, bytes = 0;   // bytes from the workspace's start
-    size_t rows, keys;
-    BackParts(const PackedCall& c, const BackCut& cut, bool round) {
+    size_t stats = 0, rounded = 0, bytes = 0;   // bytes from the workspace's start
+    int slots;
+    struct Plan {
+        PagedPieces pieces;
+        size_t units, cuts, places, least, counts_at, units_at, cuts_at, scratch_at, places_at;
+    } keys, rows;
+    BackParts(const PackedCall& c, bool round) {
         auto take = [this](size_t n) {
             const size_t at = bytes;
             bytes += (n + 255) / 256 * 256;
             return at;
         };
-        rows = c.kv_heads * (size_t)cut.rows.n.by * kRows, keys = c.kv_heads * (size_t)cut.keys.n.by * kKeys;
+        slots = (c.d == 64 ? 3 : 2) * fv_compute_units();
+        const size_t group = c.heads / c.kv_heads;
+        auto plan = [&](Plan& x, const PagedPieces& pieces, size_t steps, size_t least, size_t place_bytes) {
+            x.pieces = pieces, x.least = least;
+            const size_t n = (size_t)pieces.n.by, more = steps > least ? std::min((size_t)slots / c.kv_heads + 1, n * (steps / least)) : 0;
+            x.units = n + more, x.cuts = std::min(n, more), x.places = 2 * more;
+            x.counts_at = take(16), x.units_at = take(x.units * sizeof(BackUnit)), x.cuts_at = take(x.cuts * sizeof(BackUnit)), x.scratch_at = take(n * 8);
+            x.places_at = take(x.places * c.kv_heads * place_bytes);
+        };
         stats = take(c.tokens * c.heads * 8);
         if (round) rounded = take(c.tokens * c.heads * c.d * 2);
-        if (cut.row_shares > 1) dq = take(cut.row_shares * rows * c.d * 4);
-        if (cut.key_shares > 1) dkv = take(cut.key_shares * keys * c.d * 8);
+        plan(keys, paged_pieces(kKeys, c.seqs, c.k_tokens, c.max_k, 1), (c.max_q * group + kStep - 1) / kStep, 32, kKeys * c.d * 8);
+        plan(rows, paged_pieces(kRows, c.seqs, c.tokens, c.max_q, group), fv_packed_key_steps(c, kRows), 12, kRows * c.d * 4);
+    }
+    static BackPlan on_device(const Plan& x, uint8_t* ws) {
+        return {x.pieces, (int*)(ws + x.counts_at), (BackUnit*)(ws + x.units_at), (BackUnit*)(ws + x.cuts_at), (int2*)(ws + x.scratch_at), (int)x.units, (int)x.cuts,
+                (int)x.places, (int)x.least, (float*)(ws + x.places_at)};
     }
 };
 std::atomic<unsigned long long> lds_done{0};   // (of the one kernel that takes more than 64 KB)
@@ -696,7 +776,7 @@ size_t fv_packed_attention_backward_workspace_bytes(int dout_is_bf16, size_t hea
                                                     size_t sink) {
     const PackedCall c = {heads, kv_heads, d, seqs, q_tokens, k_tokens, std::min(max_q, q_tokens), std::min(max_k, k_tokens), nullptr, nullptr, 1.f, causal,
                           block_tokens, window, sink};
-    return fv_packed_sizes(c) ? fv::BackParts(c, fv::back_cut(c), !dout_is_bf16).bytes : 0;
+    return fv_packed_sizes(c) ? fv::BackParts(c, !dout_is_bf16).bytes : 0;
 }
 
 int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint16_t* q, size_t q_stride, const uint16_t* k, size_t k_stride,
@@ -717,15 +797,12 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     if (k_tokens > 0) x[n++] = {k, k_stride, kv_heads}, x[n++] = {v, v_stride, kv_heads}, x[n++] = {dk, kv_heads * d, kv_heads}, x[n++] = {dv, kv_heads * d, kv_heads};
     const int rc = fv_packed_args("packed attention backward", c, x, n, workspace);
     if (rc != FV_OK) return rc;
-    const fv::BackCut cut = fv::back_cut(c);
-    const fv::BackParts parts(c, cut, !dout_is_bf16);
-    if (parts.bytes > 0 && (!workspace || workspace_bytes < parts.bytes)) return fv_invalid("packed attention backward: workspace too small");
-    const size_t row_items = kv_heads * (size_t)cut.rows.n.by, key_items = kv_heads * (size_t)cut.keys.n.by;
-    const size_t rows = q_tokens * heads, stat_blocks = (rows + 2048 / d - 1) / (2048 / d);
-    const size_t sum_rows = row_items * fv::kRows / (1024 / d), sum_keys = key_items * fv::kKeys / (512 / d);
+    const fv::BackParts parts(c, !dout_is_bf16);
+    if (!workspace || workspace_bytes < parts.bytes) return fv_invalid("packed attention backward: workspace too small");
+    const size_t rows = q_tokens * heads, stat_blocks = (rows + 2048 / d - 1) / (2048 / d) + 2;
+    const size_t sum_rows = kv_heads * parts.rows.cuts * fv::kRows / (1024 / d), sum_keys = kv_heads * parts.keys.cuts * fv::kKeys / (512 / d);
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
-    if (row_items * cut.row_shares >= kMost / 2 || key_items * cut.key_shares >= kMost / 2 || stat_blocks >= kMost ||
-        (cut.row_shares > 1 && sum_rows >= kMost) || (cut.key_shares > 1 && sum_keys >= kMost))
+    if (kv_heads * parts.rows.units >= kMost / 2 || kv_heads * parts.keys.units >= kMost / 2 || stat_blocks >= kMost || sum_rows >= kMost || sum_keys >= kMost)
         return fv_decline("packed attention backward: too large for one launch");
     uint8_t* ws = (uint8_t*)workspace;
     fv::PackedBackParams p;
@@ -737,32 +814,27 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     p.dq = dq, p.dk = dk, p.dv = dv, p.grads_are_bf16 = grads_are_bf16 != 0;
     p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = fv::paged_div(heads / kv_heads);
     p.scale = scale, p.sl2 = (float)((double)scale * 1.4426950408889634);
-    p.row_pieces = cut.rows, p.key_pieces = cut.keys;
-    p.row_items = fv::packed_items(kv_heads, (size_t)cut.rows.n.by, cut.row_shares);
-    p.key_items = fv::packed_items(kv_heads, (size_t)cut.keys.n.by, cut.key_shares);
-    p.row_chunk = (int)cut.row_chunk, p.key_chunk = (int)cut.key_chunk;
-    p.part_dq = (float*)(ws + parts.dq), p.part_dkv = (float*)(ws + parts.dkv), p.part_rows = (long)parts.rows, p.part_keys = (long)parts.keys;
+    p.runs = fv::packed_runs(kv_heads);
+    p.keys = fv::BackParts::on_device(parts.keys, ws), p.rows = fv::BackParts::on_device(parts.rows, ws);
     hipStream_t st = (hipStream_t)stream;
     hipError_t e = hipSuccess;
     fv::paged_pick(d == 128, [&](auto d128) {
         constexpr int D = d128() ? 128 : 64;
-        if (q_tokens > 0)
-            fv::paged_pick(out_is_bf16 != 0, [&](auto o16) {
-                fv::paged_pick(dout_is_bf16 != 0, [&](auto g16) {
-                    hipLaunchKernelGGL((fv::packed_stats_kernel<D, o16(), g16()>), dim3((unsigned)stat_blocks), dim3(256), 0, st, dout, out, lse,
-                                       (float*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (long)q_tokens, (int)heads, p.group,
-                                       (float)(1.0 / (double)scale));
-                });
+        fv::paged_pick(out_is_bf16 != 0, [&](auto o16) {
+            fv::paged_pick(dout_is_bf16 != 0, [&](auto g16) {
+                hipLaunchKernelGGL((fv::packed_stats_kernel<D, o16(), g16()>), dim3((unsigned)stat_blocks), dim3(256), 0, st, p, dout, out, lse,
+                                   (float*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (float)(1.0 / (double)scale), parts.slots);
             });
-        if (key_items > 0) {
+        });
+        if (k_tokens > 0) {
             if (fv::KeyForm<D>::kLds > 65536) e = fv_set_max_lds_once((const void*)fv::packed_dkv_kernel<D>, fv::KeyForm<D>::kLds, fv::lds_done);
             if (e != hipSuccess) return;
-            hipLaunchKernelGGL((fv::packed_dkv_kernel<D>), dim3((unsigned)fv::packed_blocks(p.key_items)), dim3(256), fv::KeyForm<D>::kLds, st, p);
-            if (cut.key_shares > 1) hipLaunchKernelGGL((fv::packed_sum_kernel<D, true>), dim3((unsigned)sum_keys), dim3(256), 0, st, p);
+            hipLaunchKernelGGL((fv::packed_dkv_kernel<D>), dim3((unsigned)fv::packed_blocks(p.runs, parts.keys.units)), dim3(256), fv::KeyForm<D>::kLds, st, p);
+            if (parts.keys.cuts > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D, true>), dim3((unsigned)sum_keys), dim3(256), 0, st, p);
         }
-        if (row_items > 0) {
-            hipLaunchKernelGGL((fv::packed_dq_kernel<D>), dim3((unsigned)fv::packed_blocks(p.row_items)), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
-            if (cut.row_shares > 1) hipLaunchKernelGGL((fv::packed_sum_kernel<D, false>), dim3((unsigned)sum_rows), dim3(256), 0, st, p);
+        if (q_tokens > 0) {
+            hipLaunchKernelGGL((fv::packed_dq_kernel<D>), dim3((unsigned)fv::packed_blocks(p.runs, parts.rows.units)), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
+            if (parts.rows.cuts > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D, false>), dim3((unsigned)sum_rows), dim3(256), 0, st, p);
         }
     });
     if (e == hipSuccess) e = hipGetLastError();
