@@ -92,23 +92,27 @@ FV_DEV PackedWhole packed_whole(const PackedWalk& w, const PagedSight& all) {
     return {w.before(all.a / kTileRows), all.a >= all.lo ? 0 : w.before((all.lo + kTileRows - 1) / kTileRows), w.before(all.hi / kTileRows)};
 }
 
-// Workgroups to pieces: 2^xcds XCDs take the pieces of a run of whole key heads, the heads' pieces in turn, so that an L2 holds few heads' tensors and
-// the longest walks of all heads come first; the XCDs of a run take them in turn.
+// Workgroups to pieces: 2^xcds XCDs take the pieces of a run of whole key heads, in turn, so that an L2 holds few heads' tensors. Under a causal mask the
+// heads' pieces follow each other by number, so that the longest walks of all come first (one clip of 7 frames, 12 heads, three a run: 13 % over even
+// shares of the work instead of 36 %); where walks are alike, head by head (two clips, 12 heads, forward: 740 us, by number 768).
 struct PackedRuns {
     PagedDiv heads;   // of a run
-    int xcds;
+    int xcds, by_head;
 };
 struct PackedSlot {
-    int head, number;   // of the key head's pieces; past the last: none
+    int head, number;   // of the key head's pieces; head < 0: none
 };
 template <class Runs>
-FV_DEV PackedSlot packed_slot(const Runs& x, int block) {
-    const int in_run = ((block >> 3) << x.xcds) + (block & ((1 << x.xcds) - 1)), number = paged_quot(in_run, x.heads);
-    return {((block & 7) >> x.xcds) * x.heads.by + in_run - number * x.heads.by, number};
+FV_DEV PackedSlot packed_slot(const Runs& x, int block, int numbers) {
+    const int in_run = ((block >> 3) << x.xcds) + (block & ((1 << x.xcds) - 1)), first = ((block & 7) >> x.xcds) * x.heads.by;
+    if (numbers <= 0) return {-1, 0};
+    const int a = x.by_head ? in_run / numbers : paged_quot(in_run, x.heads), b = in_run - a * (x.by_head ? numbers : x.heads.by);
+    const int head = x.by_head ? a : b, number = x.by_head ? b : a;
+    return {head < x.heads.by && number < numbers ? first + head : -1, number};
 }
-inline PackedRuns packed_runs(size_t kv_heads) {
+inline PackedRuns packed_runs(size_t kv_heads, bool causal) {
     const int xcds = kv_heads % 8 == 0 ? 0 : kv_heads % 4 == 0 ? 1 : kv_heads % 2 == 0 ? 2 : 3;
-    return {paged_div(kv_heads >> (3 - xcds)), xcds};
+    return {paged_div(kv_heads >> (3 - xcds)), xcds, causal ? 0 : 1};
 }
 inline size_t packed_blocks(const PackedRuns& x, size_t numbers) {
     return (((size_t)x.heads.by * numbers + ((size_t)1 << x.xcds) - 1) >> x.xcds) * 8;

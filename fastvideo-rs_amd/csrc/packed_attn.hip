@@ -52,9 +52,9 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int q4 = lane >> 4, i16 = lane & 15;
-    const PackedSlot slot_at = packed_slot(p.runs, block);
+    const PackedSlot slot_at = packed_slot(p.runs, block, p.pieces.n.by * p.shares);
+    if (slot_at.head < 0) return true;
     const int kvh = slot_at.head, share = paged_quot(slot_at.number, p.pieces.n);
-    if (share >= p.shares) return true;
     const int number = (share + 1) * p.pieces.n.by - 1 - slot_at.number;   // (a sequence's last rows, which see most, first)
     const PagedPiece piece = paged_piece<kRows>(p.pieces, p.b, p.group.by, number);
     const PackedSeq sq = packed_seq(p.b, piece.seq);
@@ -408,7 +408,7 @@ size_t fv_packed_key_steps(const PackedCall& c, size_t rows) {
 static bool mask_fits(const PackedCall& c) { return std::max({c.block_tokens, c.window, c.sink}) <= (size_t)INT_MAX / 2; }
 bool fv_packed_sizes(const PackedCall& c) {
     return c.kv_heads > 0 && c.heads >= c.kv_heads && c.heads % c.kv_heads == 0 && c.heads <= 65535 && (c.d == 64 || c.d == 128) && c.seqs > 0 &&
-           c.seqs <= kMostSeqs && c.tokens > 0 && c.tokens <= kMostRows && c.k_tokens <= kMostRows && c.tokens * (c.heads / c.kv_heads) <= (size_t)INT_MAX / 2 &&
+           c.seqs <= kMostSeqs && c.tokens <= kMostRows && c.k_tokens <= kMostRows && c.tokens * (c.heads / c.kv_heads) <= (size_t)INT_MAX / 2 &&
            (!c.causal || (c.block_tokens > 0 && mask_fits(c)));
 }
 fv::PackedMask fv_packed_mask(const PackedCall& c) {
@@ -446,7 +446,7 @@ size_t fv_packed_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t
                                            size_t max_k, int causal, size_t block_tokens, size_t window, size_t sink) {
     const PackedCall c = {heads, kv_heads, d, seqs, q_tokens, k_tokens, std::min(max_q, q_tokens), std::min(max_k, k_tokens), nullptr, nullptr, 1.f, causal,
                           block_tokens, window, sink};
-    return fv_packed_sizes(c) && max_q > 0 ? fv::packed_cut(c).bytes(kv_heads, d) : 0;
+    return fv_packed_sizes(c) && c.max_q > 0 ? fv::packed_cut(c).bytes(kv_heads, d) : 0;
 }
 
 int fv_packed_attention(const uint16_t* q, size_t q_stride, const uint16_t* k, size_t k_stride, const uint16_t* v, size_t v_stride, void* out,
@@ -476,7 +476,7 @@ int fv_packed_attention(const uint16_t* q, size_t q_stride, const uint16_t* k, s
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     const size_t join_blocks = items * fv::kRows / (1024 / d);
     if (items * cut.shares >= kMost / 2 || (cut.shares > 1 && join_blocks >= kMost)) return fv_decline("packed attention: too large for one launch");
-    p.runs = fv::packed_runs(kv_heads), p.shares = (int)cut.shares;
+    p.runs = fv::packed_runs(kv_heads, causal != 0), p.shares = (int)cut.shares;
     p.part_rows = (long)cut.rows(kv_heads);
     p.part_o = (float*)workspace, p.part_lse = p.part_o + cut.shares * cut.rows(kv_heads) * d;
     hipStream_t st = (hipStream_t)stream;

@@ -80,6 +80,19 @@ FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group)
     k.hi = hi >= s.count ? 0x7fffffff : (int)max(hi, 0L) * group;
     return k;
 }
+// The rows of a sequence that see one key, [lo, hi): their weight is 1 and their dS nothing, exactly, where dP - D would leave the rounding of `out`.
+// packed_dkv_kernel loads zeros for their queries and -lse / scale (scores of 0, a weight of 1, no part in dk), packed_dq_kernel stores zeros. By token those are the first token's (under a window of one, without a sink, all); by blocks those of a last block of one key under such a window.
+template <class Mask>
+FV_DEV KeySight single_rows(const Mask& m, const PackedSeq& s, int group) {
+    const bool alone = m.window == 1 && m.sink == 0;
+    if (!m.causal) return {0, s.len == 1 ? 0x7fffffff : 0};
+    const int bt = m.block_tokens.by;
+    if (bt > 1 && !(s.len == 1 || (alone && s.len - paged_quot(s.len, m.block_tokens) * bt == 1))) return {0, 0};
+    const int pos = bt == 1 ? 0 : s.len - 1;   // (a row at a negative position sees none)
+    const int first = (int)min(max((long)pos - s.pos0, 0L), (long)s.count), behind = bt == 1 && alone ? s.count : (int)min(max((long)pos + 1 - s.pos0, 0L), (long)s.count);
+    return {first * group, behind * group};
+}
+
 // packed_dkv_kernel: a workgroup's keys, the rows of a step, and its LDS: V's operands | 2 x (q, dout) | 2 x (-lse / scale, -D).
 constexpr int kKeys = 128, kStep = 32;
 template <int D>
@@ -284,9 +297,9 @@ FV_DEV void key_step(const lds_u8* qt, const lds_u8* gt, const lds_u8* vt, const
         to[g][4 * x + i] = y[0], to[g][4 * x + i + 1] = y[1];
     };
     auto stat_rows = [&](int x, int which) { return *reinterpret_cast<const __attribute__((address_space(3))) f32x4*>(stat + 128 * which + (16 * x + 4 * q4) * 4); };
+    auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
     auto hide = [&](int x) {
         if (!cut) return;
-        auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
 #pragma unroll
         for (int g = 0; g < 2; g++) {
             const int r = row0 + 16 * x + 4 * q4;
@@ -342,8 +355,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
-    const PackedSlot at = packed_slot(p.runs, blockIdx.x);
-    if (at.number >= p.keys.counts[0]) return;
+    const PackedSlot at = packed_slot(p.runs, blockIdx.x, p.keys.counts[0]);
+    if (at.head < 0) return;
     const BackUnit unit = p.keys.units[at.number];
     const int kvh = at.head, group = p.group.by;
     const PackedSeq sq = packed_seq(p.b, unit.seq);
@@ -364,6 +377,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
         const KeySight a = key_sight(p.mask, sq, wkey, group), b = key_sight(p.mask, sq, to, group);
         some = {a.lo, max(a.hi, b.hi)}, all = {b.lo, key_sight(p.mask, sq, max(wkey, early), group).hi};
     }
+    const KeySight single = single_rows(p.mask, sq, group);
     const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
     const unsigned lds0 = (unsigned)(size_t)smem;
     // V: the wave's operands, 1 KB each: the lane's 16 bytes of key i16 (+ 16) and chunk 4 dc + q4
@@ -415,21 +429,30 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const 
         const int n = max(min(rows - r_last, kStep), 1), end = h0 + n - 1, dt_end = row_dt(end);   // the last row
         q_bytes = (unsigned)dt_end * qstep + (unsigned)(end + 1) * G::kRow, g_bytes = (unsigned)dt_end * gstep + (unsigned)(end + 1) * G::kRow, s_bytes = n * 4u;
     }
+    int r_at = r_last;   // the step's first row
     auto load = [&](int buf) {
+        const bool some_single = r_at < single.hi && r_at + kStep > single.lo;
         const u32x4 qd = plane_descriptor(qb, q_bytes), gd = plane_descriptor(gb, g_bytes);
         const unsigned at = lds0 + F::kSteps + buf * 2 * kHalf + wave * (kHalf / 4);
 #pragma unroll
         for (int it = 0; it < kLoads; it++) {
             const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(at + it * 1024)), m1 = m0 + kHalf;
+            unsigned from = qo[it];
+            if (some_single) {
+                const int r = r_at + (wave * kLoads + it) * G::kRowsPerDma + lane / G::kChunks;
+                from = r >= single.lo && r < single.hi ? 0x80000000u : from;   // (past the descriptor: zeros)
+            }
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
                          "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds"
-                         :: "s"(m0), "s"(m1), "v"(qo[it]), "v"(go[it]), "s"(qd), "s"(gd) : "memory");
+                         :: "s"(m0), "s"(m1), "v"(from), "v"(go[it]), "s"(qd), "s"(gd) : "memory");
         }
         if (wave < 2) {   // (32 floats, -lse / scale or -D)
             const u32x4 sd = plane_descriptor(sb, s_bytes);
             const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + F::kStats + buf * 256 + wave * 128));
-            if (lane < 32) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(m0), "v"(lane * 4), "s"(sd) : "memory");
+            const bool none = wave == 0 && r_at + lane >= single.lo && r_at + lane < single.hi;
+            if (lane < 32) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(m0), "v"(none ? 0x80000000u : lane * 4u), "s"(sd) : "memory");
         }
+        r_at -= kStep;
         q_bytes = g_bytes = 0x80000000u, s_bytes = 128;
         h0 -= back_heads;
         const bool more = h0 < 0;
@@ -594,8 +617,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
-    const PackedSlot at = packed_slot(p.runs, blockIdx.x);
-    if (at.number >= p.rows.counts[0]) return;
+    const PackedSlot at = packed_slot(p.runs, blockIdx.x, p.rows.counts[0]);
+    if (at.head < 0) return;
     const BackUnit unit = p.rows.units[at.number];
     const int kvh = at.head, group = p.group.by;
     const PackedSeq sq = packed_seq(p.b, unit.seq);
@@ -603,6 +626,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
     if (row0 >= rows) return;   // (as above)
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
     const int e0 = unit.from, e1 = min(w.n, unit.to);
+    const KeySight single = single_rows(p.mask, sq, group);
     const float sl2 = p.sl2;
 
     const int wrow = row0 + 32 * wave;
@@ -679,13 +703,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
         const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
         if (r >= rows) continue;
         const size_t dst = ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D;
+        const bool alone = r >= single.lo && r < single.hi;
         float* part = p.rows.places + (((size_t)kvh * p.rows.most_places + max(unit.place, 0)) * kRows + (r - row0)) * D;
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
             const int at = 16 * db + 4 * q4;
             f32x4 x = dq[db][g];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] *= p.scale;
+            for (int i = 0; i < 4; i++) x[i] = alone ? 0.f : x[i] * p.scale;
             if (unit.place >= 0) *reinterpret_cast<f32x4*>(part + at) = x;
             else if (p.grads_are_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.dq + dst + at) = __builtin_convertvector(x, bf16x4);
             else *reinterpret_cast<f32x4*>((float*)p.dq + dst + at) = x;
@@ -814,7 +839,7 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     p.dq = dq, p.dk = dk, p.dv = dv, p.grads_are_bf16 = grads_are_bf16 != 0;
     p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = fv::paged_div(heads / kv_heads);
     p.scale = scale, p.sl2 = (float)((double)scale * 1.4426950408889634);
-    p.runs = fv::packed_runs(kv_heads);
+    p.runs = fv::packed_runs(kv_heads, causal != 0);
     p.keys = fv::BackParts::on_device(parts.keys, ws), p.rows = fv::BackParts::on_device(parts.rows, ws);
     hipStream_t st = (hipStream_t)stream;
     hipError_t e = hipSuccess;

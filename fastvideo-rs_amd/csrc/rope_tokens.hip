@@ -29,8 +29,8 @@ struct RopeParams {
     long tokens;
     float amplitude;
     int inverse;
-    PagedDiv chunks;        // threads of a token in one piece of heads
-    PagedDiv pieces;        // pieces of a token's heads
+    PagedDiv units;         // threads of a token in one piece of heads
+    int turned;             // those of channels that are turned
     int per;                // heads a piece
 };
 
@@ -48,93 +48,90 @@ FV_DEV void turn_sincos(uint64_t turns, float& sin, float& cos) {
     sin = quarter & 2 ? -sin : sin, cos = (quarter + 1) & 2 ? -cos : cos;
 }
 
-template <bool IS16>
-FV_DEV void load_eight(const void* base, long at, float (&x)[8]) {
+// N channels: 16 bytes of bf16 or f32 in, as many or half or twice as many out.
+template <bool IS16, int N>
+FV_DEV void load_run(const void* base, long at, float (&x)[N]) {
     if constexpr (IS16) {
+        static_assert(N == 8, "16 bytes");
         const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)base + at);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[2 * i] = __builtin_bit_cast(float, w[i] << 16), x[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
     } else {
+        static_assert(N == 4, "16 bytes");
+        const f32x4 w = *reinterpret_cast<const f32x4*>((const float*)base + at);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>((const float*)base + at + 4 * h);
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[4 * h + i] = w[i];
-        }
+        for (int i = 0; i < 4; i++) x[i] = w[i];
     }
 }
-template <bool IS16>
-FV_DEV void store_eight(void* base, long at, const float (&x)[8]) {
+template <bool IS16, int N>
+FV_DEV void store_run(void* base, long at, const float (&x)[N]) {
     if constexpr (IS16) {
-        f32x8 v;
+        typedef __attribute__((ext_vector_type(N))) float fv_n;
+        typedef __attribute__((ext_vector_type(N))) __bf16 bf_n;
+        fv_n v;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = x[i];
-        *reinterpret_cast<bf16x8*>((uint16_t*)base + at) = __builtin_convertvector(v, bf16x8);
+        for (int i = 0; i < N; i++) v[i] = x[i];
+        *reinterpret_cast<bf_n*>((uint16_t*)base + at) = __builtin_convertvector(v, bf_n);
     } else {
 #pragma unroll
-        for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4*>((float*)base + at + 4 * h) = f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
+        for (int h = 0; h < N; h += 4) *reinterpret_cast<f32x4*>((float*)base + at + h) = f32x4{x[h], x[h + 1], x[h + 2], x[h + 3]};
     }
 }
 
-// A thread has 16 channels of a token: of the turned ones eight pairs (neighbours: 16 channels in a row; halves: eight and their partners), of the
-// others any, and goes through `per` heads of q and then k.
+// A thread has 16 bytes of a token's input a head (HALVES: and those of their partners), makes the angles of their pairs once, and goes through `per`
+// heads of q and then k, four on their way at a time.
 template <bool IN16, bool OUT16, bool HALVES>
 __global__ __launch_bounds__(256) void rope_tokens_kernel(const RopeParams p) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    const long unit = id / p.chunks.by;   // (token, piece of heads)
-    const int chunk = (int)(id - unit * p.chunks.by);
-    const long token = unit / p.pieces.by;
+    constexpr int N = IN16 ? 8 : 4, kPairs = HALVES ? N : N / 2, kAtOnce = 4;
+    const int id = blockIdx.x * 256 + threadIdx.x, token = paged_quot(id, p.units), unit = id - token * p.units.by;
     if (token >= p.tokens) return;
-    const int piece = (int)(unit - token * p.pieces.by);
-    const int all = p.heads + p.kv_heads, h0 = piece * p.per, h1 = min(all, h0 + p.per);
-    const bool turns = 8 * chunk < p.pairs;
-    // the two runs of eight channels
-    const int c0 = !turns ? 2 * p.pairs + 16 * (chunk - p.pairs / 8) : HALVES ? 8 * chunk : 16 * chunk, c1 = turns && HALVES ? p.pairs + 8 * chunk : c0 + 8;
-    const bool two = c1 < p.d;   // (a last run of eight channels alone that are not turned)
-    float c[8], s[8];
+    const int all = p.heads + p.kv_heads, h0 = blockIdx.y * p.per, h1 = min(all, h0 + p.per);
+    const bool turns = unit < p.turned;
+    const int c0 = turns ? N * unit : 2 * p.pairs + N * (unit - p.turned), c1 = p.pairs + c0;   // (c1: HALVES' partners)
+    const bool two = HALVES && turns;
+    float c[kPairs], s[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) c[i] = 1.f, s[i] = 0.f;
     if (turns) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int pair = 8 * chunk + i;
+        for (int i = 0; i < kPairs; i++) {
+            const int pair = kPairs * unit + i;
             int axis = p.pair_axis ? p.pair_axis[pair] : 0;
             axis = (unsigned)axis < (unsigned)p.axes ? axis : 0;
-            turn_sincos((uint64_t)(int64_t)p.positions[token * p.axes + axis] * p.freq[pair], s[i], c[i]);
+            turn_sincos((uint64_t)(int64_t)p.positions[(long)token * p.axes + axis] * p.freq[pair], s[i], c[i]);
             s[i] = (p.inverse ? -s[i] : s[i]) * p.amplitude;
             c[i] *= p.amplitude;
         }
     }
-    for (int h = h0; h < h1; h++) {
-        const bool is_k = h >= p.heads;
-        const void* in = is_k ? p.k : p.q;
-        void* out = is_k ? p.k_out : p.q_out;
-        const long col = (long)(is_k ? h - p.heads : h) * p.d, from = token * (is_k ? p.k_stride : p.q_stride) + col,
-                   to = token * (is_k ? p.k_out_stride : p.q_out_stride) + col;
-        float x[8], y[8];
-        load_eight<IN16>(in, from + c0, x);
-        if (two) load_eight<IN16>(in, from + c1, y);
-        if (turns) {
+    for (int h = h0; h < h1; h += kAtOnce) {
+        float x[kAtOnce][N], y[kAtOnce][N];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) {
+            const int head = min(h + j, h1 - 1);
+            const bool is_k = head >= p.heads;
+            const long from = token * (is_k ? p.k_stride : p.q_stride) + (long)(is_k ? head - p.heads : head) * p.d;
+            load_run<IN16>(is_k ? p.k : p.q, from + c0, x[j]);
+            if (two) load_run<IN16>(is_k ? p.k : p.q, from + c1, y[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) {
+            if (turns) {
 #pragma clang fp contract(off)
-            if constexpr (HALVES) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float a = x[i], b = y[i];
-                    x[i] = a * c[i] - b * s[i];
-                    y[i] = a * s[i] + b * c[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float a = x[2 * i], b = x[2 * i + 1];
-                    x[2 * i] = a * c[i] - b * s[i];
-                    x[2 * i + 1] = a * s[i] + b * c[i];
-                    a = y[2 * i], b = y[2 * i + 1];
-                    y[2 * i] = a * c[4 + i] - b * s[4 + i];
-                    y[2 * i + 1] = a * s[4 + i] + b * c[4 + i];
+                for (int i = 0; i < kPairs; i++) {
+                    const float a = HALVES ? x[j][i] : x[j][2 * i], b = HALVES ? y[j][i] : x[j][2 * i + 1];
+                    const float u = a * c[i] - b * s[i], w = a * s[i] + b * c[i];
+                    if constexpr (HALVES) x[j][i] = u, y[j][i] = w;
+                    else x[j][2 * i] = u, x[j][2 * i + 1] = w;
                 }
             }
+            if (h + j < h1) {
+                const bool is_k = h + j >= p.heads;
+                const long to = token * (is_k ? p.k_out_stride : p.q_out_stride) + (long)(is_k ? h + j - p.heads : h + j) * p.d;
+                store_run<OUT16>(is_k ? p.k_out : p.q_out, to + c0, x[j]);
+                if (two) store_run<OUT16>(is_k ? p.k_out : p.q_out, to + c1, y[j]);
+            }
         }
-        store_eight<OUT16>(out, to + c0, x);
-        if (two) store_eight<OUT16>(out, to + c1, y);
     }
 }
 
@@ -154,17 +151,19 @@ int fv_rope_frequencies(size_t pairs, double base, int scaling, double factor, d
     if (scaling == 2 && pairs < 2) return fv_invalid("rope frequencies: a scaled base needs two pairs");
     if (scaling == 3 && (!(original > 0.0) || !(original < 1e18) || !(high > low) || !(high < 1e18) || !(low > -1e18)))
         return fv_invalid("rope frequencies: original must be positive and low below high");
-    constexpr double kTurn = 6.283185307179586476925;
-    const double n = (double)pairs;
-    if (scaling == 2) base *= pow(factor, n / (n - 1.0));
+    // (80 bits: a double's 53 leave a turn 2^-24 off at 2^31 positions)
+    constexpr long double kTurn = 6.28318530717958647692528676655900577L;
+    const long double n = (long double)pairs;
+    long double b = base;
+    if (scaling == 2) b *= powl(factor, n / (n - 1.0L));
     for (size_t i = 0; i < pairs; i++) {
-        double theta = pow(base, -(double)i / n);
+        long double theta = powl(b, -(long double)i / n);
         if (scaling == 1) theta /= factor;
         if (scaling == 3) {
-            const double kept = std::min(1.0, std::max(0.0, (original * theta / kTurn - low) / (high - low)));
-            theta *= kept + (1.0 - kept) / factor;
+            const long double kept = std::min(1.0L, std::max(0.0L, (original * theta / kTurn - low) / (high - low)));
+            theta *= kept + (1.0L - kept) / factor;
         }
-        out[i] = (uint64_t)llrint(ldexp(theta / kTurn, 64));   // (theta is 1 at most: below 2^62)
+        out[i] = (uint64_t)llrintl(ldexpl(theta / kTurn, 64));   // (theta is 1 at most: below 2^62)
     }
     return FV_OK;
 }
@@ -203,20 +202,20 @@ int fv_rope_tokens(const void* q, size_t q_stride, void* q_out, size_t q_out_str
     p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.d = (int)d, p.pairs = (int)pairs, p.axes = (int)axes;
     p.freq = freq, p.pair_axis = pair_axis, p.positions = positions, p.tokens = (long)tokens;
     p.amplitude = amplitude, p.inverse = inverse != 0;
-    const size_t chunks = pairs / 8 + (d - 2 * pairs + 15) / 16, all = heads + kv_heads;
-    // Heads of a thread: eight where tokens are many, so that the angles are a small part of its work; fewer tokens spread over the units.
-    const size_t wanted = (size_t)fv_compute_units() * 1024;   // threads
-    size_t per = std::min<size_t>(all, 8);
-    while (per > 1 && tokens * chunks * ((all + per - 1) / per) < wanted) per = (per + 1) / 2;
-    p.per = (int)per;
-    p.chunks = fv::paged_div(chunks), p.pieces = fv::paged_div((all + per - 1) / per);
-    const size_t blocks = (tokens * chunks * ((all + per - 1) / per) + 255) / 256;
-    if (blocks >= (size_t)1 << 24) return fv_decline("rope tokens: too large for one launch");
+    const size_t run = in_is_bf16 ? 8 : 4, turned = (halves ? pairs : 2 * pairs) / run, units = turned + (d - 2 * pairs) / run, all = heads + kv_heads;
+    if (tokens * units > (size_t)INT_MAX) return fv_decline("rope tokens: too many tokens for one launch");
+    // Heads of a thread: up to 16, so that the angles are a small part of its work; fewer where that leaves units without threads.
+    const size_t wanted = (size_t)fv_compute_units() * 1024;
+    size_t per = std::min<size_t>(all, 16);
+    while (per > 1 && tokens * units * ((all + per - 1) / per) < wanted) per = (per + 1) / 2;
+    p.per = (int)per, p.turned = (int)turned, p.units = fv::paged_div(units);
+    const dim3 blocks((unsigned)((tokens * units + 255) / 256), (unsigned)((all + per - 1) / per));
+    if ((size_t)blocks.x * blocks.y >= (size_t)1 << 24) return fv_decline("rope tokens: too large for one launch");
     hipStream_t st = (hipStream_t)stream;
     fv::paged_pick(in_is_bf16 != 0, [&](auto i16) {
         fv::paged_pick(out_is_bf16 != 0, [&](auto o16) {
             fv::paged_pick(halves != 0, [&](auto h) {
-                hipLaunchKernelGGL((fv::rope_tokens_kernel<i16(), o16(), h()>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+                hipLaunchKernelGGL((fv::rope_tokens_kernel<i16(), o16(), h()>), blocks, dim3(256), 0, st, p);
             });
         });
     });

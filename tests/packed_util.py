@@ -73,6 +73,9 @@ def gradients(q, k, v, dout, out, lse, seen, scale):
     return dq, dk, dv, bq, bk, bv
 
 
+TURN = np.longdouble("6.28318530717958647692528676655900577")
+
+
 def frequencies(n, base=10000.0, scaling=None):
     """Radians a position of n pairs."""
     i = np.arange(n, dtype=np.longdouble)
@@ -83,7 +86,7 @@ def frequencies(n, base=10000.0, scaling=None):
         theta = theta / scaling[1]
     if scaling and scaling[0] == "parts":
         _, factor, original, low, high = scaling
-        kept = np.clip((original * theta / (2 * np.pi) - low) / (high - low), 0, 1)
+        kept = np.clip((original * theta / TURN - low) / (high - low), 0, 1)
         theta = theta * (kept + (1 - kept) / factor)
     return theta
 
@@ -91,7 +94,7 @@ def frequencies(n, base=10000.0, scaling=None):
 def rotate(x, positions, theta, halves, amplitude=1.0, inverse=False):
     """x [tokens, heads, d] with its first 2 len(theta) channels turned by positions [tokens, len(theta)] * theta."""
     n = len(theta)
-    angle = (positions.astype(np.longdouble) * theta[None, :]) % np.longdouble("6.28318530717958647692528676655900577")
+    angle = (positions.astype(np.longdouble) * theta[None, :]) % TURN
     c, s = (np.asarray(f(angle), dtype=np.float64)[:, None, :] * amplitude for f in (np.cos, np.sin))
     s = -s if inverse else s
     y = x.astype(np.float64).copy()
