@@ -26,17 +26,12 @@ struct PackedSeq {
     int start, count;   // first row, rows
     int k0, len;        // first key, keys
     int pos0;           // position of the first row among the keys: the last row is at the last key; negative where rows are more than keys
+    FV_DEV PackedSeq(int start_, int count_, int k0_, int len_) : start(start_), count(count_), k0(k0_), len(len_), pos0(len_ - count_) {}
 };
 template <class Batch>
 FV_DEV PackedSeq packed_seq(const Batch& b, int s) {
-    PackedSeq q;
-    q.start = min(max(b.q_start[s], 0), b.tokens);
-    const int behind = max(b.q_start[s + 1], q.start), k_behind = b.k_start[s + 1];
-    q.count = min(min(behind, b.tokens) - q.start, b.max_q);
-    q.k0 = min(max(b.k_start[s], 0), b.k_tokens);
-    q.len = min(min(max(k_behind, q.k0), b.k_tokens) - q.k0, b.max_k);
-    q.pos0 = q.len - (behind - q.start);
-    return q;
+    const int start = min(max(b.q_start[s], 0), b.tokens), k0 = min(max(b.k_start[s], 0), b.k_tokens);
+    return {start, min(min(max(b.q_start[s + 1], start), b.tokens) - start, b.max_q), k0, min(min(max(b.k_start[s + 1], k0), b.k_tokens) - k0, b.max_k)};
 }
 
 // f(0), f(1), .., f(N - 1) with the numbers as types (loops that the compiler does not unroll in time).

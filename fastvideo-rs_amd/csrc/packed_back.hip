@@ -2,7 +2,7 @@
 // of every row (token, query head) and dS = P (dout v^T - D):
 //     dv = P^T dout,    dk = scale dS^T q    (over the rows of all heads that share a key head),    dq = scale dS k.
 //
-// Three launches. A scan makes -lse / scale and -D of every row. Then the keys' gradients, a workgroup for 128 keys that walks the rows which
+// A scan makes -lse / scale and -D of every row. Then, in one launch, the keys' gradients, a workgroup for 128 keys that walks the rows which
 // see them, and the queries', a workgroup for 128 rows that walks the keys: each accumulates in registers and writes once, so the sums have one
 // order, no atomics and no cleared buffers. S and dP are made twice for that (seven products where five would do): to share them dq
 // would go through memory as f32 sums of every key tile, 512 B a row and 128 keys, at 0.19 us of matrix work for 128 x 128 pairs of five
@@ -18,18 +18,20 @@
 namespace fv {
 namespace {
 
-constexpr int kRows = 128;   // of a workgroup of packed_dq_kernel, 32 a wave
+constexpr int kRows = 128;   // of a workgroup of packed_dq_item, 32 a wave
 
 // Which workgroup takes what, made on the device from the sequences' lengths (plan_pieces): the units of a key head, the longest first, each a
 // piece of 128 rows or keys and a part [from, to) of the steps of its walk: tiles of 64 keys; of 32 rows. A walk longer than a slot's mean load is cut into
 // shares, which leave f32 sums in places of 128 rows ([kv_heads][most_places][128][d or 2 d]) and are added by packed_sum_kernel.
 struct BackUnit {
-    int seq, tile, from, to, place, shares, unused[2];   // place < 0: a whole walk; of a share: its place
+    int tile, from, to, place;    // place < 0: a whole walk; of a share: its place; kNoUnit: none. (Of a cut piece: `to` is its shares, `place` the first one's.)
+    int start, count, k0, len;    // the sequence, as packed_seq has it
+    FV_DEV PackedSeq seq() const { return {start, count, k0, len}; }
 };
+constexpr int kNoUnit = -2;
 struct BackPlan {
     PagedPieces pieces;
-    int* counts;         // units, cut pieces, places
-    BackUnit *units, *cuts;   // (of a cut piece: its first place)
+    BackUnit *units, *cuts;   // (behind the last: kNoUnit)
     int2* scratch;       // every piece number's sequence and steps
     int most_units, most_cuts, most_places, least;   // of a key head; steps below which no walk is cut
     float* places;
@@ -48,7 +50,7 @@ struct PackedBackParams {
     PagedDiv group;
     float scale, sl2;                                 // sl2 = scale * log2(e)
     PackedRuns runs;
-    BackPlan rows, keys;                              // of packed_dq_kernel, of packed_dkv_kernel
+    BackPlan rows, keys;                              // of packed_dq_item, of packed_dkv_item
 };
 
 // Chunk c of row r of a tile lies at chunk c ^ both_swz(r), so that a tile serves both kinds of operands without bank conflicts: the 8 rows of a
@@ -81,7 +83,7 @@ FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group)
     return k;
 }
 // The rows of a sequence that see one key, [lo, hi): their weight is 1 and their dS nothing, exactly, where dP - D would leave the rounding of `out`.
-// packed_dkv_kernel loads zeros for their queries and -lse / scale (scores of 0, a weight of 1, no part in dk), packed_dq_kernel stores zeros. By token those are the first token's (under a window of one, without a sink, all); by blocks those of a last block of one key under such a window.
+// packed_dkv_item loads zeros for their queries and -lse / scale (scores of 0, a weight of 1, no part in dk), packed_dq_item stores zeros. By token those are the first token's (under a window of one, without a sink, all); by blocks those of a last block of one key under such a window.
 template <class Mask>
 FV_DEV KeySight single_rows(const Mask& m, const PackedSeq& s, int group) {
     const bool alone = m.window == 1 && m.sink == 0;
@@ -93,7 +95,7 @@ FV_DEV KeySight single_rows(const Mask& m, const PackedSeq& s, int group) {
     return {first * group, behind * group};
 }
 
-// packed_dkv_kernel: a workgroup's keys, the rows of a step, and its LDS: V's operands | 2 x (q, dout) | 2 x (-lse / scale, -D).
+// packed_dkv_item: a workgroup's keys, the rows of a step, and its LDS: V's operands | 2 x (q, dout) | 2 x (-lse / scale, -D).
 constexpr int kKeys = 128, kStep = 32;
 template <int D>
 struct KeyForm {
@@ -132,7 +134,7 @@ template <bool KEYS>
 FV_DEV void plan_pieces(const PackedBackParams& p, const BackPlan& plan, int slots) {
     constexpr int kClasses = 64;
     __shared__ unsigned long long sum;
-    __shared__ int longest, units[kClasses], cuts, places;
+    __shared__ int longest, units[kClasses], cuts, places, total;
     const int tid = threadIdx.x, numbers = plan.pieces.n.by;
     if (tid == 0) sum = 0, longest = 0, cuts = 0, places = 0;
     if (tid < kClasses) units[tid] = 0;
@@ -181,24 +183,26 @@ FV_DEV void plan_pieces(const PackedBackParams& p, const BackPlan& plan, int slo
             units[c] = at;
             at += n;
         }
-        plan.counts[0] = min(at, plan.most_units);
+        total = at;
     }
     __syncthreads();
     for (int n = tid; n < numbers; n += 256) {
         const int2 x = plan.scratch[n];
         if (x.y < 0) continue;
+        const PackedSeq sq = packed_seq(p.b, x.x);
         const int k = shares_of(x.y), chunk = (x.y + k - 1) / k, tile = (int)(n - first_of(x.x));
         int u = atomicAdd(&units[class_of(x.y, k)], k), place = -1;
         if (k > 1) {
             const int c = atomicAdd(&cuts, 1);
             place = atomicAdd(&places, k);
-            if (c < plan.most_cuts) plan.cuts[c] = BackUnit{x.x, tile, 0, x.y, place, k, {0, 0}};
+            if (c < plan.most_cuts) plan.cuts[c] = BackUnit{tile, 0, k, place, sq.start, sq.count, sq.k0, sq.len};
         }
-        for (int s = 0; s < k; s++, u++)
-            if (u < plan.most_units) plan.units[u] = BackUnit{x.x, tile, s * chunk, min(x.y, (s + 1) * chunk), place < 0 ? -1 : place + s, k, {0, 0}};
+        for (int i = 0; i < k; i++, u++)
+            if (u < plan.most_units) plan.units[u] = BackUnit{tile, i * chunk, min(x.y, (i + 1) * chunk), place < 0 ? -1 : place + i, sq.start, sq.count, sq.k0, sq.len};
     }
     __syncthreads();
-    if (tid == 0) plan.counts[1] = min(cuts, plan.most_cuts);
+    for (int u = total + tid; u < plan.most_units; u += 256) plan.units[u].place = kNoUnit;
+    for (int c = cuts + tid; c < plan.most_cuts; c += 256) plan.cuts[c].place = kNoUnit;
 }
 
 // D / 8 threads a row (token, head); OUT16, DOUT16: bf16 bits. An f32 gradient is kept as bf16 bits in `rounded` [tokens, heads, d].
@@ -347,21 +351,21 @@ FV_DEV void key_step(const lds_u8* qt, const lds_u8* gt, const lds_u8* vt, const
 // registers (64 at 64 channels). K's operands stay in registers, V's in LDS as they are read: an operand is read once for two products, and an LDS
 // read a product costs nothing (at two waves a SIMD 1706 and 1715 TFLOP/s of 16x16x32 with half a ds_read_b128 each and one).
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dkv_kernel(const PackedBackParams p) {
+FV_DEV void packed_dkv_item(const PackedBackParams& p, const int wave, const int lane, const int block) {
     using G = TileGeo<D>;
     using F = KeyForm<D>;
     constexpr int kNO = D / 16, kNK = D / 32, kHalf = F::kHalf;
     constexpr int kLoads = kHalf / 4096;   // of a wave: its part of a step's q
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
-    const PackedSlot at = packed_slot(p.runs, blockIdx.x, p.keys.counts[0]);
+    const int q4 = lane >> 4, i16 = lane & 15;
+    const PackedSlot at = packed_slot(p.runs, block, p.keys.most_units);
     if (at.head < 0) return;
     const BackUnit unit = p.keys.units[at.number];
+    if (unit.place == kNoUnit) return;
     const int kvh = at.head, group = p.group.by;
-    const PackedSeq sq = packed_seq(p.b, unit.seq);
+    const PackedSeq sq = unit.seq();
     const int key0 = unit.tile * kKeys;
-    if (key0 >= sq.len) return;   // (as the plan has it; lengths changed since make no address)
     const int rows = sq.count * group, last = min(key0 + kKeys, sq.len) - 1;
     const RowWalk walk = row_walk(p.mask, sq, key0, last, group);
     const int e0 = walk.from + unit.from, e1 = min(walk.to, walk.from + unit.to);
@@ -611,19 +615,19 @@ FV_DEV void row_step(const lds_u8* kt, const lds_u8* vt, const TileReadBases& rb
 // K Q^T and dP^T = V dO^T leave the scores of two rows in a lane, dS the operand of dQ^T += K^T dS, whose K is the
 // same tile read across.
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const PackedBackParams p) {
+FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int lane, const int block) {
     using G = TileGeo<D>;
     constexpr int kNO = D / 16, kNK = D / 32, kTile = G::kTile, kIter = TileDma<4, D>::ITER, kUnits = kIter / 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     lds_u8* smem = (lds_u8*)smem_raw;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q4 = lane >> 4, i16 = lane & 15;
-    const PackedSlot at = packed_slot(p.runs, blockIdx.x, p.rows.counts[0]);
+    const int q4 = lane >> 4, i16 = lane & 15;
+    const PackedSlot at = packed_slot(p.runs, block, p.rows.most_units);
     if (at.head < 0) return;
     const BackUnit unit = p.rows.units[at.number];
+    if (unit.place == kNoUnit) return;
     const int kvh = at.head, group = p.group.by;
-    const PackedSeq sq = packed_seq(p.b, unit.seq);
+    const PackedSeq sq = unit.seq();
     const int rows = sq.count * group, row0 = unit.tile * kRows;
-    if (row0 >= rows) return;   // (as above)
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
     const int e0 = unit.from, e1 = min(w.n, unit.to);
     const KeySight single = single_rows(p.mask, sq, group);
@@ -718,17 +722,25 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(const P
     }
 }
 
+// The keys' units first, then the rows', whose shorter walks fill what the last of the keys' leave idle.
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_back_kernel(const PackedBackParams p, int key_blocks) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, block = blockIdx.x;
+    if (block < key_blocks) packed_dkv_item<D>(p, wave, lane, block);
+    else packed_dq_item<D>(p, wave, lane, block - key_blocks);
+}
+
 // The shares of cut walks, added in their order: D / 4 threads a row of dq or (KEYS) twice as many a key, dk and dv. (The grid is that of as many cut
 // pieces as there may be.)
 template <int D, bool KEYS>
-__global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams p) {
+FV_DEV void packed_sum(const PackedBackParams& p, int block) {
     constexpr int kPiece = KEYS ? kKeys : kRows, kWide = KEYS ? 2 * D : D, kPer = kWide / 4, kSum = 256 / kPer, kPerPiece = kPiece / kSum;
     const BackPlan& plan = KEYS ? p.keys : p.rows;
-    const int c = threadIdx.x % kPer, in = (int)(blockIdx.x % kPerPiece) * kSum + threadIdx.x / kPer, item = blockIdx.x / kPerPiece;
+    const int c = threadIdx.x % kPer, in = block % kPerPiece * kSum + threadIdx.x / kPer, item = block / kPerPiece;
     const int number = item / p.kv_heads, kvh = item - number * p.kv_heads, group = p.group.by;
-    if (number >= plan.counts[1]) return;
     const BackUnit cut = plan.cuts[number];
-    const PackedSeq sq = packed_seq(p.b, cut.seq);
+    if (cut.place == kNoUnit) return;
+    const PackedSeq sq = cut.seq();
     void* out;
     size_t dst;
     if constexpr (KEYS) {
@@ -745,13 +757,19 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams 
     }
     const float* part = plan.places + (((size_t)kvh * plan.most_places + cut.place) * kPiece + in) * kWide + 4 * c;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < cut.shares; s++) {
+    for (int s = 0; s < cut.to; s++) {
         const f32x4 y = *reinterpret_cast<const f32x4*>(part + (size_t)s * kPiece * kWide);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] += y[i];
     }
     if (p.grads_are_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)out + dst) = __builtin_convertvector(x, bf16x4);
     else *reinterpret_cast<f32x4*>((float*)out + dst) = x;
+}
+template <int D>
+__global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams p, int key_blocks) {
+    const int block = blockIdx.x;
+    if (block < key_blocks) packed_sum<D, true>(p, block);
+    else packed_sum<D, false>(p, block - key_blocks);
 }
 
 // A call's plans and its workspace. With a walk cut where it passes the mean load of a slot there are no more shares past the first of a piece than slots, and
@@ -762,7 +780,7 @@ struct BackParts {
     int slots;
     struct Plan {
         PagedPieces pieces;
-        size_t units, cuts, places, least, counts_at, units_at, cuts_at, scratch_at, places_at;
+        size_t units, cuts, places, least, units_at, cuts_at, scratch_at, places_at;
     } keys, rows;
     BackParts(const PackedCall& c, bool round) {
         auto take = [this](size_t n) {
@@ -776,7 +794,7 @@ struct BackParts {
             x.pieces = pieces, x.least = least;
             const size_t n = (size_t)pieces.n.by, more = steps > least ? std::min((size_t)slots / c.kv_heads + 1, n * (steps / least)) : 0;
             x.units = n + more, x.cuts = std::min(n, more), x.places = 2 * more;
-            x.counts_at = take(16), x.units_at = take(x.units * sizeof(BackUnit)), x.cuts_at = take(x.cuts * sizeof(BackUnit)), x.scratch_at = take(n * 8);
+            x.units_at = take(x.units * sizeof(BackUnit)), x.cuts_at = take(x.cuts * sizeof(BackUnit)), x.scratch_at = take(n * 8);
             x.places_at = take(x.places * c.kv_heads * place_bytes);
         };
         stats = take(c.tokens * c.heads * 8);
@@ -785,7 +803,7 @@ struct BackParts {
         plan(rows, paged_pieces(kRows, c.seqs, c.tokens, c.max_q, group), fv_packed_key_steps(c, kRows), 12, kRows * c.d * 4);
     }
     static BackPlan on_device(const Plan& x, uint8_t* ws) {
-        return {x.pieces, (int*)(ws + x.counts_at), (BackUnit*)(ws + x.units_at), (BackUnit*)(ws + x.cuts_at), (int2*)(ws + x.scratch_at), (int)x.units, (int)x.cuts,
+        return {x.pieces, (BackUnit*)(ws + x.units_at), (BackUnit*)(ws + x.cuts_at), (int2*)(ws + x.scratch_at), (int)x.units, (int)x.cuts,
                 (int)x.places, (int)x.least, (float*)(ws + x.places_at)};
     }
 };
@@ -827,7 +845,7 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     const size_t rows = q_tokens * heads, stat_blocks = (rows + 2048 / d - 1) / (2048 / d) + 2;
     const size_t sum_rows = kv_heads * parts.rows.cuts * fv::kRows / (1024 / d), sum_keys = kv_heads * parts.keys.cuts * fv::kKeys / (512 / d);
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
-    if (kv_heads * parts.rows.units >= kMost / 2 || kv_heads * parts.keys.units >= kMost / 2 || stat_blocks >= kMost || sum_rows >= kMost || sum_keys >= kMost)
+    if (kv_heads * (parts.rows.units + parts.keys.units) >= kMost / 2 || stat_blocks >= kMost || sum_rows + sum_keys >= kMost)
         return fv_decline("packed attention backward: too large for one launch");
     uint8_t* ws = (uint8_t*)workspace;
     fv::PackedBackParams p;
@@ -851,16 +869,11 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
                                    (float*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (float)(1.0 / (double)scale), parts.slots);
             });
         });
-        if (k_tokens > 0) {
-            if (fv::KeyForm<D>::kLds > 65536) e = fv_set_max_lds_once((const void*)fv::packed_dkv_kernel<D>, fv::KeyForm<D>::kLds, fv::lds_done);
-            if (e != hipSuccess) return;
-            hipLaunchKernelGGL((fv::packed_dkv_kernel<D>), dim3((unsigned)fv::packed_blocks(p.runs, parts.keys.units)), dim3(256), fv::KeyForm<D>::kLds, st, p);
-            if (parts.keys.cuts > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D, true>), dim3((unsigned)sum_keys), dim3(256), 0, st, p);
-        }
-        if (q_tokens > 0) {
-            hipLaunchKernelGGL((fv::packed_dq_kernel<D>), dim3((unsigned)fv::packed_blocks(p.runs, parts.rows.units)), dim3(256), 4 * fv::TileGeo<D>::kTile, st, p);
-            if (parts.rows.cuts > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D, false>), dim3((unsigned)sum_rows), dim3(256), 0, st, p);
-        }
+        const size_t key_blocks = fv::packed_blocks(p.runs, parts.keys.units), row_blocks = fv::packed_blocks(p.runs, parts.rows.units);
+        if (fv::KeyForm<D>::kLds > 65536) e = fv_set_max_lds_once((const void*)fv::packed_back_kernel<D>, fv::KeyForm<D>::kLds, fv::lds_done);
+        if (e != hipSuccess) return;
+        hipLaunchKernelGGL((fv::packed_back_kernel<D>), dim3((unsigned)(key_blocks + row_blocks)), dim3(256), fv::KeyForm<D>::kLds, st, p, (int)key_blocks);
+        if (sum_keys + sum_rows > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D>), dim3((unsigned)(sum_keys + sum_rows)), dim3(256), 0, st, p, (int)sum_keys);
     });
     if (e == hipSuccess) e = hipGetLastError();
     return e == hipSuccess ? FV_OK : fv_fail_hip(e, "packed_attention_backward");
