@@ -34,6 +34,28 @@ FV_DEV PackedSeq packed_seq(const Batch& b, int s) {
     return {start, min(min(max(b.q_start[s + 1], start), b.tokens) - start, b.max_q), k0, min(min(max(b.k_start[s + 1], k0), b.k_tokens) - k0, b.max_k)};
 }
 
+// The piece of a number and its sequence (of a whole wave). Up to 63 sequences: the starts come with one load of the wave, from which both the search and
+// the sequence are taken.
+struct PackedPiece {
+    PackedSeq seq;
+    int tile;   // (one that the sequence does not have: of an unused number)
+};
+template <int R, class Pieces, class Batch>
+FV_DEV PackedPiece packed_piece(const Pieces& x, const Batch& b, int group, int number) {
+    if (x.tiles.by || b.seqs > 63) {
+        const PagedPiece at = paged_piece<R>(x, b, group, number);
+        return {packed_seq(b, at.seq), at.tile};
+    }
+    const int lane = threadIdx.x & 63, row = b.q_start[min(lane, b.seqs)], key = b.k_start[min(lane, b.seqs)];
+    const long first = ((long)min(max(row, 0), b.tokens) * group + (long)(R - 1) * lane) / R;
+    const int seq = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < b.seqs && first <= number)), 1) - 1;
+    const int q0 = min(max(__builtin_amdgcn_readlane(row, seq), 0), b.tokens), k0 = min(max(__builtin_amdgcn_readlane(key, seq), 0), b.k_tokens);
+    const int q1 = max(__builtin_amdgcn_readlane(row, seq + 1), q0), k1 = max(__builtin_amdgcn_readlane(key, seq + 1), k0);
+    const long tile = number - ((long)q0 * group + (long)(R - 1) * seq) / R;
+    constexpr int kNone = 0x7fffffff / R;
+    return {{q0, min(min(q1, b.tokens) - q0, b.max_q), k0, min(min(k1, b.k_tokens) - k0, b.max_k)}, tile < 0 || tile > kNone ? kNone : (int)tile};
+}
+
 // f(0), f(1), .., f(N - 1) with the numbers as types (loops that the compiler does not unroll in time).
 template <class F, int... I>
 FV_DEV void static_for_each(F&& f, std::integer_sequence<int, I...>) {
@@ -141,7 +163,9 @@ struct PackedRun {
         at = (const uint8_t*)base + (s.k0 + key) * stride_, left = s.len - key;
         step = kTileRows * stride_, gap = (w.b0 - w.ns) * kTileRows, jump = gap * stride_;
     }
-    FV_DEV u32x4 rows(int row_bytes) const { return plane_descriptor(at, (unsigned)(min(max(left, 1), kTileRows) - 1) * stride + (unsigned)row_bytes); }
+    FV_DEV u32x4 rows(int row_bytes, bool any = true) const {   // (none: zeros)
+        return plane_descriptor(at, any && left > 0 ? (unsigned)(min(left, kTileRows) - 1) * stride + (unsigned)row_bytes : 0u);
+    }
     FV_DEV void next() {
         e++;
         at += step, left -= kTileRows;
@@ -154,6 +178,29 @@ FV_DEV void packed_issue(const u32x4& rows, unsigned o0, unsigned o1, unsigned l
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
                  "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds"
                  :: "s"(m0), "v"(o0), "v"(o1), "s"(rows) : "memory");
+}
+
+// A wave's 32 rows in bf16, x[db][g] its lanes' channels 16 db + 4 q4 .. + 3 of row 16 g + i16: through 32 x 2D bytes of LDS of the wave's own, scattered
+// 8-byte pieces in, whole rows out, 16 bytes a lane. dst(row): where a row lies, or null.
+template <int D, class Dst>
+FV_DEV void packed_store_rows(lds_u8* my, const bf16x4 (&x)[D / 16][2], int lane, Dst&& dst) {
+    constexpr int kRowB = 2 * D, kCh = kRowB / 16, kRowsPer = 64 / kCh;
+    const int q4 = lane >> 4, i16 = lane & 15;
+#pragma unroll
+    for (int db = 0; db < D / 16; db++)
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int ch = (2 * db + (q4 >> 1)) ^ (i16 & (kCh - 1));
+            *reinterpret_cast<__attribute__((address_space(3))) bf16x4*>(my + (16 * g + i16) * kRowB + (ch << 4) + 8 * (q4 & 1)) = x[db][g];
+        }
+    // (writes and reads of one wave complete in order; the compiler waits for the reads' data)
+#pragma unroll
+    for (int i = 0; i < 32 / kRowsPer; i++) {
+        const int r = i * kRowsPer + lane / kCh, c = lane % kCh;
+        const u32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(my + r * kRowB + ((c ^ (r & (kCh - 1))) << 4));
+        uint16_t* to = dst(r);
+        if (to) global_store<u32x4>(to + 8 * c, v);
+    }
 }
 
 }  // namespace fv

@@ -56,8 +56,8 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     if (slot_at.head < 0) return true;
     const int kvh = slot_at.head, share = paged_quot(slot_at.number, p.pieces.n);
     const int number = (share + 1) * p.pieces.n.by - 1 - slot_at.number;   // (a sequence's last rows, which see most, first)
-    const PagedPiece piece = paged_piece<kRows>(p.pieces, p.b, p.group.by, number);
-    const PackedSeq sq = packed_seq(p.b, piece.seq);
+    const PackedPiece piece = packed_piece<kRows>(p.pieces, p.b, p.group.by, number);
+    const PackedSeq sq = piece.seq;
     const int rows = sq.count * p.group.by, row0 = piece.tile * kRows;
     if (row0 >= rows) return true;
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
@@ -65,6 +65,19 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     if (share > 0 && e0 >= e1) return true;
     const bool split = w.n > p.chunk;
     const float sl2 = p.sl2;
+
+    unsigned koff[kIter], voff[kIter];
+    packed_offsets<D>(koff, (unsigned)p.k_stride, wave, lane, [](int r) { return G::kswz(r); });
+    packed_offsets<D>(voff, (unsigned)p.v_stride, wave, lane, [](int r) { return G::vswz(r); });
+    const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
+    const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
+    PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
+
+    if (e0 < e1) {   // (the first keys and values on their way before the queries: short walks are mostly this wait)
+        const u32x4 kd = krun.rows(G::kRow), vd = vrun.rows(G::kRow);
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + u * 2048), packed_issue(vd, voff[2 * u], voff[2 * u + 1], slot + 2 * kTile + u * 2048);
+    }
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
     const int wrow = row0 + 32 * wave;
@@ -90,13 +103,11 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     const TileReadBases rb = tile_read_bases<D>(lane);
     auto kbuf = [&](int m) -> lds_u8* { return smem + (m & 1) * kTile; };
     auto vbuf = [&](int m) -> lds_u8* { return smem + (2 + (m & 1)) * kTile; };
-    unsigned koff[kIter], voff[kIter];
-    packed_offsets<D>(koff, (unsigned)p.k_stride, wave, lane, [](int r) { return G::kswz(r); });
-    packed_offsets<D>(voff, (unsigned)p.v_stride, wave, lane, [](int r) { return G::vswz(r); });
-    const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
-    const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
-    PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
-
+    auto dst_row = [&](int r) {   // of the results
+        const int t = paged_quot(r, p.group);
+        return (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
+    };
+    auto part_row = [&](int r) { return (size_t)share * p.part_rows + (size_t)(kvh * p.pieces.n.by + number) * kRows + (r - row0); };
     f32x4 o[kNO][2], s_init[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     SoftmaxOffState st;
     st.init();
@@ -184,29 +195,24 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
 #pragma unroll
     for (int db = 0; db < kNO; db++) o[db][0] = o[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (e0 < e1) {
-        {
-            const u32x4 kd = krun.rows(G::kRow);
-#pragma unroll
-            for (int u = 0; u < kUnits; u++) packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + u * 2048);
-        }
 #pragma unroll
         for (int dk = 0; dk < D / 32; dk++) asm volatile("" : "+v"(qf[dk][0]), "+v"(qf[dk][1]));   // (waited for here, not among the tile loads)
         wait_vmcnt<0>();
         block_barrier();
         constexpr int kAhead = 3;
-        // (past the walk: its last tile again)
-        if (e0 + 1 < e1) krun.next();
-        u32x4 vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow);
+        krun.next(), vrun.next();
+        u32x4 vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow, e0 + 1 < e1);
         auto phase = [&](int m, auto first) {
             const int e = e0 + m;
             ScoreTile s;
             auto hook = [&](int i) {
+                if constexpr (first()) i += kUnits;   // (the first values are there)
                 if (i < kUnits) packed_issue(vd, voff[2 * i], voff[2 * i + 1], slot + (2 + (m & 1)) * kTile + i * 2048);
                 else if (i < 2 * kUnits) packed_issue(kd, koff[2 * (i - kUnits)], koff[2 * (i - kUnits) + 1], slot + ((m + 1) & 1) * kTile + (i - kUnits) * 2048);
             };
             if (idle) {
 #pragma unroll
-                for (int i = 0; i < 2 * kUnits; i++) hook(i);
+                for (int i = 0; i < (first() ? 1 : 2) * kUnits; i++) hook(i);
             } else {
                 __builtin_amdgcn_s_setprio(1);
                 if constexpr (first()) mfma_phase<false, kAhead, D>(vbuf(0), kbuf(0), rb, pb, o, qf, s, s_init, hook);
@@ -219,9 +225,9 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
                 else softmax_tile_off<true>(s, st, o, s_init, sl2, pb);
                 asm volatile("" ::"v"(pb[0][0]), "v"(pb[0][1]), "v"(pb[1][0]), "v"(pb[1][1]), "v"(st.l_acc[0]), "v"(st.l_acc[1]));
             }
-            vrun.next();
-            if (e + 2 < e1) krun.next();
-            vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow);
+            if constexpr (!first()) vrun.next();
+            krun.next();
+            vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow, e + 2 < e1);
             __builtin_amdgcn_sched_barrier(0);
             wait_vmcnt<0>();
             block_barrier();   // K(m + 1), V(m) resident; this phase's tiles read by every wave
@@ -270,29 +276,47 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
             block_barrier();   // (a second pass loads over the votes)
             return false;
         }
+    } else {
+        block_barrier();   // (as the votes' one: the results pass through the V buffers, which every wave has read)
     }
+    float inv[2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         const float l = quad_sum(st.l_acc[g]);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
-        if (r >= rows) continue;
-        const size_t dst = (size_t)(sq.start + t) * p.heads + kvh * p.group.by + (r - t * p.group.by);
-        const size_t part = (size_t)share * p.part_rows + (size_t)(kvh * p.pieces.n.by + number) * kRows + (r - row0);
+        inv[g] = l == 0.f ? 0.f : 1.f / l;
+        const int r = wrow + 16 * g + i16;
+        if (r >= rows || q4 != 0) continue;
         const float lse2 = l == 0.f ? neg_inf() : st.log2_offset<true>(g, sl2) + __log2f(l);
-        if (q4 == 0) {
-            if (split) p.part_lse[part] = lse2;
-            else if (p.lse) p.lse[dst] = lse2 * kLn2;
-        }
+        if (split) p.part_lse[part_row(r)] = lse2;
+        else if (p.lse) p.lse[dst_row(r)] = lse2 * kLn2;
+    }
+    if (!split && p.out_is_bf16) {   // (whole rows: 16 bytes a lane)
+        if (idle) return true;
+        bf16x4 y[kNO][2];
+#pragma unroll
+        for (int db = 0; db < kNO; db++)
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                f32x4 x;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = o[db][g][i] * inv[g];
+                y[db][g] = __builtin_convertvector(x, bf16x4);
+            }
+        packed_store_rows<D>(smem + 2 * kTile + wave * (32 * G::kRow), y, lane,
+                             [&](int r) -> uint16_t* { return wrow + r < rows ? (uint16_t*)p.out + dst_row(wrow + r) * D : nullptr; });
+        return true;
+    }
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const int r = wrow + 16 * g + i16;
+        if (r >= rows) continue;
+        float* to = split ? p.part_o + part_row(r) * D : (float*)p.out + dst_row(r) * D;
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
             f32x4 x;
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = o[db][g][i] * inv;
-            const size_t at = dst * D + 16 * db + 4 * q4;
-            if (split) *reinterpret_cast<f32x4*>(p.part_o + part * D + 16 * db + 4 * q4) = x;
-            else if (p.out_is_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.out + at) = __builtin_convertvector(x, bf16x4);
-            else *reinterpret_cast<f32x4*>((float*)p.out + at) = x;
+            for (int i = 0; i < 4; i++) x[i] = o[db][g][i] * inv[g];
+            *reinterpret_cast<f32x4*>(to + 16 * db + 4 * q4) = x;
         }
     }
     return true;
@@ -319,8 +343,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedAttnParams
     constexpr int kPer = D / 4, kJoin = 256 / kPer, kPerPiece = kRows / kJoin;
     const int c = threadIdx.x % kPer, slot = threadIdx.x / kPer;
     const int item = blockIdx.x / kPerPiece, kvh = paged_quot(item, p.pieces.n), number = item - kvh * p.pieces.n.by;
-    const PagedPiece piece = paged_piece<kRows>(p.pieces, p.b, p.group.by, number);
-    const PackedSeq sq = packed_seq(p.b, piece.seq);
+    const PackedPiece piece = packed_piece<kRows>(p.pieces, p.b, p.group.by, number);
+    const PackedSeq sq = piece.seq;
     const int rows = sq.count * p.group.by, row0 = piece.tile * kRows;
     if (row0 >= rows) return;
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));

@@ -641,6 +641,22 @@ FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int 
         mine = packed_sight(p.mask, sq.pos0 + paged_quot(min(wrow + (lane & 31), rows - 1), p.group), sq.len);
     }
     const PackedWhole whole = packed_whole(w, all_see);
+    unsigned koff[kIter], voff[kIter];
+    packed_offsets<D>(koff, (unsigned)p.k_stride, wave, lane, [](int r) { return both_swz<D>(r); });
+    packed_offsets<D>(voff, (unsigned)p.v_stride, wave, lane, [](int r) { return both_swz<D>(r); });
+    const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
+    const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
+    PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
+    auto load = [&](int buf) {
+        const u32x4 kd = krun.rows(G::kRow), vd = vrun.rows(G::kRow);
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + buf * kTile + u * 2048);
+            packed_issue(vd, voff[2 * u], voff[2 * u + 1], slot + (2 + buf) * kTile + u * 2048);
+        }
+        krun.next(), vrun.next();
+    };
+    if (e0 < e1) load(0);   // (the first keys and values on their way before the queries)
     bf16x8 qf[kNK][2], gf[kNK][2];
     f32x4 s_init[2], d_init[2];
 #pragma unroll
@@ -665,30 +681,11 @@ FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int 
         for (int i = 0; i < 4; i++) s_init[g][i] = nlse, d_init[g][i] = nd;
     }
     const TileReadBases rb = both_bases<D>(lane);
-    unsigned koff[kIter], voff[kIter];
-    packed_offsets<D>(koff, (unsigned)p.k_stride, wave, lane, [](int r) { return both_swz<D>(r); });
-    packed_offsets<D>(voff, (unsigned)p.v_stride, wave, lane, [](int r) { return both_swz<D>(r); });
-    const uint16_t *kbase = p.k + kvh * D, *vbase = p.v + kvh * D;
-    const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
-    PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
-    auto load = [&](int buf) {
-        const u32x4 kd = krun.rows(G::kRow), vd = vrun.rows(G::kRow);
-#pragma unroll
-        for (int u = 0; u < kUnits; u++) {
-            packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + buf * kTile + u * 2048);
-            packed_issue(vd, voff[2 * u], voff[2 * u + 1], slot + (2 + buf) * kTile + u * 2048);
-        }
-        krun.next(), vrun.next();
-    };
     f32x4 dq[kNO][2];
 #pragma unroll
     for (int db = 0; db < kNO; db++) dq[db][0] = dq[db][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the operands and statistics, on every path (as above)
-    if (e0 < e1) {
-        load(0);
-        wait_vmcnt<0>();
-        block_barrier();
-    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the operands and statistics, on every path (as above), and the first tile
+    if (e0 < e1) block_barrier();
 #pragma unroll 1
     for (int e = e0; e < e1; e++) {
         const int buf = (e - e0) & 1;
