@@ -495,28 +495,39 @@ FV_DEV void packed_dkv_item(const PackedBackParams& p, const int wave, const int
         block_barrier();   // the next step resident; this one's read by every wave
         __builtin_amdgcn_sched_barrier(0);
     }
+    auto dst_key = [&](int key) { return ((size_t)(sq.k0 + key) * p.kv_heads + kvh) * D; };
+#pragma unroll
+    for (int db = 0; db < kNO; db++)
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) dk[db][g][i] *= p.scale;
+    if (unit.place < 0 && p.grads_are_bf16) {   // (through the wave's own LDS of its fragments, which are of no more use)
+        if (idle) return;
+        lds_u8* my = smem + wave * F::kFrags * 1024;
+        bf16x4 y[kNO][2];
+        auto rounded = [&](const f32x4 (&x)[kNO][2]) {
+#pragma unroll
+            for (int db = 0; db < kNO; db++)
+#pragma unroll
+                for (int g = 0; g < 2; g++) y[db][g] = __builtin_convertvector(x[db][g], bf16x4);
+        };
+        rounded(dk);
+        packed_store_rows<D>(my, y, lane, [&](int r) -> uint16_t* { return wkey + r < sq.len ? (uint16_t*)p.dk + dst_key(wkey + r) : nullptr; });
+        rounded(dv);
+        packed_store_rows<D>(my, y, lane, [&](int r) -> uint16_t* { return wkey + r < sq.len ? (uint16_t*)p.dv + dst_key(wkey + r) : nullptr; });
+        return;
+    }
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         const int key = wkey + 16 * g + i16;
         if (key >= sq.len) continue;
-        const size_t dst = ((size_t)(sq.k0 + key) * p.kv_heads + kvh) * D;
         float* part = p.keys.places + (((size_t)kvh * p.keys.most_places + max(unit.place, 0)) * kKeys + (key - key0)) * 2 * D;
+        float *to_dk = unit.place >= 0 ? part : (float*)p.dk + dst_key(key), *to_dv = unit.place >= 0 ? part + D : (float*)p.dv + dst_key(key);
 #pragma unroll
         for (int db = 0; db < kNO; db++) {
-            const int at = 16 * db + 4 * q4;
-            f32x4 x = dk[db][g];
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] *= p.scale;
-            if (unit.place >= 0) {
-                *reinterpret_cast<f32x4*>(part + at) = x;
-                *reinterpret_cast<f32x4*>(part + D + at) = dv[db][g];
-            } else if (p.grads_are_bf16) {
-                *reinterpret_cast<bf16x4*>((uint16_t*)p.dk + dst + at) = __builtin_convertvector(x, bf16x4);
-                *reinterpret_cast<bf16x4*>((uint16_t*)p.dv + dst + at) = __builtin_convertvector(dv[db][g], bf16x4);
-            } else {
-                *reinterpret_cast<f32x4*>((float*)p.dk + dst + at) = x;
-                *reinterpret_cast<f32x4*>((float*)p.dv + dst + at) = dv[db][g];
-            }
+            *reinterpret_cast<f32x4*>(to_dk + 16 * db + 4 * q4) = dk[db][g];
+            *reinterpret_cast<f32x4*>(to_dv + 16 * db + 4 * q4) = dv[db][g];
         }
     }
 }
@@ -699,23 +710,36 @@ FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int 
         block_barrier();
         __builtin_amdgcn_sched_barrier(0);
     }
+    auto dst_row = [&](int r) {
+        const int t = paged_quot(r, p.group);
+        return ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D;
+    };
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
-        if (r >= rows) continue;
-        const size_t dst = ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D;
+        const int r = wrow + 16 * g + i16;
         const bool alone = r >= single.lo && r < single.hi;
-        float* part = p.rows.places + (((size_t)kvh * p.rows.most_places + max(unit.place, 0)) * kRows + (r - row0)) * D;
 #pragma unroll
-        for (int db = 0; db < kNO; db++) {
-            const int at = 16 * db + 4 * q4;
-            f32x4 x = dq[db][g];
+        for (int db = 0; db < kNO; db++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = alone ? 0.f : x[i] * p.scale;
-            if (unit.place >= 0) *reinterpret_cast<f32x4*>(part + at) = x;
-            else if (p.grads_are_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)p.dq + dst + at) = __builtin_convertvector(x, bf16x4);
-            else *reinterpret_cast<f32x4*>((float*)p.dq + dst + at) = x;
-        }
+            for (int i = 0; i < 4; i++) dq[db][g][i] = alone ? 0.f : dq[db][g][i] * p.scale;
+    }
+    if (unit.place < 0 && p.grads_are_bf16) {   // (through the tiles' LDS, which every wave has read)
+        if (idle) return;
+        bf16x4 y[kNO][2];
+#pragma unroll
+        for (int db = 0; db < kNO; db++)
+#pragma unroll
+            for (int g = 0; g < 2; g++) y[db][g] = __builtin_convertvector(dq[db][g], bf16x4);
+        packed_store_rows<D>(smem + wave * (32 * G::kRow), y, lane, [&](int r) -> uint16_t* { return wrow + r < rows ? (uint16_t*)p.dq + dst_row(wrow + r) : nullptr; });
+        return;
+    }
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const int r = wrow + 16 * g + i16;
+        if (r >= rows) continue;
+        float* to = unit.place >= 0 ? p.rows.places + (((size_t)kvh * p.rows.most_places + max(unit.place, 0)) * kRows + (r - row0)) * D : (float*)p.dq + dst_row(r);
+#pragma unroll
+        for (int db = 0; db < kNO; db++) *reinterpret_cast<f32x4*>(to + 16 * db + 4 * q4) = dq[db][g];
     }
 }
 
