@@ -31,6 +31,11 @@ def _tokens(t, name, heads, d, device, dtypes=(_BF16,)):
     return h, a if n > 1 else h * d
 
 
+def _like(t, dtype):
+    """An uninitialised contiguous [tokens, heads, d] beside a checked t (empty_like, where it serves, is the shorter call; it lays slices out densely)."""
+    return torch.empty_like(t) if t.dtype is dtype else torch.empty(t.shape, device=t.device, dtype=dtype)
+
+
 def _on(device, name):
     if device < 0:
         raise ValueError(f"{name}: want CUDA tensors")
@@ -103,8 +108,8 @@ def rope_tokens(rope, positions, q, k=None, inverse=False, out_bf16=None, in_pla
         q_out, k_out, qos, kos = q, k, qs, ks
     else:
         dtype = _BF16 if out16 else _F32
-        q_out, qos = torch.empty((tokens, heads, d), device=q.device, dtype=dtype), heads * d
-        k_out, kos = (torch.empty((tokens, kvh, d), device=q.device, dtype=dtype), kvh * d) if k is not None else (None, 0)
+        q_out, qos = _like(q, dtype), heads * d
+        k_out, kos = (_like(k, dtype), kvh * d) if k is not None else (None, 0)
     _lib.check(_lib.lib().fv_rope_tokens(
         q.data_ptr(), qs, q_out.data_ptr(), qos, heads, k.data_ptr() if k is not None else None, ks, k_out.data_ptr() if k is not None else None, kos, kvh, d,
         1 if is16 else 0, 1 if out16 else 0, rope._freq.data_ptr(), rope._pair_axis.data_ptr() if rope._pair_axis is not None else None, rope._rot // 2,
@@ -169,7 +174,7 @@ def packed_attention(q, k, v, seqs, mask=None, causal=True, scale=None, out_bf16
     tokens, keys = q.shape[0], k.shape[0]
     dtype = _BF16 if out_bf16 else _F32
     if out is None:
-        out = torch.empty((tokens, heads, d), device=q.device, dtype=dtype)
+        out = _like(q, dtype)
     else:
         _dense(out, "out", (tokens, heads, d), (dtype,), dev)
     lse = torch.empty((tokens, heads), device=q.device, dtype=_F32) if with_lse else None
@@ -194,8 +199,7 @@ def packed_attention_backward(dout, q, k, v, out, lse, seqs, mask=None, causal=T
     _dense(out, "out", (tokens, heads, d), (_BF16, _F32), dev)
     _dense(lse, "lse", (tokens, heads), (_F32,), dev)
     dtype = _BF16 if grads_bf16 else _F32
-    dq = torch.empty((tokens, heads, d), device=q.device, dtype=dtype)
-    dk, dv = (torch.empty((keys, kvh, d), device=q.device, dtype=dtype) for _ in range(2))
+    dq, dk, dv = _like(q, dtype), _like(k, dtype), _like(v, dtype)
     lib, n, g16 = _lib.lib(), seqs._args[2], 1 if dout.dtype is _BF16 else 0
     numbers = (heads, kvh, d, n, tokens, keys, seqs.max_q, seqs.max_k, 1 if causal else 0, *m)
     nbytes = lib.fv_packed_attention_backward_workspace_bytes(g16, *numbers)
