@@ -4,7 +4,7 @@
 //
 // Rows of one key head lie together (token by token, the heads of its group in turn), so a tile of keys serves a whole group, and a few
 // tokens of many heads fill a tile of rows as well as many tokens of one. Scores, offsets, sums and O are f32; the probabilities are
-// rounded to bf16 for the second product (each off by 2^-9 of itself, as much as a result in bf16 is).
+// rounded to bf16 for the second product (each off by up to 2^-8 of itself, as much as a result in bf16 is).
 #include <limits.h>
 
 #include <algorithm>

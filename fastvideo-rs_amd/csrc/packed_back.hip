@@ -7,7 +7,7 @@
 // order, no atomics and no cleared buffers. S and dP are made twice for that (seven products where five would do): to share them dq
 // would go through memory as f32 sums of every key tile, 512 B a row and 128 keys, at 0.19 us of matrix work for 128 x 128 pairs of five
 // products an atomic stream of 64 KB, in an order that changes. Both statistics ride in the C operands of the products that
-// make S and dP. Sums are f32; P and dS are rounded to bf16 for the second products (2^-9 of each).
+// make S and dP. Sums are f32; P and dS are rounded to bf16 for the second products (up to 2^-8 of each).
 #include <limits.h>
 
 #include <algorithm>

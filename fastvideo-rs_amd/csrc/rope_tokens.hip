@@ -203,7 +203,7 @@ int fv_rope_tokens(const void* q, size_t q_stride, void* q_out, size_t q_out_str
     p.freq = freq, p.pair_axis = pair_axis, p.positions = positions, p.tokens = (long)tokens;
     p.amplitude = amplitude, p.inverse = inverse != 0;
     const size_t run = in_is_bf16 ? 8 : 4, turned = (halves ? pairs : 2 * pairs) / run, units = turned + (d - 2 * pairs) / run, all = heads + kv_heads;
-    if (tokens * units > (size_t)INT_MAX) return fv_decline("rope tokens: too many tokens for one launch");
+    if (tokens * units > (size_t)INT_MAX - 255) return fv_decline("rope tokens: too many tokens for one launch");
     // Heads of a thread: up to 16, so that the angles are a small part of its work; fewer where that leaves units without threads.
     const size_t wanted = (size_t)fv_compute_units() * 1024;
     size_t per = std::min<size_t>(all, 16);

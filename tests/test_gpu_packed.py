@@ -123,6 +123,31 @@ def test_against_64_bits(seqs, mask, heads):
     c.check_backward(out, lse, grads, tag)
 
 
+@pytest.mark.parametrize("heads", [HEADS[1], HEADS[2]], ids=str)
+def test_many_sequences(heads):
+    """More than a wave's lanes have starts, some without rows, some without keys."""
+    rng = np.random.Generator(np.random.PCG64(31))
+    counts = [(int(a), int(a + b)) for a, b in zip(rng.integers(0, 50, 150), rng.integers(-20, 20, 150).clip(0))]
+    announce(f"150 sequences, {heads}")
+    for mask in ("causal", "full"):
+        c = Case(counts, *heads, MASKS[mask], seed=8)
+        out, lse, grads = run_both(c)
+        c.check_forward(out, lse, f"150 sequences {mask}")
+        c.check_backward(out, lse, grads, f"150 sequences {mask} backward")
+
+
+def test_starts_outside_the_tensors():
+    """Starts are bounded to the tensors: the same bits as from starts that end with them."""
+    c = Case([(90, 90), (310, 310), (205, 205)], 6, 2, 64, MASKS["causal"], seed=10, lead=0, trail=0)
+    announce("starts before and behind the tensors")
+    out, lse, grads = run_both(c)
+    starts = torch.tensor([-7, 90, 400, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    c.batch = fv_sdpa.PackedSeqs(starts, 310)
+    again, lse2, grads2 = run_both(c)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again) and torch.equal(lse, lse2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))
+
+
 def run_both(c, **kw):
     out, lse = fv_sdpa.packed_attention(c.q, c.k, c.v, c.batch, with_lse=True, **c.how)
     return out, lse, fv_sdpa.packed_attention_backward(c.dout, c.q, c.k, c.v, out, lse, c.batch, **c.how, **kw)
@@ -201,6 +226,15 @@ def test_second_pass():
             assert torch.equal(again[before], out[before]), "rows before it"
             assert torch.equal(again[int(c.q0[1]):int(c.q0[2])], out[int(c.q0[1]):int(c.q0[2])]), "the other sequence"
             assert not torch.isfinite(again[behind, :2, 5]).any() and torch.isfinite(again[behind, 2:]).all()
+        announce(f"a key that is not a number, d {d}")
+        k = c.k.clone()
+        k[at, 0, 5] = float("nan")
+        again = fv_sdpa.packed_attention(c.q, k, c.v, c.batch)
+        # (either pass is within a half step of its weights and one of its result: 2^-8 + 2^-8 of the largest value)
+        room = 4 * pu.BF16_HALF * c.v[int(c.k0[0]):int(c.k0[-1])].abs().max()
+        inside = slice(int(c.q0[1]), int(c.q0[2]))
+        assert ((again[before].float() - out[before].float()).abs() <= room).all() and torch.equal(again[inside], out[inside])
+        assert again[behind, :2].isnan().all() and torch.equal(again[behind, 2:], out[behind, 2:])
 
 
 def raw_backward(c, out, lse, dq, dk, dv, starts=None, nbytes=None):
@@ -243,7 +277,6 @@ def test_far_tokens():
     for i, x in enumerate((c.q, c.k, c.v)):
         base.view(tokens, wide)[rows, i * 1024:i * 1024 + x.shape[1] * d] = x.reshape(len(rows), -1)
     q, k, v = (base[:, i * 1024:i * 1024 + h * d].unflatten(1, (h, d)) for i, h in enumerate((4, 2, 2)))
-    starts = torch.tensor([0, 190, tokens - 260, tokens], dtype=torch.int32, device="cuda")   # (the middle one is cut to its first rows)
     batch = fv_sdpa.PackedSeqs(torch.tensor([tokens - 260, tokens], dtype=torch.int32, device="cuda"), 260)
     announce("past 4 GB, forward")
     out, lse = fv_sdpa.packed_attention(q, k, v, batch, with_lse=True)
@@ -256,7 +289,6 @@ def test_far_tokens():
     grads = fv_sdpa.packed_attention_backward(dout, q, k, v, out, lse, batch)
     want = fv_sdpa.packed_attention_backward(c.dout, c.q, c.k, c.v, small, small_lse, c.batch)
     torch.cuda.synchronize()
-    del starts
     for a, b in zip(grads, want):
         x, y = a[tokens - 260:].float(), b[190:].float()
         assert (x - y).abs().max() <= 2.0 ** -7 * y.abs().max()   # (cut elsewhere: other sums)
