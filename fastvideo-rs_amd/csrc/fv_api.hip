@@ -464,6 +464,7 @@ int fv_sdpa_init(void) {
     hipError_t e = fv_internal_init_flash();
     if (e == hipSuccess) e = fv_internal_init_vsa();
     if (e == hipSuccess) e = fv_internal_init_composed();
+    if (e == hipSuccess) e = fv_internal_init_packed();
     void* p = nullptr;
     if (e == hipSuccess) e = static_scratch(&p);
     return e == hipSuccess ? FV_OK : fail_hip(e, "fv_sdpa_init");

@@ -76,7 +76,10 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     if (e0 < e1) {   // (the first keys and values on their way before the queries: short walks are mostly this wait)
         const u32x4 kd = krun.rows(G::kRow), vd = vrun.rows(G::kRow);
 #pragma unroll
-        for (int u = 0; u < kUnits; u++) packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + u * 2048), packed_issue(vd, voff[2 * u], voff[2 * u + 1], slot + 2 * kTile + u * 2048);
+        for (int u = 0; u < kUnits; u++) {
+            packed_issue(kd, koff[2 * u], koff[2 * u + 1], slot + u * 2048);
+            packed_issue(vd, voff[2 * u], voff[2 * u + 1], slot + 2 * kTile + u * 2048);
+        }
     }
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)

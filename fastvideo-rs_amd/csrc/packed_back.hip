@@ -83,7 +83,8 @@ FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group)
     return k;
 }
 // The rows of a sequence that see one key, [lo, hi): their weight is 1 and their dS nothing, exactly, where dP - D would leave the rounding of `out`.
-// packed_dkv_item loads zeros for their queries and -lse / scale (scores of 0, a weight of 1, no part in dk), packed_dq_item stores zeros. By token those are the first token's (under a window of one, without a sink, all); by blocks those of a last block of one key under such a window.
+// packed_dkv_item loads zeros for their queries and -lse / scale (scores of 0, a weight of 1, no part in dk), packed_dq_item stores zeros. By
+// token those are the first token's (under a window of one, without a sink, all); by blocks those of a last block of one key under such a window.
 template <class Mask>
 FV_DEV KeySight single_rows(const Mask& m, const PackedSeq& s, int group) {
     const bool alone = m.window == 1 && m.sink == 0;
@@ -262,8 +263,9 @@ __global__ __launch_bounds__(256) void packed_stats_kernel(const PackedBackParam
 
 // ---- the keys' gradients ---------------------------------------------------------------------------------------------
 
-// A wave's part in a step of 32 rows at `qt` and `gt` (q and dout), `cut`: with keys that rows do not see, whose scores become -inf. The products, two to a unit that shares an operand read: S = Q K^T - lse / scale, 16 rows after 16; dP = dO V^T - D; dV^T += dO^T P; dK^T += Q^T dS. The vector work lies
-// in their shadow: a 16x16x32 product holds the matrix pipe for four instructions' time, of which two others of the same wave cost
+// A wave's part in a step of 32 rows at `qt` and `gt` (q and dout), `cut`: with keys that rows do not see, whose scores become -inf. The
+// products, two to a unit that shares an operand read: S = Q K^T - lse / scale, 16 rows after 16; dP = dO V^T - D; dV^T += dO^T P; dK^T += Q^T dS.
+// The vector work lies in their shadow: a 16x16x32 product holds the matrix pipe for four instructions' time, of which two others of the same wave cost
 // nothing (measured, with one wave a SIMD: 8.1 ns a product with none, 8.7 with two multiplications, 10.3 with three; an exponential counts for two). So the
 // exponentials of the first 16 rows run under the scores of the others and dP, dS under dV. With the softmax by itself between dP and dV: 5 to 6 %
 // slower. Operands are read three units ahead: one, 15 % slower; four need registers that are not there.
@@ -347,8 +349,8 @@ FV_DEV void key_step(const lds_u8* qt, const lds_u8* gt, const lds_u8* vt, const
 }
 
 // 128 keys of one (sequence, key head), 32 a wave, over steps of 32 rows of q and dout that pass through LDS, two buffers each (three, a step's
-// rows on their way for two: 6 to 9 % slower). A lane has two keys (columns lane % 16 and 16 + lane % 16 of its wave's): S and dP [rows x keys] come out of the products in the layout that the second ones take P and dS in, and dV^T, dK^T [d x keys] stay in 128
-// registers (64 at 64 channels). K's operands stay in registers, V's in LDS as they are read: an operand is read once for two products, and an LDS
+// rows on their way for two: 6 to 9 % slower). A lane has two keys (columns lane % 16 and 16 + lane % 16 of its wave's): S and dP [rows x keys]
+// come out of the products in the layout that the second ones take P and dS in, and dV^T, dK^T [d x keys] stay in 128 registers (64 at 64 channels). K's operands stay in registers, V's in LDS as they are read: an operand is read once for two products, and an LDS
 // read a product costs nothing (at two waves a SIMD 1706 and 1715 TFLOP/s of 16x16x32 with half a ds_read_b128 each and one).
 template <int D>
 FV_DEV void packed_dkv_item(const PackedBackParams& p, const int wave, const int lane, const int block) {
@@ -793,9 +795,9 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams 
     else packed_sum<D, false>(p, block - key_blocks);
 }
 
-// A call's plans and its workspace. With a walk cut where it passes the mean load of a slot there are no more shares past the first of a piece than slots, and
-// no more places than twice as many; walks of no more than `least` steps are not cut: a share costs its place's traffic (of 128 keys 256 KB, of 128 rows 128), some 18
-// steps of 32 rows or 8 tiles.
+// A call's plans and its workspace. With a walk cut where it passes the mean load of a slot there are no more shares past the first of a piece
+// than slots, and no more places than twice as many; walks of no more than `least` steps are not cut: a share costs its place's traffic (of 128
+// keys 256 KB, of 128 rows 128), some 18 steps of 32 rows or 8 tiles.
 struct BackParts {
     size_t stats = 0, rounded = 0, bytes = 0;   // bytes from the workspace's start
     int slots;
@@ -828,10 +830,17 @@ struct BackParts {
                 (int)x.places, (int)x.least, (float*)(ws + x.places_at)};
     }
 };
-std::atomic<unsigned long long> lds_done{0};   // (of the one kernel that takes more than 64 KB)
+// (the one kernel here that takes more than 64 KB)
+hipError_t packed_prepare() {
+    static std::atomic<unsigned long long> done{0};
+    static_assert(KeyForm<64>::kLds <= 65536, "no attribute");
+    return fv_set_max_lds_once((const void*)packed_back_kernel<128>, KeyForm<128>::kLds, done);
+}
 
 }  // namespace
 }  // namespace fv
+
+extern "C" hipError_t fv_internal_init_packed(void) { return fv::packed_prepare(); }
 
 extern "C" {
 
@@ -891,7 +900,7 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
             });
         });
         const size_t key_blocks = fv::packed_blocks(p.runs, parts.keys.units), row_blocks = fv::packed_blocks(p.runs, parts.rows.units);
-        if (fv::KeyForm<D>::kLds > 65536) e = fv_set_max_lds_once((const void*)fv::packed_back_kernel<D>, fv::KeyForm<D>::kLds, fv::lds_done);
+        if (D == 128) e = fv::packed_prepare();
         if (e != hipSuccess) return;
         hipLaunchKernelGGL((fv::packed_back_kernel<D>), dim3((unsigned)(key_blocks + row_blocks)), dim3(256), fv::KeyForm<D>::kLds, st, p, (int)key_blocks);
         if (sum_keys + sum_rows > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D>), dim3((unsigned)(sum_keys + sum_rows)), dim3(256), 0, st, p, (int)sum_keys);
