@@ -111,7 +111,7 @@ FV_DEV PackedWhole packed_whole(const PackedWalk& w, const PagedSight& all) {
 
 // Workgroups to pieces: 2^xcds XCDs take the pieces of a run of whole key heads, in turn, so that an L2 holds few heads' tensors. Under a causal mask the
 // heads' pieces follow each other by number, so that the longest walks of all come first (one clip of 7 frames, 12 heads, three a run: 13 % over even
-// shares of the work instead of 36 %); where walks are alike, head by head (two clips, 12 heads, forward: 740 us, by number 768).
+// shares of the work instead of 36 %); where walks are alike, head by head (two clips, 12 heads, forward: 727 us, by number 751).
 struct PackedRuns {
     PagedDiv heads;   // of a run
     int xcds, by_head;

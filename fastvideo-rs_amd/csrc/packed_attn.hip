@@ -41,6 +41,9 @@ struct PackedAttnParams {
 // 128 rows of one (sequence, key head), 32 a wave, over tiles of 64 keys that pass through LDS as in the dense kernels
 // (attn_core.h): two buffers for K, two for V, so that a unit holds two workgroups, whose matrix and vector phases fall beside each other.
 // A phase is one key tile: O += P V of the tile before and S = K Q^T with the next K and this V on their way in, the softmax, one barrier.
+// (Three buffers of 64 channels, loads a phase earlier: the same time. What bounds it: long walks of 128 channels the chip's power limit, 1.2 to
+// 1.28 PFLOP/s; of 64 channels the softmax, 1.0 PFLOP/s; walks of a few tiles their ends, of 15 us for 8 tiles of 64 channels 1.6 to the piece,
+// 0.7 to its loads, 1.8 for them and 1.9 from the last scores to the stores.)
 // FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop). Exact as
 // long as nothing overflows or vanishes, which is checked before anything is stored: the sum of every row that sees a key of the
 // walk within 2^-60 .. 2^100 and its values finite, or the workgroup makes the pass again with the running maximum and an eye on
