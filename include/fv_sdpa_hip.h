@@ -423,6 +423,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
  * sees key j as in fv_paged_attention: ti = i / block_tokens, tj <= ti && (window == 0 || ti - tj < window || tj < sink). A row that sees no key
  * (a sequence without keys, or with more rows than keys) is zeros, with lse -inf and no gradient. What a row does not see does not
  * reach its result, whatever is stored there; the gradients of a sequence are numbers only where all its operands are.
+ * A row that sees one key has no gradient by its score, exactly. Outputs may not overlap inputs or each other.
  *
  * out [q_tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale q k^T) v; lse (NULL: not wanted) f32 [q_tokens, heads] = the natural
  * logarithm of sum e^(scale q k^T). Results are the same bits from call to call with the same bounds and workspace.
