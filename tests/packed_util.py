@@ -60,6 +60,8 @@ def gradients(q, k, v, dout, out, lse, seen, scale):
     dp = _products(dout, v)
     delta = (dout * out).sum(1, keepdims=True)
     ds = p * (dp - delta)
+    # a row that sees one key: its weight is 1 whatever the score, so dS is 0, where the rounding of the given result would leave some 2^-8 of dp
+    ds = np.where(seen.sum(1, keepdims=True) == 1, 0.0, ds)
     dq, dk, dv = ds @ k * scale, ds.T @ q * scale, p.T @ dout
     # P: its score's error, -lse's rounding and the exponential's; dP - D: products in f32
     off = _score_error(q, k, scale, seen) + 2 * F32_HALF * np.abs(np.where(np.isfinite(lse), lse, 0.0))[:, None] + 2.0 ** -20

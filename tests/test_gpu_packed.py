@@ -186,7 +186,8 @@ def test_types(d):
 
 
 @pytest.mark.parametrize("causal,block,window,sink,seqs", [
-    (True, 1, 0, 0, [(1, 1)] * 9), (False, 1, 0, 0, [(7, 1), (130, 1)]), (True, 1, 1, 0, [(200, 200), (3, 40)]), (True, 4, 1, 0, [(65, 65), (1, 129)])])
+    (True, 1, 0, 0, [(1, 1)] * 9), (False, 1, 0, 0, [(7, 1), (130, 1)]), (True, 1, 1, 0, [(200, 200), (3, 40)]), (True, 4, 1, 0, [(65, 65), (1, 129)]),
+    (True, 1, 1, 0, [(700, 500), (40, 900)])])
 def test_rows_that_see_one_key(causal, block, window, sink, seqs):
     """Their scores have no gradient: exact zeros, and the values' gradient is that of the results."""
     announce(f"{causal} {block} {window} {sink} {seqs}")
