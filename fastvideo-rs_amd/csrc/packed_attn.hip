@@ -456,7 +456,7 @@ int fv_packed_args(const char* who, const PackedCall& c, const PackedOperand* x,
     if (c.heads > 65535) return say("too many heads", true);
     if (c.seqs > kMostSeqs || c.tokens > kMostRows || c.k_tokens > kMostRows || c.tokens * (c.heads / c.kv_heads) > (size_t)INT_MAX / 2)
         return say("too many sequences or rows for one launch", true);
-    if (!(c.scale > 0.f) || !(c.scale <= 2e38f)) return say("scale must be positive and finite", true);
+    if (!(c.scale >= 1e-30f) || !(c.scale <= 1e30f)) return say("scale must lie within 1e-30 and 1e30", true);   // (the gradients' lse / scale is a number)
     if (c.causal && c.block_tokens == 0) return say("block_tokens must be positive", false);
     if (c.causal && !mask_fits(c)) return say("mask too large", true);
     for (size_t i = 0; i < operands; i++) {

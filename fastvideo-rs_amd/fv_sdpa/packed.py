@@ -1,5 +1,6 @@
 """Training on packed sequences (include/fv_sdpa_hip.h, `fv_packed_*`, `fv_rope_*`; no counterpart in the reference): sequences of different
-lengths one behind the other, attention with shared key heads inside each of them, its gradients, and rotary positions without tables.
+lengths one behind the other, attention with shared key heads inside each of them, its gradients, and rotary positions without tables. They
+record no graph: a caller's autograd function calls them.
 """
 import ctypes as C
 import math

@@ -425,7 +425,7 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
  * reach its result, whatever is stored there; the gradients of a sequence are numbers only where all its operands are.
  * A row that sees one key has no gradient by its score, exactly. Outputs may not overlap inputs or each other.
  *
- * out [q_tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale q k^T) v; lse (NULL: not wanted) f32 [q_tokens, heads] = the natural
+ * out [q_tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale q k^T) v, scale within 1e-30 and 1e30; lse (NULL: not wanted) f32 [q_tokens, heads] = the natural
  * logarithm of sum e^(scale q k^T). Results are the same bits from call to call with the same bounds and workspace.
  * workspace: fv_packed_attention_workspace_bytes of the same numbers (0: none), 256-byte aligned, this call's alone until its work is done; too small or
  * NULL: walks are not split among workgroups, which costs time only. */

@@ -185,6 +185,18 @@ def test_types(d):
         assert torch.equal(a[at], b[at].bfloat16())
 
 
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 3.0, 50.0])
+def test_scales(scale):
+    """Nearly even weights to one key a row (and the pass with the running maximum)."""
+    announce(f"scale {scale}")
+    c = Case(SEQS["long"], 4, 2, 64, MASKS["causal"], seed=12)
+    c.scale = scale
+    out, lse = fv_sdpa.packed_attention(c.q, c.k, c.v, c.batch, scale=scale, with_lse=True)
+    c.check_forward(out, lse, f"scale {scale}")
+    grads = fv_sdpa.packed_attention_backward(c.dout, c.q, c.k, c.v, out, lse, c.batch, scale=scale)
+    c.check_backward(out, lse, grads, f"scale {scale} backward")
+
+
 @pytest.mark.parametrize("causal,block,window,sink,seqs", [
     (True, 1, 0, 0, [(1, 1)] * 9), (False, 1, 0, 0, [(7, 1), (130, 1)]), (True, 1, 1, 0, [(200, 200), (3, 40)]), (True, 4, 1, 0, [(65, 65), (1, 129)]),
     (True, 1, 1, 0, [(700, 500), (40, 900)])])

@@ -53,7 +53,7 @@ BOTH = ["fv_packed_attention", "fv_packed_attention_backward"]
     (dict(d=96), DECLINED, "head dim"), (dict(d=0), DECLINED, "head dim"), (dict(d=256), DECLINED, "head dim"),
     (dict(heads=65536, q_stride=65536 * 128), DECLINED, "too many heads"), (dict(seqs=1 << 25), DECLINED, "too many"), (dict(q_tokens=1 << 27), DECLINED, "too many"),
     (dict(k_tokens=1 << 27), DECLINED, "too many"), (dict(q_tokens=1 << 26, heads=64, q_stride=64 * 128), DECLINED, "too many"),
-    (dict(scale=0.0), DECLINED, "scale"), (dict(scale=-1.0), DECLINED, "scale"), (dict(scale=float("nan")), DECLINED, "scale"), (dict(scale=float("inf")), DECLINED, "scale"),
+    (dict(scale=0.0), DECLINED, "scale"), (dict(scale=-1.0), DECLINED, "scale"), (dict(scale=float("nan")), DECLINED, "scale"), (dict(scale=float("inf")), DECLINED, "scale"), (dict(scale=1e-31), DECLINED, "scale"), (dict(scale=1e31), DECLINED, "scale"),
     (dict(block_tokens=0), INVALID, "block_tokens"), (dict(window=1 << 31), DECLINED, "mask too large"), (dict(sink=1 << 31), DECLINED, "mask too large"),
     (dict(q=P + 8), INVALID, "16-byte aligned"), (dict(v=P + 2), INVALID, "16-byte aligned"), (dict(out=P + 4), INVALID, "16-byte aligned"),
     (dict(q_stride=504), INVALID, "tokens overlap"), (dict(k_stride=0), INVALID, "tokens overlap"), (dict(v_stride=260), DECLINED, "multiples of 8"),
