@@ -41,7 +41,8 @@ struct PackedAttnParams {
 // 128 rows of one (sequence, key head), 32 a wave, over tiles of 64 keys that pass through LDS as in the dense kernels
 // (attn_core.h): two buffers for K, two for V, so that a unit holds two workgroups, whose matrix and vector phases fall beside each other.
 // A phase is one key tile: O += P V of the tile before and S = K Q^T with the next K and this V on their way in, the softmax, one barrier.
-// (Three buffers of 64 channels, loads a phase earlier: the same time. What bounds it: long walks of 128 channels the chip's power limit, 1.2 to
+// (The softmax dealt out over the gaps between the products, as in the gradients: 4 % slower, the other workgroup's wave fills them better. Three
+// buffers of 64 channels, loads a phase earlier: the same time. What bounds it: long walks of 128 channels the chip's power limit, 1.2 to
 // 1.28 PFLOP/s; of 64 channels the softmax, 1.0 PFLOP/s; walks of a few tiles their ends, of 15 us for 8 tiles of 64 channels 1.6 to the piece,
 // 0.7 to its loads, 1.8 for them and 1.9 from the last scores to the stores.)
 // FIXED: a row's softmax offset stays at the largest score of the first tile (no row maximum and no rescale decision in the loop). Exact as
@@ -205,7 +206,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
         for (int dk = 0; dk < D / 32; dk++) asm volatile("" : "+v"(qf[dk][0]), "+v"(qf[dk][1]));   // (waited for here, not among the tile loads)
         wait_vmcnt<0>();
         block_barrier();
-        constexpr int kAhead = 3;
+        constexpr int kAhead = 4;   // (three: 0.6 % slower, eight 1.2 %)
         krun.next(), vrun.next();
         u32x4 vd = vrun.rows(G::kRow), kd = krun.rows(G::kRow, e0 + 1 < e1);
         auto phase = [&](int m, auto first) {
