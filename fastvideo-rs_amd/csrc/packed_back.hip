@@ -33,7 +33,7 @@ struct BackPlan {
     PagedPieces pieces;
     BackUnit *units, *cuts;   // (behind the last: kNoUnit)
     int2* scratch;       // every piece number's sequence and steps
-    int most_units, most_cuts, most_places, least;   // of a key head; steps below which no walk is cut
+    int most_units, most_cuts, most_places;   // of a key head
     float* places;
 };
 
@@ -128,71 +128,103 @@ FV_DEV int back_steps(const PackedBackParams& p, const PackedSeq& sq, int tile) 
         return packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group)).n;
     }
 }
-// One workgroup makes a plan: the walks' lengths; their sum, and from it the mean load of a slot, past which a walk is cut into equal shares; the units
+// Steps below which no walk is cut; a step of a row's walk (64 keys x 128 rows, three products) in steps of a key's (128 keys x 32 rows, four); what a
+// share costs: with S steps in all, shares of A steps take A steps' time and leave S / A places, each 1 / kShares of a step for its traffic (of 128
+// keys 256 KB, of 128 rows 128), which is least for A = sqrt(S / kShares). (Five sequences of some 100 rows and keys, 16 heads on one: 50 -> 32 us.)
+constexpr int kLeastKeys = 4, kLeastRows = 3, kSharesKeys = 10, kSharesRows = 25;
+constexpr float kRowStep = 1.5f;
+// The first piece of a sequence; the sequence and the steps of a piece (steps < 0: of an unused number).
+template <bool KEYS>
+FV_DEV long plan_first(const PackedBackParams& p, const PackedBatch& b, const BackPlan& plan, int seq) {
+    constexpr int R = KEYS ? kKeys : kRows;
+    const PackedKeys kb = {b.k_start, b.seqs, b.k_tokens};
+    return KEYS ? paged_first_piece<R>(plan.pieces, kb, 1, seq) : paged_first_piece<R>(plan.pieces, b, p.group.by, seq);
+}
+template <bool KEYS>
+FV_DEV int2 plan_piece(const PackedBackParams& p, const PackedBatch& b, const BackPlan& plan, int n) {
+    constexpr int R = KEYS ? kKeys : kRows;
+    auto first_of = [&](int seq) { return plan_first<KEYS>(p, b, plan, seq); };
+    int seq = 0;
+    if (plan.pieces.tiles.by) {
+        seq = paged_quot(n, plan.pieces.tiles);
+    } else {
+        int behind = b.seqs;   // the last of sequences seq .. behind - 1 whose first piece is no later
+        while (behind - seq > 1) {
+            const int mid = seq + (behind - seq) / 2;
+            if (first_of(mid) <= n) seq = mid;
+            else behind = mid;
+        }
+    }
+    const long tile = n - first_of(seq);
+    return {seq, tile < 0 || tile > 0x7fffffff / R ? -1 : back_steps<KEYS>(p, packed_seq(b, seq), (int)tile)};
+}
+// One workgroup makes a plan: the walks' lengths; their sum, and from it the length past which a walk is cut into equal shares; the units
 // sorted by their lengths into 64 classes, longest first (in a class in any order: it changes no result). By itself the order of the pieces left slots idle
 // for a third of the time (one clip of 7 frames, 12 heads, 1032 pieces on 512 slots) or for two thirds (a window with a sink, whose keys all rows see).
+// The rows' walks are cut past their mean load of a slot, the keys' past the mean load of both kinds, since the rows' units come behind and fill
+// what is idle (21 prompts of up to 702 tokens, 32 / 8 heads: 227 -> 206 us).
 template <bool KEYS>
 FV_DEV void plan_pieces(const PackedBackParams& p, const BackPlan& plan, int slots) {
-    constexpr int kClasses = 64;
-    __shared__ unsigned long long sum;
-    __shared__ int longest, units[kClasses], cuts, places, total;
+    constexpr int kClasses = 64, kHeld = 1024;
+    __shared__ unsigned long long sum, others;
+    __shared__ int longest, units[kClasses], cuts, places, total, held[2][kHeld];
     const int tid = threadIdx.x, numbers = plan.pieces.n.by;
-    if (tid == 0) sum = 0, longest = 0, cuts = 0, places = 0;
+    if (tid == 0) sum = 0, others = 0, longest = 0, cuts = 0, places = 0;
     if (tid < kClasses) units[tid] = 0;
+    PackedBatch b = p.b;
+    if (b.seqs < kHeld) {   // (a search makes a chain of reads: from LDS)
+        for (int i = tid; i <= b.seqs; i += 256) held[0][i] = b.q_start[i], held[1][i] = b.k_start[i];
+        b.q_start = held[0], b.k_start = held[1];
+    }
     __syncthreads();
-    const PackedKeys kb = {p.b.k_start, p.b.seqs, p.b.k_tokens};
-    const int group = KEYS ? 1 : p.group.by;
-    constexpr int R = KEYS ? kKeys : kRows;
-    auto first_of = [&](int seq) { return KEYS ? paged_first_piece<R>(plan.pieces, kb, group, seq) : paged_first_piece<R>(plan.pieces, p.b, group, seq); };
-    unsigned long long mine = 0;
+    unsigned long long mine = 0, theirs = 0;
     int most = 0;
-    for (int n = tid; n < numbers; n += 256) {
-        int seq = 0;
-        if (plan.pieces.tiles.by) {
-            seq = paged_quot(n, plan.pieces.tiles);
-        } else {
-            int behind = p.b.seqs;   // the last of sequences seq .. behind - 1 whose first piece is no later
-            while (behind - seq > 1) {
-                const int mid = seq + (behind - seq) / 2;
-                if (first_of(mid) <= n) seq = mid;
-                else behind = mid;
-            }
+    const int rows_at = (numbers + 63) & ~63;   // (the other kind in the same turns, by other waves)
+    for (int n = tid; n < (KEYS ? rows_at + p.rows.pieces.n.by : numbers); n += 256) {
+        if (n < numbers) {
+            const int2 x = plan_piece<KEYS>(p, b, plan, n);
+            plan.scratch[n] = x;
+            mine += (unsigned long long)max(x.y, 0), most = max(most, x.y);
+        } else if (n >= rows_at) {
+            theirs += (unsigned long long)max(plan_piece<false>(p, b, p.rows, n - rows_at).y, 0);
         }
-        const long tile = n - first_of(seq);
-        const int steps = tile < 0 || tile > 0x7fffffff / R ? -1 : back_steps<KEYS>(p, packed_seq(p.b, seq), (int)tile);
-        plan.scratch[n] = int2{seq, steps};
-        mine += (unsigned long long)max(steps, 0), most = max(most, steps);
     }
     atomicAdd(&sum, mine);
     atomicMax(&longest, most);
+    if constexpr (KEYS) atomicAdd(&others, theirs);
     __syncthreads();
-    const int load = max(plan.least, (int)min((sum * p.kv_heads + slots - 1) / slots, 0x7fffffffull));
+    const float all = (float)sum * (float)p.kv_heads, behind = KEYS ? kRowStep * (float)others * (float)p.kv_heads : 0.f;
+    const float least = __builtin_sqrtf(all / (KEYS ? kSharesKeys : kSharesRows));
+    const int load = (int)min(max(max((all + behind) / (float)slots, least) + 1.f, (float)(KEYS ? kLeastKeys : kLeastRows)), 1e9f);
     auto shares_of = [&](int steps) { return steps > load ? (steps + load - 1) / load : 1; };
-    const int top = min(longest, load) + 1;
-    auto class_of = [&](int steps, int shares) { return kClasses - 1 - (int)((long)((steps + shares - 1) / shares) * kClasses / top); };   // 0: the longest
+    const float per_step = (float)kClasses / (float)(min(longest, load) + 1);
+    auto class_of = [&](int chunk) { return kClasses - 1 - min((int)((float)chunk * per_step), kClasses - 1); };   // 0: the longest
+    auto chunk_of = [](int steps, int shares) { return shares == 1 ? steps : (steps + shares - 1) / shares; };
     for (int n = tid; n < numbers; n += 256) {
         const int steps = plan.scratch[n].y;
         if (steps < 0) continue;
         const int k = shares_of(steps);
-        atomicAdd(&units[class_of(steps, k)], k);
+        atomicAdd(&units[class_of(chunk_of(steps, k))], k);
     }
     __syncthreads();
-    if (tid == 0) {
-        int at = 0;
-        for (int c = 0; c < kClasses; c++) {
-            const int n = units[c];
-            units[c] = at;
-            at += n;
+    if (tid < kClasses) {   // (a wave)
+        const int n = units[tid];
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < kClasses; d <<= 1) {
+            const int x = __shfl_up(upto, d, 64);
+            upto += tid >= d ? x : 0;
         }
-        total = at;
+        units[tid] = upto - n;
+        if (tid == kClasses - 1) total = upto;
     }
     __syncthreads();
     for (int n = tid; n < numbers; n += 256) {
         const int2 x = plan.scratch[n];
         if (x.y < 0) continue;
-        const PackedSeq sq = packed_seq(p.b, x.x);
-        const int k = shares_of(x.y), chunk = (x.y + k - 1) / k, tile = (int)(n - first_of(x.x));
-        int u = atomicAdd(&units[class_of(x.y, k)], k), place = -1;
+        const PackedSeq sq = packed_seq(b, x.x);
+        const int k = shares_of(x.y), chunk = chunk_of(x.y, k), tile = (int)(n - plan_first<KEYS>(p, b, plan, x.x));
+        int u = atomicAdd(&units[class_of(chunk)], k), place = -1;
         if (k > 1) {
             const int c = atomicAdd(&cuts, 1);
             place = atomicAdd(&places, k);
@@ -753,57 +785,61 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_back_kernel(const
     else packed_dq_item<D>(p, wave, lane, block - key_blocks);
 }
 
-// The shares of cut walks, added in their order: D / 4 threads a row of dq or (KEYS) twice as many a key, dk and dv. (The grid is that of as many cut
-// pieces as there may be.)
+// The shares of cut walks, added in their order: D / 4 threads a row of dq or (KEYS) twice as many a key, dk and dv, `per` rows or keys a workgroup. (The
+// grid is that of as many cut pieces as there may be.)
 template <int D, bool KEYS>
-FV_DEV void packed_sum(const PackedBackParams& p, int block) {
-    constexpr int kPiece = KEYS ? kKeys : kRows, kWide = KEYS ? 2 * D : D, kPer = kWide / 4, kSum = 256 / kPer, kPerPiece = kPiece / kSum;
+FV_DEV void packed_sum(const PackedBackParams& p, int block, int per) {
+    constexpr int kPiece = KEYS ? kKeys : kRows, kWide = KEYS ? 2 * D : D, kPer = kWide / 4, kSum = 256 / kPer, kAtOnce = 4;
     const BackPlan& plan = KEYS ? p.keys : p.rows;
-    const int c = threadIdx.x % kPer, in = block % kPerPiece * kSum + threadIdx.x / kPer, item = block / kPerPiece;
+    const int c = threadIdx.x % kPer, parts = kPiece / per, item = block / parts, in0 = (block - item * parts) * per;
     const int number = item / p.kv_heads, kvh = item - number * p.kv_heads, group = p.group.by;
     const BackUnit cut = plan.cuts[number];
     if (cut.place == kNoUnit) return;
     const PackedSeq sq = cut.seq();
-    void* out;
-    size_t dst;
-    if constexpr (KEYS) {
-        const int key = cut.tile * kKeys + in;
-        if (key >= sq.len) return;
-        out = 4 * c < D ? p.dk : p.dv;
-        dst = ((size_t)(sq.k0 + key) * p.kv_heads + kvh) * D + 4 * c % D;
-    } else {
-        const int r = cut.tile * kRows + in;
-        if (r >= sq.count * group) return;
-        const int t = paged_quot(r, p.group);
-        out = p.dq;
-        dst = ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D + 4 * c;
-    }
-    const float* part = plan.places + (((size_t)kvh * plan.most_places + cut.place) * kPiece + in) * kWide + 4 * c;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < cut.to; s++) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(part + (size_t)s * kPiece * kWide);
+    const int rows = KEYS ? sq.len : sq.count * group;
+    for (int in = in0 + threadIdx.x / kPer; in < in0 + per; in += kSum) {
+        const int r = cut.tile * kPiece + in;
+        if (r >= rows) return;
+        const float* part = plan.places + (((size_t)kvh * plan.most_places + cut.place) * kPiece + in) * kWide + 4 * c;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < cut.to; s += kAtOnce) {
+            f32x4 y[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] += y[i];
+            for (int u = 0; u < kAtOnce; u++) y[u] = *reinterpret_cast<const f32x4*>(part + (size_t)min(s + u, cut.to - 1) * kPiece * kWide);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] += s + u < cut.to ? y[u][i] : 0.f;
+        }
+        void* out;
+        size_t dst;
+        if constexpr (KEYS) {
+            out = 4 * c < D ? p.dk : p.dv;
+            dst = ((size_t)(sq.k0 + r) * p.kv_heads + kvh) * D + 4 * c % D;
+        } else {
+            const int t = paged_quot(r, p.group);
+            out = p.dq;
+            dst = ((size_t)(sq.start + t) * p.heads + kvh * group + (r - t * group)) * D + 4 * c;
+        }
+        if (p.grads_are_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)out + dst) = __builtin_convertvector(x, bf16x4);
+        else *reinterpret_cast<f32x4*>((float*)out + dst) = x;
     }
-    if (p.grads_are_bf16) *reinterpret_cast<bf16x4*>((uint16_t*)out + dst) = __builtin_convertvector(x, bf16x4);
-    else *reinterpret_cast<f32x4*>((float*)out + dst) = x;
 }
 template <int D>
-__global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams p, int key_blocks) {
+__global__ __launch_bounds__(256) void packed_sum_kernel(const PackedBackParams p, int key_blocks, int per) {
     const int block = blockIdx.x;
-    if (block < key_blocks) packed_sum<D, true>(p, block);
-    else packed_sum<D, false>(p, block - key_blocks);
+    if (block < key_blocks) packed_sum<D, true>(p, block, per);
+    else packed_sum<D, false>(p, block - key_blocks, per);
 }
 
 // A call's plans and its workspace. With a walk cut where it passes the mean load of a slot there are no more shares past the first of a piece
-// than slots, and no more places than twice as many; walks of no more than `least` steps are not cut: a share costs its place's traffic (of 128
-// keys 256 KB, of 128 rows 128), some 18 steps of 32 rows or 8 tiles.
+// than slots, and no more places than twice as many; walks of no more than `least` steps are not cut.
 struct BackParts {
     size_t stats = 0, rounded = 0, bytes = 0;   // bytes from the workspace's start
     int slots;
     struct Plan {
         PagedPieces pieces;
-        size_t units, cuts, places, least, units_at, cuts_at, scratch_at, places_at;
+        size_t units, cuts, places, units_at, cuts_at, scratch_at, places_at;
     } keys, rows;
     BackParts(const PackedCall& c, bool round) {
         auto take = [this](size_t n) {
@@ -814,7 +850,7 @@ struct BackParts {
         slots = (c.d == 64 ? 3 : 2) * fv_compute_units();
         const size_t group = c.heads / c.kv_heads;
         auto plan = [&](Plan& x, const PagedPieces& pieces, size_t steps, size_t least, size_t place_bytes) {
-            x.pieces = pieces, x.least = least;
+            x.pieces = pieces;
             const size_t n = (size_t)pieces.n.by, more = steps > least ? std::min((size_t)slots / c.kv_heads + 1, n * (steps / least)) : 0;
             x.units = n + more, x.cuts = std::min(n, more), x.places = 2 * more;
             x.units_at = take(x.units * sizeof(BackUnit)), x.cuts_at = take(x.cuts * sizeof(BackUnit)), x.scratch_at = take(n * 8);
@@ -822,12 +858,12 @@ struct BackParts {
         };
         stats = take(c.tokens * c.heads * 8);
         if (round) rounded = take(c.tokens * c.heads * c.d * 2);
-        plan(keys, paged_pieces(kKeys, c.seqs, c.k_tokens, c.max_k, 1), (c.max_q * group + kStep - 1) / kStep, 32, kKeys * c.d * 8);
-        plan(rows, paged_pieces(kRows, c.seqs, c.tokens, c.max_q, group), fv_packed_key_steps(c, kRows), 12, kRows * c.d * 4);
+        plan(keys, paged_pieces(kKeys, c.seqs, c.k_tokens, c.max_k, 1), (c.max_q * group + kStep - 1) / kStep, kLeastKeys, kKeys * c.d * 8);
+        plan(rows, paged_pieces(kRows, c.seqs, c.tokens, c.max_q, group), fv_packed_key_steps(c, kRows), kLeastRows, kRows * c.d * 4);
     }
     static BackPlan on_device(const Plan& x, uint8_t* ws) {
         return {x.pieces, (BackUnit*)(ws + x.units_at), (BackUnit*)(ws + x.cuts_at), (int2*)(ws + x.scratch_at), (int)x.units, (int)x.cuts,
-                (int)x.places, (int)x.least, (float*)(ws + x.places_at)};
+                (int)x.places, (float*)(ws + x.places_at)};
     }
 };
 // (the one kernel here that takes more than 64 KB)
@@ -873,7 +909,12 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     const fv::BackParts parts(c, !dout_is_bf16);
     if (!workspace || workspace_bytes < parts.bytes) return fv_invalid("packed attention backward: workspace too small");
     const size_t rows = q_tokens * heads, stat_blocks = (rows + 2048 / d - 1) / (2048 / d) + 2;
-    const size_t sum_rows = kv_heads * parts.rows.cuts * fv::kRows / (1024 / d), sum_keys = kv_heads * parts.keys.cuts * fv::kKeys / (512 / d);
+    // Rows or keys of a workgroup of the sums: 8 where few pieces may be cut (their shares are many, a wait each), up to 32 where the grid would hold
+    // thousands without work (8 us of 25000).
+    size_t per = 8;
+    static_assert(fv::kRows == fv::kKeys, "one number for both");
+    while (per < 32 && kv_heads * (parts.rows.cuts + parts.keys.cuts) * (fv::kRows / per) > 4096) per *= 2;
+    const size_t sum_rows = kv_heads * parts.rows.cuts * (fv::kRows / per), sum_keys = kv_heads * parts.keys.cuts * (fv::kKeys / per);
     constexpr size_t kMost = (size_t)1 << 24;   // (a launch holds fewer than 2^32 work-items)
     if (kv_heads * (parts.rows.units + parts.keys.units) >= kMost / 2 || stat_blocks >= kMost || sum_rows + sum_keys >= kMost)
         return fv_decline("packed attention backward: too large for one launch");
@@ -903,7 +944,7 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
         if (D == 128) e = fv::packed_prepare();
         if (e != hipSuccess) return;
         hipLaunchKernelGGL((fv::packed_back_kernel<D>), dim3((unsigned)(key_blocks + row_blocks)), dim3(256), fv::KeyForm<D>::kLds, st, p, (int)key_blocks);
-        if (sum_keys + sum_rows > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D>), dim3((unsigned)(sum_keys + sum_rows)), dim3(256), 0, st, p, (int)sum_keys);
+        if (sum_keys + sum_rows > 0) hipLaunchKernelGGL((fv::packed_sum_kernel<D>), dim3((unsigned)(sum_keys + sum_rows)), dim3(256), 0, st, p, (int)sum_keys, (int)per);
     });
     if (e == hipSuccess) e = hipGetLastError();
     return e == hipSuccess ? FV_OK : fv_fail_hip(e, "packed_attention_backward");
