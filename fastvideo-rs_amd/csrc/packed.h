@@ -194,12 +194,17 @@ FV_DEV void packed_store_rows(lds_u8* my, const bf16x4 (&x)[D / 16][2], int lane
             *reinterpret_cast<__attribute__((address_space(3))) bf16x4*>(my + (16 * g + i16) * kRowB + (ch << 4) + 8 * (q4 & 1)) = x[db][g];
         }
     // (writes and reads of one wave complete in order; the compiler waits for the reads' data)
+    const int c = lane % kCh;
+    u32x4 v[32 / kRowsPer];
 #pragma unroll
     for (int i = 0; i < 32 / kRowsPer; i++) {
-        const int r = i * kRowsPer + lane / kCh, c = lane % kCh;
-        const u32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(my + r * kRowB + ((c ^ (r & (kCh - 1))) << 4));
-        uint16_t* to = dst(r);
-        if (to) global_store<u32x4>(to + 8 * c, v);
+        const int r = i * kRowsPer + lane / kCh;
+        v[i] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(my + r * kRowB + ((c ^ (r & (kCh - 1))) << 4));
+    }
+#pragma unroll
+    for (int i = 0; i < 32 / kRowsPer; i++) {
+        uint16_t* to = dst(i * kRowsPer + lane / kCh);
+        if (to) global_store<u32x4>(to + 8 * c, v[i]);
     }
 }
 

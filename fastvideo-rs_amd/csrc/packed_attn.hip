@@ -98,14 +98,10 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     bf16x8 qf[D / 32][2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
+        const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
         const uint16_t* q = (const uint16_t*)((const uint8_t*)p.q + (long)(sq.start + t) * p.q_stride) + (kvh * p.group.by + r - t * p.group.by) * D + 8 * q4;
 #pragma unroll
-        for (int dk = 0; dk < D / 32; dk++) {
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (r < rows) x = *reinterpret_cast<const u32x4*>(q + 32 * dk);
-            qf[dk][g] = __builtin_bit_cast(bf16x8, x);
-        }
+        for (int dk = 0; dk < D / 32; dk++) qf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 32 * dk));
     }
     const TileReadBases rb = tile_read_bases<D>(lane);
     auto kbuf = [&](int m) -> lds_u8* { return smem + (m & 1) * kTile; };
@@ -270,7 +266,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
 #pragma unroll
                 for (int i = 0; i < 4; i++) chk = __builtin_fmaf(o[db][g][i], 0.f, chk);
         }
-        // (of rows past the last nothing is stored; their values are those of queries of zeros)
+        // (of rows past the last nothing is stored; their values are the last's)
         const bool wave_ok = idle || __builtin_amdgcn_ballot_w64(!(fine && chk == 0.f)) == 0;
         // (the K buffer that neither the last P V nor the load past the walk's end uses is the one of this tile; all reads of it are behind a barrier)
         auto* votes = (__attribute__((address_space(3))) unsigned*)kbuf(e1 - e0 - 1);

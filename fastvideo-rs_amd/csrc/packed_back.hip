@@ -431,14 +431,10 @@ FV_DEV void packed_dkv_item(const PackedBackParams& p, const int wave, const int
     }
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        const int key = wkey + 16 * g + i16;
+        const int key = min(wkey + 16 * g + i16, sq.len - 1);   // (past the last: the last again, not stored)
         const uint16_t* at = (const uint16_t*)((const uint8_t*)kbase + (long)(sq.k0 + key) * p.k_stride) + 8 * q4;
 #pragma unroll
-        for (int dk = 0; dk < kNK; dk++) {
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (key < sq.len) x = *reinterpret_cast<const u32x4*>(at + 32 * dk);
-            kf[dk][g] = __builtin_bit_cast(bf16x8, x);
-        }
+        for (int dk = 0; dk < kNK; dk++) kf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(at + 32 * dk));
     }
     // Steps are loaded from the walk's last to its first: their rows' tokens t0 .. and the h0 heads of t0 before them, and where t0 and the statistics lie, go
     // back by 32 rows a step. (The same from the step's number, 50 scalar instructions in a row, cost 13 to 17 % of the time.) Row x of a step is token t0 + dt,
@@ -706,22 +702,17 @@ FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int 
     f32x4 s_init[2], d_init[2];
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        const int r = wrow + 16 * g + i16, t = paged_quot(r, p.group);
+        const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
         const long in = (long)(kvh * group + r - t * group) * G::kRow + 16 * q4;
         const uint8_t* q = (const uint8_t*)p.q + (long)(sq.start + t) * p.q_stride + in;
         const uint8_t* go = (const uint8_t*)p.dout + (long)(sq.start + t) * p.dout_stride + in;
 #pragma unroll
         for (int dk = 0; dk < kNK; dk++) {
-            u32x4 x = {0u, 0u, 0u, 0u}, y = x;
-            if (r < rows) x = *reinterpret_cast<const u32x4*>(q + 64 * dk), y = *reinterpret_cast<const u32x4*>(go + 64 * dk);
-            qf[dk][g] = __builtin_bit_cast(bf16x8, x);
-            gf[dk][g] = __builtin_bit_cast(bf16x8, y);
+            qf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 64 * dk));
+            gf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(go + 64 * dk));
         }
-        float nlse = 0.f, nd = 0.f;
-        if (r < rows) {
-            const float* at = p.stats + ((long)kvh * p.b.tokens + sq.start) * group + r;
-            nlse = at[0], nd = at[p.stat_rows];
-        }
+        const float* at = p.stats + ((long)kvh * p.b.tokens + sq.start) * group + r;
+        const float nlse = at[0], nd = at[p.stat_rows];
 #pragma unroll
         for (int i = 0; i < 4; i++) s_init[g][i] = nlse, d_init[g][i] = nd;
     }
