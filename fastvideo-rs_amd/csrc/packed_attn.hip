@@ -64,6 +64,16 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     const PackedSeq sq = piece.seq;
     const int rows = sq.count * p.group.by, row0 = piece.tile * kRows;
     if (row0 >= rows) return true;
+    const int wrow = row0 + 32 * wave;
+    const bool idle = wrow >= rows;   // (brings its part of the tiles and no more)
+    bf16x8 qf[D / 32][2];
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
+        const uint16_t* q = (const uint16_t*)((const uint8_t*)p.q + (long)(sq.start + t) * p.q_stride) + (kvh * p.group.by + r - t * p.group.by) * D + 8 * q4;
+#pragma unroll
+        for (int dk = 0; dk < D / 32; dk++) qf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 32 * dk));
+    }
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
     const int e0 = share * p.chunk, e1 = min(w.n, e0 + p.chunk);
     if (share > 0 && e0 >= e1) return true;
@@ -87,22 +97,12 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     }
 
     // the wave's rows: the keys that all of them see, those of one of them a lane (row lane % 32; exchanged where a tile asks)
-    const int wrow = row0 + 32 * wave;
-    const bool idle = wrow >= rows;   // (brings its part of the tiles and no more)
     PagedSight all_see = {0x7fffffff, 0, 0x7fffffff}, mine = {0, 0, 0};
     if (!idle) {
         all_see = packed_all(p.mask, sq, paged_quot(wrow, p.group), paged_quot(min(wrow + 32, rows) - 1, p.group));
         mine = packed_sight(p.mask, sq.pos0 + paged_quot(min(wrow + (lane & 31), rows - 1), p.group), sq.len);
     }
     const PackedWhole whole = packed_whole(w, all_see);
-    bf16x8 qf[D / 32][2];
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-        const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
-        const uint16_t* q = (const uint16_t*)((const uint8_t*)p.q + (long)(sq.start + t) * p.q_stride) + (kvh * p.group.by + r - t * p.group.by) * D + 8 * q4;
-#pragma unroll
-        for (int dk = 0; dk < D / 32; dk++) qf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 32 * dk));
-    }
     const TileReadBases rb = tile_read_bases<D>(lane);
     auto kbuf = [&](int m) -> lds_u8* { return smem + (m & 1) * kTile; };
     auto vbuf = [&](int m) -> lds_u8* { return smem + (2 + (m & 1)) * kTile; };
