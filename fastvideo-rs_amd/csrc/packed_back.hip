@@ -669,13 +669,31 @@ FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int 
     const int kvh = at.head, group = p.group.by;
     const PackedSeq sq = unit.seq();
     const int rows = sq.count * group, row0 = unit.tile * kRows;
+    const int wrow = row0 + 32 * wave;
+    const bool idle = wrow >= rows;
+    bf16x8 qf[kNK][2], gf[kNK][2];
+    f32x4 s_init[2], d_init[2];
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
+        const long in = (long)(kvh * group + r - t * group) * G::kRow + 16 * q4;
+        const uint8_t* q = (const uint8_t*)p.q + (long)(sq.start + t) * p.q_stride + in;
+        const uint8_t* go = (const uint8_t*)p.dout + (long)(sq.start + t) * p.dout_stride + in;
+#pragma unroll
+        for (int dk = 0; dk < kNK; dk++) {
+            qf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 64 * dk));
+            gf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(go + 64 * dk));
+        }
+        const float* at = p.stats + ((long)kvh * p.b.tokens + sq.start) * group + r;
+        const float nlse = at[0], nd = at[p.stat_rows];
+#pragma unroll
+        for (int i = 0; i < 4; i++) s_init[g][i] = nlse, d_init[g][i] = nd;
+    }
     const PackedWalk w = packed_walk(p.mask, sq, paged_quot(row0, p.group), paged_quot(min(row0 + kRows, rows) - 1, p.group));
     const int e0 = unit.from, e1 = min(w.n, unit.to);
     const KeySight single = single_rows(p.mask, sq, group);
     const float sl2 = p.sl2;
 
-    const int wrow = row0 + 32 * wave;
-    const bool idle = wrow >= rows;
     PagedSight all_see = {0x7fffffff, 0, 0x7fffffff}, mine = {0, 0, 0};
     if (!idle) {
         all_see = packed_all(p.mask, sq, paged_quot(wrow, p.group), paged_quot(min(wrow + 32, rows) - 1, p.group));
@@ -697,25 +715,7 @@ FV_DEV void packed_dq_item(const PackedBackParams& p, const int wave, const int 
         }
         krun.next(), vrun.next();
     };
-    if (e0 < e1) load(0);   // (the first keys and values on their way before the queries)
-    bf16x8 qf[kNK][2], gf[kNK][2];
-    f32x4 s_init[2], d_init[2];
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-        const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
-        const long in = (long)(kvh * group + r - t * group) * G::kRow + 16 * q4;
-        const uint8_t* q = (const uint8_t*)p.q + (long)(sq.start + t) * p.q_stride + in;
-        const uint8_t* go = (const uint8_t*)p.dout + (long)(sq.start + t) * p.dout_stride + in;
-#pragma unroll
-        for (int dk = 0; dk < kNK; dk++) {
-            qf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 64 * dk));
-            gf[dk][g] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(go + 64 * dk));
-        }
-        const float* at = p.stats + ((long)kvh * p.b.tokens + sq.start) * group + r;
-        const float nlse = at[0], nd = at[p.stat_rows];
-#pragma unroll
-        for (int i = 0; i < 4; i++) s_init[g][i] = nlse, d_init[g][i] = nd;
-    }
+    if (e0 < e1) load(0);   // (the first keys and values on their way beside the operands')
     const TileReadBases rb = both_bases<D>(lane);
     f32x4 dq[kNO][2];
 #pragma unroll
