@@ -239,8 +239,12 @@ FV_DEV void plan_pieces(const PackedBackParams& p, const BackPlan& plan, int slo
 }
 
 // D / 8 threads a row (token, head); OUT16, DOUT16: bf16 bits. An f32 gradient is kept as bf16 bits in `rounded` [tokens, heads, d].
-template <int D, bool OUT16, bool DOUT16>
-__global__ __launch_bounds__(256) void packed_stats_kernel(const PackedBackParams p, const void* dout, const void* out, const float* lse, float* stats, uint16_t* rounded,
+// FEW, in calls whose rows see 64 keys at most: one that sees up to kFew has sum_j p_j (dout . v_j) in place of sum(dout out). The rounding of `out` is up to
+// 2^-8 of it, which is as much as what dS is made of where few keys share a row and one has most of its weight (dq and dk of sequences of 2 to 4 tokens
+// were 0.0051 of their size off, are 0.0032). The search for its sequence costs every row as much as the rest (5 prompts of up to 6000: 55 -> 79 us).
+constexpr int kFew = 8, kFewKeys = 64;
+template <int D, bool OUT16, bool DOUT16, bool FEW>
+__global__ __launch_bounds__(256, 8) void packed_stats_kernel(const PackedBackParams p, const void* dout, const void* out, const float* lse, float* stats, uint16_t* rounded,
                                                            long rows, float inv_scale, int slots) {
     if (blockIdx.x < 2) {   // (the first two: the plans)
         if (blockIdx.x == 0) plan_pieces<true>(p, p.keys, slots);
@@ -283,10 +287,64 @@ __global__ __launch_bounds__(256) void packed_stats_kernel(const PackedBackParam
     for (int i = 0; i < 8; i++) sum = __builtin_fmaf(g[i], o[i], sum);
 #pragma unroll
     for (int s = 1; s < kPer; s <<= 1) sum += __shfl_xor(sum, s, 64);
+    const long t = row / heads;
+    const int h = (int)(row - t * heads), kvh = paged_quot(h, group);
+    const float l = lse[row];
+    if constexpr (FEW) {
+        // the last sequence that begins no later than the token: for the wave's first by scalar reads, from there on by the lane
+        using Starts = const __attribute__((address_space(4))) int*;
+        const int t0 = __builtin_amdgcn_readfirstlane((int)t);
+        int seq = 0;
+        for (int behind = p.b.seqs; behind - seq > 1;) {
+            const int mid = seq + (behind - seq) / 2;
+            if (((Starts)p.b.q_start)[mid] <= t0) seq = mid;
+            else behind = mid;
+        }
+        if (seq + 1 < p.b.seqs && p.b.q_start[seq + 1] <= t) {
+            seq++;
+            for (int behind = p.b.seqs; behind - seq > 1;) {
+                const int mid = seq + (behind - seq) / 2;
+                if (p.b.q_start[mid] <= t) seq = mid;
+                else behind = mid;
+            }
+        }
+        const PackedSeq sq = packed_seq(p.b, seq);
+        const int in = (int)t - sq.start;
+        const PagedSight sees = in >= 0 && in < sq.count ? packed_sight(p.mask, sq.pos0 + in, sq.len) : PagedSight{0, 0, 0};
+        const int band = max(sees.lo, sees.a), keys = sees.a + max(sees.hi - band, 0);
+        if (keys > 1 && keys <= kFew) {
+            auto bits = [](const uint16_t* at, float (&x)[8]) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[2 * i] = __builtin_bit_cast(float, w[i] << 16), x[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+            };
+            float qx[8];
+            bits((const uint16_t*)((const uint8_t*)p.q + t * p.q_stride) + h * D + 8 * c, qx);
+            sum = 0.f;
+#pragma unroll 1
+            for (int j = 0; j < keys; j += 2) {
+                float s[2], dp[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int x = min(j + u, keys - 1);
+                    const long key = sq.k0 + (x < sees.a ? x : band + x - sees.a);
+                    float kx[8], vx[8];
+                    bits((const uint16_t*)((const uint8_t*)p.k + key * p.k_stride) + kvh * D + 8 * c, kx);
+                    bits((const uint16_t*)((const uint8_t*)p.v + key * p.v_stride) + kvh * D + 8 * c, vx);
+                    s[u] = dp[u] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s[u] = __builtin_fmaf(qx[i], kx[i], s[u]), dp[u] = __builtin_fmaf(g[i], vx[i], dp[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+#pragma unroll
+                    for (int x = 1; x < kPer; x <<= 1) s[u] += __shfl_xor(s[u], x, 64), dp[u] += __shfl_xor(dp[u], x, 64);
+                    if (j + u < keys) sum += fast_exp2((s[u] - l * inv_scale) * p.sl2) * dp[u];
+                }
+            }
+        }
+    }
     if (c == 0) {
-        const long t = row / heads;
-        const int h = (int)(row - t * heads), kvh = paged_quot(h, group);
-        const float l = lse[row];
         float* at = stats + ((long)kvh * tokens + t) * group.by + (h - kvh * group.by);
         at[0] = l == neg_inf() ? l : -l * inv_scale;
         at[rows] = -sum;
@@ -921,14 +979,17 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
     p.scale = scale, p.sl2 = (float)((double)scale * 1.4426950408889634);
     p.runs = fv::packed_runs(kv_heads, causal != 0);
     p.keys = fv::BackParts::on_device(parts.keys, ws), p.rows = fv::BackParts::on_device(parts.rows, ws);
+    const bool few = c.max_k <= (size_t)fv::kFewKeys || (causal && window > 0 && (window + sink) * block_tokens <= (size_t)fv::kFewKeys);   // (below 2^32 each)
     hipStream_t st = (hipStream_t)stream;
     hipError_t e = hipSuccess;
     fv::paged_pick(d == 128, [&](auto d128) {
         constexpr int D = d128() ? 128 : 64;
         fv::paged_pick(out_is_bf16 != 0, [&](auto o16) {
             fv::paged_pick(dout_is_bf16 != 0, [&](auto g16) {
-                hipLaunchKernelGGL((fv::packed_stats_kernel<D, o16(), g16()>), dim3((unsigned)stat_blocks), dim3(256), 0, st, p, dout, out, lse,
-                                   (float*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (float)(1.0 / (double)scale), parts.slots);
+                fv::paged_pick(few, [&](auto f) {
+                    hipLaunchKernelGGL((fv::packed_stats_kernel<D, o16(), g16(), f()>), dim3((unsigned)stat_blocks), dim3(256), 0, st, p, dout, out, lse,
+                                       (float*)(ws + parts.stats), (uint16_t*)(ws + parts.rounded), (long)rows, (float)(1.0 / (double)scale), parts.slots);
+                });
             });
         });
         const size_t key_blocks = fv::packed_blocks(p.runs, parts.keys.units), row_blocks = fv::packed_blocks(p.runs, parts.rows.units);

@@ -440,7 +440,8 @@ int fv_packed_attention(const uint16_t* q, size_t q_stride, const uint16_t* k, s
  * dout [q_tokens, heads, d] (contiguous, f32 or bf16 bits: dout_is_bf16; f32 is rounded to bf16 first) by the result of
  * fv_packed_attention on the same operands and numbers, its out (contiguous, out_is_bf16) and lse: with P = e^(scale q k^T - lse), dv = P^T dout,
  * dS = P (dout v^T - sum(dout out)), dq = scale dS k, dk = scale dS^T q, summed over the heads that share a key head, always in one order (no
- * atomics). P and dS are rounded to bf16 for the second products. workspace: fv_packed_attention_backward_workspace_bytes, which it cannot do without. */
+ * atomics). (Rows that see up to 8 keys, in calls whose max_k or window and sink leave no row more than 64: with sum_j P_j (dout . v_j) in place of
+ * sum(dout out), whose rounding would be as much as their dS.) P and dS are rounded to bf16 for the second products. workspace: fv_packed_attention_backward_workspace_bytes, which it cannot do without. */
 size_t fv_packed_attention_backward_workspace_bytes(int dout_is_bf16, size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t q_tokens,
                                                     size_t k_tokens, size_t max_q, size_t max_k, int causal, size_t block_tokens,
                                                     size_t window, size_t sink);

@@ -48,9 +48,9 @@ def attention(q, k, v, seen, scale, out_bf16):
     return out, lse, bound, off + sums + 2.0 ** -18 + 4 * F32_HALF * np.abs(np.where(some, lse, 0.0))
 
 
-def gradients(q, k, v, dout, out, lse, seen, scale):
+def gradients(q, k, v, dout, out, lse, seen, scale, few=0):
     """One head of one sequence, with the result and the logarithms that the kernels are given: (dq, dk, dv, bounds of each before the
-    results' own rounding)."""
+    results' own rounding). Rows that see up to `few` keys: with sum_j p_j dp_j in place of sum(dout out)."""
     n, m, d = q.shape[0], k.shape[0], q.shape[1]
     if m == 0 or n == 0:
         z = np.zeros((n, d)), np.zeros((m, d)), np.zeros((m, d))
@@ -58,7 +58,8 @@ def gradients(q, k, v, dout, out, lse, seen, scale):
     s = np.where(seen, _products(q, k), 0.0) * scale
     p = np.where(seen, np.exp(s - np.where(np.isfinite(lse), lse, 0.0)[:, None]), 0.0)
     dp = _products(dout, v)
-    delta = (dout * out).sum(1, keepdims=True)
+    some = seen.sum(1, keepdims=True) <= few
+    delta = np.where(some, np.where(seen, p * dp, 0.0).sum(1, keepdims=True), (dout * out).sum(1, keepdims=True))
     ds = p * (dp - delta)
     # a row that sees one key: its weight is 1 whatever the score, so dS is 0, where the rounding of the given result would leave some 2^-8 of dp
     ds = np.where(seen.sum(1, keepdims=True) == 1, 0.0, ds)
@@ -66,6 +67,8 @@ def gradients(q, k, v, dout, out, lse, seen, scale):
     # P: its score's error, -lse's rounding and the exponential's; dP - D: products in f32
     off = _score_error(q, k, scale, seen) + 2 * F32_HALF * np.abs(np.where(np.isfinite(lse), lse, 0.0))[:, None] + 2.0 ** -20
     off_dp = (d + 4) * F32_HALF * (_products(np.abs(dout), np.abs(v)) + (np.abs(dout) * np.abs(out)).sum(1, keepdims=True))
+    # (few keys: each p_j of their sum is off as P is, each dp_j as dP)
+    off_dp = off_dp + np.where(some, np.where(seen, p * (off * np.abs(dp) + (d + 4 + few) * F32_HALF * _products(np.abs(dout), np.abs(v))), 0.0).sum(1, keepdims=True), 0.0)
     ep = p * (off + BF16_HALF)
     es = np.abs(ds) * (off + BF16_HALF + 2 * F32_HALF) + p * off_dp
     acc = F32_HALF * (max(n, m) / 16 + 64)          # f32 sums of the products over rows, or keys

@@ -62,6 +62,11 @@ class Case:
         self.how = {"causal": self.causal, "mask": fv_sdpa.BlockCausal(self.block, self.window, self.sink) if self.causal and (self.block, self.window, self.sink) != (1, 0, 0) else None}
         self.scale = 1.0 / np.sqrt(d)
 
+    def few(self):
+        """Rows that see up to so many keys have their sum of p dp made from these (where no row sees more than 64)."""
+        band = (self.window + self.sink) * self.block if self.causal and self.window else 1 << 40
+        return 8 if min(self.batch.max_k, self.nk, band) <= 64 else 0
+
     def heads_of(self):
         """(rows, keys, head, key head, mask) of every head of every sequence."""
         for s, (a, b) in enumerate(self.seqs):
@@ -94,7 +99,7 @@ class Case:
         dq, dk, dv = (np.zeros((n, h, self.d)) for n, h in ((self.nq, self.heads), (self.nk, self.kvh), (self.nk, self.kvh)))
         bq, bk, bv = np.zeros_like(dq), np.zeros_like(dk), np.zeros_like(dv)
         for rows, keys, h, y, seen in self.heads_of():
-            r = pu.gradients(q[rows, h], k[keys, y], v[keys, y], g[rows, h], o[rows, h], l[rows, h], seen, self.scale)
+            r = pu.gradients(q[rows, h], k[keys, y], v[keys, y], g[rows, h], o[rows, h], l[rows, h], seen, self.scale, self.few())
             dq[rows, h], bq[rows, h] = r[0], r[3]
             for to, x in ((dk, r[1]), (dv, r[2]), (bk, r[4]), (bv, r[5])):
                 to[keys, y] += x
@@ -377,7 +382,7 @@ def test_gradients_against_differences():
     got = [x.double().cpu().numpy() for x in grads]
     bound = [np.zeros_like(x) for x in got]
     for r, s, h, y, seen in c.heads_of():
-        b = pu.gradients(q[r, h], k[s, y], v[s, y], g[r, h], out.double().cpu().numpy()[r, h], lse.double().cpu().numpy()[r, h], seen, c.scale)
+        b = pu.gradients(q[r, h], k[s, y], v[s, y], g[r, h], out.double().cpu().numpy()[r, h], lse.double().cpu().numpy()[r, h], seen, c.scale, c.few())
         # the given result is rounded to bf16: dP - D is off by its half step's part
         off = (np.abs(g[r, h]) * np.abs(out.double().cpu().numpy()[r, h])).sum(1, keepdims=True) * pu.BF16_HALF
         p = np.where(seen, np.exp(np.where(seen, q[r, h] @ k[s, y].T, 0) * c.scale - lse.double().cpu().numpy()[r, h][:, None]), 0)
