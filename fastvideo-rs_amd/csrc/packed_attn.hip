@@ -66,7 +66,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     if (row0 >= rows) return true;
     const int wrow = row0 + 32 * wave;
     const bool idle = wrow >= rows;   // (brings its part of the tiles and no more)
-    bf16x8 qf[D / 32][2];
+    bf16x8 qf[D / 32][2];             // (on their way before the walk is worked out: they come from the farthest)
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         const int r = min(wrow + 16 * g + i16, rows - 1), t = paged_quot(r, p.group);   // (past the last: the last again, not stored)
@@ -87,7 +87,7 @@ FV_DEV bool packed_item_pass(const Params& p, const int wave, const int lane, co
     const unsigned slot = (unsigned)(size_t)smem + wave * kIter * 1024;
     PackedRun krun(kbase, p.k_stride, sq, w, e0), vrun(vbase, p.v_stride, sq, w, e0);
 
-    if (e0 < e1) {   // (the first keys and values on their way before the queries: short walks are mostly this wait)
+    if (e0 < e1) {   // (with the queries: short walks are mostly this wait)
         const u32x4 kd = krun.rows(G::kRow), vd = vrun.rows(G::kRow);
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {

@@ -167,11 +167,12 @@ def test_more_heads(heads, seqs, mask):
     c.check_backward(out, lse, grads, "backward")
 
 
+@pytest.mark.parametrize("seqs", ["long", "short"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_types(d):
+def test_types(d, seqs):
     """f32 results, f32 gradients in (rounded first) and out, each against the same bounds with its own rounding."""
-    c = Case(SEQS["long"], 4, 2, d, MASKS["causal"], seed=3)
-    announce(f"f32 result, d {d}")
+    c = Case(SEQS[seqs], 4, 2, d, MASKS["causal"], seed=3)
+    announce(f"f32 result, d {d}, {seqs}")
     out, lse = fv_sdpa.packed_attention(c.q, c.k, c.v, c.batch, out_bf16=False, with_lse=True)
     assert out.dtype is torch.float32
     c.check_forward(out, lse, "f32 result", out_bf16=False)
