@@ -331,10 +331,12 @@ def test_the_same_bits_and_streams():
             assert torch.equal(a[at], b[at])
 
 
-def test_a_captured_step_replays_with_other_lengths():
+@pytest.mark.parametrize("most,batches", [
+    (300, [[(300, 300), (1, 1), (77, 77), (0, 0)], [(10, 10), (300, 300), (129, 129), (64, 64)], [(0, 0), (0, 0), (5, 5), (33, 33)]]),
+    (40, [[(40, 40), (1, 1), (7, 7), (0, 0)], [(3, 3), (2, 2), (40, 40), (5, 5)], [(0, 0), (0, 0), (5, 5), (33, 33)]])])
+def test_a_captured_step_replays_with_other_lengths(most, batches):
     """Forward and backward captured once, replayed with other starts within the bounds, each replay against its own eager calls."""
-    heads, kvh, d, n, most = 4, 2, 128, 4, 300
-    batches = [[(300, 300), (1, 1), (77, 77), (0, 0)], [(10, 10), (300, 300), (129, 129), (64, 64)], [(0, 0), (0, 0), (5, 5), (33, 33)]]
+    heads, kvh, d, n = 4, 2, 128, 4
     tokens = 520
     g = torch.Generator(device="cuda").manual_seed(11)
     q = torch.randn(tokens, heads, d, device="cuda", generator=g).bfloat16()
