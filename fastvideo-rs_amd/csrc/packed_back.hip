@@ -942,9 +942,9 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
                                  int grads_are_bf16, size_t heads, size_t kv_heads, size_t d, const int32_t* q_start, const int32_t* k_start,
                                  size_t seqs, size_t q_tokens, size_t k_tokens, size_t max_q, size_t max_k, float scale, int causal,
                                  size_t block_tokens, size_t window, size_t sink, void* workspace, size_t workspace_bytes, void* stream) {
-    if (seqs == 0 || (q_tokens == 0 && k_tokens == 0)) return FV_OK;   // (empty arrays may have no address)
     const PackedCall c = {heads, kv_heads, d, seqs, q_tokens, k_tokens, std::min(max_q, q_tokens), std::min(max_k, k_tokens), q_start, k_start, scale,
                           causal, block_tokens, window, sink};
+    if (seqs == 0 || (c.max_q == 0 && c.max_k == 0)) return FV_OK;   // (no unit to launch; empty arrays may have no address)
     PackedOperand x[9];
     size_t n = 0;
     if (q_tokens > 0) {
