@@ -14,7 +14,7 @@ namespace fv {
 struct PackedBatch {
     const int* q_start;
     const int* k_start;
-    int seqs, tokens, k_tokens, max_q, max_k;   // (what lies past the bounds that the launch is sized by is left out)
+    int seqs, tokens, k_tokens, max_q, max_k;   // (a sequence's rows and keys past the bounds that the launch is sized by are left out)
 };
 // The keys' side alone, for numbering pieces of keys.
 struct PackedKeys {
@@ -25,13 +25,17 @@ struct PackedKeys {
 struct PackedSeq {
     int start, count;   // first row, rows
     int k0, len;        // first key, keys
-    int pos0;           // position of the first row among the keys: the last row is at the last key; negative where rows are more than keys
-    FV_DEV PackedSeq(int start_, int count_, int k0_, int len_) : start(start_), count(count_), k0(k0_), len(len_), pos0(len_ - count_) {}
-};
+    int pos0;           // position of the first row among the keys: the last row of the whole sequence is at its last key, also where max_q or max_k
+};                      // leave some out; negative where rows are more than keys
+// Of the rows [q0, q1) and the keys [k0, k1) those within the bounds.
+template <class Batch>
+FV_DEV PackedSeq packed_within(const Batch& b, int q0, int q1, int k0, int k1) {
+    return {q0, min(q1 - q0, b.max_q), k0, min(k1 - k0, b.max_k), (k1 - k0) - (q1 - q0)};
+}
 template <class Batch>
 FV_DEV PackedSeq packed_seq(const Batch& b, int s) {
-    const int start = min(max(b.q_start[s], 0), b.tokens), k0 = min(max(b.k_start[s], 0), b.k_tokens);
-    return {start, min(min(max(b.q_start[s + 1], start), b.tokens) - start, b.max_q), k0, min(min(max(b.k_start[s + 1], k0), b.k_tokens) - k0, b.max_k)};
+    const int q0 = min(max(b.q_start[s], 0), b.tokens), k0 = min(max(b.k_start[s], 0), b.k_tokens);
+    return packed_within(b, q0, min(max(b.q_start[s + 1], q0), b.tokens), k0, min(max(b.k_start[s + 1], k0), b.k_tokens));
 }
 
 // The piece of a number and its sequence (of a whole wave). Up to 63 sequences: the starts come with one load of the wave, from which both the search and
@@ -50,10 +54,10 @@ FV_DEV PackedPiece packed_piece(const Pieces& x, const Batch& b, int group, int 
     const long first = ((long)min(max(row, 0), b.tokens) * group + (long)(R - 1) * lane) / R;
     const int seq = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < b.seqs && first <= number)), 1) - 1;
     const int q0 = min(max(__builtin_amdgcn_readlane(row, seq), 0), b.tokens), k0 = min(max(__builtin_amdgcn_readlane(key, seq), 0), b.k_tokens);
-    const int q1 = max(__builtin_amdgcn_readlane(row, seq + 1), q0), k1 = max(__builtin_amdgcn_readlane(key, seq + 1), k0);
+    const int q1 = min(max(__builtin_amdgcn_readlane(row, seq + 1), q0), b.tokens), k1 = min(max(__builtin_amdgcn_readlane(key, seq + 1), k0), b.k_tokens);
     const long tile = number - ((long)q0 * group + (long)(R - 1) * seq) / R;
     constexpr int kNone = 0x7fffffff / R;
-    return {{q0, min(min(q1, b.tokens) - q0, b.max_q), k0, min(min(k1, b.k_tokens) - k0, b.max_k)}, tile < 0 || tile > kNone ? kNone : (int)tile};
+    return {packed_within(b, q0, q1, k0, k1), tile < 0 || tile > kNone ? kNone : (int)tile};
 }
 
 // f(0), f(1), .., f(N - 1) with the numbers as types (loops that the compiler does not unroll in time).

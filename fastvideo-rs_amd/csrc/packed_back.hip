@@ -24,9 +24,9 @@ constexpr int kRows = 128;   // of a workgroup of packed_dq_item, 32 a wave
 // piece of 128 rows or keys and a part [from, to) of the steps of its walk: tiles of 64 keys; of 32 rows. A walk longer than a slot's mean load is cut into
 // shares, which leave f32 sums in places of 128 rows ([kv_heads][most_places][128][d or 2 d]) and are added by packed_sum_kernel.
 struct BackUnit {
-    int tile, from, to, place;    // place < 0: a whole walk; of a share: its place; kNoUnit: none. (Of a cut piece: `to` is its shares, `place` the first one's.)
-    int start, count, k0, len;    // the sequence, as packed_seq has it
-    FV_DEV PackedSeq seq() const { return {start, count, k0, len}; }
+    int tile, from, to, place;         // place < 0: a whole walk; of a share: its place; kNoUnit: none. (Of a cut piece: `to` is its shares, `place` the first one's.)
+    int start, count, k0, len, pos0;   // the sequence, as packed_seq has it
+    FV_DEV PackedSeq seq() const { return {start, count, k0, len, pos0}; }
 };
 constexpr int kNoUnit = -2;
 struct BackPlan {
@@ -85,6 +85,7 @@ FV_DEV KeySight key_sight(const Mask& m, const PackedSeq& s, int key, int group)
 // The rows of a sequence that see one key, [lo, hi): their weight is 1 and their dS nothing, exactly, where dP - D would leave the rounding of `out`.
 // packed_dkv_item loads zeros for their queries and -lse / scale (scores of 0, a weight of 1, no part in dk), packed_dq_item stores zeros. By
 // token those are the first token's (under a window of one, without a sink, all); by blocks those of a last block of one key under such a window.
+// (Others see one of the keys that max_k keeps and are not among these: their dS is what dP - D leaves.)
 template <class Mask>
 FV_DEV KeySight single_rows(const Mask& m, const PackedSeq& s, int group) {
     const bool alone = m.window == 1 && m.sink == 0;
@@ -228,10 +229,10 @@ FV_DEV void plan_pieces(const PackedBackParams& p, const BackPlan& plan, int slo
         if (k > 1) {
             const int c = atomicAdd(&cuts, 1);
             place = atomicAdd(&places, k);
-            if (c < plan.most_cuts) plan.cuts[c] = BackUnit{tile, 0, k, place, sq.start, sq.count, sq.k0, sq.len};
+            if (c < plan.most_cuts) plan.cuts[c] = BackUnit{tile, 0, k, place, sq.start, sq.count, sq.k0, sq.len, sq.pos0};
         }
         for (int i = 0; i < k; i++, u++)
-            if (u < plan.most_units) plan.units[u] = BackUnit{tile, i * chunk, min(x.y, (i + 1) * chunk), place < 0 ? -1 : place + i, sq.start, sq.count, sq.k0, sq.len};
+            if (u < plan.most_units) plan.units[u] = BackUnit{tile, i * chunk, min(x.y, (i + 1) * chunk), place < 0 ? -1 : place + i, sq.start, sq.count, sq.k0, sq.len, sq.pos0};
     }
     __syncthreads();
     for (int u = total + tid; u < plan.most_units; u += 256) plan.units[u].place = kNoUnit;

@@ -120,7 +120,8 @@ def rope_tokens(rope, positions, q, k=None, inverse=False, out_bf16=None, in_pla
 
 class PackedSeqs:
     """The sequences of a call: int32 CUDA tensors q_start [n + 1] and k_start [n + 1] (None: q_start), the first row and key of each and the end
-    of the last; max_q and max_k (None: max_q) bound the rows and keys of a sequence (host numbers: the launches are sized by them).
+    of the last; max_q and max_k (None: max_q) bound the rows and keys of a sequence (host numbers: the launches are sized by
+    them; of a longer sequence the first rows and keys, at the positions that they have in the whole, are taken).
     The tensors' addresses are taken here: other numbers go into them, other tensors are another PackedSeqs."""
 
     __slots__ = ("_q_start", "_k_start", "max_q", "max_k", "_args", "_device")

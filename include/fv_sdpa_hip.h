@@ -416,14 +416,15 @@ int fv_paged_attention(const uint16_t* q, size_t q_stride, void* out, int out_is
  * fused projection), 16-byte aligned; heads / kv_heads neighbouring heads share a key head. Sequence s is rows q_start[s] .. q_start[s + 1]
  * and keys k_start[s] .. k_start[s + 1] (int32 [seqs + 1] device arrays, ascending; self-attention passes one array for both). They are read when the
  * call's work runs, and every index from them is bounded to the tensors, so a captured call may be replayed with other lengths. max_q / max_k bound the rows and
- * keys of a sequence (host numbers that the launch is sized by; what lies past them may be left out). Rows at q_start[seqs] and
- * behind, and keys' gradients likewise, are left as they were.
+ * keys of a sequence (host numbers that the launch is sized by): of a longer one the first max_q rows see what they see of its first max_k keys, at the
+ * positions that they have in the whole, and the rest is left out. Rows left out, rows at q_start[seqs] and behind, and keys' gradients likewise, are left as
+ * they were.
  *
  * causal == 0: every row sees every key of its sequence. Else a sequence's last row is at its last key's position, and the row at position i
  * sees key j as in fv_paged_attention: ti = i / block_tokens, tj <= ti && (window == 0 || ti - tj < window || tj < sink). A row that sees no key
  * (a sequence without keys, or with more rows than keys) is zeros, with lse -inf and no gradient. What a row does not see does not
  * reach its result, whatever is stored there; the gradients of a sequence are numbers only where all its operands are.
- * A row that sees one key has no gradient by its score, exactly. Outputs may not overlap inputs or each other.
+ * A row that sees one key (of a sequence within max_k) has no gradient by its score, exactly. Outputs may not overlap inputs or each other.
  *
  * out [q_tokens, heads, d] (contiguous, f32 or bf16 bits) = softmax(scale q k^T) v, scale within 1e-30 and 1e30; lse (NULL: not wanted) f32 [q_tokens, heads] = the natural
  * logarithm of sum e^(scale q k^T). Results are the same bits from call to call with the same bounds and workspace.
