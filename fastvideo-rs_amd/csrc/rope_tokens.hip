@@ -210,6 +210,7 @@ int fv_rope_tokens(const void* q, size_t q_stride, void* q_out, size_t q_out_str
     const size_t wanted = (size_t)fv_compute_units() * 1024;
     size_t per = std::min<size_t>(all, 16);
     while (per > 1 && tokens * units * ((all + per - 1) / per) < wanted) per = (per + 1) / 2;
+    per = std::max(per, (all + 65534) / 65535);   // (a grid's y is below 2^16)
     p.per = (int)per, p.turned = (int)turned, p.units = fv::paged_div(units);
     const dim3 blocks((unsigned)((tokens * units + 255) / 256), (unsigned)((all + per - 1) / per));
     if ((size_t)blocks.x * blocks.y >= (size_t)1 << 24) return fv_decline("rope tokens: too large for one launch");
