@@ -1,12 +1,14 @@
 """Training on packed sequences (include/fv_sdpa_hip.h, `fv_packed_*`, `fv_rope_*`; no counterpart in the reference): sequences of different
 lengths one behind the other, attention with shared key heads inside each of them, its gradients, and rotary positions without tables. They
-record no graph: a caller's autograd function calls them.
+record no graph: a caller's autograd function calls them. Elsewhere, of tensors that autograd watches, the results are such that a gradient
+asked for through them is an error (not silently left out), and a rotation in place is refused.
 """
 import ctypes as C
 import math
 from operator import attrgetter
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -42,6 +44,24 @@ def _on(device, name):
         raise ValueError(f"{name}: want CUDA tensors")
     if torch._C._cuda_getDevice() != device:
         raise ValueError(f"{name}: the tensors are on cuda:{device}, which is not the current device")
+
+
+def _watched(a, b=None, c=None):
+    """Whether autograd would record a call on these tensors."""
+    return (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)) and torch.is_grad_enabled()
+
+
+class _NoGraph(torch.autograd.Function):
+    """The results of call() (which runs with autograd off) for tensors that autograd watches: their backward says what is missing."""
+
+    @staticmethod
+    def forward(ctx, name, call, *watched):
+        ctx.name = name
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} records no graph: its gradient goes through an autograd function of the caller's (or call it under torch.no_grad())")
 
 
 class Rope:
@@ -88,6 +108,10 @@ def rope_tokens(rope, positions, q, k=None, inverse=False, out_bf16=None, in_pla
     """q [tokens, heads, d] (and k [tokens, kv_heads, d]), f32 or bf16, turned by the angles of positions, int32 [tokens] or [tokens, axes].
     inverse: turned back, which is the gradients' way. Returns contiguous tensors of the inputs' type (out_bf16: another one), or with
     in_place the inputs themselves; with k both."""
+    if _watched(q, k):
+        if in_place:
+            raise ValueError("rope_tokens: autograd watches q or k and would not see them turned in place")
+        return _NoGraph.apply("rope_tokens", lambda: rope_tokens(rope, positions, q, k, inverse, out_bf16), q, *(() if k is None else (k,)))
     dev, d = rope._device, rope._d
     _on(dev, "rope_tokens")
     dtypes = (q.dtype,) if q.dtype is _BF16 or q.dtype is _F32 else (_F32, _BF16)
@@ -115,6 +139,8 @@ def rope_tokens(rope, positions, q, k=None, inverse=False, out_bf16=None, in_pla
         q.data_ptr(), qs, q_out.data_ptr(), qos, heads, k.data_ptr() if k is not None else None, ks, k_out.data_ptr() if k is not None else None, kos, kvh, d,
         1 if is16 else 0, 1 if out16 else 0, rope._freq.data_ptr(), rope._pair_axis.data_ptr() if rope._pair_axis is not None else None, rope._rot // 2,
         positions.data_ptr(), axes, tokens, rope._amplitude, 1 if rope._halves else 0, 1 if inverse else 0, _lib.stream()))
+    if in_place:   # (written by their addresses: tensors saved for a gradient are known to be others now)
+        increment_version(q if k is None else (q, k))
     return q_out if k is None else (q_out, k_out)
 
 
@@ -172,10 +198,13 @@ def packed_attention(q, k, v, seqs, mask=None, causal=True, scale=None, out_bf16
     projection do) -> [tokens, heads, d]. causal: by token, the last row at the last key, or by a BlockCausal `mask` whose sink blocks are not
     seen before their time; not causal: every key of the sequence. with_lse: also f32 [tokens, heads], the logarithm of every row's
     sum, for packed_attention_backward. Rows behind the last sequence are not written."""
+    if _watched(q, k, v):
+        return _NoGraph.apply("packed_attention", lambda: packed_attention(q, k, v, seqs, mask, causal, scale, out_bf16, out, with_lse), q, k, v)
     dev, d, heads, kvh, qs, ks, vs, m = _operands("packed_attention", q, k, v, seqs, mask, causal)
     tokens, keys = q.shape[0], k.shape[0]
     dtype = _BF16 if out_bf16 else _F32
-    if out is None:
+    given = out is not None
+    if not given:
         out = _like(q, dtype)
     else:
         _dense(out, "out", (tokens, heads, d), (dtype,), dev)
@@ -188,6 +217,8 @@ def packed_attention(q, k, v, seqs, mask=None, causal=True, scale=None, out_bf16
         q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), 1 if out_bf16 else 0, lse.data_ptr() if with_lse else None, heads, kvh, d,
         *seqs._args, tokens, keys, seqs.max_q, seqs.max_k, 1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0, *m,
         work.data_ptr() if nbytes else None, nbytes, _lib.stream()))
+    if given:
+        increment_version(out)
     return (out, lse) if with_lse else out
 
 
@@ -195,6 +226,8 @@ def packed_attention_backward(dout, q, k, v, out, lse, seqs, mask=None, causal=T
     """The gradients (dq, dk, dv), contiguous, of a scalar from its gradient dout [tokens, heads, d] (f32 or bf16) by packed_attention's result:
     q, k, v, seqs, mask, causal and scale as that call had them, out and lse as it returned them. Rows and keys behind the last sequence
     are not written."""
+    if _watched(dout):   # (gradients of gradients)
+        return _NoGraph.apply("packed_attention_backward", lambda: packed_attention_backward(dout, q, k, v, out, lse, seqs, mask, causal, scale, grads_bf16), dout)
     dev, d, heads, kvh, qs, ks, vs, m = _operands("packed_attention_backward", q, k, v, seqs, mask, causal)
     tokens, keys = q.shape[0], k.shape[0]
     _dense(dout, "dout", (tokens, heads, d), (_BF16, _F32), dev)
