@@ -215,7 +215,7 @@ def packed_attention(q, k, v, seqs, mask=None, causal=True, scale=None, out_bf16
     work = torch.empty(nbytes, device=q.device, dtype=_U8) if nbytes else None
     _lib.check(lib.fv_packed_attention(
         q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), 1 if out_bf16 else 0, lse.data_ptr() if with_lse else None, heads, kvh, d,
-        *seqs._args, tokens, keys, seqs.max_q, seqs.max_k, 1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0, *m,
+        *seqs._args, tokens, keys, seqs.max_q, seqs.max_k, 1.0 / math.sqrt(d or 1) if scale is None else scale, 1 if causal else 0, *m,
         work.data_ptr() if nbytes else None, nbytes, _lib.stream()))
     if given:
         increment_version(out)
@@ -242,5 +242,5 @@ def packed_attention_backward(dout, q, k, v, out, lse, seqs, mask=None, causal=T
     _lib.check(lib.fv_packed_attention_backward(
         dout.data_ptr(), g16, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), 1 if out.dtype is _BF16 else 0, lse.data_ptr(),
         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), 1 if grads_bf16 else 0, heads, kvh, d, *seqs._args, tokens, keys, seqs.max_q, seqs.max_k,
-        1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0, *m, work.data_ptr() if nbytes else None, nbytes, _lib.stream()))
+        1.0 / math.sqrt(d or 1) if scale is None else scale, 1 if causal else 0, *m, work.data_ptr() if nbytes else None, nbytes, _lib.stream()))
     return dq, dk, dv

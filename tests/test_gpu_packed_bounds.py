@@ -78,3 +78,14 @@ def test_rows_and_keys_past_the_bounds_are_left():
     rows, keys = c.left_out()
     for x, rest in zip(grads, (rows, keys, keys)):
         assert (x[rest] == 7).all() and torch.isfinite(x).all()
+
+
+def test_heads_of_no_channels():
+    """Refused by the library, as every head dim but 64 and 128 is."""
+    none = torch.zeros(5, 2, 0, dtype=torch.bfloat16, device="cuda")
+    starts = torch.tensor([0, 5], dtype=torch.int32, device="cuda")
+    lse = torch.zeros(5, 2, device="cuda")
+    for call in (lambda: fv_sdpa.packed_attention(none, none, none, fv_sdpa.PackedSeqs(starts, 5)),
+                 lambda: fv_sdpa.packed_attention_backward(none, none, none, none, none, lse, fv_sdpa.PackedSeqs(starts, 5))):
+        with pytest.raises(fv_sdpa.FvDeclined, match="head dim"):
+            call()
