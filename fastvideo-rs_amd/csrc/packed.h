@@ -230,5 +230,5 @@ int fv_packed_args(const char* who, const PackedCall& c, const PackedOperand* x,
 fv::PackedMask fv_packed_mask(const PackedCall& c);
 // Numbers whose workspace is asked for, within what the entries take.
 bool fv_packed_sizes(const PackedCall& c);
-// Steps of `step` keys (or rows) that the walk of a piece may have, on the call's bounds.
+// Tiles of 64 keys that the walk of a piece of `rows` rows may have, by the call's bounds.
 size_t fv_packed_key_steps(const PackedCall& c, size_t rows);

@@ -420,7 +420,6 @@ PackedCut packed_cut(const PackedCall& c) {
 }  // namespace
 }  // namespace fv
 
-// Tiles of 64 keys that the walk of `rows` rows may have.
 size_t fv_packed_key_steps(const PackedCall& c, size_t rows) {
     size_t steps = (c.max_k + fv::kTileRows - 1) / fv::kTileRows;
     if (c.causal && c.window > 0) {   // the first token's window and the blocks to the last token's, a step more (they begin anywhere in one); the sink

@@ -224,8 +224,9 @@ def packed_attention(q, k, v, seqs, mask=None, causal=True, scale=None, out_bf16
 
 def packed_attention_backward(dout, q, k, v, out, lse, seqs, mask=None, causal=True, scale=None, grads_bf16=True):
     """The gradients (dq, dk, dv), contiguous, of a scalar from its gradient dout [tokens, heads, d] (f32 or bf16) by packed_attention's result:
-    q, k, v, seqs, mask, causal and scale as that call had them, out and lse as it returned them. Rows and keys behind the last sequence
-    are not written."""
+    q, k, v, seqs, mask, causal and scale as that call had them, out and lse as it returned them. An f32 dout is rounded to bf16 first. By an f32
+    out rows that see few keys are nearer (in calls whose rows see 64 keys at most they are so by either). Rows and keys behind the last
+    sequence are not written."""
     if _watched(dout):   # (gradients of gradients)
         return _NoGraph.apply("packed_attention_backward", lambda: packed_attention_backward(dout, q, k, v, out, lse, seqs, mask, causal, scale, grads_bf16), dout)
     dev, d, heads, kvh, qs, ks, vs, m = _operands("packed_attention_backward", q, k, v, seqs, mask, causal)

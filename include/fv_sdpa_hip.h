@@ -442,7 +442,7 @@ int fv_packed_attention(const uint16_t* q, size_t q_stride, const uint16_t* k, s
  * fv_packed_attention on the same operands and numbers, its out (contiguous, out_is_bf16) and lse: with P = e^(scale q k^T - lse), dv = P^T dout,
  * dS = P (dout v^T - sum(dout out)), dq = scale dS k, dk = scale dS^T q, summed over the heads that share a key head, always in one order (no
  * atomics). (Rows that see up to 8 keys, in calls whose max_k or window and sink leave no row more than 64: with sum_j P_j (dout . v_j) in place of
- * sum(dout out), whose rounding would be as much as their dS.) P and dS are rounded to bf16 for the second products. workspace: fv_packed_attention_backward_workspace_bytes, which it cannot do without. */
+ * sum(dout out), whose rounding would be as much as their dS; in other calls a result in f32, out_is_bf16 0, keeps such rows free of that rounding.) P and dS are rounded to bf16 for the second products. workspace: fv_packed_attention_backward_workspace_bytes, which it cannot do without. */
 size_t fv_packed_attention_backward_workspace_bytes(int dout_is_bf16, size_t heads, size_t kv_heads, size_t d, size_t seqs, size_t q_tokens,
                                                     size_t k_tokens, size_t max_q, size_t max_k, int causal, size_t block_tokens,
                                                     size_t window, size_t sink);
@@ -457,7 +457,8 @@ int fv_packed_attention_backward(const void* dout, int dout_is_bf16, const uint1
  *   scaling 0: not (factor is not read); 1: theta / factor; 2: with base * factor^(pairs / (pairs - 1)) in place of base, which leaves the first
  *   pair and slows the last by factor (pairs > 1); 3: by parts: theta (c + (1 - c) / factor), c = clamp((original theta / 2 pi - low) / (high - low), 0, 1), so
  *   that pairs of more than `high` turns in the `original` context stay and those of fewer than `low` are slowed (original, low, high are read here alone);
- * as turns a position in units of 2^-64: angles of any 32-bit position are exact to 2^-33 turns, with no table to make. */
+ * as turns a position in units of 2^-64, with no table to make: the product with any 32-bit position is within 2^-33 turns, the angle whose sine and cosine are
+ * taken, in f32, within 2^-26 at any position. */
 int fv_rope_frequencies(size_t pairs, double base, int scaling, double factor, double original, double low, double high,
                         uint64_t* out);
 /* q [tokens, heads, d] (and k [tokens, kv_heads, d]; NULL: none) with the first 2 * pairs channels of each head turned by angles positions[token *
